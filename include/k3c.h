@@ -560,6 +560,92 @@ int k3c_moe_prefill_tc(float *out, const void *x, int x_dtype, int ntok,
 int k3c_moe_combine(float *out, const float *contrib, const float *wt, const int *idx, int n_experts,
                     int ntok, int topk, int hidden, int has_shared, k3c_stream_t stream);
 
+/* ------------------------------------------------------------------------------------
+ * Tokens sorted by expert and back (no reference counterpart as operators: the reference visits
+ * a token's experts one by one, src/core/k3_ops.c:630-645). Pair p = t * topk + j is token t's
+ * j-th expert idx[t][j]. An id outside [0, n_experts) (another rank's expert, a dropped one) has
+ * no row: pos = -1, and every operator below passes over it. A token may name an expert more
+ * than once. ntok may be 0. Nothing here synchronises the host or allocates.
+ * ------------------------------------------------------------------------------------ */
+/* Stable sort of the pairs by expert: off[n_experts + 1] first rows (off[n_experts] rows in
+ * all), pos[ntok][topk] each pair's row or -1, pair[ntok * topk] each row's pair, -1 behind the
+ * last row. n_experts <= 2048. scratch: k3c_moe_sort_scratch bytes (0 for small calls: may be
+ * NULL), not shared between calls that may overlap. */
+size_t k3c_moe_sort_scratch(int ntok, int topk, int n_experts);
+int k3c_moe_sort(int *pos, int *pair, int *off, const int *idx, int ntok, int topk, int n_experts,
+                 void *scratch, size_t scratch_bytes, k3c_stream_t stream);
+/* rows[pos[t][j]] = x[t]: x [ntok] rows of ldx elements, rows [ntok * topk][hidden] of the same
+ * type (K3C_F32 or K3C_BF16); rows no pair has are left as they were. */
+int k3c_moe_permute(void *rows, const void *x, int dtype, int64_t ldx, const int *pos, int ntok, int topk,
+                    int hidden, k3c_stream_t stream);
+/* Its gradient: dx[t] = sum_j drows[pos[t][j]], fp32 sums in the order of j, rounded once; a
+ * token without rows gets zeros. */
+int k3c_moe_permute_bwd(void *dx, const void *drows, int dtype, const int *pos, int ntok, int topk,
+                        int hidden, k3c_stream_t stream);
+/* The permute and k3c_mxfp4_quant in one pass: packed [ntok * topk][hidden / 2] and scales
+ * [ntok * topk][hidden / 32] rows, as k3c_mxfp4_mm reads them. hidden a multiple of 32, packed
+ * 16-byte aligned. */
+int k3c_moe_permute_mxfp4(uint8_t *packed, uint8_t *scales, const void *x, int x_dtype, int64_t ldx,
+                          const int *pos, int ntok, int topk, int hidden, k3c_stream_t stream);
+/* out[t] = sum_j wt[t][j] * y[pos[t][j]], products and sums rounded separately in fp32 in the
+ * order of j (src/core/k3_ops.c:641-642), rounded once to out's type; y [ntok * topk][hidden]. */
+int k3c_moe_unpermute(void *out, int out_dtype, const void *y, int y_dtype, const float *wt, const int *pos,
+                      int ntok, int topk, int hidden, k3c_stream_t stream);
+/* Its gradients: dy[pos[t][j]] = wt[t][j] * dout[t] (y's type; rows no pair has are left as they
+ * were) and dwt[t][j] = <dout[t], y[pos[t][j]]> (fp32; 0 for a pair without a row). Either may be
+ * NULL; y is not read when dwt is. dy must not overlap y. */
+int k3c_moe_unpermute_bwd(void *dy, float *dwt, const void *dout, int out_dtype, const void *y, int y_dtype,
+                          const float *wt, const int *pos, int ntok, int topk, int hidden,
+                          k3c_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * MXFP4 quantisation and products (E2M1 x E2M1 on tcgen05 kind::mxf4; no reference counterpart,
+ * the packed format is the reference's).
+ * ------------------------------------------------------------------------------------ */
+/* x [rows] rows of ldx elements (x_dtype K3C_F32 or K3C_BF16) to packed [rows][in/2] and scales
+ * [rows][ceil(in/32)]: per 32 elements scale byte clamp(floor(log2 max|x|) - 2 + 127, 0, 254),
+ * codes round(x * 2^(127-byte)) to the nearest E2M1 value, ties to even, saturating at +-6. An
+ * infinity makes its group's byte 253 and reads back as an infinity; a NaN makes it 255 with
+ * zero codes, which k3c_mxfp4_mm reads as NaN and k3c_mxfp4_dequant, like the reference, as 0.
+ * in even. */
+int k3c_mxfp4_quant(uint8_t *packed, uint8_t *scales, const void *x, int x_dtype, int64_t ldx, int rows, int in,
+                    k3c_stream_t stream);
+/* A product's right operand: n_mats matrices [rows][in] as codes [rows][in/2], code_stride
+ * bytes apart, and their scales in atoms of 512 bytes, atom_stride bytes apart:
+ * [ceil(rows/128)][ceil(in/128)] atoms, row r's scale of group g at byte
+ * 16 * (r % 32) + 4 * (r % 128 / 32) + g % 4 of atom [r / 128][g / 4] (rows and groups past the
+ * matrix hold 127). That is what k3c_mxfp4_pack writes, and how a pool-format run holds an
+ * expert's matrices: codes = arena + the matrix's offset in the run, both strides the run
+ * stride, mat_of = the layer's run_of. Group g multiplies matrix mat_of[g] (device; NULL: g
+ * itself); an index outside [0, n_mats) makes the group's results zeros. in a multiple of 32,
+ * every address and stride of 16 bytes. */
+typedef struct {
+    const uint8_t *codes, *atoms;
+    size_t code_stride, atom_stride;
+    int n_mats, rows, in;
+    const int *mat_of;
+} k3c_mxfp4_mat;
+size_t k3c_mxfp4_atom_bytes(int rows, int in);
+/* n_mats matrices from the reference layout (packed [n_mats][rows][in/2], scales
+ * [n_mats][rows][in/32]) to codes and atoms, densely; a group with scale 255 (the reference skips
+ * it) becomes zero codes under scale 127. codes may be packed itself. */
+int k3c_mxfp4_pack(uint8_t *codes, uint8_t *atoms, const uint8_t *packed, const uint8_t *scales, int n_mats,
+                   int rows, int in, k3c_stream_t stream);
+/* y[r][o] = sum_i A[r][i] W_g[o][i], A as k3c_mxfp4_quant writes it (a [M][in/2] 16-byte aligned,
+ * a_scales [M][in/32]); rows off[g] .. off[g+1] - 1 (device, n_groups + 1 ints, ascending;
+ * offsets outside 0..M are clamped) belong to group g, rows outside every group are left as they
+ * were; off NULL with n_groups 1: all rows. Exact products, fp32 accumulation, one rounding to
+ * y_dtype; y rows ldy >= rows elements apart. n_groups <= 1024. The result does not depend on
+ * how the work is spread. */
+int k3c_mxfp4_mm(void *y, int y_dtype, int64_t ldy, const uint8_t *a, const uint8_t *a_scales, int M,
+                 const k3c_mxfp4_mat *W, const int *off, int n_groups, k3c_stream_t stream);
+/* The gradient with respect to A's values: da[r][i] = sum_o dy[r][o] W_g[o][i], dy bf16 rows of
+ * lddy elements (a multiple of 8, dy 16-byte aligned), fp32 accumulation, one rounding to
+ * da_dtype. Weights past fp32's range (scale bytes above 251) enter as infinities, as in
+ * k3_matmul_mxfp4. Quantisation passes gradients straight through; packed weights are constants. */
+int k3c_mxfp4_mm_bwd(void *da, int da_dtype, int64_t ldda, const void *dy, int64_t lddy, int M,
+                     const k3c_mxfp4_mat *W, const int *off, int n_groups, k3c_stream_t stream);
+
 /* ---- Expert-parallel prefill over peer memory (no reference counterpart: the reference is
  * a single-process CPU engine). The ranks of one node each own a set of routed experts (the
  * layer's run table marks the others -1) and their own tokens. Per layer, with a cross-rank

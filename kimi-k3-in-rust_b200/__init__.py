@@ -67,6 +67,14 @@ class MoeLatentLayerC(C.Structure):
                 + [("cache_only", C.c_int)])
 
 
+class Mxfp4MatC(C.Structure):
+    """Mirror of k3c_mxfp4_mat (include/k3c.h): packed matrices on the device."""
+
+    _fields_ = [("codes", C.c_void_p), ("atoms", C.c_void_p), ("code_stride", C.c_size_t),
+                ("atom_stride", C.c_size_t), ("n_mats", C.c_int), ("rows", C.c_int), ("in_", C.c_int),
+                ("mat_of", C.c_void_p)]
+
+
 class TensorC(C.Structure):
     """Mirror of k3c_tensor (include/k3c.h)."""
 
@@ -262,6 +270,18 @@ def lib():
         "k3c_expert_ref": ([vp, i, i, C.POINTER(ExpertRunC)], i),
         "k3c_expert_read": ([vp, C.POINTER(ExpertRunC), vp, C.c_int64, C.POINTER(C.c_int64)], C.c_int64),
         "k3c_expert_upload": ([vp, C.POINTER(ExpertRunC), vp, vp, vp], i),
+        "k3c_moe_sort_scratch": ([i, i, i], sz),
+        "k3c_moe_sort": ([vp, vp, vp, vp, i, i, i, vp, sz, vp], i),
+        "k3c_moe_permute": ([vp, vp, i, C.c_int64, vp, i, i, i, vp], i),
+        "k3c_moe_permute_bwd": ([vp, vp, i, vp, i, i, i, vp], i),
+        "k3c_moe_permute_mxfp4": ([vp, vp, vp, i, C.c_int64, vp, i, i, i, vp], i),
+        "k3c_moe_unpermute": ([vp, i, vp, i, vp, vp, i, i, i, vp], i),
+        "k3c_moe_unpermute_bwd": ([vp, vp, vp, i, vp, i, vp, vp, i, i, i, vp], i),
+        "k3c_mxfp4_quant": ([vp, vp, vp, i, C.c_int64, i, i, vp], i),
+        "k3c_mxfp4_atom_bytes": ([i, i], sz),
+        "k3c_mxfp4_pack": ([vp, vp, vp, vp, i, i, i, vp], i),
+        "k3c_mxfp4_mm": ([vp, i, C.c_int64, vp, vp, i, C.POINTER(Mxfp4MatC), vp, i, vp], i),
+        "k3c_mxfp4_mm_bwd": ([vp, i, C.c_int64, vp, C.c_int64, i, C.POINTER(Mxfp4MatC), vp, i, vp], i),
         "k3c_moe_latent_decode": ([vp, vp, i, C.POINTER(MoeLatentLayerC), vp, vp, vp, vp, sz, vp], i),
     }
     for name, (args, res) in sig.items():
@@ -976,6 +996,303 @@ class LatentMoeLayer:
                                                   self._scratch.numel(), _stream()),
                "k3c_moe_latent_decode_routed")
         return out
+
+
+# ------------------------------------------------------------------ expert dispatch, MXFP4 products
+# These wrappers check what the C entry points cannot see (element types, shapes, devices), run on
+# the tensors' own device and on that device's current stream, and allocate only their results.
+
+
+class _On:
+    """The tensors' device made current for a call where it is not."""
+
+    __slots__ = ("dev", "prev")
+
+    def __init__(self, t):
+        self.dev = t.device.index
+
+    def __enter__(self):
+        import torch
+        prev = torch.cuda.current_device()
+        self.prev = None
+        if prev != self.dev:
+            torch.cuda.set_device(self.dev)
+            self.prev = prev
+        return C.c_void_p(torch.cuda.current_stream(self.dev).cuda_stream)
+
+    def __exit__(self, *exc):
+        if self.prev is not None:
+            import torch
+            torch.cuda.set_device(self.prev)
+
+
+def _need(ok, what):
+    if not ok:
+        raise K3CError(what)
+
+
+def _arg(t, name, dtypes, shape, like=None):
+    """t is a CUDA tensor of one of dtypes and of shape (None: any extent), contiguous."""
+    if t.dtype not in dtypes or t.dim() != len(shape) or any(s is not None and s != n for s, n in zip(shape, t.shape)):
+        raise K3CError(f"{name}: {t.dtype} {tuple(t.shape)}, expected {dtypes} {tuple(shape)}")
+    if not t.is_cuda or (like is not None and t.device != like.device):
+        raise K3CError(f"{name}: on {t.device}" + (f", expected {like.device}" if like is not None else ""))
+    if not t.is_contiguous():
+        raise K3CError(f"{name}: not contiguous (strides {t.stride()})")
+    return t
+
+
+def _rows_arg(t, name, dtypes, like=None):
+    """A 2-D CUDA tensor whose rows are contiguous; returns its row stride in elements."""
+    if t.dtype not in dtypes or t.dim() != 2:
+        raise K3CError(f"{name}: {t.dtype} {tuple(t.shape)}, expected 2-D {dtypes}")
+    if not t.is_cuda or (like is not None and t.device != like.device):
+        raise K3CError(f"{name}: on {t.device}" + (f", expected {like.device}" if like is not None else ""))
+    rows, n = t.shape
+    if rows <= 1:
+        ok, ld = n <= 1 or t.stride(1) == 1, n
+    else:
+        ok, ld = (n <= 1 or t.stride(1) == 1) and t.stride(0) >= n, t.stride(0)
+    if not ok:
+        raise K3CError(f"{name}: rows are not contiguous (strides {t.stride()})")
+    return ld
+
+
+def _types():
+    import torch
+    return (torch.float32, torch.bfloat16), torch
+
+
+def moe_sort(idx, n_experts):
+    """Stable sort of a routing's pairs by expert: idx [T][topk] int32 -> (pos [T][topk], pair
+    [T * topk], off [n_experts + 1]) int32. pos is a pair's row, -1 for ids outside
+    0..n_experts-1; pair a row's pair t * topk + j, -1 behind the last row (off[n_experts])."""
+    _, torch = _types()
+    _arg(idx, "idx", (torch.int32,), (None, None))
+    T, K = idx.shape
+    L = lib()
+    pos, pair = torch.empty_like(idx), torch.empty(T * K, dtype=torch.int32, device=idx.device)
+    off = torch.empty(n_experts + 1, dtype=torch.int32, device=idx.device)
+    n = L.k3c_moe_sort_scratch(T, K, n_experts)
+    ws = torch.empty(n, dtype=torch.uint8, device=idx.device) if n else None
+    with _On(idx) as s:
+        _check(L.k3c_moe_sort(_ptr(pos), _ptr(pair), _ptr(off), _ptr(idx), T, K, n_experts, _ptr(ws), n, s),
+               "k3c_moe_sort")
+    return pos, pair, off
+
+
+def moe_permute(x, pos, out=None):
+    """Every pair's token row in expert order: out[pos[t][j]] = x[t], x [T][H] bf16 or fp32 (rows
+    may be strided), out [T * topk][H]. Rows no pair has are left as they were (in a new out:
+    undefined)."""
+    ft, torch = _types()
+    ld = _rows_arg(x, "x", ft)
+    T, H = x.shape
+    _arg(pos, "pos", (torch.int32,), (T, None), x)
+    K = pos.shape[1]
+    if out is None:
+        out = torch.empty((T * K, H), dtype=x.dtype, device=x.device)
+    else:
+        _arg(out, "out", (x.dtype,), (T * K, H), x)
+    with _On(x) as s:
+        _check(lib().k3c_moe_permute(_ptr(out), _ptr(x), _dtype_code(x), ld, _ptr(pos), T, K, H, s), "k3c_moe_permute")
+    return out
+
+
+def moe_permute_bwd(drows, pos, out=None):
+    """moe_permute's gradient: dx[t] = sum_j drows[pos[t][j]], drows [T * topk][H]."""
+    ft, torch = _types()
+    _arg(pos, "pos", (torch.int32,), (None, None))
+    T, K = pos.shape
+    _arg(drows, "drows", ft, (T * K, None), pos)
+    H = drows.shape[1]
+    if out is None:
+        out = torch.empty((T, H), dtype=drows.dtype, device=drows.device)
+    else:
+        _arg(out, "out", (drows.dtype,), (T, H), drows)
+    with _On(drows) as s:
+        _check(lib().k3c_moe_permute_bwd(_ptr(out), _ptr(drows), _dtype_code(drows), _ptr(pos), T, K, H, s),
+               "k3c_moe_permute_bwd")
+    return out
+
+
+def moe_permute_mxfp4(x, pos):
+    """moe_permute and mxfp4_quant in one pass: (packed [T * topk][H / 2], scales
+    [T * topk][H / 32]) uint8 in expert order. H a multiple of 32."""
+    ft, torch = _types()
+    ld = _rows_arg(x, "x", ft)
+    T, H = x.shape
+    _arg(pos, "pos", (torch.int32,), (T, None), x)
+    K = pos.shape[1]
+    packed = torch.empty((T * K, H // 2), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((T * K, H // 32), dtype=torch.uint8, device=x.device)
+    with _On(x) as s:
+        _check(lib().k3c_moe_permute_mxfp4(_ptr(packed), _ptr(scales), _ptr(x), _dtype_code(x), ld, _ptr(pos), T, K, H, s),
+               "k3c_moe_permute_mxfp4")
+    return packed, scales
+
+
+def moe_unpermute(y, pos, wt, out=None, out_dtype=None):
+    """out[t] = sum_j wt[t][j] * y[pos[t][j]]: y [T * topk][H] in expert order, wt [T][topk] fp32;
+    out [T][H] of out_dtype (default: y's)."""
+    ft, torch = _types()
+    _arg(pos, "pos", (torch.int32,), (None, None))
+    T, K = pos.shape
+    _arg(y, "y", ft, (T * K, None), pos)
+    _arg(wt, "wt", (torch.float32,), (T, K), pos)
+    H = y.shape[1]
+    if out is None:
+        out = torch.empty((T, H), dtype=out_dtype or y.dtype, device=y.device)
+    _arg(out, "out", ft if out_dtype is None else (out_dtype,), (T, H), y)
+    with _On(y) as s:
+        _check(lib().k3c_moe_unpermute(_ptr(out), _dtype_code(out), _ptr(y), _dtype_code(y), _ptr(wt), _ptr(pos), T, K, H, s),
+               "k3c_moe_unpermute")
+    return out
+
+
+def moe_unpermute_bwd(dout, y, pos, wt, dy=None, dwt=None):
+    """moe_unpermute's gradients (dy [T * topk][H] of y's type, dwt [T][topk] fp32). Rows of dy no
+    pair has are left as they were (in a new dy: undefined)."""
+    ft, torch = _types()
+    _arg(pos, "pos", (torch.int32,), (None, None))
+    T, K = pos.shape
+    _arg(y, "y", ft, (T * K, None), pos)
+    H = y.shape[1]
+    _arg(dout, "dout", ft, (T, H), pos)
+    _arg(wt, "wt", (torch.float32,), (T, K), pos)
+    dy = torch.empty_like(y) if dy is None else _arg(dy, "dy", (y.dtype,), (T * K, H), y)
+    dwt = torch.empty_like(wt) if dwt is None else _arg(dwt, "dwt", (torch.float32,), (T, K), y)
+    with _On(y) as s:
+        _check(lib().k3c_moe_unpermute_bwd(_ptr(dy), _ptr(dwt), _ptr(dout), _dtype_code(dout), _ptr(y), _dtype_code(y),
+                                           _ptr(wt), _ptr(pos), T, K, H, s), "k3c_moe_unpermute_bwd")
+    return dy, dwt
+
+
+def mxfp4_quant(x):
+    """x [rows][in] bf16 or fp32 (rows may be strided, in even) -> (packed [rows][in/2], scales
+    [rows][ceil(in/32)]) uint8, the layout mxfp4_dequant, mxfp4_gemv and mxfp4_mm read."""
+    ft, torch = _types()
+    ld = _rows_arg(x, "x", ft)
+    M, K = x.shape
+    packed = torch.empty((M, K // 2), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((M, (K + 31) // 32), dtype=torch.uint8, device=x.device)
+    with _On(x) as s:
+        _check(lib().k3c_mxfp4_quant(_ptr(packed), _ptr(scales), _ptr(x), _dtype_code(x), ld, M, K, s), "k3c_mxfp4_quant")
+    return packed, scales
+
+
+def mxfp4_pack(packed, scales):
+    """Matrices in the reference layout (packed [n][rows][in/2], scales [n][rows][in/32] uint8; or
+    one without the leading extent) -> (codes, atoms) as Mxfp4Mat takes them."""
+    _, torch = _types()
+    if packed.dim() == 2 and scales.dim() == 2:
+        packed, scales = packed.unsqueeze(0), scales.unsqueeze(0)
+    _arg(packed, "packed", (torch.uint8,), (None, None, None))
+    n, rows, half = packed.shape
+    _arg(scales, "scales", (torch.uint8,), (n, rows, half // 16), packed)
+    codes = torch.empty_like(packed)
+    atoms = torch.empty((n, (rows + 127) // 128, (2 * half + 127) // 128, 512), dtype=torch.uint8, device=packed.device)
+    with _On(packed) as s:
+        _check(lib().k3c_mxfp4_pack(_ptr(codes), _ptr(atoms), _ptr(packed), _ptr(scales), n, rows, 2 * half, s),
+               "k3c_mxfp4_pack")
+    return codes, atoms
+
+
+class Mxfp4Mat:
+    """Packed matrices as the right operand of mxfp4_mm: codes [n][rows][in/2] and atoms
+    [n][ceil(rows/128)][ceil(in/128)][512] as mxfp4_pack returns them, or one matrix of every run
+    of a PoolMoeLayer (from_pool). The tensors are kept, not copied."""
+
+    __slots__ = ("c", "keep", "device")
+
+    def __init__(self, codes, atoms, mat_of=None):
+        """mat_of: device int32, the matrix of each group of rows (default: group g's is g)."""
+        _, torch = _types()
+        _arg(codes, "codes", (torch.uint8,), (None, None, None))
+        n, rows, half = codes.shape
+        _arg(atoms, "atoms", (torch.uint8,), (n, (rows + 127) // 128, (2 * half + 127) // 128, 512), codes)
+        if mat_of is not None:
+            _arg(mat_of, "mat_of", (torch.int32,), (None,), codes)
+        self.c = Mxfp4MatC(codes.data_ptr(), atoms.data_ptr(), rows * half, atoms.stride(0), n, rows, 2 * half,
+                           None if mat_of is None else mat_of.data_ptr())
+        self.keep, self.device = (codes, atoms, mat_of), codes.device
+
+    @classmethod
+    def from_pool(cls, layer, which):
+        """The experts' matrices of a PoolMoeLayer in its arena, by expert id: "gate_up" [2 * inter]
+        [hidden] (64 gate rows, the matching 64 up rows, and so on) or "down" [hidden][inter].
+        Experts without a run give zeros."""
+        H, I = layer.c.hidden, layer.c.inter
+        if which not in ("gate_up", "down"):
+            raise K3CError(f"from_pool: {which!r}")
+        lay, _ = pool_layout(H, I)
+        p, s = ("gu_p", "gu_s") if which == "gate_up" else ("d_p", "d_s")
+        rows, in_ = (2 * I, H) if which == "gate_up" else (H, I)
+        base = layer.arena.data_ptr()
+        m = cls.__new__(cls)
+        m.c = Mxfp4MatC(base + lay[p][0], base + lay[s][0], layer.stride, layer.stride, layer.c.n_runs, rows, in_,
+                        layer.run_of.data_ptr())
+        m.keep, m.device = (layer.arena, layer.run_of, None), layer.arena.device
+        return m
+
+    @property
+    def groups(self):
+        """Groups of rows an `off` may name: one per entry of mat_of, or per matrix."""
+        mat_of = self.keep[2] if self.keep[2] is not None else (self.keep[1] if self.c.mat_of else None)
+        return self.c.n_mats if mat_of is None else mat_of.numel()
+
+
+def _mm_groups(W, off, like):
+    """(off pointer, number of groups) of a product."""
+    _, torch = _types()
+    if W.device != like.device:
+        raise K3CError(f"matrices on {W.device}, rows on {like.device}")
+    if off is None:
+        return None, 1
+    _arg(off, "off", (torch.int32,), (None,), like)
+    G = off.numel() - 1
+    if G < 1 or G > W.groups:
+        raise K3CError(f"off: {G} groups, {W.groups} matrices")
+    return _ptr(off), G
+
+
+def mxfp4_mm(a, a_scales, W, off=None, out=None, out_dtype=None):
+    """y[r] = W_g a[r]: a [M][in/2] and a_scales [M][in/32] as mxfp4_quant or moe_permute_mxfp4
+    return them, W an Mxfp4Mat. Without off every row multiplies W's first matrix (mat_of[0]);
+    with off [G + 1] int32 (moe_sort's) rows off[g]..off[g+1]-1 multiply group g's and rows
+    outside every group are left as they were (in a new out: undefined). out [M][rows] of
+    out_dtype (default bf16), rows may be strided."""
+    ft, torch = _types()
+    _arg(a, "a", (torch.uint8,), (None, W.c.in_ // 2))
+    M = a.shape[0]
+    _arg(a_scales, "a_scales", (torch.uint8,), (M, W.c.in_ // 32), a)
+    po, G = _mm_groups(W, off, a)
+    if out is None:
+        out = torch.empty((M, W.c.rows), dtype=out_dtype or torch.bfloat16, device=a.device)
+    ld = _rows_arg(out, "out", ft if out_dtype is None else (out_dtype,), a)
+    _need(out.shape == (M, W.c.rows), f"out: {tuple(out.shape)}, expected {(M, W.c.rows)}")
+    with _On(a) as s:
+        _check(lib().k3c_mxfp4_mm(_ptr(out), _dtype_code(out), ld, _ptr(a), _ptr(a_scales), M, C.byref(W.c), po, G, s),
+               "k3c_mxfp4_mm")
+    return out
+
+
+def mxfp4_mm_bwd(dy, W, off=None, out=None, out_dtype=None):
+    """mxfp4_mm's gradient with respect to a's values: da[r] = W_g^T dy[r], dy [M][rows] bf16 (rows
+    may be strided, the stride a multiple of 8). out [M][in] of out_dtype (default bf16)."""
+    ft, torch = _types()
+    ldd = _rows_arg(dy, "dy", (torch.bfloat16,))
+    M = dy.shape[0]
+    _need(dy.shape[1] == W.c.rows, f"dy: {tuple(dy.shape)}, {W.c.rows} columns expected")
+    po, G = _mm_groups(W, off, dy)
+    if out is None:
+        out = torch.empty((M, W.c.in_), dtype=out_dtype or torch.bfloat16, device=dy.device)
+    ld = _rows_arg(out, "out", ft if out_dtype is None else (out_dtype,), dy)
+    _need(out.shape == (M, W.c.in_), f"out: {tuple(out.shape)}, expected {(M, W.c.in_)}")
+    with _On(dy) as s:
+        _check(lib().k3c_mxfp4_mm_bwd(_ptr(out), _dtype_code(out), ld, _ptr(dy), ldd, M, C.byref(W.c), po, G, s),
+               "k3c_mxfp4_mm_bwd")
+    return out
 
 
 # ------------------------------------------------------------------ checkpoint experts

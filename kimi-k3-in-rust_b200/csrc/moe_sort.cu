@@ -1,0 +1,610 @@
+// moe_sort.cu -- (token, expert) pairs sorted by expert and back, as operators of their own:
+// the sort, the copy of every pair's token row into expert order (plain, or quantised to MXFP4
+// on the way), the weighted sum back per token, and the gradients of both copies. No reference
+// counterpart (the reference visits a token's experts one after another,
+// src/core/k3_ops.c:630-645); the order of a token's sum is the reference's.
+//
+// With pairs p = t*topk + j:
+//     pos[p]  = off[idx[p]] + #{q < p : idx[q] = idx[p]}       (stable counting sort)
+//     rows[pos[t][j]] = x[t]                                    permute
+//     dx[t]   = sum_j drows[pos[t][j]]                          its gradient
+//     out[t]  = sum_j wt[t][j] * y[pos[t][j]]                   unpermute
+//     dy[pos[t][j]] = wt[t][j] * dout[t],  dwt[t][j] = <dout[t], y[pos[t][j]]>
+// Sums run in the order of j in fp32, each result is rounded once. Every output element has one
+// writer, so no result depends on the order in which blocks run.
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "common.cuh"
+#include "mx4_quant.cuh"
+
+namespace k3c {
+
+namespace {
+
+// ------------------------------------------------------------------ sort
+constexpr int SORT_TH = 1024;
+constexpr int SORT_WARPS = SORT_TH / 32;
+constexpr int SORT_SUB = 4096;                    // pairs placed per pass of a block
+constexpr int SORT_ROUNDS = SORT_SUB / SORT_TH;   // 32-pair rounds per warp and pass
+constexpr int SORT_BLOCKS = 128;                  // blocks at most: every one reads all blocks' counts
+constexpr int SORT_EMAX = 2048;
+
+__device__ __forceinline__ int expert_of(const int *idx, int p, int P, int E) {
+    if (p >= P) return -1;
+    const int e = __ldg(idx + p);
+    return (unsigned)e < (unsigned)E ? e : -1;
+}
+
+// Counts of a block's pairs per expert: cnt[block][E].
+__global__ void __launch_bounds__(SORT_TH) k_sort_count(int *__restrict__ cnt, const int *__restrict__ idx, int P,
+                                                        int E, int chunk) {
+    extern __shared__ int sort_sm[];
+    for (int e = threadIdx.x; e < E; e += SORT_TH) sort_sm[e] = 0;
+    __syncthreads();
+    const int lo = blockIdx.x * chunk, hi = min(P - lo, chunk) + lo;
+    for (int p = lo + threadIdx.x; p < hi; p += SORT_TH) {
+        const int e = expert_of(idx, p, P, E);
+        if (e >= 0) atomicAdd(&sort_sm[e], 1);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += SORT_TH) cnt[(size_t)blockIdx.x * E + e] = sort_sm[e];
+}
+
+// Each block finds its experts' first rows from all blocks' counts (nblk == 1: from its own
+// pairs) and places its chunk, SORT_SUB pairs at a time. A warp owns 128 consecutive pairs of
+// a pass, so a pair's rank is (earlier passes) + (earlier warps) + (earlier rounds of the warp)
+// + (lower lanes with the same expert, from one match per round): no atomics, and a stable order.
+__global__ void __launch_bounds__(SORT_TH) k_sort_place(int *__restrict__ pos, int *__restrict__ pair,
+                                                        int *__restrict__ off, const int *__restrict__ idx,
+                                                        const int *__restrict__ cnt, int P, int E, int chunk, int nblk) {
+    extern __shared__ int sort_sm[];
+    int *base = sort_sm;                                       // [E] next free row of each expert
+    uint16_t *wh = reinterpret_cast<uint16_t *>(base + E);     // [warps][E] counts, then ranks, of a pass
+    __shared__ int warp_tot[SORT_WARPS];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int lo = blockIdx.x * chunk, hi = min(P - lo, chunk) + lo;
+
+    if (nblk == 1) {
+        for (int e = tid; e < E; e += SORT_TH) base[e] = 0;
+        __syncthreads();
+        for (int p = lo + tid; p < hi; p += SORT_TH) {
+            const int e = expert_of(idx, p, P, E);
+            if (e >= 0) atomicAdd(&base[e], 1);
+        }
+        __syncthreads();
+    }
+    int run = 0;   // pairs of the experts before this round of the scan
+    for (int e0 = 0; e0 < E; e0 += SORT_TH) {
+        const int e = e0 + tid;
+        int tot = 0, before = 0;
+        if (e < E) {
+            if (nblk == 1) tot = base[e];
+            else
+                for (int b = 0; b < nblk; b++) {
+                    const int c = cnt[(size_t)b * E + e];
+                    before += b < (int)blockIdx.x ? c : 0;
+                    tot += c;
+                }
+        }
+        int inc = tot;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        if (lane == 31) warp_tot[warp] = inc;
+        __syncthreads();
+        int pre = 0, all = 0;
+        for (int w = 0; w < SORT_WARPS; w++) {
+            const int v = warp_tot[w];
+            pre += w < warp ? v : 0;
+            all += v;
+        }
+        if (e < E) {
+            const int first = run + pre + inc - tot;
+            base[e] = first + before;
+            if (blockIdx.x == 0) off[e] = first;
+        }
+        run += all;
+        __syncthreads();
+    }
+    if (blockIdx.x == 0 && tid == 0) off[E] = run;
+    for (int r = lo + tid; r < hi; r += SORT_TH)   // rows behind the last pair
+        if (r >= run) pair[r] = -1;
+
+    uint16_t *mine = wh + (size_t)warp * E;
+    const uint32_t below = (1u << lane) - 1u;
+    for (int s0 = lo; s0 < hi; s0 += SORT_SUB) {
+        for (int i = tid; i < SORT_WARPS * E; i += SORT_TH) wh[i] = 0;
+        __syncthreads();
+        int ex[SORT_ROUNDS];
+        uint32_t same[SORT_ROUNDS];
+        const int w0 = s0 + warp * (SORT_ROUNDS * 32) + lane;
+#pragma unroll
+        for (int r = 0; r < SORT_ROUNDS; r++) {
+            ex[r] = expert_of(idx, w0 + 32 * r, hi, E);
+            same[r] = __match_any_sync(0xffffffffu, ex[r]);
+            if (ex[r] >= 0 && (same[r] & below) == 0) mine[ex[r]] += (uint16_t)__popc(same[r]);
+            __syncwarp();
+        }
+        __syncthreads();
+        for (int e = tid; e < E; e += SORT_TH) {
+            int at = 0;
+            for (int w = 0; w < SORT_WARPS; w++) {
+                const int c = wh[(size_t)w * E + e];
+                wh[(size_t)w * E + e] = (uint16_t)at;
+                at += c;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < SORT_ROUNDS; r++) {
+            const int p = w0 + 32 * r;
+            int row = -1;
+            if (ex[r] >= 0) row = base[ex[r]] + mine[ex[r]] + __popc(same[r] & below);
+            __syncwarp();
+            if (ex[r] >= 0 && (same[r] & below) == 0) mine[ex[r]] += (uint16_t)__popc(same[r]);
+            __syncwarp();
+            if (p < hi) {
+                pos[p] = row;
+                if (row >= 0) pair[row] = p;
+            }
+        }
+        __syncthreads();
+        // the last warp's running ranks are the pass's counts
+        for (int e = tid; e < E; e += SORT_TH) base[e] += wh[(size_t)(SORT_WARPS - 1) * E + e];
+        __syncthreads();
+    }
+}
+
+// ------------------------------------------------------------------ elements
+// 16 bytes of T as floats and back; V elements.
+template <typename T>
+struct Vec;
+template <>
+struct Vec<float> {
+    static constexpr int V = 4;
+    static __device__ __forceinline__ void get(const uint4 &u, float (&f)[4]) {
+        f[0] = __uint_as_float(u.x);
+        f[1] = __uint_as_float(u.y);
+        f[2] = __uint_as_float(u.z);
+        f[3] = __uint_as_float(u.w);
+    }
+    static __device__ __forceinline__ uint4 put(const float (&f)[4]) {
+        return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    }
+    static __device__ __forceinline__ float one(float v) { return v; }
+    static __device__ __forceinline__ float back(float v) { return v; }
+};
+template <>
+struct Vec<uint16_t> {   // bf16 bits
+    static constexpr int V = 8;
+    static __device__ __forceinline__ void get(const uint4 &u, float (&f)[8]) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            f[2 * i] = __uint_as_float(w[i] << 16);
+            f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    }
+    static __device__ __forceinline__ uint4 put(const float (&f)[8]) {
+        return make_uint4(f32x2_to_bf16x2(f[0], f[1]), f32x2_to_bf16x2(f[2], f[3]), f32x2_to_bf16x2(f[4], f[5]),
+                          f32x2_to_bf16x2(f[6], f[7]));
+    }
+    static __device__ __forceinline__ float one(uint16_t v) { return bf16_bits_to_f32(v); }
+    static __device__ __forceinline__ uint16_t back(float v) { return (uint16_t)(f32x2_to_bf16x2(v, 0.0f) & 0xFFFFu); }
+};
+
+__device__ __forceinline__ uint4 ld16(const void *p) { return ldg_nc_v4(p); }
+// Rows are written once and read by a later kernel: streaming stores keep x and pos in L2.
+__device__ __forceinline__ void st16(void *p, const uint4 &v) { __stcs(reinterpret_cast<uint4 *>(p), v); }
+
+// The row of pair (t, j): -1 for a dropped pair or anything outside [0, P).
+__device__ __forceinline__ int row_of(const int *__restrict__ pos, size_t p, int P) {
+    const int r = __ldg(pos + p);
+    return (unsigned)r < (unsigned)P ? r : -1;
+}
+
+constexpr int PM_TH = 256;
+
+// ------------------------------------------------------------------ permute
+// Block (t, h): 16-byte chunks h*PM_TH.. of token t, read once and stored into the token's rows.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(PM_TH) k_permute(T *__restrict__ rows, const T *__restrict__ x, int64_t ldx,
+                                                   const int *__restrict__ pos, int P, int topk, int H) {
+    const int t = blockIdx.x;
+    const T *xr = x + (size_t)t * ldx;
+    const int *pt = pos + (size_t)t * topk;
+    if constexpr (VEC) {
+        const int n = H / Vec<T>::V, stride = gridDim.y * PM_TH;
+        for (int c = blockIdx.y * PM_TH + threadIdx.x; c < n; c += stride) {
+            const uint4 v = ld16(xr + (size_t)c * Vec<T>::V);
+            for (int j = 0; j < topk; j++) {
+                const int r = row_of(pt, j, P);
+                if (r >= 0) st16(rows + (size_t)r * H + (size_t)c * Vec<T>::V, v);
+            }
+        }
+    } else {
+        for (int i = blockIdx.y * PM_TH + threadIdx.x; i < H; i += gridDim.y * PM_TH) {
+            const T v = xr[i];
+            for (int j = 0; j < topk; j++) {
+                const int r = row_of(pt, j, P);
+                if (r >= 0) rows[(size_t)r * H + i] = v;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------ sums back per token
+// out[t] = sum_j w_j y[pos[t][j]]; wt NULL: w_j = 1 (the gradient of the permute). Four rows'
+// loads are in flight before the first is added; the additions keep the order of j.
+template <typename T, typename O, bool VEC>
+__global__ void __launch_bounds__(PM_TH) k_gather_sum(O *__restrict__ out, const T *__restrict__ y,
+                                                      const float *__restrict__ wt, const int *__restrict__ pos, int P,
+                                                      int topk, int H) {
+    const int t = blockIdx.x;
+    const size_t p0 = (size_t)t * topk;
+    if constexpr (VEC) {
+        constexpr int V = Vec<T>::V;
+        const int n = H / V, stride = gridDim.y * PM_TH;
+        for (int c = blockIdx.y * PM_TH + threadIdx.x; c < n; c += stride) {
+            float acc[V];
+#pragma unroll
+            for (int i = 0; i < V; i++) acc[i] = 0.0f;
+            for (int j0 = 0; j0 < topk; j0 += 4) {
+                uint4 u[4];
+                float w[4];
+                bool on[4];
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const int j = j0 + q;
+                    const int r = j < topk ? row_of(pos, p0 + j, P) : -1;
+                    on[q] = r >= 0;
+                    if (on[q]) {
+                        u[q] = ld16(y + (size_t)r * H + (size_t)c * V);
+                        w[q] = wt ? __ldg(wt + p0 + j) : 1.0f;
+                    }
+                }
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+                    if (on[q]) {
+                        float f[V];
+                        Vec<T>::get(u[q], f);
+#pragma unroll
+                        for (int i = 0; i < V; i++) acc[i] = __fadd_rn(acc[i], __fmul_rn(w[q], f[i]));
+                    }
+            }
+            O *o = out + (size_t)t * H + (size_t)c * V;
+            constexpr int VO = Vec<O>::V;
+            if constexpr (VO == V) {
+                st16(o, Vec<O>::put(acc));
+            } else if constexpr (VO < V) {   // bf16 rows, fp32 sums: two stores
+#pragma unroll
+                for (int h = 0; h < V / VO; h++) {
+                    float part[VO];
+#pragma unroll
+                    for (int i = 0; i < VO; i++) part[i] = acc[h * VO + i];
+                    st16(o + h * VO, Vec<O>::put(part));
+                }
+            } else {                         // fp32 rows, bf16 sums: half a store
+                *reinterpret_cast<uint2 *>(o) = make_uint2(f32x2_to_bf16x2(acc[0], acc[1]), f32x2_to_bf16x2(acc[2], acc[3]));
+            }
+        }
+    } else {
+        for (int i = blockIdx.y * PM_TH + threadIdx.x; i < H; i += gridDim.y * PM_TH) {
+            float acc = 0.0f;
+            for (int j = 0; j < topk; j++) {
+                const int r = row_of(pos, p0 + j, P);
+                if (r >= 0)
+                    acc = __fadd_rn(acc, __fmul_rn(wt ? __ldg(wt + p0 + j) : 1.0f, Vec<T>::one(y[(size_t)r * H + i])));
+            }
+            out[(size_t)t * H + i] = Vec<O>::back(acc);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ unpermute's gradients
+// One block per token: dout[t] is read once per batch of JB pairs, each pair's y row once; the
+// products for dwt are summed per thread in fp32, then across the block in a fixed tree.
+constexpr int UB_JB = 8;
+template <typename T, typename D, bool VEC>
+__global__ void __launch_bounds__(PM_TH) k_unpermute_bwd(T *__restrict__ dy, float *__restrict__ dwt,
+                                                         const D *__restrict__ dout, const T *__restrict__ y,
+                                                         const float *__restrict__ wt, const int *__restrict__ pos,
+                                                         int P, int topk, int H) {
+    __shared__ float part[PM_TH / 32][UB_JB];
+    const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const size_t p0 = (size_t)t * topk;
+    const D *dr = dout + (size_t)t * H;
+    for (int j0 = 0; j0 < topk; j0 += UB_JB) {
+        int r[UB_JB];
+        float w[UB_JB], dot[UB_JB];
+#pragma unroll
+        for (int q = 0; q < UB_JB; q++) {
+            r[q] = j0 + q < topk ? row_of(pos, p0 + j0 + q, P) : -1;
+            w[q] = r[q] >= 0 ? __ldg(wt + p0 + j0 + q) : 0.0f;
+            dot[q] = 0.0f;
+        }
+        if constexpr (VEC) {
+            constexpr int V = Vec<T>::V, VD = Vec<D>::V;
+            for (int c = threadIdx.x; c < H / V; c += PM_TH) {
+                float d[V];
+                if constexpr (VD >= V) {
+                    if constexpr (VD == V) {
+                        Vec<D>::get(ld16(dr + (size_t)c * V), d);
+                    } else {   // bf16 dout, fp32 rows: half a load
+                        const uint2 u = *reinterpret_cast<const uint2 *>(dr + (size_t)c * V);
+                        d[0] = __uint_as_float(u.x << 16);
+                        d[1] = __uint_as_float(u.x & 0xFFFF0000u);
+                        d[2] = __uint_as_float(u.y << 16);
+                        d[3] = __uint_as_float(u.y & 0xFFFF0000u);
+                    }
+                } else {       // fp32 dout, bf16 rows: two loads
+#pragma unroll
+                    for (int h = 0; h < V / VD; h++) {
+                        float g[VD];
+                        Vec<D>::get(ld16(dr + (size_t)c * V + h * VD), g);
+#pragma unroll
+                        for (int i = 0; i < VD; i++) d[h * VD + i] = g[i];
+                    }
+                }
+#pragma unroll
+                for (int q0 = 0; q0 < UB_JB; q0 += 4) {
+                    uint4 u[4];
+                    if (dwt) {
+#pragma unroll
+                        for (int q = 0; q < 4; q++)
+                            if (r[q0 + q] >= 0) u[q] = ld16(y + (size_t)r[q0 + q] * H + (size_t)c * V);
+                    }
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const int a = q0 + q;
+                        if (r[a] < 0) continue;
+                        if (dwt) {
+                            float f[V];
+                            Vec<T>::get(u[q], f);
+#pragma unroll
+                            for (int i = 0; i < V; i++) dot[a] = fmaf(d[i], f[i], dot[a]);
+                        }
+                        if (dy) {
+                            float f[V];
+#pragma unroll
+                            for (int i = 0; i < V; i++) f[i] = w[a] * d[i];
+                            st16(dy + (size_t)r[a] * H + (size_t)c * V, Vec<T>::put(f));
+                        }
+                    }
+                }
+            }
+        } else {
+            for (int i = threadIdx.x; i < H; i += PM_TH) {
+                const float d = Vec<D>::one(dr[i]);
+#pragma unroll
+                for (int q = 0; q < UB_JB; q++) {
+                    if (r[q] < 0) continue;
+                    const size_t at = (size_t)r[q] * H + i;
+                    if (dwt) dot[q] = fmaf(d, Vec<T>::one(y[at]), dot[q]);
+                    if (dy) dy[at] = Vec<T>::back(w[q] * d);
+                }
+            }
+        }
+        if (dwt) {
+#pragma unroll
+            for (int q = 0; q < UB_JB; q++) {
+                const float s = warp_sum(dot[q]);
+                if (lane == 0) part[warp][q] = s;
+            }
+            __syncthreads();
+            if (threadIdx.x < UB_JB && j0 + (int)threadIdx.x < topk) {
+                float s = 0.0f;
+#pragma unroll
+                for (int w2 = 0; w2 < PM_TH / 32; w2++) s += part[w2][threadIdx.x];
+                dwt[p0 + j0 + threadIdx.x] = s;   // a dropped pair's products are all absent: 0
+            }
+            __syncthreads();
+        }
+    }
+}
+
+// ------------------------------------------------------------------ quantising permute
+// One thread per 32-element group of a token: read and quantised once, its 16 bytes of codes
+// and its scale byte stored into each of the token's rows.
+template <typename T>
+__global__ void __launch_bounds__(PM_TH) k_permute_mx4(uint8_t *__restrict__ packed, uint8_t *__restrict__ scales,
+                                                       const T *__restrict__ x, int64_t ldx,
+                                                       const int *__restrict__ pos, int P, int topk, int H, int vec) {
+    const int t = blockIdx.x, G = H / 32;
+    for (int g = blockIdx.y * PM_TH + threadIdx.x; g < G; g += gridDim.y * PM_TH) {
+        float v[32];
+        mx4_load32(v, x + (size_t)t * ldx + (size_t)g * 32, 32, vec);
+        uint4 codes;
+        const uint8_t sb = mx4_quant32(v, codes);
+        for (int j = 0; j < topk; j++) {
+            const int r = row_of(pos, (size_t)t * topk + j, P);
+            if (r < 0) continue;
+            *reinterpret_cast<uint4 *>(packed + (size_t)r * (H / 2) + (size_t)g * 16) = codes;
+            scales[(size_t)r * G + g] = sb;
+        }
+    }
+}
+
+// ------------------------------------------------------------------ host side
+bool al16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+bool known(int dt) { return dt == K3C_F32 || dt == K3C_BF16; }
+size_t size_of(int dt) { return dt == K3C_F32 ? 4 : 2; }
+
+// Blocks along a row: enough blocks to fill the SMs when there are few tokens.
+int row_blocks(int ntok, int units) {
+    const int most = (units + PM_TH - 1) / PM_TH;
+    int want = (2 * 148 + ntok - 1) / ntok;
+    if (want > most) want = most;
+    return want < 1 ? 1 : want;
+}
+
+int check_pairs(const char *what, int ntok, int topk, int hidden) {
+    if (ntok < 0 || topk < 1 || topk > K3_MAX_TOPK || hidden < 1)
+        return set_error(K3C_EINVAL, "%s: ntok=%d topk=%d (1..%d) hidden=%d", what, ntok, topk, K3_MAX_TOPK, hidden);
+    if ((int64_t)ntok * topk > 0x7FFFFFFF - 2 * SORT_BLOCKS * SORT_SUB)
+        return set_error(K3C_EINVAL, "%s: %d x %d pairs exceed 32 bits", what, ntok, topk);
+    return K3C_OK;
+}
+
+int sort_blocks(int64_t P) {
+    // One block up to two passes: a second launch costs more than the passes it saves.
+    const int64_t n = (P + SORT_SUB - 1) / SORT_SUB;
+    return n <= 2 ? 1 : (int)(n < SORT_BLOCKS ? n : SORT_BLOCKS);
+}
+
+template <typename T, typename O>
+int run_gather(O *out, const T *y, const float *wt, const int *pos, int ntok, int topk, int H, cudaStream_t s) {
+    const bool vec = al16(y) && al16(out) && H % Vec<T>::V == 0 && H % Vec<O>::V == 0;
+    const dim3 grid(ntok, row_blocks(ntok, vec ? H / Vec<T>::V : H));
+    if (vec) k_gather_sum<T, O, true><<<grid, PM_TH, 0, s>>>(out, y, wt, pos, ntok * topk, topk, H);
+    else k_gather_sum<T, O, false><<<grid, PM_TH, 0, s>>>(out, y, wt, pos, ntok * topk, topk, H);
+    K3C_CHECK_LAUNCH();
+    return K3C_OK;
+}
+
+template <typename T, typename D>
+int run_unpermute_bwd(T *dy, float *dwt, const D *dout, const T *y, const float *wt, const int *pos, int ntok, int topk,
+                      int H, cudaStream_t s) {
+    const bool vec = al16(y) && al16(dy) && al16(dout) && H % Vec<T>::V == 0 && H % Vec<D>::V == 0;
+    if (vec) k_unpermute_bwd<T, D, true><<<ntok, PM_TH, 0, s>>>(dy, dwt, dout, y, wt, pos, ntok * topk, topk, H);
+    else k_unpermute_bwd<T, D, false><<<ntok, PM_TH, 0, s>>>(dy, dwt, dout, y, wt, pos, ntok * topk, topk, H);
+    K3C_CHECK_LAUNCH();
+    return K3C_OK;
+}
+
+}  // namespace
+}  // namespace k3c
+
+using namespace k3c;
+
+extern "C" size_t k3c_moe_sort_scratch(int ntok, int topk, int n_experts) {
+    if (ntok <= 0 || topk <= 0 || n_experts <= 0) return 0;
+    const int nb = sort_blocks((int64_t)ntok * topk);
+    return nb == 1 ? 0 : (size_t)nb * n_experts * sizeof(int);
+}
+
+extern "C" int k3c_moe_sort(int *pos, int *pair, int *off, const int *idx, int ntok, int topk, int n_experts,
+                            void *scratch, size_t scratch_bytes, k3c_stream_t stream) {
+    clear_error();
+    K3C_TRY(check_pairs("moe_sort", ntok, topk, 1));
+    if (n_experts < 1 || n_experts > SORT_EMAX)
+        return set_error(K3C_EINVAL, "moe_sort: n_experts=%d (1..%d)", n_experts, SORT_EMAX);
+    if (!off || (ntok && (!pos || !pair || !idx))) return set_error(K3C_EINVAL, "moe_sort: NULL array");
+    const size_t need = k3c_moe_sort_scratch(ntok, topk, n_experts);
+    if (need && (!scratch || scratch_bytes < need || ((uintptr_t)scratch & 3)))
+        return set_error(K3C_EINVAL, "moe_sort: scratch of %zu bytes, %zu needed (4-byte aligned)", scratch_bytes, need);
+    cudaStream_t s = (cudaStream_t)stream;
+    const int P = ntok * topk, nblk = sort_blocks(P);
+    const int64_t n = ((int64_t)P + SORT_SUB - 1) / SORT_SUB;
+    const int chunk = (int)((n + nblk - 1) / nblk) * SORT_SUB;
+    const size_t sm = (size_t)n_experts * (sizeof(int) + SORT_WARPS * sizeof(uint16_t));
+    static bool attr_of[64] = {};
+    bool &attr = attr_of[cur_dev()];
+    if (!attr) {
+        K3C_TRY_CUDA(cudaFuncSetAttribute(k_sort_place, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          SORT_EMAX * (int)(sizeof(int) + SORT_WARPS * sizeof(uint16_t))));
+        attr = true;
+    }
+    if (nblk > 1) {
+        k_sort_count<<<nblk, SORT_TH, n_experts * sizeof(int), s>>>((int *)scratch, idx, P, n_experts, chunk);
+        K3C_CHECK_LAUNCH();
+    }
+    k_sort_place<<<nblk, SORT_TH, sm, s>>>(pos, pair, off, idx, (const int *)scratch, P, n_experts, chunk, nblk);
+    K3C_CHECK_LAUNCH();
+    return K3C_OK;
+}
+
+extern "C" int k3c_moe_permute(void *rows, const void *x, int dtype, int64_t ldx, const int *pos, int ntok, int topk,
+                               int hidden, k3c_stream_t stream) {
+    clear_error();
+    K3C_TRY(check_pairs("moe_permute", ntok, topk, hidden));
+    if (!known(dtype) || ldx < hidden) return set_error(K3C_EINVAL, "moe_permute: dtype=%d ldx=%lld", dtype, (long long)ldx);
+    if (!ntok) return K3C_OK;
+    if (!rows || !x || !pos) return set_error(K3C_EINVAL, "moe_permute: NULL array");
+    cudaStream_t s = (cudaStream_t)stream;
+    const int V = dtype == K3C_F32 ? 4 : 8, P = ntok * topk;
+    const bool vec = al16(rows) && al16(x) && hidden % V == 0 && ldx % V == 0;
+    const dim3 grid(ntok, row_blocks(ntok, vec ? hidden / V : hidden));
+    if (dtype == K3C_F32) {
+        if (vec) k_permute<float, true><<<grid, PM_TH, 0, s>>>((float *)rows, (const float *)x, ldx, pos, P, topk, hidden);
+        else k_permute<float, false><<<grid, PM_TH, 0, s>>>((float *)rows, (const float *)x, ldx, pos, P, topk, hidden);
+    } else {
+        if (vec) k_permute<uint16_t, true><<<grid, PM_TH, 0, s>>>((uint16_t *)rows, (const uint16_t *)x, ldx, pos, P, topk, hidden);
+        else k_permute<uint16_t, false><<<grid, PM_TH, 0, s>>>((uint16_t *)rows, (const uint16_t *)x, ldx, pos, P, topk, hidden);
+    }
+    K3C_CHECK_LAUNCH();
+    return K3C_OK;
+}
+
+extern "C" int k3c_moe_permute_bwd(void *dx, const void *drows, int dtype, const int *pos, int ntok, int topk, int hidden,
+                                   k3c_stream_t stream) {
+    clear_error();
+    K3C_TRY(check_pairs("moe_permute_bwd", ntok, topk, hidden));
+    if (!known(dtype)) return set_error(K3C_EINVAL, "moe_permute_bwd: dtype=%d", dtype);
+    if (!ntok) return K3C_OK;
+    if (!dx || !drows || !pos) return set_error(K3C_EINVAL, "moe_permute_bwd: NULL array");
+    cudaStream_t s = (cudaStream_t)stream;
+    if (dtype == K3C_F32) return run_gather((float *)dx, (const float *)drows, nullptr, pos, ntok, topk, hidden, s);
+    return run_gather((uint16_t *)dx, (const uint16_t *)drows, nullptr, pos, ntok, topk, hidden, s);
+}
+
+extern "C" int k3c_moe_permute_mxfp4(uint8_t *packed, uint8_t *scales, const void *x, int x_dtype, int64_t ldx,
+                                     const int *pos, int ntok, int topk, int hidden, k3c_stream_t stream) {
+    clear_error();
+    K3C_TRY(check_pairs("moe_permute_mxfp4", ntok, topk, hidden));
+    if (!known(x_dtype) || ldx < hidden || hidden % 32)
+        return set_error(K3C_EINVAL, "moe_permute_mxfp4: dtype=%d ldx=%lld hidden=%d (a multiple of 32)", x_dtype,
+                         (long long)ldx, hidden);
+    if (!ntok) return K3C_OK;
+    if (!packed || !scales || !x || !pos) return set_error(K3C_EINVAL, "moe_permute_mxfp4: NULL array");
+    if (!al16(packed)) return set_error(K3C_EINVAL, "moe_permute_mxfp4: packed must be 16-byte aligned");
+    cudaStream_t s = (cudaStream_t)stream;
+    const dim3 grid(ntok, row_blocks(ntok, hidden / 32));
+    const int vec = al16(x) && (ldx * size_of(x_dtype)) % 16 == 0;
+    if (x_dtype == K3C_F32)
+        k_permute_mx4<<<grid, PM_TH, 0, s>>>(packed, scales, (const float *)x, ldx, pos, ntok * topk, topk, hidden, vec);
+    else
+        k_permute_mx4<<<grid, PM_TH, 0, s>>>(packed, scales, (const uint16_t *)x, ldx, pos, ntok * topk, topk, hidden, vec);
+    K3C_CHECK_LAUNCH();
+    return K3C_OK;
+}
+
+extern "C" int k3c_moe_unpermute(void *out, int out_dtype, const void *y, int y_dtype, const float *wt, const int *pos,
+                                 int ntok, int topk, int hidden, k3c_stream_t stream) {
+    clear_error();
+    K3C_TRY(check_pairs("moe_unpermute", ntok, topk, hidden));
+    if (!known(out_dtype) || !known(y_dtype))
+        return set_error(K3C_EINVAL, "moe_unpermute: out_dtype=%d y_dtype=%d", out_dtype, y_dtype);
+    if (!ntok) return K3C_OK;
+    if (!out || !y || !wt || !pos) return set_error(K3C_EINVAL, "moe_unpermute: NULL array");
+    cudaStream_t s = (cudaStream_t)stream;
+    if (y_dtype == K3C_F32) {
+        if (out_dtype == K3C_F32) return run_gather((float *)out, (const float *)y, wt, pos, ntok, topk, hidden, s);
+        return run_gather((uint16_t *)out, (const float *)y, wt, pos, ntok, topk, hidden, s);
+    }
+    if (out_dtype == K3C_F32) return run_gather((float *)out, (const uint16_t *)y, wt, pos, ntok, topk, hidden, s);
+    return run_gather((uint16_t *)out, (const uint16_t *)y, wt, pos, ntok, topk, hidden, s);
+}
+
+extern "C" int k3c_moe_unpermute_bwd(void *dy, float *dwt, const void *dout, int out_dtype, const void *y, int y_dtype,
+                                     const float *wt, const int *pos, int ntok, int topk, int hidden,
+                                     k3c_stream_t stream) {
+    clear_error();
+    K3C_TRY(check_pairs("moe_unpermute_bwd", ntok, topk, hidden));
+    if (!known(out_dtype) || !known(y_dtype))
+        return set_error(K3C_EINVAL, "moe_unpermute_bwd: out_dtype=%d y_dtype=%d", out_dtype, y_dtype);
+    if (!ntok || (!dy && !dwt)) return K3C_OK;
+    if (!dout || !wt || !pos || (dwt && !y)) return set_error(K3C_EINVAL, "moe_unpermute_bwd: NULL array");
+    cudaStream_t s = (cudaStream_t)stream;
+    if (y_dtype == K3C_F32) {
+        if (out_dtype == K3C_F32)
+            return run_unpermute_bwd((float *)dy, dwt, (const float *)dout, (const float *)y, wt, pos, ntok, topk, hidden, s);
+        return run_unpermute_bwd((float *)dy, dwt, (const uint16_t *)dout, (const float *)y, wt, pos, ntok, topk, hidden, s);
+    }
+    if (out_dtype == K3C_F32)
+        return run_unpermute_bwd((uint16_t *)dy, dwt, (const float *)dout, (const uint16_t *)y, wt, pos, ntok, topk, hidden, s);
+    return run_unpermute_bwd((uint16_t *)dy, dwt, (const uint16_t *)dout, (const uint16_t *)y, wt, pos, ntok, topk, hidden, s);
+}

@@ -1,0 +1,914 @@
+// mxfp4_mm.cu -- MXFP4 quantisation, the product of two MXFP4 matrices, and the product's
+// gradient with respect to its activations. No reference counterpart (the reference multiplies
+// fp32 activations with packed weights, src/core/k3_ops.c:1363-1768); the packed formats are the
+// reference's (E2M1 nibbles, low nibble even; one E8M0 byte per 32 elements).
+//
+//   quant   x -> (codes [rows][in/2], scales [rows][ceil(in/32)])            mx4_quant.cuh
+//   pack    a weight's scales re-ordered into 512-byte atoms of 128 rows x 4 groups, which
+//           tcgen05.cp copies to TMEM as they are; scale 255 (the reference: skip the group)
+//           becomes zero codes under scale 127, as in the pool format
+//   mm      y[r][o] = sum_i A[r][i] W_g[o][i]: E2M1 x E2M1 on tcgen05.mma kind::mxf4 with both
+//           block scales applied by the MMA, fp32 accumulation, one rounding to y's type.
+//           Rows [off[g], off[g+1]) of A multiply matrix g (grouped by expert), or all rows
+//           one matrix.
+//   mm_bwd  dA[r][i] = sum_o dY[r][o] W_g[o][i]: the contraction runs over W's rows, which the
+//           4-bit MMA cannot read (it wants the contracted index contiguous), so W tiles are
+//           widened to bf16 in shared memory (exact: two significant bits and a power of two)
+//           and multiplied by kind::f16, fp32 accumulation.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+#include <stdlib.h>
+
+#include "common.cuh"
+#include "mx4_quant.cuh"
+#include "tc_common.cuh"
+#include "tc_host.cuh"
+
+namespace k3c {
+
+namespace {
+
+constexpr int MX_GMAX = 1024;   // groups of a product
+
+static __device__ int g_mx_err;
+
+__device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// ------------------------------------------------------------------ quantisation
+// One thread per 32-element group.
+template <typename T>
+__global__ void __launch_bounds__(256) k_mx4_quant(uint8_t *__restrict__ packed, uint8_t *__restrict__ scales,
+                                                   const T *__restrict__ x, int64_t ldx, int rows, int in, int vec) {
+    grid_dep_launch();
+    const int G = (in + 31) / 32;
+    const size_t n = (size_t)rows * G;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
+        const size_t r = i / G;
+        const int g = (int)(i - r * G), left = min(32, in - 32 * g);
+        float v[32];
+        mx4_load32(v, x + r * ldx + (size_t)g * 32, left, vec);
+        uint4 c;
+        scales[i] = mx4_quant32(v, c);
+        uint8_t *d = packed + r * (in / 2) + (size_t)g * 16;
+        if (vec && left == 32) *reinterpret_cast<uint4 *>(d) = c;
+        else {
+            const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+            for (int b = 0; b < 16; b++)
+                if (2 * b < left) d[b] = (uint8_t)(w[b >> 2] >> (8 * (b & 3)));
+        }
+    }
+}
+
+// Byte of row m (0..127), group g (0..3) in a scale atom.
+__device__ __forceinline__ int sf_byte(int m, int g) { return 16 * (m & 31) + 4 * (m >> 5) + g; }
+
+// One thread per group of the padded matrix: scale byte into its atom, codes copied (packed and
+// codes may be the same array).
+__global__ void __launch_bounds__(256) k_mx4_pack(uint8_t *codes, uint8_t *__restrict__ atoms, const uint8_t *packed,
+                                                  const uint8_t *__restrict__ scales, int n_mats, int rows, int in) {
+    const int G = in / 32, RA = (rows + 127) / 128, KA = (in + 127) / 128;
+    const size_t per = (size_t)RA * 128 * KA * 4, n = per * n_mats;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
+        const size_t m = i / per, q = i - m * per;
+        const int r = (int)(q / (KA * 4)), g = (int)(q % (KA * 4));
+        uint8_t sb = 127;
+        if (r < rows && g < G) {
+            const size_t row = m * rows + r;
+            sb = scales[row * G + g];
+            uint4 c = *reinterpret_cast<const uint4 *>(packed + row * (in / 2) + (size_t)g * 16);
+            if (sb == 255) {
+                c = make_uint4(0, 0, 0, 0);
+                sb = 127;
+            }
+            *reinterpret_cast<uint4 *>(codes + row * (in / 2) + (size_t)g * 16) = c;
+        }
+        atoms[((m * RA + r / 128) * KA + g / 4) * 512 + sf_byte(r & 127, g & 3)] = sb;
+    }
+}
+
+// ------------------------------------------------------------------ work items
+// Groups own consecutive rows; an item is one row tile of one group x one column tile. tbase[g]
+// (shared memory) is the number of row tiles before group g.
+struct Item {
+    int mat;         // matrix index, -1: none (the rows' results are zeros)
+    int row0, n;     // first row, rows of the tile
+    int nt;          // column tile
+};
+
+__device__ __forceinline__ void group_rows(const int *off, int g, int M, int &lo, int &hi) {
+    if (!off) {
+        lo = 0;
+        hi = M;
+        return;
+    }
+    lo = min(max(__ldg(off + g), 0), M);   // offsets outside the rows cannot leave them
+    hi = min(max(__ldg(off + g + 1), lo), M);
+}
+
+// tbase[0..G] by all THREADS of the block; returns the number of row tiles.
+template <int THREADS>
+__device__ int plan_tiles(int *tbase, int *warp_tot, const int *off, int G, int M, int tile) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    int run = 0;
+    for (int g0 = 0; g0 < G; g0 += THREADS) {
+        const int g = g0 + tid;
+        int n = 0;
+        if (g < G) {
+            int lo, hi;
+            group_rows(off, g, M, lo, hi);
+            n = (hi - lo + tile - 1) / tile;
+        }
+        int inc = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        if (lane == 31) warp_tot[warp] = inc;
+        __syncthreads();
+        int pre = 0, all = 0;
+#pragma unroll
+        for (int w = 0; w < THREADS / 32; w++) {
+            pre += w < warp ? warp_tot[w] : 0;
+            all += warp_tot[w];
+        }
+        if (g < G) tbase[g] = run + pre + inc - n;
+        run += all;
+        __syncthreads();
+    }
+    if (tid == 0) tbase[G] = run;
+    __syncthreads();
+    return run;
+}
+
+// Items of a group run through its row tiles first, RB of them at a time, so that the CTAs
+// working side by side share W tiles and a bounded set of A rows in L2.
+constexpr int MX_RB = 16;
+__device__ __forceinline__ Item item_of(int it, const int *tbase, const int *off, const int *mat_of, int n_mats, int G,
+                                        int M, int NTL, int tile) {
+    const int tt = it / NTL;
+    int g = 0, h = G;   // tbase[g] <= tt < tbase[h]
+    while (h - g > 1) {
+        const int c = (g + h) >> 1;
+        if (tbase[c] <= tt) g = c;
+        else h = c;
+    }
+    const int i = it - tbase[g] * NTL, mt = tbase[g + 1] - tbase[g];
+    const int b = i / (MX_RB * NTL), mb = min(MX_RB, mt - MX_RB * b), r = i - b * MX_RB * NTL;
+    int lo, hi;
+    group_rows(off, g, M, lo, hi);
+    Item x;
+    x.nt = r / mb;
+    const int m = MX_RB * b + r % mb;
+    x.row0 = lo + m * tile;
+    x.n = min(tile, hi - x.row0);
+    const int mat = mat_of ? __ldg(mat_of + g) : (off ? g : 0);
+    x.mat = mat >= 0 && mat < n_mats ? mat : -1;
+    return x;
+}
+
+struct MxArgs {
+    void *y;
+    int64_t ldy;
+    int y_bf16, vec;             // vec: rows of y start on 16-byte boundaries
+    int M, N, K, G, NTL;         // A [M][K], W [N][K]
+    const int *off, *mat_of;
+    int n_mats;
+    const uint8_t *as;           // A's scales [M][K/32]
+    const uint8_t *atoms;        // W's scale atoms, atom_stride bytes per matrix
+    size_t atom_stride;
+    int *err;
+};
+
+// 32 columns of 32 rows (a warp's share of the accumulator) to y: staged in 2 KB of shared
+// memory, 64 bytes per row with the 16-byte chunks rotated by the row, and stored 64 bytes per
+// row by four lanes. rows: valid rows of this warp's 32; c0: first column; N: columns of y.
+__device__ __forceinline__ void store_rows(uint8_t *stg, const uint32_t (&v)[32], const MxArgs &p, int64_t row, int rows,
+                                           int c0, int N, bool ok) {
+    const int lane = threadIdx.x & 31;
+    const uint32_t sw = (lane >> 1) & 3;
+    const int esz = p.y_bf16 ? 2 : 4, per = 64 / esz;   // columns per 64-byte piece
+    char *base = reinterpret_cast<char *>(p.y);
+    for (int h = 0; h < 32 / per; h++) {
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            uint4 o;
+            if (p.y_bf16) {
+                uint32_t w[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    w[k] = ok ? f32x2_to_bf16x2(__uint_as_float(v[8 * i + 2 * k]), __uint_as_float(v[8 * i + 2 * k + 1]))
+                              : 0x7FC07FC0u;
+                o = make_uint4(w[0], w[1], w[2], w[3]);
+            } else {
+                uint32_t w[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) w[k] = !ok ? 0x7FC00000u : h ? v[16 + 4 * i + k] : v[4 * i + k];
+                o = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            *reinterpret_cast<uint4 *>(stg + lane * 64 + 16 * (i ^ sw)) = o;
+        }
+        __syncwarp();
+        const int c = c0 + h * per;
+        if (p.vec && c + per <= N) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int r = (lane >> 2) + 8 * i, k = lane & 3;
+                const uint4 o = *reinterpret_cast<const uint4 *>(stg + r * 64 + 16 * (k ^ ((r >> 1) & 3)));
+                if (r < rows) *reinterpret_cast<uint4 *>(base + ((row + r) * p.ldy + c) * esz + k * 16) = o;
+            }
+        } else {
+            for (int i = 0; i < per; i++) {   // 32 elements at a time, a row's columns side by side
+                const int e = i * 32 + lane, r = e / per, k = e % per;
+                const int at = k * esz;
+                const uint8_t *s = stg + r * 64 + 16 * ((at >> 4) ^ ((r >> 1) & 3)) + (at & 15);
+                if (r < rows && c + k < N) {
+                    if (p.y_bf16)
+                        reinterpret_cast<uint16_t *>(base)[(row + r) * p.ldy + c + k] = *reinterpret_cast<const uint16_t *>(s);
+                    else
+                        reinterpret_cast<uint32_t *>(base)[(row + r) * p.ldy + c + k] = *reinterpret_cast<const uint32_t *>(s);
+                }
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------ MXFP4 x MXFP4
+// kind::mxf4: E2M1 A and B, K-major, UE8M0 scales per 32 (scale_vec::2X), M = 128, K = 64.
+__host__ __device__ constexpr uint32_t idesc_mxf4(uint32_t n, uint32_t sf_id) {
+    return (sf_id << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((128u >> 4) << 24) | (sf_id << 29);
+}
+__device__ __forceinline__ void tc_mma_mx4(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sfa,
+                                           uint32_t sfb, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d),
+        "l"(da), "l"(db), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)
+        : "memory");
+}
+
+constexpr int MM_M = 128;
+constexpr int MM_ABOX = 32;                      // rows per A copy: short tiles copy only what they have
+constexpr int MM_A = MM_M * 128;                 // 128 rows x 256 codes
+constexpr int MM_THREADS = 384;                  // copies, MMA, A scales, (idle), 8 epilogue warps
+constexpr int MM_EPI = 8;
+template <int NT>
+struct MmCfg {
+    static constexpr int B = NT * 128;
+    static constexpr int NA = NT / 128 ? NT / 128 : 1;    // 128-row scale atoms of a column tile
+    static constexpr int SF = 1024 + NA * 1024;           // A's and W's scales of 256 elements
+    static constexpr int STAGE = MM_A + B + SF;
+    static constexpr int STAGES = NT == 256 ? 4 : NT == 128 ? 6 : 7;
+    static constexpr int NACC = NT == 256 ? 1 : 2;        // accumulators in TMEM
+    static constexpr uint32_t SFW = 2 * (4 + 4 * NA);     // TMEM columns of a stage's scales
+    static constexpr uint32_t SF_COL = NT * NACC;
+    static constexpr int BAR = 256;
+    static constexpr int BYTES = 1024 + STAGES * STAGE + BAR + MM_EPI * 2048 + (MX_GMAX + 1) * 4 + 64;
+    static_assert(STAGE % 1024 == 0, "stage bases stay 1024-byte aligned");
+    static_assert(SF_COL + STAGES * SFW <= 512, "TMEM columns");
+    static_assert(BYTES <= 227 * 1024, "one CTA per SM");
+    static_assert((2 * STAGES + 2 * NACC) * 8 + 4 <= BAR, "barriers");
+};
+
+template <int NT>
+__global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant__ CUtensorMap tmA,
+                                                          const __grid_constant__ CUtensorMap tmW, MxArgs p) {
+    using C = MmCfg<NT>;
+    extern __shared__ uint8_t mm_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)mm_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::STAGES * C::STAGE);
+    uint64_t *empty = full + C::STAGES, *tfull = empty + C::STAGES, *tempty = tfull + C::NACC;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tempty + C::NACC);
+    uint8_t *stg_all = smem + C::STAGES * C::STAGE + C::BAR;
+    int *tbase = reinterpret_cast<int *>(stg_all + MM_EPI * 2048);
+    __shared__ int warp_tot[MM_THREADS / 32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::STAGES; i++) {
+            tc::mbar_init(&full[i], 2);     // the copies' thread and the A scales' warp
+            tc::mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < C::NACC; i++) {
+            tc::mbar_init(&tfull[i], 1);
+            tc::mbar_init(&tempty[i], MM_EPI);
+        }
+        tc::fence_mbar_init();
+        tc::prefetch_tmap(&tmA);
+        tc::prefetch_tmap(&tmW);
+    }
+    if (warp == 1) tc::tmem_alloc(tmem_slot, 512);
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    grid_dep_wait();   // everything read from here on may come from the kernel before
+    const int tiles = plan_tiles<MM_THREADS>(tbase, warp_tot, p.off, p.G, p.M, MM_M);
+    const int n_items = tiles * p.NTL;
+    const int KB = (p.K + 255) / 256;
+    const int KA = (p.K + 127) / 128;              // scale atoms along K
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ copies
+        if (lane == 0) {
+            bool ok = tc::tc_check((tc::smem_u32(smem) & 1023) == 0, p.err, 80);
+            uint32_t ki = 0;
+            for (int it = blockIdx.x; ok && it < n_items; it += gridDim.x) {
+                const Item x = item_of(it, tbase, p.off, p.mat_of, p.n_mats, p.G, p.M, p.NTL, MM_M);
+                if (x.mat < 0) continue;
+                const int boxes = (x.n + MM_ABOX - 1) / MM_ABOX;
+                const int arow = NT >= 128 ? x.nt * C::NA : x.nt / 2;         // W's 128-row atom
+                const int atoms = min(C::NA, (p.N + 127) / 128 - arow);        // the last tile may end early
+                const uint8_t *wsf = p.atoms + (size_t)x.mat * p.atom_stride + (size_t)arow * KA * 512;
+                for (int kb = 0; kb < KB; kb++, ki++) {
+                    const int st = ki % C::STAGES;
+                    const uint32_t ph = (ki / C::STAGES) & 1u;
+                    if (ki >= C::STAGES && !tc::mbar_wait(&empty[st], ph ^ 1u, p.err, 81)) { ok = false; break; }
+                    uint8_t *sa = smem + st * C::STAGE, *sb = sa + MM_A, *sf = sb + C::B + 1024;
+                    const uint32_t sfb = min(2, KA - 2 * kb) * 512;            // W's scales of this K block
+                    tc::mbar_expect_tx(&full[st], boxes * MM_ABOX * 128 + C::B + atoms * sfb);
+                    tc::tma_load_3d(sb, &tmW, &full[st], kb * 128, x.nt * NT, x.mat);
+                    for (int a = 0; a < atoms; a++)
+                        tc::bulk_load(sf + a * 1024, wsf + ((size_t)a * KA + 2 * kb) * 512, sfb, &full[st]);
+                    for (int b = 0; b < boxes; b++)
+                        tc::tma_load_3d(sa + b * (MM_ABOX * 128), &tmA, &full[st], kb * 128, x.row0 + b * MM_ABOX, 0);
+                }
+            }
+            // no copy may still be landing when the CTA exits
+            for (uint32_t i = ki > C::STAGES ? ki - C::STAGES : 0; i < ki; i++)
+                tc::mbar_wait(&full[i % C::STAGES], (i / C::STAGES) & 1u, p.err, 82);
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA
+        if (lane == 0) {
+            uint32_t ki = 0, li = 0;
+            bool ok = true;
+            for (int it = blockIdx.x; ok && it < n_items; it += gridDim.x) {
+                const Item x = item_of(it, tbase, p.off, p.mat_of, p.n_mats, p.G, p.M, p.NTL, MM_M);
+                if (x.mat < 0) continue;
+                const uint32_t a = li % C::NACC, use = li / C::NACC;
+                li++;
+                if (use >= 1 && !tc::mbar_wait(&tempty[a], (use - 1) & 1u, p.err, 83)) { ok = false; break; }
+                tc::tc_fence_after();
+                const uint32_t d = tmem + a * NT;
+                const uint32_t shift = NT == 64 ? 2u * (x.nt & 1) : 0u;   // rows 64..127 of an atom: two columns on
+                for (int kb = 0; kb < KB; kb++, ki++) {
+                    const int st = ki % C::STAGES;
+                    if (!tc::mbar_wait(&full[st], (ki / C::STAGES) & 1u, p.err, 84)) { ok = false; break; }
+                    tc::tc_fence_after();
+                    const uint32_t sa = tc::smem_u32(smem + st * C::STAGE), sb = sa + MM_A, sf = sb + C::B;
+                    const uint32_t col = tmem + C::SF_COL + st * C::SFW;
+                    const int steps = min(4, (p.K - 256 * kb + 63) / 64);
+                    // per 128 elements: A's four columns, then W's four per 128 rows
+                    for (int j = 0; 2 * j < steps; j++) {
+                        tc::tc_cp_sf(col + j * (C::SFW / 2), tc::desc_sf_atom(sf + j * 512));
+#pragma unroll
+                        for (int q = 0; q < C::NA; q++)
+                            tc::tc_cp_sf(col + j * (C::SFW / 2) + 4 + 4 * q, tc::desc_sf_atom(sf + 1024 + q * 1024 + j * 512));
+                    }
+                    for (int k = 0; k < steps; k++) {
+                        const uint32_t id = 2u * (k & 1), sfa = col + (k >> 1) * (C::SFW / 2);
+                        tc_mma_mx4(d, tc::desc_kmajor_sw128(sa + 32 * k), tc::desc_kmajor_sw128(sb + 32 * k),
+                                   idesc_mxf4(NT, id), sfa | (id << 30), (sfa + 4 + shift) | (id << 30), (kb | k) != 0);
+                    }
+                    tc::tc_commit(&empty[st]);
+                }
+                if (ok) tc::tc_commit(&tfull[a]);
+            }
+        }
+    } else if (warp == 2) {
+        // ------------------------------------------------------------ A's scales
+        // Lane i fetches the eight scale bytes of rows i, 32+i, 64+i and 96+i and stores the
+        // four rows' words of each atom as one 16-byte piece (sf_byte's order).
+        const int SR = p.K / 32;
+        const int wide = SR % 8 == 0 && ((uintptr_t)p.as & 7) == 0;
+        uint32_t ki = 0;
+        bool ok = true;
+        for (int it = blockIdx.x; ok && it < n_items; it += gridDim.x) {
+            const Item x = item_of(it, tbase, p.off, p.mat_of, p.n_mats, p.G, p.M, p.NTL, MM_M);
+            if (x.mat < 0) continue;
+            for (int kb = 0; kb < KB; kb++, ki++) {
+                uint32_t w[2][4];
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    w[0][q] = w[1][q] = 0x7F7F7F7Fu;   // rows past the tile, groups past K: scale 1
+                    const int r = 32 * q + lane;
+                    if (r < x.n) {
+                        const uint8_t *s = p.as + (size_t)(x.row0 + r) * SR + 8 * kb;
+                        if (wide) {
+                            const uint2 u = __ldg(reinterpret_cast<const uint2 *>(s));
+                            w[0][q] = u.x;
+                            w[1][q] = u.y;
+                        } else {
+                            const int n = min(8, SR - 8 * kb);
+#pragma unroll
+                            for (int b = 0; b < 8; b++)
+                                if (b < n) {
+                                    const uint32_t sh = 8 * (b & 3);
+                                    w[b >> 2][q] = (w[b >> 2][q] & ~(0xFFu << sh)) | ((uint32_t)__ldg(s + b) << sh);
+                                }
+                        }
+                    }
+                }
+                const int st = ki % C::STAGES;
+                const uint32_t ph = (ki / C::STAGES) & 1u;
+                if (ki >= C::STAGES && !tc::mbar_wait(&empty[st], ph ^ 1u, p.err, 85)) { ok = false; break; }
+                uint8_t *sf = smem + st * C::STAGE + MM_A + C::B;
+                *reinterpret_cast<uint4 *>(sf + 16 * lane) = make_uint4(w[0][0], w[0][1], w[0][2], w[0][3]);
+                *reinterpret_cast<uint4 *>(sf + 512 + 16 * lane) = make_uint4(w[1][0], w[1][1], w[1][2], w[1][3]);
+                tc::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&full[st]);
+            }
+        }
+    } else if (warp >= 4) {
+        // ------------------------------------------------------------ epilogue
+        const int q = warp & 3, half = (warp - 4) >> 2;   // TMEM lane quadrant, half of the columns
+        constexpr int NC = NT / 64;                       // 32-column pieces per half
+        const uint32_t lane_base = (uint32_t)(32 * q) << 16;
+        uint8_t *stg = stg_all + (warp - 4) * 2048;
+        uint32_t li = 0;
+        bool alive = true;   // false after a wait gave up: the remaining results are NaN
+        for (int it = blockIdx.x; it < n_items; it += gridDim.x) {
+            const Item x = item_of(it, tbase, p.off, p.mat_of, p.n_mats, p.G, p.M, p.NTL, MM_M);
+            const int rows = min(32, x.n - 32 * q);
+            uint32_t v[NC][32];
+            bool ok = true;   // zeros of a group without a matrix stay zeros
+            if (x.mat < 0) {
+#pragma unroll
+                for (int c = 0; c < NC; c++)
+#pragma unroll
+                    for (int i = 0; i < 32; i++) v[c][i] = 0;
+            } else {
+                const uint32_t a = li % C::NACC, use = li / C::NACC;
+                li++;
+                ok = alive = alive && tc::mbar_wait(&tfull[a], use & 1u, p.err, 86);
+                __syncwarp();
+                tc::tc_fence_after();
+                // the whole share goes to registers first, so the accumulator is free again
+#pragma unroll
+                for (int c = 0; c < NC; c++) tc::tmem_ld32(tmem + lane_base + a * NT + 32u * (half * NC + c), v[c]);
+                tc::tmem_ld_wait();
+                tc::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&tempty[a]);
+            }
+            if (rows > 0) {
+#pragma unroll
+                for (int c = 0; c < NC; c++)
+                    store_rows(stg, v[c], p, x.row0 + 32 * q, rows, x.nt * NT + 32 * (half * NC + c), p.N, ok);
+            }
+        }
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    if (warp == 1) tc::tmem_dealloc(tmem, 512);
+}
+
+// ------------------------------------------------------------------ gradient of the activations
+constexpr int MB_M = 256;                        // rows per item: two accumulators share a widened W tile
+constexpr int MB_N = 256;                        // columns (W's in) per item
+constexpr int MB_KB = 64;                        // W rows per K block
+constexpr int MB_A = MB_M * 128;                 // dY: 256 rows x 64 bf16
+constexpr int MB_B = MB_N * MB_KB * 2;           // widened W: 4 blocks of 64 columns x 64 rows
+constexpr int MB_W = MB_KB * 128;                // packed W: 64 rows x 256 codes
+constexpr int MB_SF = 1024;                      // its two scale atoms
+constexpr int MB_STAGE = MB_A + MB_B + MB_W + MB_SF;
+constexpr int MB_STAGES = 3;
+constexpr int MB_WARPS = 8;                      // widening, then the epilogue
+constexpr int MB_THREADS = 64 + 32 * MB_WARPS;
+constexpr int MB_BYTES = 1024 + MB_STAGES * MB_STAGE + 256;
+static_assert(MB_STAGE % 1024 == 0, "stage bases stay 1024-byte aligned");
+static_assert(MB_BYTES + (MX_GMAX + 1) * 4 + 128 <= 227 * 1024, "one CTA per SM");
+
+// kind::f16: bf16 A (K-major) and B (N-major: transpose bit 16), fp32 accumulator, M = 128.
+__host__ __device__ constexpr uint32_t idesc_bf16_tb(uint32_t n) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+__device__ __forceinline__ void tc_mma_bf16(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// N-major operand, 128-byte swizzle: rows of 64 N-elements, 8 of the contracted index per 1024
+// bytes (SBO), blocks of 64 N-elements MB_KB * 128 bytes apart (LBO).
+__device__ __forceinline__ uint64_t desc_nmajor_sw128(uint32_t addr) { return tc::smem_desc(addr, MB_KB * 128, 1024, 2); }
+
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+// Eight E2M1 codes to eight bf16 (element k in half k): table bytes through permutes, as
+// e2m1x8_to_f32, without the widening.
+__device__ __forceinline__ void e2m1x8_to_bf16(uint32_t w, uint32_t (&o)[4]) {
+    const uint32_t m = w & 0x77777777u, mh = m >> 16, w4 = w << 4;
+    const uint32_t lo_a = __byte_perm(0xC0800000u, 0xC0804000u, m), hi_a = __byte_perm(0x3F3F3F00u, 0x40404040u, m);
+    const uint32_t lo_b = __byte_perm(0xC0800000u, 0xC0804000u, mh), hi_b = __byte_perm(0x3F3F3F00u, 0x40404040u, mh);
+    o[0] = __byte_perm(lo_a, hi_a, 0x5140u) | (__byte_perm(w4, w, 0x4000u) & 0x80008000u);
+    o[1] = __byte_perm(lo_a, hi_a, 0x7362u) | (__byte_perm(w4, w, 0x5010u) & 0x80008000u);
+    o[2] = __byte_perm(lo_b, hi_b, 0x5140u) | (__byte_perm(w4, w, 0x6020u) & 0x80008000u);
+    o[3] = __byte_perm(lo_b, hi_b, 0x7362u) | (__byte_perm(w4, w, 0x7030u) & 0x80008000u);
+}
+
+__global__ void __launch_bounds__(MB_THREADS, 1) k_mx4_bwd(const __grid_constant__ CUtensorMap tmD,
+                                                           const __grid_constant__ CUtensorMap tmW, MxArgs p) {
+    extern __shared__ uint8_t mb_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)mb_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + MB_STAGES * MB_STAGE);
+    uint64_t *wide = full + MB_STAGES, *empty = wide + MB_STAGES, *tfull = empty + MB_STAGES, *tempty = tfull + 1;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tempty + 1);
+    __shared__ int tbase[MX_GMAX + 1];
+    __shared__ int warp_tot[MB_THREADS / 32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < MB_STAGES; i++) {
+            tc::mbar_init(&full[i], 1);
+            tc::mbar_init(&wide[i], MB_WARPS);
+            tc::mbar_init(&empty[i], 1);
+        }
+        tc::mbar_init(tfull, 1);
+        tc::mbar_init(tempty, MB_WARPS);
+        tc::fence_mbar_init();
+        tc::prefetch_tmap(&tmD);
+        tc::prefetch_tmap(&tmW);
+    }
+    if (warp == 1) tc::tmem_alloc(tmem_slot, 512);
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    grid_dep_wait();
+    const int tiles = plan_tiles<MB_THREADS>(tbase, warp_tot, p.off, p.G, p.M, MB_M);
+    const int n_items = tiles * p.NTL;
+    const int KB = (p.N + MB_KB - 1) / MB_KB;      // contracted: W's rows
+    const int KA = (p.K + 127) / 128;
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ copies
+        if (lane == 0) {
+            bool ok = tc::tc_check((tc::smem_u32(smem) & 1023) == 0, p.err, 90);
+            uint32_t ki = 0;
+            for (int it = blockIdx.x; ok && it < n_items; it += gridDim.x) {
+                const Item x = item_of(it, tbase, p.off, p.mat_of, p.n_mats, p.G, p.M, p.NTL, MB_M);
+                if (x.mat < 0) continue;
+                const int boxes = (x.n + 31) / 32;
+                const uint32_t sfb = min(2, KA - 2 * x.nt) * 512;
+                const uint8_t *wsf = p.atoms + (size_t)x.mat * p.atom_stride + (size_t)(2 * x.nt) * 512;
+                for (int kb = 0; kb < KB; kb++, ki++) {
+                    const int st = ki % MB_STAGES;
+                    const uint32_t ph = (ki / MB_STAGES) & 1u;
+                    if (ki >= MB_STAGES && !tc::mbar_wait(&empty[st], ph ^ 1u, p.err, 91)) { ok = false; break; }
+                    uint8_t *sa = smem + st * MB_STAGE, *sw = sa + MB_A + MB_B;
+                    tc::mbar_expect_tx(&full[st], boxes * 32 * 128 + MB_W + sfb);
+                    tc::tma_load_3d(sw, &tmW, &full[st], x.nt * 128, kb * MB_KB, x.mat);
+                    tc::bulk_load(sw + MB_W, wsf + (size_t)(kb / 2) * KA * 512, sfb, &full[st]);
+                    for (int b = 0; b < boxes; b++)
+                        tc::tma_load_3d(sa + b * (32 * 128), &tmD, &full[st], kb * MB_KB, x.row0 + b * 32, 0);
+                }
+            }
+            for (uint32_t i = ki > MB_STAGES ? ki - MB_STAGES : 0; i < ki; i++)
+                tc::mbar_wait(&full[i % MB_STAGES], (i / MB_STAGES) & 1u, p.err, 92);
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA
+        if (lane == 0) {
+            uint32_t ki = 0, li = 0;
+            bool ok = true;
+            constexpr uint32_t idesc = idesc_bf16_tb(MB_N);
+            for (int it = blockIdx.x; ok && it < n_items; it += gridDim.x) {
+                const Item x = item_of(it, tbase, p.off, p.mat_of, p.n_mats, p.G, p.M, p.NTL, MB_M);
+                if (x.mat < 0) continue;
+                if (li >= 1 && !tc::mbar_wait(tempty, (li - 1) & 1u, p.err, 93)) { ok = false; break; }
+                li++;
+                tc::tc_fence_after();
+                for (int kb = 0; kb < KB; kb++, ki++) {
+                    const int st = ki % MB_STAGES;
+                    const uint32_t ph = (ki / MB_STAGES) & 1u;
+                    if (!tc::mbar_wait(&full[st], ph, p.err, 94) || !tc::mbar_wait(&wide[st], ph, p.err, 95)) { ok = false; break; }
+                    tc::tc_fence_after();
+                    const uint32_t sa = tc::smem_u32(smem + st * MB_STAGE), sb = sa + MB_A;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const uint64_t db = desc_nmajor_sw128(sb + 2048 * k);
+                        tc_mma_bf16(tmem, tc::desc_kmajor_sw128(sa + 32 * k), db, idesc, (kb | k) != 0);
+                        if (x.n > 128)
+                            tc_mma_bf16(tmem + MB_N, tc::desc_kmajor_sw128(sa + 128 * 128 + 32 * k), db, idesc, (kb | k) != 0);
+                    }
+                    tc::tc_commit(&empty[st]);
+                }
+                if (ok) tc::tc_commit(tfull);
+            }
+        }
+    } else {
+        // ------------------------------------------------------------ widening, then the epilogue
+        const int w8 = warp - 2;
+        const int q = warp & 3, acc = w8 >> 2;     // TMEM lane quadrant; accumulator drained by this warp
+        const uint32_t lane_base = (uint32_t)(32 * q) << 16;
+        uint32_t ki = 0, li = 0;
+        bool ok = true;
+        for (int it = blockIdx.x; it < n_items; it += gridDim.x) {
+            const Item x = item_of(it, tbase, p.off, p.mat_of, p.n_mats, p.G, p.M, p.NTL, MB_M);
+            if (x.mat >= 0) {
+                for (int kb = 0; ok && kb < KB; kb++, ki++) {
+                    const int st = ki % MB_STAGES;
+                    if (!tc::mbar_wait(&full[st], (ki / MB_STAGES) & 1u, p.err, 96)) { ok = false; break; }
+                    uint8_t *sb = smem + st * MB_STAGE + MB_A, *sw = sb + MB_B, *sf = sw + MB_W;
+                    // a lane widens 32 codes of one W row: rows 8 w8 + (lane & 7), groups lane / 8 and
+                    // 4 + lane / 8 (eight lanes touch eight rows: the swizzle spreads them over the banks)
+                    const int n = 8 * w8 + (lane & 7), m = (kb & 1) * 64 + n;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const int g = 4 * h + (lane >> 3);
+                        const uint4 c = *reinterpret_cast<const uint4 *>(sw + n * 128 + 16 * (g ^ (n & 7)));
+                        const uint32_t s = sf[h * 512 + sf_byte(m, g & 3)];
+                        const uint32_t s16 = s ? s << 7 : 0x40u;    // 2^(s-127) in bf16
+                        const uint32_t s2 = s16 | (s16 << 16);
+                        const uint32_t cw[4] = {c.x, c.y, c.z, c.w};
+                        uint8_t *row = sb + (g >> 1) * (MB_KB * 128) + n * 128;
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            uint32_t o[4];
+                            e2m1x8_to_bf16(cw[k], o);
+#pragma unroll
+                            for (int i = 0; i < 4; i++) o[i] = mul_bf16x2(o[i], s2);
+                            *reinterpret_cast<uint4 *>(row + 16 * (((g & 1) * 4 + k) ^ (n & 7))) =
+                                make_uint4(o[0], o[1], o[2], o[3]);
+                        }
+                    }
+                    tc::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&wide[st]);
+                }
+                ok = ok && tc::mbar_wait(tfull, li & 1u, p.err, 97);
+                li++;
+                __syncwarp();
+                tc::tc_fence_after();
+            }
+            const int row = 128 * acc + 32 * q + lane;
+            const bool live = row < x.n;
+            const bool full_warp = 128 * acc + 32 * q < x.n;     // warp-uniform
+#pragma unroll 1
+            for (int c0 = 0; c0 < MB_N; c0 += 32) {
+                if (!full_warp) break;
+                uint32_t v[32];
+                if (x.mat >= 0) {
+                    tc::tmem_ld32(tmem + lane_base + acc * MB_N + c0, v);
+                    tc::tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; i++) v[i] = 0;
+                }
+                const int col = x.nt * MB_N + c0;
+                if (!live || col >= p.K) continue;
+                if (x.mat >= 0 && !ok)
+#pragma unroll
+                    for (int i = 0; i < 32; i++) v[i] = 0x7FC00000u;
+                if (p.y_bf16) {
+                    uint16_t *d = reinterpret_cast<uint16_t *>(p.y) + (x.row0 + row) * p.ldy + col;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        uint32_t o[4];
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            o[k] = f32x2_to_bf16x2(__uint_as_float(v[8 * i + 2 * k]), __uint_as_float(v[8 * i + 2 * k + 1]));
+                        if (p.vec) reinterpret_cast<uint4 *>(d)[i] = make_uint4(o[0], o[1], o[2], o[3]);
+                        else
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                d[8 * i + 2 * k] = (uint16_t)o[k];
+                                d[8 * i + 2 * k + 1] = (uint16_t)(o[k] >> 16);
+                            }
+                    }
+                } else {
+                    uint32_t *d = reinterpret_cast<uint32_t *>(p.y) + (x.row0 + row) * p.ldy + col;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        if (p.vec) reinterpret_cast<uint4 *>(d)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                        else
+#pragma unroll
+                            for (int k = 0; k < 4; k++) d[4 * i + k] = v[4 * i + k];
+                    }
+                }
+            }
+            if (x.mat >= 0) {
+                tc::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(tempty);
+            }
+        }
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    if (warp == 1) tc::tmem_dealloc(tmem, 512);
+}
+
+// ------------------------------------------------------------------ host side
+bool al16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+int known(int dt) { return dt == K3C_F32 || dt == K3C_BF16; }
+
+int check_mat(const char *what, const k3c_mxfp4_mat *W, int M, const int *off, int n_groups) {
+    if (!W || !W->codes || !W->atoms || W->rows < 1 || W->in < 32 || W->in % 32 || W->n_mats < 1)
+        return set_error(K3C_EINVAL, "%s: matrix rows=%d in=%d (a multiple of 32) n_mats=%d", what, W ? W->rows : 0,
+                         W ? W->in : 0, W ? W->n_mats : 0);
+    if (!al16(W->codes) || !al16(W->atoms) || W->code_stride % 16 || W->atom_stride % 16)
+        return set_error(K3C_EINVAL, "%s: codes, atoms and their strides must be 16-byte aligned", what);
+    const size_t cb = (size_t)W->rows * (W->in / 2), ab = k3c_mxfp4_atom_bytes(W->rows, W->in);
+    if (W->n_mats > 1 && (W->code_stride < cb || W->atom_stride < ab))
+        return set_error(K3C_EINVAL, "%s: strides %zu, %zu below a matrix's %zu, %zu bytes", what, W->code_stride,
+                         W->atom_stride, cb, ab);
+    if (M < 0 || n_groups < 1 || n_groups > MX_GMAX || (!off && n_groups != 1))
+        return set_error(K3C_EINVAL, "%s: M=%d n_groups=%d (1..%d; 1 without offsets)", what, M, n_groups, MX_GMAX);
+    if (off && !W->mat_of && n_groups > W->n_mats)
+        return set_error(K3C_EINVAL, "%s: %d groups, %d matrices", what, n_groups, W->n_mats);
+    return K3C_OK;
+}
+
+int map_weights(CUtensorMap *m, const k3c_mxfp4_mat *W, int box_rows) {
+    const size_t stride = W->n_mats > 1 ? W->code_stride : (size_t)W->rows * (W->in / 2);
+    return make_map3(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, W->codes, W->in / 2, W->rows, W->n_mats, W->in / 2,
+                     (stride + 15) / 16 * 16, 128, box_rows);
+}
+
+int err_slot(int **err) {
+    static int *err_of[64] = {};
+    int *&e = err_of[cur_dev()];
+    if (!e) K3C_TRY_CUDA(cudaGetSymbolAddress((void **)&e, g_mx_err));
+    *err = e;
+    return K3C_OK;
+}
+
+int check_waits(const char *what, int *err, cudaStream_t s) {
+    static const int sync_check = getenv("K3C_SYNC_CHECK") ? 1 : 0;
+    if (!sync_check) return K3C_OK;
+    int code = 0;
+    K3C_TRY_CUDA(cudaStreamSynchronize(s));
+    K3C_TRY_CUDA(cudaMemcpy(&code, err, sizeof(int), cudaMemcpyDeviceToHost));
+    if (code) {
+        const int zero = 0;
+        cudaMemcpy(err, &zero, sizeof(int), cudaMemcpyHostToDevice);
+        return set_error(K3C_ETIMEOUT, "%s: device check code %d", what, code);
+    }
+    return K3C_OK;
+}
+
+int check_items(const char *what, int64_t items) {
+    return items < 0x7FFFFFFF ? K3C_OK : set_error(K3C_EINVAL, "%s: %lld tiles exceed 32 bits", what, (long long)items);
+}
+
+// Row tiles of at most `tile` rows that n_groups groups of M rows can have together.
+int64_t most_tiles(int M, int n_groups, int tile) { return (int64_t)M / tile + (n_groups < M ? n_groups : M); }
+
+template <int NT>
+int launch_mm(const CUtensorMap &ma, const CUtensorMap &mw, MxArgs p, cudaStream_t s) {
+    static bool attr_of[64] = {};
+    bool &attr = attr_of[cur_dev()];
+    if (!attr) {
+        K3C_TRY_CUDA(cudaFuncSetAttribute(k_mx4_mm<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, MmCfg<NT>::BYTES));
+        attr = true;
+    }
+    p.NTL = (p.N + NT - 1) / NT;
+    const int64_t items = most_tiles(p.M, p.G, MM_M) * p.NTL;
+    K3C_TRY(check_items("mxfp4_mm", items));
+    const int grid = (int)(items < sm_count() ? items : sm_count());
+    K3C_TRY_CUDA(launch_pdl(k_mx4_mm<NT>, dim3(grid), dim3(MM_THREADS), MmCfg<NT>::BYTES, s, ma, mw, p));
+    K3C_CHECK_LAUNCH();
+    return K3C_OK;
+}
+
+}  // namespace
+}  // namespace k3c
+
+using namespace k3c;
+
+extern "C" int k3c_mxfp4_quant(uint8_t *packed, uint8_t *scales, const void *x, int x_dtype, int64_t ldx, int rows, int in,
+                               k3c_stream_t stream) {
+    clear_error();
+    if (rows < 0 || in < 2 || in % 2 || ldx < in || !known(x_dtype))
+        return set_error(K3C_EINVAL, "mxfp4_quant: rows=%d in=%d (even) ldx=%lld dtype=%d", rows, in, (long long)ldx, x_dtype);
+    if (!rows) return K3C_OK;
+    if (!packed || !scales || !x) return set_error(K3C_EINVAL, "mxfp4_quant: NULL array");
+    cudaStream_t s = (cudaStream_t)stream;
+    const size_t groups = (size_t)rows * ((in + 31) / 32);
+    const unsigned grid = (unsigned)((groups + 255) / 256 < 148 * 64 ? (groups + 255) / 256 : 148 * 64);
+    const int esz = x_dtype == K3C_F32 ? 4 : 2;
+    const int vec = al16(x) && al16(packed) && in % 32 == 0 && (ldx * esz) % 16 == 0;
+    if (x_dtype == K3C_F32) k_mx4_quant<<<grid, 256, 0, s>>>(packed, scales, (const float *)x, ldx, rows, in, vec);
+    else k_mx4_quant<<<grid, 256, 0, s>>>(packed, scales, (const uint16_t *)x, ldx, rows, in, vec);
+    K3C_CHECK_LAUNCH();
+    return K3C_OK;
+}
+
+extern "C" size_t k3c_mxfp4_atom_bytes(int rows, int in) {
+    if (rows < 1 || in < 1) return 0;
+    return (size_t)((rows + 127) / 128) * ((in + 127) / 128) * 512;
+}
+
+extern "C" int k3c_mxfp4_pack(uint8_t *codes, uint8_t *atoms, const uint8_t *packed, const uint8_t *scales, int n_mats,
+                              int rows, int in, k3c_stream_t stream) {
+    clear_error();
+    if (n_mats < 1 || rows < 1 || in < 32 || in % 32)
+        return set_error(K3C_EINVAL, "mxfp4_pack: n_mats=%d rows=%d in=%d (a multiple of 32)", n_mats, rows, in);
+    if (!codes || !atoms || !packed || !scales) return set_error(K3C_EINVAL, "mxfp4_pack: NULL array");
+    if (!al16(codes) || !al16(packed)) return set_error(K3C_EINVAL, "mxfp4_pack: codes and packed must be 16-byte aligned");
+    const size_t n = (size_t)n_mats * k3c_mxfp4_atom_bytes(rows, in);   // one byte per group
+    const unsigned grid = (unsigned)((n + 255) / 256 < 148 * 64 ? (n + 255) / 256 : 148 * 64);
+    k_mx4_pack<<<grid, 256, 0, (cudaStream_t)stream>>>(codes, atoms, packed, scales, n_mats, rows, in);
+    K3C_CHECK_LAUNCH();
+    return K3C_OK;
+}
+
+extern "C" int k3c_mxfp4_mm(void *y, int y_dtype, int64_t ldy, const uint8_t *a, const uint8_t *a_scales, int M,
+                            const k3c_mxfp4_mat *W, const int *off, int n_groups, k3c_stream_t stream) {
+    clear_error();
+    K3C_TRY(check_mat("mxfp4_mm", W, M, off, n_groups));
+    if (!known(y_dtype) || ldy < W->rows)
+        return set_error(K3C_EINVAL, "mxfp4_mm: y_dtype=%d ldy=%lld rows=%d", y_dtype, (long long)ldy, W->rows);
+    if (!M) return K3C_OK;
+    if (!y || !a || !a_scales) return set_error(K3C_EINVAL, "mxfp4_mm: NULL array");
+    if (!al16(a)) return set_error(K3C_EINVAL, "mxfp4_mm: a must be 16-byte aligned");
+    cudaStream_t s = (cudaStream_t)stream;
+    MxArgs p = {};
+    K3C_TRY(err_slot(&p.err));
+    p.y = y;
+    p.ldy = ldy;
+    p.y_bf16 = y_dtype == K3C_BF16;
+    p.vec = al16(y) && (ldy * (p.y_bf16 ? 2 : 4)) % 16 == 0;
+    p.M = M;
+    p.N = W->rows;
+    p.K = W->in;
+    p.G = n_groups;
+    p.off = off;
+    p.mat_of = W->mat_of;
+    p.n_mats = W->n_mats;
+    p.as = a_scales;
+    p.atoms = W->atoms;
+    p.atom_stride = W->atom_stride;
+    // Column tile: the widest that still gives every SM an item; with fewer items a narrower
+    // tile spreads W's bytes over more SMs.
+    const int64_t tiles = off ? most_tiles(M, n_groups, MM_M) : (M + MM_M - 1) / MM_M;
+    int nt = 256;
+    while (nt > 64 && tiles * ((p.N + nt - 1) / nt) < sm_count()) nt /= 2;
+    CUtensorMap ma, mw;
+    K3C_TRY(make_map3(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, a, p.K / 2, M, 1, p.K / 2, (uint64_t)(p.K / 2) * M, 128, MM_ABOX));
+    K3C_TRY(map_weights(&mw, W, nt));
+    if (nt == 256) K3C_TRY(launch_mm<256>(ma, mw, p, s));
+    else if (nt == 128) K3C_TRY(launch_mm<128>(ma, mw, p, s));
+    else K3C_TRY(launch_mm<64>(ma, mw, p, s));
+    return check_waits("mxfp4_mm", p.err, s);
+}
+
+extern "C" int k3c_mxfp4_mm_bwd(void *da, int da_dtype, int64_t ldda, const void *dy, int64_t lddy, int M,
+                                const k3c_mxfp4_mat *W, const int *off, int n_groups, k3c_stream_t stream) {
+    clear_error();
+    K3C_TRY(check_mat("mxfp4_mm_bwd", W, M, off, n_groups));
+    if (!known(da_dtype) || ldda < W->in || lddy < W->rows || lddy % 8)
+        return set_error(K3C_EINVAL, "mxfp4_mm_bwd: da_dtype=%d ldda=%lld in=%d lddy=%lld (a multiple of 8) rows=%d", da_dtype,
+                         (long long)ldda, W->in, (long long)lddy, W->rows);
+    if (!M) return K3C_OK;
+    if (!da || !dy) return set_error(K3C_EINVAL, "mxfp4_mm_bwd: NULL array");
+    if (!al16(dy)) return set_error(K3C_EINVAL, "mxfp4_mm_bwd: dy must be 16-byte aligned");
+    cudaStream_t s = (cudaStream_t)stream;
+    MxArgs p = {};
+    K3C_TRY(err_slot(&p.err));
+    p.y = da;
+    p.ldy = ldda;
+    p.y_bf16 = da_dtype == K3C_BF16;
+    p.vec = al16(da) && (ldda * (p.y_bf16 ? 2 : 4)) % 16 == 0;
+    p.M = M;
+    p.N = W->rows;
+    p.K = W->in;
+    p.G = n_groups;
+    p.off = off;
+    p.mat_of = W->mat_of;
+    p.n_mats = W->n_mats;
+    p.atoms = W->atoms;
+    p.atom_stride = W->atom_stride;
+    p.NTL = (p.K + MB_N - 1) / MB_N;
+    CUtensorMap md, mw;
+    K3C_TRY(make_map3(&md, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dy, p.N, M, 1, lddy * 2, (uint64_t)lddy * 2 * M, 64, 32));
+    K3C_TRY(map_weights(&mw, W, MB_KB));
+    static bool attr_of[64] = {};
+    bool &attr = attr_of[cur_dev()];
+    if (!attr) {
+        K3C_TRY_CUDA(cudaFuncSetAttribute(k_mx4_bwd, cudaFuncAttributeMaxDynamicSharedMemorySize, MB_BYTES));
+        attr = true;
+    }
+    const int64_t items = most_tiles(M, n_groups, MB_M) * p.NTL;
+    K3C_TRY(check_items("mxfp4_mm_bwd", items));
+    const int grid = (int)(items < sm_count() ? items : sm_count());
+    K3C_TRY_CUDA(launch_pdl(k_mx4_bwd, dim3(grid), dim3(MB_THREADS), MB_BYTES, s, md, mw, p));
+    K3C_CHECK_LAUNCH();
+    return check_waits("mxfp4_mm_bwd", p.err, s);
+}

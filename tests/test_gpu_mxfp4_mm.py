@@ -1,0 +1,421 @@
+"""MXFP4 quantisation (k3c_mxfp4_quant), packing and the products k3c_mxfp4_mm and
+k3c_mxfp4_mm_bwd against plain 64-bit arithmetic on the same codes.
+
+Tolerances. Quantisation and packing are exact. In the products every term is exact in fp32 (E2M1
+x E2M1 under powers of two; bf16 x E2M1 under a power of two). A 64-wide (mm) or 16-wide (mm_bwd)
+step adds its terms to the accumulator with at most one unit (2^-23, a truncation) of the running
+magnitude, which sum|terms| bounds; 8 more units stand for the additions within steps. Rounding
+to bf16 adds 2^-8 of the result, to fp32 nothing."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+GRID = np.array([0, .5, 1, 1.5, 2, 3, 4, 6])
+
+
+@pytest.fixture(scope="module")
+def dev():
+    import torch
+    return torch.device("cuda:0")
+
+
+def quant_plain(v):
+    """v [rows][in] float64 (finite or not, no NaN) -> (codes 0..15 [rows][in], scale bytes): the
+    nearest grid value by distance, the even code on ties."""
+    rows, n = v.shape
+    G = -(-n // 32)
+    pad = np.zeros((rows, G * 32))
+    pad[:, :n] = v
+    g = pad.reshape(rows, G, 32)
+    top = np.abs(g).max(-1)
+    with np.errstate(divide="ignore"):
+        e = np.where(np.isinf(top), 128, np.floor(np.log2(np.where(np.isinf(top), 1, top))))
+    byte = np.clip(np.where(top == 0, -1000, e) - 2 + 127, 0, 254)
+    a = np.minimum(np.abs(g) / 2.0 ** (byte - 127)[..., None], 6.0)
+    d = np.abs(a[..., None] - GRID)
+    best = d.min(-1, keepdims=True)
+    near = d == best
+    even = near & (np.arange(8) % 2 == 0)
+    code = np.where(even.any(-1), even.argmax(-1), near.argmax(-1))
+    code = code + 8 * np.signbit(g)
+    return code.reshape(rows, -1)[:, :n].astype(np.uint8), byte.astype(np.uint8)
+
+
+def values(codes, byte):
+    """float64 values of codes [rows][in] (0..15) under scale bytes [rows][in/32 rounded up]."""
+    v = GRID[codes & 7] * np.where(codes & 8, -1.0, 1.0)
+    sc = 2.0 ** (byte.astype(np.float64) - 127)
+    return v * np.repeat(sc, 32, axis=1)[:, :codes.shape[1]]
+
+
+def pack_nibbles(codes):
+    return (codes[:, 0::2] | (codes[:, 1::2] << 4)).astype(np.uint8)
+
+
+def unpack(packed):
+    return np.stack([packed & 15, packed >> 4], -1).reshape(packed.shape[0], -1)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,n,pad", [(1, 2, 0), (1, 32, 0), (3, 34, 0), (5, 96, 1), (7, 1000, 24), (64, 7168, 0),
+                                        (513, 352, 32)])
+def test_quant(k3, dev, rows, n, pad, dtype):
+    import torch
+    g = np.random.default_rng(rows + n)
+    x = g.standard_normal((rows, n + pad)) * 2.0 ** g.integers(-140, 120, (rows, 1))
+    x[:, ::7] = g.choice([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.0, -0.25, -5.0, 0.0, -0.0], x[:, ::7].shape)   # ties
+    x[0, :] = 0
+    t = torch.from_numpy(x).float()
+    t = t.bfloat16() if dtype == "bf16" else t
+    packed, scales = k3.mxfp4_quant(t.to(dev)[:, :n])
+    codes, byte = quant_plain(t.double().numpy()[:, :n])
+    assert np.array_equal(scales.cpu().numpy(), byte)
+    assert np.array_equal(unpack(packed.cpu().numpy())[:, :n], codes)
+
+
+def test_quant_borders_of_the_range(k3, dev):
+    """Subnormal groups, the largest finite value, infinities (read back as infinities) and NaN
+    (scale byte 255, zero codes)."""
+    import torch
+    x = torch.zeros(7, 32)
+    x[0, 3] = 2.0 ** -149
+    x[1, :] = 2.0 ** -127
+    x[2, 5], x[2, 6] = torch.finfo(torch.float32).max, 1.0
+    x[3, 0], x[3, 1], x[3, 2] = float("inf"), -float("inf"), 3.0
+    x[4, 31], x[4, 0] = float("nan"), 5.0
+    x[5, :] = torch.linspace(-1.9e-38, 1.9e-38, 32)
+    x[6, 0], x[6, 1] = 2.0 ** -125, -2.0 ** -127
+    packed, scales = k3.mxfp4_quant(x.to(dev))
+    ok = [0, 1, 2, 3, 5, 6]
+    codes, byte = quant_plain(x.double().numpy()[ok])
+    assert np.array_equal(scales.cpu().numpy()[ok], byte)
+    assert np.array_equal(unpack(packed.cpu().numpy())[ok], codes)
+    assert scales[4, 0] == 255 and (packed[4] == 0).all()
+    back = k3.mxfp4_dequant(packed, scales).cpu()
+    assert back[3, 0] == float("inf") and back[3, 1] == -float("inf") and torch.isfinite(back[2, 6])
+
+
+@pytest.mark.parametrize("n,rows,in_", [(1, 1, 32), (3, 130, 96), (2, 256, 4128)])
+def test_pack(k3, dev, n, rows, in_):
+    import torch
+    g = np.random.default_rng(in_)
+    p = g.integers(0, 256, (n, rows, in_ // 2), dtype=np.uint8)
+    s = g.integers(0, 256, (n, rows, in_ // 32), dtype=np.uint8)
+    s[:, ::3, 0] = 255
+    codes, atoms = (t.cpu().numpy() for t in k3.mxfp4_pack(torch.from_numpy(p).to(dev), torch.from_numpy(s).to(dev)))
+    want = np.full_like(atoms, 127)
+    for r in range(rows):
+        for q in range(in_ // 32):
+            b = s[:, r, q]
+            want[:, r // 128, q // 4, 16 * (r % 32) + 4 * (r % 128 // 32) + q % 4] = np.where(b == 255, 127, b)
+    assert np.array_equal(atoms, want)
+    skip = np.repeat(s == 255, 16, axis=2)
+    assert np.array_equal(codes, np.where(skip, 0, p))
+
+
+def operand(seed, rows, in_, lo=116, hi=132):
+    g = np.random.default_rng(seed)
+    codes = g.integers(0, 16, (rows, in_), dtype=np.uint8)
+    byte = g.integers(lo, hi, (rows, in_ // 32), dtype=np.uint8)
+    return codes, byte
+
+
+def to_dev(dev, *arrays):
+    import torch
+    return [torch.from_numpy(np.ascontiguousarray(a)).to(dev) for a in arrays]
+
+
+def check(got, want, mag, steps, bf16):
+    lim = (steps + 8) * 2.0 ** -23 * mag + (2.0 ** -8 * np.abs(want) if bf16 else 0)
+    bad = np.abs(got - want) > lim
+    assert not bad.any(), (int(bad.sum()), float((np.abs(got - want) / np.maximum(lim, 1e-300)).max()))
+
+
+def matrices(k3, dev, seed, n, rows, in_):
+    """n packed matrices: (Mxfp4Mat, float64 values [n][rows][in])."""
+    cs, bs, vs = [], [], []
+    for i in range(n):
+        c, b = operand(seed + i, rows, in_)
+        cs.append(pack_nibbles(c))
+        bs.append(b)
+        vs.append(values(c, b))
+    return k3.Mxfp4Mat(*k3.mxfp4_pack(*to_dev(dev, np.stack(cs), np.stack(bs)))), np.stack(vs)
+
+
+DENSE = [(1, 1, 32), (1, 64, 64), (2, 65, 96), (1, 7168, 2048), (31, 130, 160), (33, 200, 256), (127, 384, 288),
+         (128, 128, 512), (129, 257, 1056), (300, 1000, 3616), (64, 7168, 7168), (1000, 640, 352), (2200, 4100, 64)]
+
+
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("M,N,K", DENSE)
+def test_mm(k3, dev, M, N, K, out):
+    import torch
+    W, w = matrices(k3, dev, 5, 1, N, K)
+    c, b = operand(6, M, K)
+    a, s = to_dev(dev, pack_nibbles(c), b)
+    y = k3.mxfp4_mm(a, s, W, out_dtype=torch.float32 if out == "f32" else torch.bfloat16)
+    av = torch.from_numpy(values(c, b)).to(dev)
+    wv = torch.from_numpy(w[0]).to(dev)
+    check(y.double().cpu().numpy(), (av @ wv.T).cpu().numpy(), (av.abs() @ wv.abs().T).cpu().numpy(), -(-K // 64),
+          out == "bf16")
+    assert torch.equal(y, k3.mxfp4_mm(a, s, W, out_dtype=y.dtype))      # the same bits again
+
+
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("M,N,K", [m for m in DENSE if m[1] % 8 == 0])
+def test_mm_bwd(k3, dev, M, N, K, out):
+    import torch
+    W, w = matrices(k3, dev, 7, 1, N, K)
+    g = torch.Generator().manual_seed(M + N)
+    dy = torch.randn((M, N), generator=g).bfloat16().to(dev)
+    da = k3.mxfp4_mm_bwd(dy, W, out_dtype=torch.float32 if out == "f32" else torch.bfloat16)
+    wv = torch.from_numpy(w[0]).to(dev)
+    check(da.double().cpu().numpy(), (dy.double() @ wv).cpu().numpy(), (dy.double().abs() @ wv.abs()).cpu().numpy(),
+          -(-N // 16), out == "bf16")
+    assert torch.equal(da, k3.mxfp4_mm_bwd(dy, W, out_dtype=da.dtype))
+
+
+# rows per group: empty groups at both ends and in the middle, groups that end inside a tile, one
+# row, several tiles
+GROUPS = [[0], [1], [0, 0, 5, 0], [1] * 9, [130, 0, 1, 257, 32], [0, 40, 33, 128, 129, 1, 0, 300, 0], [2300, 1]]
+
+
+@pytest.mark.parametrize("N,K", [(64, 32), (200, 416), (520, 1056)])
+@pytest.mark.parametrize("sizes", GROUPS, ids=lambda s: "-".join(map(str, s)))
+def test_grouped_products(k3, dev, sizes, N, K):
+    """Both products over ragged groups; rows behind the last group stay as they were."""
+    import torch
+    G, n = len(sizes), sum(sizes)
+    M = n + 3
+    off = np.concatenate([[0], np.cumsum(sizes)]).astype(np.int32)
+    W, w = matrices(k3, dev, 11, G, N, K)
+    c, b = operand(12, M, K)
+    a, s, po = to_dev(dev, pack_nibbles(c), b, off)
+    y = torch.full((M, N), 7.0, device=dev)
+    k3.mxfp4_mm(a, s, W, off=po, out=y)
+    g = torch.Generator().manual_seed(N)
+    dy = torch.randn((M, N), generator=g).bfloat16().to(dev)
+    da = torch.full((M, K), 7.0, device=dev)
+    k3.mxfp4_mm_bwd(dy, W, off=po, out=da)
+    assert (y[n:] == 7).all() and (da[n:] == 7).all()
+    av, dv = values(c, b), dy.double().cpu().numpy()
+    for e in range(G):
+        r = slice(off[e], off[e + 1])
+        check(y[r].double().cpu().numpy(), av[r] @ w[e].T, np.abs(av[r]) @ np.abs(w[e]).T, -(-K // 64), False)
+        check(da[r].double().cpu().numpy(), dv[r] @ w[e], np.abs(dv[r]) @ np.abs(w[e]), -(-N // 16), False)
+
+
+def test_matrix_map_and_strided_rows(k3, dev):
+    """mat_of picks each group's matrix, an index without one gives zeros; out and dy rows may be
+    strided, with an odd stride or base (element stores) or an even one; columns beside them stay."""
+    import torch
+    N, K, M = 72, 96, 50
+    W, w = matrices(k3, dev, 21, 3, N, K)
+    mat_of = [2, -1, 0, 0, 3]
+    off = [0, 20, 30, 30, 45, 50]
+    W = k3.Mxfp4Mat(W.keep[0], W.keep[1], mat_of=torch.tensor(mat_of, dtype=torch.int32, device=dev))
+    assert W.groups == 5
+    c, b = operand(22, M, K)
+    a, s = to_dev(dev, pack_nibbles(c), b)
+    po = torch.tensor(off, dtype=torch.int32, device=dev)
+    dyb = torch.randn((M, N + 24), device=dev).bfloat16()
+    dy = dyb[:, 8:8 + N]
+    av, dv = values(c, b), dy.double().cpu().numpy()
+    for pad, dt in ((0, torch.float32), (5, torch.float32), (8, torch.float32), (3, torch.bfloat16), (8, torch.bfloat16)):
+        yb = torch.full((M, N + 2 * pad), 7.0, dtype=dt, device=dev)
+        db = torch.full((M, K + 2 * pad), 7.0, dtype=dt, device=dev)
+        k3.mxfp4_mm(a, s, W, off=po, out=yb[:, pad:pad + N])
+        k3.mxfp4_mm_bwd(dy, W, off=po, out=db[:, pad:pad + K])
+        assert (yb[:, :pad] == 7).all() and (yb[:, pad + N:] == 7).all()
+        assert (db[:, :pad] == 7).all() and (db[:, pad + K:] == 7).all()
+        y, d = yb[:, pad:pad + N].double().cpu().numpy(), db[:, pad:pad + K].double().cpu().numpy()
+        for g, m in enumerate(mat_of):
+            r = slice(off[g], off[g + 1])
+            if not 0 <= m < 3:
+                assert (y[r] == 0).all() and (d[r] == 0).all()
+                continue
+            check(y[r], av[r] @ w[m].T, np.abs(av[r]) @ np.abs(w[m]).T, 2, dt == torch.bfloat16)
+            check(d[r], dv[r] @ w[m], np.abs(dv[r]) @ np.abs(w[m]), 5, dt == torch.bfloat16)
+
+
+def test_offsets_outside_the_rows_are_clamped(k3, dev):
+    """Bad offsets (negative, descending, past the rows) touch nothing outside the result."""
+    import torch
+    N, K, M = 64, 64, 40
+    W, w = matrices(k3, dev, 31, 4, N, K)
+    c, b = operand(32, M, K)
+    a, s = to_dev(dev, pack_nibbles(c), b)
+    buf = torch.full((M + 2, N), 7.0, device=dev)
+    off = torch.tensor([-5, 10, 4, 30, 10 ** 9], dtype=torch.int32, device=dev)
+    k3.mxfp4_mm(a, s, W, off=off, out=buf[1:M + 1])
+    assert (buf[0] == 7).all() and (buf[M + 1] == 7).all()
+    got, av = buf[1:M + 1].double().cpu().numpy(), values(c, b)
+    for r, e in ((slice(0, 4), 0), (slice(30, M), 3)):   # scales span 30 binades: not exact in fp32
+        check(got[r], av[r] @ w[e].T, np.abs(av[r]) @ np.abs(w[e]).T, 1, False)
+
+
+def test_nan_scale_makes_its_row_nan(k3, dev):
+    """An activation group with scale 255 (the format's NaN) makes its row NaN and no other row;
+    infinities pass through as the reference's arithmetic has them."""
+    import torch
+    x = torch.randn(5, 256, device=dev)
+    x[2, 100] = float("nan")
+    W, w = matrices(k3, dev, 41, 1, 200, 256)
+    y = k3.mxfp4_mm(*k3.mxfp4_quant(x), W, out_dtype=torch.float32)
+    assert torch.isnan(y[2]).all() and torch.isfinite(y[[0, 1, 3, 4]]).all()
+
+
+def test_scales_over_the_whole_range(k3, dev):
+    """Scale bytes 0..254 on either side; results inside fp32's range are right, and the widened
+    weights of mm_bwd keep subnormal scales."""
+    import torch
+    N, K = 64, 64
+    c, b = operand(51, N, K)
+    for wb, ab in ((0, 254), (1, 250), (254, 0), (200, 30), (127, 127)):
+        wbyte = np.full_like(b, wb)
+        W = k3.Mxfp4Mat(*k3.mxfp4_pack(*to_dev(dev, pack_nibbles(c)[None], wbyte[None])))
+        ac, _ = operand(52, 9, K)
+        abyte = np.full((9, K // 32), ab, np.uint8)
+        a, s = to_dev(dev, pack_nibbles(ac), abyte)
+        y = k3.mxfp4_mm(a, s, W, out_dtype=torch.float32).double().cpu().numpy()
+        assert np.array_equal(y, values(ac, abyte) @ values(c, wbyte).T)
+        if wb > 251:
+            continue        # 6 * 2^(wb - 127) exceeds fp32: infinities, as in the reference's flat path
+        dy = (torch.randint(-3, 4, (9, N), device=dev).double() * 2.0 ** (100 if wb < 100 else 0)).bfloat16()
+        da = k3.mxfp4_mm_bwd(dy, W, out_dtype=torch.float32).double().cpu().numpy()
+        assert np.array_equal(da, dy.double().cpu().numpy() @ values(c, wbyte))
+
+
+def test_gradient_is_the_adjoint(k3, dev):
+    """<dY, mm(A)> = <mm_bwd(dY), A>, and one code changed moves the product by that column of W:
+    small integers everywhere, so both hold exactly."""
+    import torch
+    N, K, M = 136, 160, 21
+    g = np.random.default_rng(3)
+    c = g.choice([2, 4, 6, 10, 12, 0], (N, K)).astype(np.uint8)      # +-1, 2, 4
+    one = np.full((N, K // 32), 127, np.uint8)
+    W = k3.Mxfp4Mat(*k3.mxfp4_pack(*to_dev(dev, pack_nibbles(c)[None], one[None])))
+    ac = g.choice([2, 4, 10, 12, 0], (M, K)).astype(np.uint8)
+    a, s = to_dev(dev, pack_nibbles(ac), one[:M, :])
+    dy = torch.randint(-4, 5, (M, N), device=dev).bfloat16()
+    y = k3.mxfp4_mm(a, s, W, out_dtype=torch.float32)
+    da = k3.mxfp4_mm_bwd(dy, W, out_dtype=torch.float32)
+    av = torch.from_numpy(values(ac, one[:M])).to(dev)
+    assert (dy.double() * y.double()).sum() == (da.double() * av).sum()
+    ac2 = ac.copy()
+    ac2[:, 77] = np.where(ac[:, 77] == 2, 4, 2)
+    y2 = k3.mxfp4_mm(to_dev(dev, pack_nibbles(ac2))[0], s, W, out_dtype=torch.float32)
+    step = values(ac2, one[:M])[:, 77] - values(ac, one[:M])[:, 77]
+    assert np.array_equal((y2 - y).double().cpu().numpy(), step[:, None] * values(c, one)[:, 77][None])
+
+
+def test_captured_and_on_two_streams(k3, dev):
+    import torch
+    W, _ = matrices(k3, dev, 61, 6, 384, 512)
+    off = torch.tensor([0, 100, 100, 350, 351, 380, 400], dtype=torch.int32, device=dev)
+
+    def chain(x, dy):
+        y = k3.mxfp4_mm(*k3.mxfp4_quant(x), W, off=off)
+        return y, k3.mxfp4_mm_bwd(dy, W, off=off)
+
+    def inputs(seed):
+        g = torch.Generator().manual_seed(seed)
+        return torch.randn((400, 512), generator=g).to(dev), torch.randn((400, 384), generator=g).bfloat16().to(dev)
+    a, b = inputs(1), inputs(2)
+    wa, wb = chain(*a), chain(*b)
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        with torch.cuda.stream(s1):
+            ga = chain(*a)
+        with torch.cuda.stream(s2):
+            gb = chain(*b)
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(ga + gb, wa + wb))
+    held = [t.clone() for t in a]
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = chain(*held)
+    for src, want in ((b, wb), (a, wa)):
+        for h, t in zip(held, src):
+            h.copy_(t)
+        gr.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, want))
+
+
+def test_experts_of_a_pool_layer_together(k3, dev):
+    """The operators as a layer uses them, on a pool layer's own arena and run table: router, sort,
+    quantising permute, gate/up product, SwiGLU, quantise, down product, weighted sum -- each
+    step against 64 bits on the step's own inputs; then back through every step."""
+    import torch
+    H, I, E, K, T = 512, 256, 12, 3, 37
+    g = k3.synth.rng(77)
+    experts = [k3.synth.expert(g, H, I) for _ in range(E)]
+    _, wb = k3.synth.router_weights(g, E, H)
+    Wr = torch.from_numpy(wb.view(np.int16)).to(dev).view(torch.bfloat16)
+    pl = k3.PoolMoeLayer.pack([k3.DeviceExpert.from_host(e, dev) for e in experts], None, Wr, None, H, I, K, dev)
+    pl.run_of[5] = -1                                   # an expert that is not resident
+    _, xb = k3.synth.activations(g, T, H)
+    x = torch.from_numpy(xb.view(np.int16)).to(dev).view(torch.bfloat16)
+    idx, wt, _ = k3.router(x, Wr, None, K)
+    pos, pair, off = k3.moe_sort(idx, E)
+    GU, D = k3.Mxfp4Mat.from_pool(pl, "gate_up"), k3.Mxfp4Mat.from_pool(pl, "down")
+    a, sa = k3.moe_permute_mxfp4(x, pos)
+    gu = k3.mxfp4_mm(a, sa, GU, off=off, out_dtype=torch.float32)
+    blocks = gu.view(T * K, I // 64, 2, 64)
+    gate, up = blocks[:, :, 0].reshape(T * K, I), blocks[:, :, 1].reshape(T * K, I)
+    h = torch.nn.functional.silu(gate) * up
+    b, sb = k3.mxfp4_quant(h)
+    y = k3.mxfp4_mm(b, sb, D, off=off, out_dtype=torch.float32)
+    out = k3.moe_unpermute(y, pos, wt)
+
+    def mat(e, name):
+        return values(unpack(e[name + "_p"]), e[name + "_s"])
+
+    av, bv = values(unpack(a.cpu().numpy()), sa.cpu().numpy()), values(unpack(b.cpu().numpy()), sb.cpu().numpy())
+    offn, idn, pn, wn = off.cpu().numpy(), idx.cpu().numpy(), pos.cpu().numpy(), wt.double().cpu().numpy()
+    assert offn[-1] == T * K
+    yn = y.double().cpu().numpy()
+    dout = torch.randn((T, H), device=dev)
+    dy, dwt = k3.moe_unpermute_bwd(dout, y, pos, wt)
+    dh = k3.mxfp4_mm_bwd(dy.bfloat16(), D, off=off, out_dtype=torch.float32)
+    sg = torch.sigmoid(gate)
+    dgate, dup = dh * up * sg * (1 + gate * (1 - sg)), dh * gate * sg
+    dgu = torch.stack([dgate.view(T * K, I // 64, 64), dup.view(T * K, I // 64, 64)], 2).reshape(T * K, 2 * I).bfloat16()
+    da = k3.mxfp4_mm_bwd(dgu, GU, off=off, out_dtype=torch.float32)
+    dx = k3.moe_permute_bwd(da, pos)
+    for e in range(E):
+        r = slice(offn[e], offn[e + 1])
+        if e == 5:
+            assert (gu[r] == 0).all() and (yn[r] == 0).all() and (da[r] == 0).all()
+            continue
+        wg, wu, wd = mat(experts[e], "gate"), mat(experts[e], "up"), mat(experts[e], "down")
+        check(gate[r].double().cpu().numpy(), av[r] @ wg.T, np.abs(av[r]) @ np.abs(wg).T, H // 64, False)
+        check(up[r].double().cpu().numpy(), av[r] @ wu.T, np.abs(av[r]) @ np.abs(wu).T, H // 64, False)
+        check(yn[r], bv[r] @ wd.T, np.abs(bv[r]) @ np.abs(wd).T, I // 64, False)
+        d = dy[r].bfloat16().double().cpu().numpy()
+        check(dh[r].double().cpu().numpy(), d @ wd, np.abs(d) @ np.abs(wd), H // 16, False)
+        wgu = np.stack([wg.reshape(I // 64, 64, H), wu.reshape(I // 64, 64, H)], 1).reshape(2 * I, H)
+        d = dgu[r].double().cpu().numpy()
+        check(da[r].double().cpu().numpy(), d @ wgu, np.abs(d) @ np.abs(wgu), 2 * I // 16, False)
+    want = (wn[:, :, None] * yn[pn]).sum(1)
+    lim = (K + 2) * 2.0 ** -24 * (np.abs(wn)[:, :, None] * np.abs(yn[pn])).sum(1)
+    assert (np.abs(out.double().cpu().numpy() - want) <= lim).all()
+    want = da.double().cpu().numpy()[pn]
+    assert (np.abs(dx.double().cpu().numpy() - want.sum(1)) <= (K + 2) * 2.0 ** -24 * np.abs(want).sum(1)).all()
+
+
+def test_products_match_the_gemv_and_dequant(k3, dev):
+    """The same codes through the framework's own fp32-activation GEMV and dequantiser."""
+    import torch
+    N, K = 96, 256
+    c, b = operand(71, N, K, 118, 125)
+    p, s = to_dev(dev, pack_nibbles(c), b)
+    x = torch.randn((5, K), device=dev)
+    a, sa = k3.mxfp4_quant(x)
+    y = k3.mxfp4_mm(a, sa, k3.Mxfp4Mat(*k3.mxfp4_pack(p, s)), out_dtype=torch.float32)
+    ref = k3.mxfp4_gemv(k3.mxfp4_dequant(a, sa), p, s)
+    mag = np.abs(values(unpack(a.cpu().numpy()), sa.cpu().numpy())) @ np.abs(values(c, b)).T
+    assert (np.abs((y - ref).double().cpu().numpy()) <= (K + 16) * 2.0 ** -23 * mag).all()

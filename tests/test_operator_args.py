@@ -1,0 +1,123 @@
+"""Refusals of the sort / permute / MXFP4-product entry points, without a GPU: the C functions
+validate before any CUDA call, and the Python wrappers refuse tensors of the wrong type, shape,
+layout or place."""
+import ctypes as C
+
+import pytest
+
+BUF = 1 << 20            # an aligned address nothing dereferences
+
+
+def err(k3):
+    return k3.lib().k3c_last_error().decode()
+
+
+def mat(k3, **kw):
+    d = dict(codes=BUF, atoms=BUF, code_stride=64 * 16, atom_stride=512, n_mats=1, rows=64, in_=32, mat_of=None)
+    d.update(kw)
+    return k3.Mxfp4MatC(*(d[n] for n in ("codes", "atoms", "code_stride", "atom_stride", "n_mats", "rows", "in_", "mat_of")))
+
+
+def test_sort_refusals(k3):
+    L = k3.lib()
+    for args, word in (((BUF, BUF, BUF, BUF, -1, 8, 4, None, 0, None), "ntok"),
+                       ((BUF, BUF, BUF, BUF, 4, 0, 4, None, 0, None), "topk"),
+                       ((BUF, BUF, BUF, BUF, 4, 65, 4, None, 0, None), "topk"),
+                       ((BUF, BUF, BUF, BUF, 4, 8, 0, None, 0, None), "n_experts"),
+                       ((BUF, BUF, BUF, BUF, 4, 8, 2049, None, 0, None), "n_experts"),
+                       ((BUF, BUF, BUF, BUF, 1 << 30, 8, 4, None, 0, None), "32 bits"),
+                       ((None, BUF, BUF, BUF, 4, 8, 4, None, 0, None), "NULL"),
+                       ((BUF, BUF, None, BUF, 0, 8, 4, None, 0, None), "NULL"),
+                       ((BUF, BUF, BUF, BUF, 4096, 8, 4, None, 0, None), "scratch"),
+                       ((BUF, BUF, BUF, BUF, 4096, 8, 4, BUF, 8, None), "scratch"),
+                       ((BUF, BUF, BUF, BUF, 4096, 8, 4, BUF + 1, 1 << 20, None), "scratch")):
+        assert L.k3c_moe_sort(*args) == -1 and word in err(k3), (args, err(k3))
+    assert L.k3c_moe_sort_scratch(16, 8, 384) == 0
+    assert L.k3c_moe_sort_scratch(4096, 8, 384) == 8 * 384 * 4
+    assert L.k3c_moe_sort_scratch(-1, 8, 384) == 0
+
+
+def test_permute_refusals(k3):
+    L = k3.lib()
+    assert L.k3c_moe_permute(BUF, BUF, 2, 64, BUF, 4, 2, 64, None) == -1 and "dtype" in err(k3)
+    assert L.k3c_moe_permute(BUF, BUF, 0, 63, BUF, 4, 2, 64, None) == -1 and "ldx" in err(k3)
+    assert L.k3c_moe_permute(BUF, BUF, 0, 64, BUF, 4, 2, 0, None) == -1 and "hidden" in err(k3)
+    assert L.k3c_moe_permute(None, BUF, 0, 64, BUF, 4, 2, 64, None) == -1 and "NULL" in err(k3)
+    assert L.k3c_moe_permute_bwd(BUF, BUF, 7, BUF, 4, 2, 64, None) == -1 and "dtype" in err(k3)
+    assert L.k3c_moe_permute_bwd(BUF, BUF, 0, None, 4, 2, 64, None) == -1 and "NULL" in err(k3)
+    assert L.k3c_moe_permute_mxfp4(BUF, BUF, BUF, 0, 48, BUF, 4, 2, 48, None) == -1 and "multiple of 32" in err(k3)
+    assert L.k3c_moe_permute_mxfp4(BUF + 8, BUF, BUF, 0, 64, BUF, 4, 2, 64, None) == -1 and "aligned" in err(k3)
+    assert L.k3c_moe_unpermute(BUF, 0, BUF, 3, BUF, BUF, 4, 2, 64, None) == -1 and "dtype" in err(k3)
+    assert L.k3c_moe_unpermute(BUF, 0, BUF, 0, None, BUF, 4, 2, 64, None) == -1 and "NULL" in err(k3)
+    assert L.k3c_moe_unpermute_bwd(BUF, BUF, BUF, 0, None, 0, BUF, BUF, 4, 2, 64, None) == -1 and "NULL" in err(k3)
+    assert L.k3c_moe_unpermute_bwd(BUF, BUF, BUF, -1, BUF, 0, BUF, BUF, 4, 2, 64, None) == -1 and "dtype" in err(k3)
+
+
+def test_quant_and_pack_refusals(k3):
+    L = k3.lib()
+    assert L.k3c_mxfp4_quant(BUF, BUF, BUF, 0, 33, 4, 33, None) == -1 and "even" in err(k3)
+    assert L.k3c_mxfp4_quant(BUF, BUF, BUF, 0, 32, 4, 34, None) == -1 and "ldx" in err(k3)
+    assert L.k3c_mxfp4_quant(BUF, BUF, BUF, 9, 32, 4, 32, None) == -1 and "dtype" in err(k3)
+    assert L.k3c_mxfp4_quant(BUF, BUF, None, 0, 32, 4, 32, None) == -1 and "NULL" in err(k3)
+    assert L.k3c_mxfp4_pack(BUF, BUF, BUF, BUF, 1, 4, 48, None) == -1 and "multiple of 32" in err(k3)
+    assert L.k3c_mxfp4_pack(BUF, BUF, BUF, BUF, 0, 4, 64, None) == -1 and "n_mats" in err(k3)
+    assert L.k3c_mxfp4_pack(BUF + 4, BUF, BUF, BUF, 1, 4, 64, None) == -1 and "aligned" in err(k3)
+    assert L.k3c_mxfp4_atom_bytes(129, 160) == 4 * 512 and L.k3c_mxfp4_atom_bytes(0, 32) == 0
+
+
+def test_mm_refusals(k3):
+    L = k3.lib()
+
+    def mm(W, y=BUF, dt=0, ldy=64, a=BUF, M=4, off=None, G=1):
+        return L.k3c_mxfp4_mm(y, dt, ldy, a, BUF, M, None if W is None else C.byref(W), off, G, None)
+
+    def bwd(W, da=BUF, dt=0, ld=64, dy=BUF, lddy=64, M=4, off=None, G=1):
+        return L.k3c_mxfp4_mm_bwd(da, dt, ld, dy, lddy, M, None if W is None else C.byref(W), off, G, None)
+
+    for f in (mm, bwd):
+        for W, word in ((None, "matrix"), (mat(k3, in_=48), "multiple of 32"), (mat(k3, rows=0), "rows"),
+                        (mat(k3, codes=BUF + 8), "aligned"), (mat(k3, n_mats=2, atom_stride=520), "aligned"),
+                        (mat(k3, n_mats=2, code_stride=512), "strides"), (mat(k3, n_mats=0), "n_mats")):
+            assert f(W) == -1 and word in err(k3), (word, err(k3))
+        assert f(mat(k3), M=-1) == -1 and "M=" in err(k3)
+        assert f(mat(k3), G=2) == -1 and "n_groups" in err(k3)
+        assert f(mat(k3), off=BUF, G=0) == -1 and "n_groups" in err(k3)
+        assert f(mat(k3, n_mats=2000, mat_of=BUF), off=BUF, G=1025) == -1 and "n_groups" in err(k3)
+        assert f(mat(k3), off=BUF, G=2) == -1 and "matrices" in err(k3)
+        assert f(mat(k3), dt=4) == -1 and "dtype" in err(k3)
+        assert f(mat(k3), M=0) == 0
+    assert mm(mat(k3), ldy=63) == -1 and "ldy" in err(k3)
+    assert mm(mat(k3), a=BUF + 8) == -1 and "aligned" in err(k3)
+    assert mm(mat(k3), y=None) == -1 and "NULL" in err(k3)
+    assert bwd(mat(k3), ld=31) == -1 and "ldda" in err(k3)
+    assert bwd(mat(k3), lddy=60) == -1 and "lddy" in err(k3)
+    assert bwd(mat(k3), lddy=68) == -1 and "lddy" in err(k3)
+    assert bwd(mat(k3), dy=BUF + 2) == -1 and "aligned" in err(k3)
+
+
+def test_wrappers_refuse(k3):
+    import torch
+    i32, f = torch.zeros((4, 2), dtype=torch.int32), torch.zeros((4, 64))
+    for call in (lambda: k3.moe_sort(i32, 8),                       # not on a GPU
+                 lambda: k3.moe_sort(i32.long(), 8), lambda: k3.moe_sort(i32[0], 8),
+                 lambda: k3.moe_permute(f, i32), lambda: k3.moe_permute(f.half(), i32),
+                 lambda: k3.moe_permute_bwd(f, i32), lambda: k3.moe_permute_mxfp4(f, i32),
+                 lambda: k3.moe_unpermute(f, i32, f[:, :2]), lambda: k3.moe_unpermute_bwd(f, f, i32, f),
+                 lambda: k3.mxfp4_quant(f), lambda: k3.mxfp4_quant(f.double()),
+                 lambda: k3.mxfp4_pack(f, f), lambda: k3.Mxfp4Mat(f, f)):
+        with pytest.raises(k3.K3CError):
+            call()
+
+
+def test_mat_struct_layout_matches_header(k3, tmp_path):
+    import os
+    import subprocess
+    from conftest import ROOT
+    src = tmp_path / "t.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "k3c.h"\nint main(void) { printf("%zu %zu %zu %zu\\n",'
+                   ' sizeof(k3c_mxfp4_mat), offsetof(k3c_mxfp4_mat, code_stride), offsetof(k3c_mxfp4_mat, rows),'
+                   ' offsetof(k3c_mxfp4_mat, mat_of)); return 0; }\n')
+    subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(tmp_path / "t")], check=True)
+    got = [int(v) for v in subprocess.run([str(tmp_path / "t")], capture_output=True, text=True).stdout.split()]
+    m = k3.Mxfp4MatC
+    assert got == [C.sizeof(m), m.code_stride.offset, m.rows.offset, m.mat_of.offset]
