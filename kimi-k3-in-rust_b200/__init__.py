@@ -1001,83 +1001,94 @@ class LatentMoeLayer:
 # ------------------------------------------------------------------ expert dispatch, MXFP4 products
 # These wrappers check what the C entry points cannot see (element types, shapes, devices), run on
 # the tensors' own device and on that device's current stream, and allocate only their results.
+# A decode step makes several of these calls on a few tokens, where the host's time is the call's:
+# hence the plain comparisons, and addresses passed as integers.
+_rt = None
 
 
-class _On:
-    """The tensors' device made current for a call where it is not."""
+class _Runtime:
+    """What every call below needs, looked up once."""
 
-    __slots__ = ("dev", "prev")
-
-    def __init__(self, t):
-        self.dev = t.device.index
-
-    def __enter__(self):
+    def __init__(self):
         import torch
-        prev = torch.cuda.current_device()
-        self.prev = None
-        if prev != self.dev:
-            torch.cuda.set_device(self.dev)
-            self.prev = prev
-        return C.c_void_p(torch.cuda.current_stream(self.dev).cuda_stream)
-
-    def __exit__(self, *exc):
-        if self.prev is not None:
-            import torch
-            torch.cuda.set_device(self.prev)
+        self.torch = torch
+        self.lib = lib()
+        self.floats = (torch.float32, torch.bfloat16)
+        self.code = {torch.float32: K3C_F32, torch.bfloat16: K3C_BF16}
+        self.i32, self.u8, self.f32 = torch.int32, torch.uint8, torch.float32
+        torch.cuda.init()
+        self.device = torch._C._cuda_getDevice
+        self.stream = torch._C._cuda_getCurrentRawStream
 
 
-def _need(ok, what):
-    if not ok:
-        raise K3CError(what)
+def _runtime(t):
+    """The runtime; t (a call's first tensor) must be on a GPU."""
+    global _rt
+    if not t.is_cuda:
+        raise K3CError(f"a CUDA tensor expected, got one on {t.device}")
+    if _rt is None:
+        _rt = _Runtime()
+    return _rt
 
 
-def _arg(t, name, dtypes, shape, like=None):
-    """t is a CUDA tensor of one of dtypes and of shape (None: any extent), contiguous."""
-    if t.dtype not in dtypes or t.dim() != len(shape) or any(s is not None and s != n for s, n in zip(shape, t.shape)):
-        raise K3CError(f"{name}: {t.dtype} {tuple(t.shape)}, expected {dtypes} {tuple(shape)}")
-    if not t.is_cuda or (like is not None and t.device != like.device):
-        raise K3CError(f"{name}: on {t.device}" + (f", expected {like.device}" if like is not None else ""))
-    if not t.is_contiguous():
-        raise K3CError(f"{name}: not contiguous (strides {t.stride()})")
-    return t
-
-
-def _rows_arg(t, name, dtypes, like=None):
-    """A 2-D CUDA tensor whose rows are contiguous; returns its row stride in elements."""
-    if t.dtype not in dtypes or t.dim() != 2:
-        raise K3CError(f"{name}: {t.dtype} {tuple(t.shape)}, expected 2-D {dtypes}")
-    if not t.is_cuda or (like is not None and t.device != like.device):
-        raise K3CError(f"{name}: on {t.device}" + (f", expected {like.device}" if like is not None else ""))
-    rows, n = t.shape
-    if rows <= 1:
-        ok, ld = n <= 1 or t.stride(1) == 1, n
+def _launch(rt, name, dev, *args):
+    """The C entry point on device dev's current stream, with dev current."""
+    fn = getattr(rt.lib, name)
+    if rt.device() == dev:
+        rc = fn(*args, rt.stream(dev))
     else:
-        ok, ld = (n <= 1 or t.stride(1) == 1) and t.stride(0) >= n, t.stride(0)
-    if not ok:
-        raise K3CError(f"{name}: rows are not contiguous (strides {t.stride()})")
-    return ld
+        with rt.torch.cuda.device(dev):
+            rc = fn(*args, rt.stream(dev))
+    if rc:
+        _check(rc, name)
 
 
-def _types():
-    import torch
-    return (torch.float32, torch.bfloat16), torch
+def _bad(t, name, want):
+    raise K3CError(f"{name}: {t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}, expected {want}")
+
+
+def _mat_arg(t, name, dev, dtypes, d0=None, d1=None):
+    """A contiguous 2-D tensor on device dev; its extents (None: any)."""
+    sh = t.shape
+    if (t.dtype not in dtypes or len(sh) != 2 or (d0 is not None and sh[0] != d0) or (d1 is not None and sh[1] != d1)
+            or t.get_device() != dev or not t.is_contiguous()):
+        _bad(t, name, f"contiguous {dtypes} {(d0, d1)} on device {dev}")
+    return sh
+
+
+def _vec_arg(t, name, dev, dtype):
+    if t.dtype != dtype or t.dim() != 1 or t.get_device() != dev or not t.is_contiguous():
+        _bad(t, name, f"contiguous 1-D {dtype} on device {dev}")
+    return t.shape[0]
+
+
+def _rows_arg(t, name, dev, dtypes):
+    """A 2-D tensor on device dev whose rows are contiguous: (rows, columns, row stride)."""
+    if t.dtype not in dtypes or t.dim() != 2 or t.get_device() != dev:
+        _bad(t, name, f"2-D {dtypes} on device {dev}")
+    rows, n = t.shape
+    if t.is_contiguous():
+        return rows, n, n
+    ld, inner = t.stride()
+    if rows <= 1:
+        ld = n
+    if (n > 1 and inner != 1) or ld < n:
+        _bad(t, name, "contiguous rows that do not overlap")
+    return rows, n, ld
 
 
 def moe_sort(idx, n_experts):
     """Stable sort of a routing's pairs by expert: idx [T][topk] int32 -> (pos [T][topk], pair
     [T * topk], off [n_experts + 1]) int32. pos is a pair's row, -1 for ids outside
     0..n_experts-1; pair a row's pair t * topk + j, -1 behind the last row (off[n_experts])."""
-    _, torch = _types()
-    _arg(idx, "idx", (torch.int32,), (None, None))
-    T, K = idx.shape
-    L = lib()
-    pos, pair = torch.empty_like(idx), torch.empty(T * K, dtype=torch.int32, device=idx.device)
-    off = torch.empty(n_experts + 1, dtype=torch.int32, device=idx.device)
-    n = L.k3c_moe_sort_scratch(T, K, n_experts)
-    ws = torch.empty(n, dtype=torch.uint8, device=idx.device) if n else None
-    with _On(idx) as s:
-        _check(L.k3c_moe_sort(_ptr(pos), _ptr(pair), _ptr(off), _ptr(idx), T, K, n_experts, _ptr(ws), n, s),
-               "k3c_moe_sort")
+    rt = _runtime(idx)
+    dev = idx.get_device()
+    T, K = _mat_arg(idx, "idx", dev, (rt.i32,))
+    n = rt.lib.k3c_moe_sort_scratch(T, K, n_experts)
+    pos, pair, off = rt.torch.empty_like(idx), idx.new_empty(T * K), idx.new_empty(max(n_experts, 0) + 1)
+    ws = idx.new_empty(n // 4) if n else None
+    _launch(rt, "k3c_moe_sort", dev, pos.data_ptr(), pair.data_ptr(), off.data_ptr(), idx.data_ptr(), T, K, n_experts,
+            ws.data_ptr() if n else None, n)
     return pos, pair, off
 
 
@@ -1085,116 +1096,115 @@ def moe_permute(x, pos, out=None):
     """Every pair's token row in expert order: out[pos[t][j]] = x[t], x [T][H] bf16 or fp32 (rows
     may be strided), out [T * topk][H]. Rows no pair has are left as they were (in a new out:
     undefined)."""
-    ft, torch = _types()
-    ld = _rows_arg(x, "x", ft)
-    T, H = x.shape
-    _arg(pos, "pos", (torch.int32,), (T, None), x)
-    K = pos.shape[1]
+    rt = _runtime(x)
+    dev = x.get_device()
+    T, H, ld = _rows_arg(x, "x", dev, rt.floats)
+    K = _mat_arg(pos, "pos", dev, (rt.i32,), T)[1]
     if out is None:
-        out = torch.empty((T * K, H), dtype=x.dtype, device=x.device)
+        out = x.new_empty((T * K, H))
     else:
-        _arg(out, "out", (x.dtype,), (T * K, H), x)
-    with _On(x) as s:
-        _check(lib().k3c_moe_permute(_ptr(out), _ptr(x), _dtype_code(x), ld, _ptr(pos), T, K, H, s), "k3c_moe_permute")
+        _mat_arg(out, "out", dev, (x.dtype,), T * K, H)
+    _launch(rt, "k3c_moe_permute", dev, out.data_ptr(), x.data_ptr(), rt.code[x.dtype], ld, pos.data_ptr(), T, K, H)
     return out
 
 
 def moe_permute_bwd(drows, pos, out=None):
     """moe_permute's gradient: dx[t] = sum_j drows[pos[t][j]], drows [T * topk][H]."""
-    ft, torch = _types()
-    _arg(pos, "pos", (torch.int32,), (None, None))
-    T, K = pos.shape
-    _arg(drows, "drows", ft, (T * K, None), pos)
-    H = drows.shape[1]
+    rt = _runtime(drows)
+    dev = drows.get_device()
+    T, K = _mat_arg(pos, "pos", dev, (rt.i32,))
+    H = _mat_arg(drows, "drows", dev, rt.floats, T * K)[1]
     if out is None:
-        out = torch.empty((T, H), dtype=drows.dtype, device=drows.device)
+        out = drows.new_empty((T, H))
     else:
-        _arg(out, "out", (drows.dtype,), (T, H), drows)
-    with _On(drows) as s:
-        _check(lib().k3c_moe_permute_bwd(_ptr(out), _ptr(drows), _dtype_code(drows), _ptr(pos), T, K, H, s),
-               "k3c_moe_permute_bwd")
+        _mat_arg(out, "out", dev, (drows.dtype,), T, H)
+    _launch(rt, "k3c_moe_permute_bwd", dev, out.data_ptr(), drows.data_ptr(), rt.code[drows.dtype], pos.data_ptr(), T, K, H)
     return out
 
 
 def moe_permute_mxfp4(x, pos):
     """moe_permute and mxfp4_quant in one pass: (packed [T * topk][H / 2], scales
     [T * topk][H / 32]) uint8 in expert order. H a multiple of 32."""
-    ft, torch = _types()
-    ld = _rows_arg(x, "x", ft)
-    T, H = x.shape
-    _arg(pos, "pos", (torch.int32,), (T, None), x)
-    K = pos.shape[1]
-    packed = torch.empty((T * K, H // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((T * K, H // 32), dtype=torch.uint8, device=x.device)
-    with _On(x) as s:
-        _check(lib().k3c_moe_permute_mxfp4(_ptr(packed), _ptr(scales), _ptr(x), _dtype_code(x), ld, _ptr(pos), T, K, H, s),
-               "k3c_moe_permute_mxfp4")
+    rt = _runtime(x)
+    dev = x.get_device()
+    T, H, ld = _rows_arg(x, "x", dev, rt.floats)
+    K = _mat_arg(pos, "pos", dev, (rt.i32,), T)[1]
+    packed, scales = pos.new_empty((T * K, H // 2), dtype=rt.u8), pos.new_empty((T * K, H // 32), dtype=rt.u8)
+    _launch(rt, "k3c_moe_permute_mxfp4", dev, packed.data_ptr(), scales.data_ptr(), x.data_ptr(), rt.code[x.dtype], ld,
+            pos.data_ptr(), T, K, H)
     return packed, scales
 
 
 def moe_unpermute(y, pos, wt, out=None, out_dtype=None):
     """out[t] = sum_j wt[t][j] * y[pos[t][j]]: y [T * topk][H] in expert order, wt [T][topk] fp32;
     out [T][H] of out_dtype (default: y's)."""
-    ft, torch = _types()
-    _arg(pos, "pos", (torch.int32,), (None, None))
-    T, K = pos.shape
-    _arg(y, "y", ft, (T * K, None), pos)
-    _arg(wt, "wt", (torch.float32,), (T, K), pos)
-    H = y.shape[1]
+    rt = _runtime(y)
+    dev = y.get_device()
+    T, K = _mat_arg(pos, "pos", dev, (rt.i32,))
+    H = _mat_arg(y, "y", dev, rt.floats, T * K)[1]
+    _mat_arg(wt, "wt", dev, (rt.f32,), T, K)
     if out is None:
-        out = torch.empty((T, H), dtype=out_dtype or y.dtype, device=y.device)
-    _arg(out, "out", ft if out_dtype is None else (out_dtype,), (T, H), y)
-    with _On(y) as s:
-        _check(lib().k3c_moe_unpermute(_ptr(out), _dtype_code(out), _ptr(y), _dtype_code(y), _ptr(wt), _ptr(pos), T, K, H, s),
-               "k3c_moe_unpermute")
+        out = y.new_empty((T, H), dtype=out_dtype or y.dtype)
+    _mat_arg(out, "out", dev, rt.floats if out_dtype is None else (out_dtype,), T, H)
+    if out.dtype not in rt.code:
+        raise K3CError(f"out_dtype {out_dtype}: fp32 or bf16")
+    _launch(rt, "k3c_moe_unpermute", dev, out.data_ptr(), rt.code[out.dtype], y.data_ptr(), rt.code[y.dtype], wt.data_ptr(),
+            pos.data_ptr(), T, K, H)
     return out
 
 
 def moe_unpermute_bwd(dout, y, pos, wt, dy=None, dwt=None):
     """moe_unpermute's gradients (dy [T * topk][H] of y's type, dwt [T][topk] fp32). Rows of dy no
-    pair has are left as they were (in a new dy: undefined)."""
-    ft, torch = _types()
-    _arg(pos, "pos", (torch.int32,), (None, None))
-    T, K = pos.shape
-    _arg(y, "y", ft, (T * K, None), pos)
-    H = y.shape[1]
-    _arg(dout, "dout", ft, (T, H), pos)
-    _arg(wt, "wt", (torch.float32,), (T, K), pos)
-    dy = torch.empty_like(y) if dy is None else _arg(dy, "dy", (y.dtype,), (T * K, H), y)
-    dwt = torch.empty_like(wt) if dwt is None else _arg(dwt, "dwt", (torch.float32,), (T, K), y)
-    with _On(y) as s:
-        _check(lib().k3c_moe_unpermute_bwd(_ptr(dy), _ptr(dwt), _ptr(dout), _dtype_code(dout), _ptr(y), _dtype_code(y),
-                                           _ptr(wt), _ptr(pos), T, K, H, s), "k3c_moe_unpermute_bwd")
+    pair has are left as they were (in a new dy: undefined). dy may not be y."""
+    rt = _runtime(y)
+    dev = y.get_device()
+    T, K = _mat_arg(pos, "pos", dev, (rt.i32,))
+    H = _mat_arg(y, "y", dev, rt.floats, T * K)[1]
+    _mat_arg(dout, "dout", dev, rt.floats, T, H)
+    _mat_arg(wt, "wt", dev, (rt.f32,), T, K)
+    if dy is None:
+        dy = rt.torch.empty_like(y)
+    else:
+        _mat_arg(dy, "dy", dev, (y.dtype,), T * K, H)
+        if dy.data_ptr() == y.data_ptr() and dy.numel():
+            raise K3CError("dy: may not be y")
+    if dwt is None:
+        dwt = rt.torch.empty_like(wt)
+    else:
+        _mat_arg(dwt, "dwt", dev, (rt.f32,), T, K)
+    _launch(rt, "k3c_moe_unpermute_bwd", dev, dy.data_ptr(), dwt.data_ptr(), dout.data_ptr(), rt.code[dout.dtype],
+            y.data_ptr(), rt.code[y.dtype], wt.data_ptr(), pos.data_ptr(), T, K, H)
     return dy, dwt
 
 
 def mxfp4_quant(x):
     """x [rows][in] bf16 or fp32 (rows may be strided, in even) -> (packed [rows][in/2], scales
     [rows][ceil(in/32)]) uint8, the layout mxfp4_dequant, mxfp4_gemv and mxfp4_mm read."""
-    ft, torch = _types()
-    ld = _rows_arg(x, "x", ft)
-    M, K = x.shape
-    packed = torch.empty((M, K // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((M, (K + 31) // 32), dtype=torch.uint8, device=x.device)
-    with _On(x) as s:
-        _check(lib().k3c_mxfp4_quant(_ptr(packed), _ptr(scales), _ptr(x), _dtype_code(x), ld, M, K, s), "k3c_mxfp4_quant")
+    rt = _runtime(x)
+    dev = x.get_device()
+    M, K, ld = _rows_arg(x, "x", dev, rt.floats)
+    packed, scales = x.new_empty((M, K // 2), dtype=rt.u8), x.new_empty((M, (K + 31) // 32), dtype=rt.u8)
+    _launch(rt, "k3c_mxfp4_quant", dev, packed.data_ptr(), scales.data_ptr(), x.data_ptr(), rt.code[x.dtype], ld, M, K)
     return packed, scales
 
 
 def mxfp4_pack(packed, scales):
     """Matrices in the reference layout (packed [n][rows][in/2], scales [n][rows][in/32] uint8; or
     one without the leading extent) -> (codes, atoms) as Mxfp4Mat takes them."""
-    _, torch = _types()
+    rt = _runtime(packed)
+    dev = packed.get_device()
     if packed.dim() == 2 and scales.dim() == 2:
         packed, scales = packed.unsqueeze(0), scales.unsqueeze(0)
-    _arg(packed, "packed", (torch.uint8,), (None, None, None))
+    if packed.dim() != 3 or packed.dtype != rt.u8 or not packed.is_contiguous():
+        _bad(packed, "packed", "contiguous uint8 [n][rows][in/2]")
     n, rows, half = packed.shape
-    _arg(scales, "scales", (torch.uint8,), (n, rows, half // 16), packed)
-    codes = torch.empty_like(packed)
-    atoms = torch.empty((n, (rows + 127) // 128, (2 * half + 127) // 128, 512), dtype=torch.uint8, device=packed.device)
-    with _On(packed) as s:
-        _check(lib().k3c_mxfp4_pack(_ptr(codes), _ptr(atoms), _ptr(packed), _ptr(scales), n, rows, 2 * half, s),
-               "k3c_mxfp4_pack")
+    if (scales.shape != (n, rows, half // 16) or scales.dtype != rt.u8 or scales.get_device() != dev
+            or not scales.is_contiguous()):
+        _bad(scales, "scales", f"contiguous uint8 {(n, rows, half // 16)} on device {dev}")
+    codes = rt.torch.empty_like(packed)
+    atoms = packed.new_empty((n, (rows + 127) // 128, (2 * half + 127) // 128, 512))
+    _launch(rt, "k3c_mxfp4_pack", dev, codes.data_ptr(), atoms.data_ptr(), packed.data_ptr(), scales.data_ptr(), n, rows,
+            2 * half)
     return codes, atoms
 
 
@@ -1203,19 +1213,26 @@ class Mxfp4Mat:
     [n][ceil(rows/128)][ceil(in/128)][512] as mxfp4_pack returns them, or one matrix of every run
     of a PoolMoeLayer (from_pool). The tensors are kept, not copied."""
 
-    __slots__ = ("c", "keep", "device")
+    __slots__ = ("c", "ref", "rows", "in_", "groups", "dev", "keep")
 
     def __init__(self, codes, atoms, mat_of=None):
         """mat_of: device int32, the matrix of each group of rows (default: group g's is g)."""
-        _, torch = _types()
-        _arg(codes, "codes", (torch.uint8,), (None, None, None))
+        rt = _runtime(codes)
+        dev = codes.get_device()
+        if codes.dim() != 3 or codes.dtype != rt.u8 or not codes.is_contiguous():
+            _bad(codes, "codes", "contiguous uint8 [n][rows][in/2]")
         n, rows, half = codes.shape
-        _arg(atoms, "atoms", (torch.uint8,), (n, (rows + 127) // 128, (2 * half + 127) // 128, 512), codes)
-        if mat_of is not None:
-            _arg(mat_of, "mat_of", (torch.int32,), (None,), codes)
-        self.c = Mxfp4MatC(codes.data_ptr(), atoms.data_ptr(), rows * half, atoms.stride(0), n, rows, 2 * half,
-                           None if mat_of is None else mat_of.data_ptr())
-        self.keep, self.device = (codes, atoms, mat_of), codes.device
+        want = (n, (rows + 127) // 128, (2 * half + 127) // 128, 512)
+        if atoms.shape != want or atoms.dtype != rt.u8 or atoms.get_device() != dev or not atoms.is_contiguous():
+            _bad(atoms, "atoms", f"contiguous uint8 {want} on device {dev}")
+        groups = n if mat_of is None else _vec_arg(mat_of, "mat_of", dev, rt.i32)
+        self._set(Mxfp4MatC(codes.data_ptr(), atoms.data_ptr(), rows * half, want[1] * want[2] * 512, n, rows, 2 * half,
+                            None if mat_of is None else mat_of.data_ptr()), groups, dev, (codes, atoms, mat_of))
+
+    def _set(self, c, groups, dev, keep):
+        self.c, self.ref, self.rows, self.in_ = c, C.byref(c), c.rows, c.in_
+        self.groups = groups      # groups of rows that `off` may name
+        self.dev, self.keep = dev, keep
 
     @classmethod
     def from_pool(cls, layer, which):
@@ -1230,30 +1247,31 @@ class Mxfp4Mat:
         rows, in_ = (2 * I, H) if which == "gate_up" else (H, I)
         base = layer.arena.data_ptr()
         m = cls.__new__(cls)
-        m.c = Mxfp4MatC(base + lay[p][0], base + lay[s][0], layer.stride, layer.stride, layer.c.n_runs, rows, in_,
-                        layer.run_of.data_ptr())
-        m.keep, m.device = (layer.arena, layer.run_of, None), layer.arena.device
+        m._set(Mxfp4MatC(base + lay[p][0], base + lay[s][0], layer.stride, layer.stride, layer.c.n_runs, rows, in_,
+                         layer.run_of.data_ptr()), layer.run_of.numel(), layer.arena.get_device(),
+               (layer.arena, layer.run_of))
         return m
 
-    @property
-    def groups(self):
-        """Groups of rows an `off` may name: one per entry of mat_of, or per matrix."""
-        mat_of = self.keep[2] if self.keep[2] is not None else (self.keep[1] if self.c.mat_of else None)
-        return self.c.n_mats if mat_of is None else mat_of.numel()
 
-
-def _mm_groups(W, off, like):
-    """(off pointer, number of groups) of a product."""
-    _, torch = _types()
-    if W.device != like.device:
-        raise K3CError(f"matrices on {W.device}, rows on {like.device}")
+def _mm_groups(rt, W, off, dev):
+    """(off address, number of groups) of a product."""
+    if W.dev != dev:
+        raise K3CError(f"matrices on device {W.dev}, rows on device {dev}")
     if off is None:
         return None, 1
-    _arg(off, "off", (torch.int32,), (None,), like)
-    G = off.numel() - 1
+    G = _vec_arg(off, "off", dev, rt.i32) - 1
     if G < 1 or G > W.groups:
         raise K3CError(f"off: {G} groups, {W.groups} matrices")
-    return _ptr(off), G
+    return off.data_ptr(), G
+
+
+def _mm_out(rt, like, M, n, dev, out, out_dtype):
+    if out is None:
+        out = like.new_empty((M, n), dtype=out_dtype or rt.torch.bfloat16)
+    rows, cols, ld = _rows_arg(out, "out", dev, rt.floats if out_dtype is None else (out_dtype,))
+    if rows != M or cols != n or out.dtype not in rt.code:
+        _bad(out, "out", f"fp32 or bf16 {(M, n)}")
+    return out, ld
 
 
 def mxfp4_mm(a, a_scales, W, off=None, out=None, out_dtype=None):
@@ -1262,36 +1280,27 @@ def mxfp4_mm(a, a_scales, W, off=None, out=None, out_dtype=None):
     with off [G + 1] int32 (moe_sort's) rows off[g]..off[g+1]-1 multiply group g's and rows
     outside every group are left as they were (in a new out: undefined). out [M][rows] of
     out_dtype (default bf16), rows may be strided."""
-    ft, torch = _types()
-    _arg(a, "a", (torch.uint8,), (None, W.c.in_ // 2))
-    M = a.shape[0]
-    _arg(a_scales, "a_scales", (torch.uint8,), (M, W.c.in_ // 32), a)
-    po, G = _mm_groups(W, off, a)
-    if out is None:
-        out = torch.empty((M, W.c.rows), dtype=out_dtype or torch.bfloat16, device=a.device)
-    ld = _rows_arg(out, "out", ft if out_dtype is None else (out_dtype,), a)
-    _need(out.shape == (M, W.c.rows), f"out: {tuple(out.shape)}, expected {(M, W.c.rows)}")
-    with _On(a) as s:
-        _check(lib().k3c_mxfp4_mm(_ptr(out), _dtype_code(out), ld, _ptr(a), _ptr(a_scales), M, C.byref(W.c), po, G, s),
-               "k3c_mxfp4_mm")
+    rt = _runtime(a)
+    dev = a.get_device()
+    M = _mat_arg(a, "a", dev, (rt.u8,), None, W.in_ // 2)[0]
+    _mat_arg(a_scales, "a_scales", dev, (rt.u8,), M, W.in_ // 32)
+    po, G = _mm_groups(rt, W, off, dev)
+    out, ld = _mm_out(rt, a, M, W.rows, dev, out, out_dtype)
+    _launch(rt, "k3c_mxfp4_mm", dev, out.data_ptr(), rt.code[out.dtype], ld, a.data_ptr(), a_scales.data_ptr(), M, W.ref, po, G)
     return out
 
 
 def mxfp4_mm_bwd(dy, W, off=None, out=None, out_dtype=None):
     """mxfp4_mm's gradient with respect to a's values: da[r] = W_g^T dy[r], dy [M][rows] bf16 (rows
     may be strided, the stride a multiple of 8). out [M][in] of out_dtype (default bf16)."""
-    ft, torch = _types()
-    ldd = _rows_arg(dy, "dy", (torch.bfloat16,))
-    M = dy.shape[0]
-    _need(dy.shape[1] == W.c.rows, f"dy: {tuple(dy.shape)}, {W.c.rows} columns expected")
-    po, G = _mm_groups(W, off, dy)
-    if out is None:
-        out = torch.empty((M, W.c.in_), dtype=out_dtype or torch.bfloat16, device=dy.device)
-    ld = _rows_arg(out, "out", ft if out_dtype is None else (out_dtype,), dy)
-    _need(out.shape == (M, W.c.in_), f"out: {tuple(out.shape)}, expected {(M, W.c.in_)}")
-    with _On(dy) as s:
-        _check(lib().k3c_mxfp4_mm_bwd(_ptr(out), _dtype_code(out), ld, _ptr(dy), ldd, M, C.byref(W.c), po, G, s),
-               "k3c_mxfp4_mm_bwd")
+    rt = _runtime(dy)
+    dev = dy.get_device()
+    M, n, ldd = _rows_arg(dy, "dy", dev, (rt.torch.bfloat16,))
+    if n != W.rows:
+        _bad(dy, "dy", f"{W.rows} columns")
+    po, G = _mm_groups(rt, W, off, dev)
+    out, ld = _mm_out(rt, dy, M, W.in_, dev, out, out_dtype)
+    _launch(rt, "k3c_mxfp4_mm_bwd", dev, out.data_ptr(), rt.code[out.dtype], ld, dy.data_ptr(), ldd, M, W.ref, po, G)
     return out
 
 

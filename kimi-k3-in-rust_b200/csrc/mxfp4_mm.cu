@@ -33,6 +33,18 @@ constexpr int MX_GMAX = 1024;   // groups of a product
 
 static __device__ int g_mx_err;
 
+// One lane of a converged warp. The compiler knows a branch on elect.sync to be taken by one
+// thread; behind `lane == 0` it guards every tcgen05 and TMA instruction's uniform operands
+// against several (~100 cycles an instruction: the copy and MMA loops below ran 3x slower).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xFFFFFFFF;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
 __device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
@@ -238,6 +250,31 @@ __device__ __forceinline__ void store_rows(uint8_t *stg, const uint32_t (&v)[32]
 }
 
 // ------------------------------------------------------------------ MXFP4 x MXFP4
+// Scale rows that do not start on 16-byte boundaries: 4 * W scale bytes at s as words. Word
+// loads only, nine for eight words, shifted together. A word that ends past the array (hi) reads
+// as `tail`, its bytes below hi, and one past it as 0; their loads go to `any` instead, without a
+// branch, so that all loads stay in flight together. n bytes from s on belong to the row, the
+// rest read as 127 (scale 1). The array starts on a word boundary.
+template <int W>
+__device__ __forceinline__ void scales_at(uint32_t (&v)[W], const uint8_t *s, int n, const uint8_t *any, const uint8_t *hi,
+                                          uint32_t tail) {
+    const uint8_t *a = reinterpret_cast<const uint8_t *>((uintptr_t)s & ~(uintptr_t)3);
+    const uint32_t sh = 8 * (uint32_t)((uintptr_t)s & 3);
+    uint32_t w[W + 1];
+#pragma unroll
+    for (int i = 0; i <= W; i++) {
+        const uint8_t *c = a + 4 * i;
+        const bool in = c + 4 <= hi;
+        const uint32_t u = __ldg(reinterpret_cast<const uint32_t *>(in ? c : any));
+        w[i] = in ? u : c < hi ? tail : 0u;
+    }
+#pragma unroll
+    for (int i = 0; i < W; i++) {
+        const int left = n - 4 * i;
+        const uint32_t keep = left >= 4 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+        v[i] = (__funnelshift_r(w[i], w[i + 1], sh) & keep) | (0x7F7F7F7Fu & ~keep);
+    }
+}
 // kind::mxf4: E2M1 A and B, K-major, UE8M0 scales per 32 (scale_vec::2X), M = 128, K = 64.
 __host__ __device__ constexpr uint32_t idesc_mxf4(uint32_t n, uint32_t sf_id) {
     return (sf_id << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((128u >> 4) << 24) | (sf_id << 29);
@@ -253,10 +290,11 @@ __device__ __forceinline__ void tc_mma_mx4(uint32_t d, uint64_t da, uint64_t db,
 }
 
 constexpr int MM_M = 128;
-constexpr int MM_ABOX = 32;                      // rows per A copy: short tiles copy only what they have
+constexpr int MM_ABOX = 32;                      // rows per A copy of a short tile; a full one takes one copy
 constexpr int MM_A = MM_M * 128;                 // 128 rows x 256 codes
 constexpr int MM_THREADS = 384;                  // copies, MMA, A scales, (idle), 8 epilogue warps
 constexpr int MM_EPI = 8;
+constexpr int MM_KS = 4;                         // K blocks per fetch of A scales: one 32-byte sector a row
 template <int NT>
 struct MmCfg {
     static constexpr int B = NT * 128;
@@ -277,6 +315,7 @@ struct MmCfg {
 
 template <int NT>
 __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant__ CUtensorMap tmA,
+                                                          const __grid_constant__ CUtensorMap tmA1,
                                                           const __grid_constant__ CUtensorMap tmW, MxArgs p) {
     using C = MmCfg<NT>;
     extern __shared__ uint8_t mm_raw[];
@@ -315,9 +354,9 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant_
 
     if (warp == 0) {
         // ------------------------------------------------------------ copies
-        if (lane == 0) {
+        if (elect_one()) {
             bool ok = tc::tc_check((tc::smem_u32(smem) & 1023) == 0, p.err, 80);
-            uint32_t ki = 0;
+            uint32_t ki = 0, st = 0, ph = 0;
             for (int it = blockIdx.x; ok && it < n_items; it += gridDim.x) {
                 const Item x = item_of(it, tbase, p.off, p.mat_of, p.n_mats, p.G, p.M, p.NTL, MM_M);
                 if (x.mat < 0) continue;
@@ -326,8 +365,6 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant_
                 const int atoms = min(C::NA, (p.N + 127) / 128 - arow);        // the last tile may end early
                 const uint8_t *wsf = p.atoms + (size_t)x.mat * p.atom_stride + (size_t)arow * KA * 512;
                 for (int kb = 0; kb < KB; kb++, ki++) {
-                    const int st = ki % C::STAGES;
-                    const uint32_t ph = (ki / C::STAGES) & 1u;
                     if (ki >= C::STAGES && !tc::mbar_wait(&empty[st], ph ^ 1u, p.err, 81)) { ok = false; break; }
                     uint8_t *sa = smem + st * C::STAGE, *sb = sa + MM_A, *sf = sb + C::B + 1024;
                     const uint32_t sfb = min(2, KA - 2 * kb) * 512;            // W's scales of this K block
@@ -335,8 +372,15 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant_
                     tc::tma_load_3d(sb, &tmW, &full[st], kb * 128, x.nt * NT, x.mat);
                     for (int a = 0; a < atoms; a++)
                         tc::bulk_load(sf + a * 1024, wsf + ((size_t)a * KA + 2 * kb) * 512, sfb, &full[st]);
-                    for (int b = 0; b < boxes; b++)
-                        tc::tma_load_3d(sa + b * (MM_ABOX * 128), &tmA, &full[st], kb * 128, x.row0 + b * MM_ABOX, 0);
+                    if (boxes == MM_M / MM_ABOX)
+                        tc::tma_load_3d(sa, &tmA, &full[st], kb * 128, x.row0, 0);
+                    else
+                        for (int b = 0; b < boxes; b++)
+                            tc::tma_load_3d(sa + b * (MM_ABOX * 128), &tmA1, &full[st], kb * 128, x.row0 + b * MM_ABOX, 0);
+                    if (++st == C::STAGES) {
+                        st = 0;
+                        ph ^= 1u;
+                    }
                 }
             }
             // no copy may still be landing when the CTA exits
@@ -345,86 +389,138 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant_
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA
-        if (lane == 0) {
-            uint32_t ki = 0, li = 0;
+        if (elect_one()) {
+            uint32_t st = 0, ph = 0, a = 0, aph = 1;   // aph: parity of an accumulator's last release
             bool ok = true;
+            // descriptors of stage 0; a stage, a K step and an atom on are additions to the low words
+            const uint64_t da0 = tc::desc_kmajor_sw128(tc::smem_u32(smem)), db0 = tc::desc_kmajor_sw128(tc::smem_u32(smem) + MM_A);
+            const uint64_t dsf0 = tc::desc_sf_atom(tc::smem_u32(smem) + MM_A + C::B);
             for (int it = blockIdx.x; ok && it < n_items; it += gridDim.x) {
                 const Item x = item_of(it, tbase, p.off, p.mat_of, p.n_mats, p.G, p.M, p.NTL, MM_M);
                 if (x.mat < 0) continue;
-                const uint32_t a = li % C::NACC, use = li / C::NACC;
-                li++;
-                if (use >= 1 && !tc::mbar_wait(&tempty[a], (use - 1) & 1u, p.err, 83)) { ok = false; break; }
+                if (!tc::mbar_wait(&tempty[a], aph, p.err, 83)) { ok = false; break; }
                 tc::tc_fence_after();
                 const uint32_t d = tmem + a * NT;
                 const uint32_t shift = NT == 64 ? 2u * (x.nt & 1) : 0u;   // rows 64..127 of an atom: two columns on
-                for (int kb = 0; kb < KB; kb++, ki++) {
-                    const int st = ki % C::STAGES;
-                    if (!tc::mbar_wait(&full[st], (ki / C::STAGES) & 1u, p.err, 84)) { ok = false; break; }
+                for (int kb = 0; kb < KB; kb++) {
+                    if (!tc::mbar_wait(&full[st], ph, p.err, 84)) { ok = false; break; }
+                    tc::fence_proxy_async_smem();   // A's scales, stored by warp 2
                     tc::tc_fence_after();
-                    const uint32_t sa = tc::smem_u32(smem + st * C::STAGE), sb = sa + MM_A, sf = sb + C::B;
+                    const uint64_t so = (uint64_t)(st * (C::STAGE >> 4));
+                    const uint64_t da = da0 + so, db = db0 + so, dsf = dsf0 + so;
                     const uint32_t col = tmem + C::SF_COL + st * C::SFW;
-                    const int steps = min(4, (p.K - 256 * kb + 63) / 64);
                     // per 128 elements: A's four columns, then W's four per 128 rows
-                    for (int j = 0; 2 * j < steps; j++) {
-                        tc::tc_cp_sf(col + j * (C::SFW / 2), tc::desc_sf_atom(sf + j * 512));
+                    auto scales = [&](int j) {
+                        tc::tc_cp_sf(col + j * (C::SFW / 2), dsf + j * 32);
 #pragma unroll
-                        for (int q = 0; q < C::NA; q++)
-                            tc::tc_cp_sf(col + j * (C::SFW / 2) + 4 + 4 * q, tc::desc_sf_atom(sf + 1024 + q * 1024 + j * 512));
-                    }
-                    for (int k = 0; k < steps; k++) {
+                        for (int q = 0; q < C::NA; q++) tc::tc_cp_sf(col + j * (C::SFW / 2) + 4 + 4 * q, dsf + 64 + q * 64 + j * 32);
+                    };
+                    auto step = [&](int k, uint32_t acc) {
                         const uint32_t id = 2u * (k & 1), sfa = col + (k >> 1) * (C::SFW / 2);
-                        tc_mma_mx4(d, tc::desc_kmajor_sw128(sa + 32 * k), tc::desc_kmajor_sw128(sb + 32 * k),
-                                   idesc_mxf4(NT, id), sfa | (id << 30), (sfa + 4 + shift) | (id << 30), (kb | k) != 0);
+                        tc_mma_mx4(d, da + 2 * k, db + 2 * k, idesc_mxf4(NT, id), sfa | (id << 30), (sfa + 4 + shift) | (id << 30), acc);
+                    };
+                    const int left = p.K - 256 * kb;
+                    scales(0);
+                    if (left >= 256) {
+                        scales(1);
+                        step(0, kb != 0);
+#pragma unroll
+                        for (int k = 1; k < 4; k++) step(k, 1);
+                    } else {
+                        if (left > 128) scales(1);
+                        for (int k = 0; 64 * k < left; k++) step(k, (kb | k) != 0);
                     }
                     tc::tc_commit(&empty[st]);
+                    if (++st == C::STAGES) {
+                        st = 0;
+                        ph ^= 1u;
+                    }
                 }
                 if (ok) tc::tc_commit(&tfull[a]);
+                if (++a == C::NACC) {
+                    a = 0;
+                    aph ^= 1u;
+                }
             }
         }
     } else if (warp == 2) {
         // ------------------------------------------------------------ A's scales
-        // Lane i fetches the eight scale bytes of rows i, 32+i, 64+i and 96+i and stores the
-        // four rows' words of each atom as one 16-byte piece (sf_byte's order).
+        // Lane i fetches the scale bytes of rows i, 32+i, 64+i and 96+i and stores the four rows'
+        // words of each atom as one 16-byte piece (sf_byte's order). MM_KS K blocks are fetched
+        // at a time, while the MM_KS before them are stored, across items. The stores become
+        // visible to tcgen05.cp by the MMA thread's proxy fence: one here would wait for the
+        // fetches in flight.
         const int SR = p.K / 32;
-        const int wide = SR % 8 == 0 && ((uintptr_t)p.as & 7) == 0;
-        uint32_t ki = 0;
+        const int wide = SR % 16 == 0 && ((uintptr_t)p.as & 15) == 0;
+        const uint8_t *as_end = p.as + (size_t)p.M * SR;
+        uint32_t tail = 0;   // the bytes of the array's last word, if it is no whole one
+        for (const uint8_t *c = reinterpret_cast<const uint8_t *>((uintptr_t)as_end & ~(uintptr_t)3); c < as_end; c++)
+            tail |= (uint32_t)__ldg(c) << (8 * ((uintptr_t)c & 3));
+        uint32_t st = 0, ph = 1, w[4][2 * MM_KS];
         bool ok = true;
-        for (int it = blockIdx.x; ok && it < n_items; it += gridDim.x) {
-            const Item x = item_of(it, tbase, p.off, p.mat_of, p.n_mats, p.G, p.M, p.NTL, MM_M);
-            if (x.mat < 0) continue;
-            for (int kb = 0; kb < KB; kb++, ki++) {
-                uint32_t w[2][4];
+        auto next_item = [&](int &it, Item &x) {   // the first item from `it` on that has a matrix
+            for (; it < n_items; it += gridDim.x) {
+                x = item_of(it, tbase, p.off, p.mat_of, p.n_mats, p.G, p.M, p.NTL, MM_M);
+                if (x.mat >= 0) return;
+            }
+        };
+        auto fetch = [&](uint32_t (&v)[4][2 * MM_KS], const Item &x, int k0) {
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    w[0][q] = w[1][q] = 0x7F7F7F7Fu;   // rows past the tile, groups past K: scale 1
-                    const int r = 32 * q + lane;
-                    if (r < x.n) {
-                        const uint8_t *s = p.as + (size_t)(x.row0 + r) * SR + 8 * kb;
-                        if (wide) {
-                            const uint2 u = __ldg(reinterpret_cast<const uint2 *>(s));
-                            w[0][q] = u.x;
-                            w[1][q] = u.y;
-                        } else {
-                            const int n = min(8, SR - 8 * kb);
+            for (int q = 0; q < 4; q++) {
 #pragma unroll
-                            for (int b = 0; b < 8; b++)
-                                if (b < n) {
-                                    const uint32_t sh = 8 * (b & 3);
-                                    w[b >> 2][q] = (w[b >> 2][q] & ~(0xFFu << sh)) | ((uint32_t)__ldg(s + b) << sh);
-                                }
-                        }
+                for (int i = 0; i < 2 * MM_KS; i++) v[q][i] = 0x7F7F7F7Fu;   // rows past the tile, groups past K: scale 1
+                if (32 * q + lane < x.n) {
+                    const uint8_t *s = p.as + (size_t)(x.row0 + 32 * q + lane) * SR + 8 * k0;
+                    if (wide) {   // SR is a multiple of 16: two K blocks at a time, all of them inside the row
+#pragma unroll
+                        for (int h = 0; h < MM_KS / 2; h++)
+                            if (k0 + 2 * h < KB) {
+                                const uint4 u = __ldg(reinterpret_cast<const uint4 *>(s + 16 * h));
+                                v[q][4 * h] = u.x;
+                                v[q][4 * h + 1] = u.y;
+                                v[q][4 * h + 2] = u.z;
+                                v[q][4 * h + 3] = u.w;
+                            }
+                    } else {
+                        scales_at<2 * MM_KS>(v[q], s, SR - 8 * k0, p.atoms, as_end, tail);
                     }
                 }
-                const int st = ki % C::STAGES;
-                const uint32_t ph = (ki / C::STAGES) & 1u;
-                if (ki >= C::STAGES && !tc::mbar_wait(&empty[st], ph ^ 1u, p.err, 85)) { ok = false; break; }
+            }
+        };
+        int it = blockIdx.x, k0 = 0;
+        Item x = {};
+        next_item(it, x);
+        if (it < n_items) fetch(w, x, 0);
+        while (ok && it < n_items) {
+            uint32_t nx[4][2 * MM_KS] = {};
+            const int kn = min(MM_KS, KB - k0);
+            k0 += MM_KS;
+            if (k0 >= KB) {
+                k0 = 0;
+                it += gridDim.x;
+                next_item(it, x);
+            }
+            if (it < n_items) fetch(nx, x, k0);
+#pragma unroll
+            for (int e = 0; e < MM_KS; e++) {
+                if (!ok || e >= kn) continue;
+                ok = __all_sync(0xFFFFFFFFu, tc::mbar_wait(&empty[st], ph, p.err, 85));   // the warp gives up together
+                if (!ok) continue;
                 uint8_t *sf = smem + st * C::STAGE + MM_A + C::B;
-                *reinterpret_cast<uint4 *>(sf + 16 * lane) = make_uint4(w[0][0], w[0][1], w[0][2], w[0][3]);
-                *reinterpret_cast<uint4 *>(sf + 512 + 16 * lane) = make_uint4(w[1][0], w[1][1], w[1][2], w[1][3]);
-                tc::fence_proxy_async_smem();
+                *reinterpret_cast<uint4 *>(sf + 16 * lane) = make_uint4(w[0][2 * e], w[1][2 * e], w[2][2 * e], w[3][2 * e]);
+                *reinterpret_cast<uint4 *>(sf + 512 + 16 * lane) =
+                    make_uint4(w[0][2 * e + 1], w[1][2 * e + 1], w[2][2 * e + 1], w[3][2 * e + 1]);
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&full[st]);
+                if (++st == C::STAGES) {
+                    st = 0;
+                    ph ^= 1u;
+                }
             }
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+#pragma unroll
+                for (int i = 0; i < 2 * MM_KS; i++) w[q][i] = nx[q][i];
         }
     } else if (warp >= 4) {
         // ------------------------------------------------------------ epilogue
@@ -481,7 +577,8 @@ constexpr int MB_W = MB_KB * 128;                // packed W: 64 rows x 256 code
 constexpr int MB_SF = 1024;                      // its two scale atoms
 constexpr int MB_STAGE = MB_A + MB_B + MB_W + MB_SF;
 constexpr int MB_STAGES = 3;
-constexpr int MB_WARPS = 8;                      // widening, then the epilogue
+constexpr int MB_GROUP = 8;                      // warps that widen one K block
+constexpr int MB_WARPS = 2 * MB_GROUP;           // two groups take K blocks in turn; all drain the accumulators
 constexpr int MB_THREADS = 64 + 32 * MB_WARPS;
 constexpr int MB_BYTES = 1024 + MB_STAGES * MB_STAGE + 256;
 static_assert(MB_STAGE % 1024 == 0, "stage bases stay 1024-byte aligned");
@@ -534,7 +631,7 @@ __global__ void __launch_bounds__(MB_THREADS, 1) k_mx4_bwd(const __grid_constant
     if (threadIdx.x == 0) {
         for (int i = 0; i < MB_STAGES; i++) {
             tc::mbar_init(&full[i], 1);
-            tc::mbar_init(&wide[i], MB_WARPS);
+            tc::mbar_init(&wide[i], MB_GROUP);
             tc::mbar_init(&empty[i], 1);
         }
         tc::mbar_init(tfull, 1);
@@ -556,7 +653,7 @@ __global__ void __launch_bounds__(MB_THREADS, 1) k_mx4_bwd(const __grid_constant
 
     if (warp == 0) {
         // ------------------------------------------------------------ copies
-        if (lane == 0) {
+        if (elect_one()) {
             bool ok = tc::tc_check((tc::smem_u32(smem) & 1023) == 0, p.err, 90);
             uint32_t ki = 0;
             for (int it = blockIdx.x; ok && it < n_items; it += gridDim.x) {
@@ -582,7 +679,7 @@ __global__ void __launch_bounds__(MB_THREADS, 1) k_mx4_bwd(const __grid_constant
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA
-        if (lane == 0) {
+        if (elect_one()) {
             uint32_t ki = 0, li = 0;
             bool ok = true;
             constexpr uint32_t idesc = idesc_bf16_tb(MB_N);
@@ -612,8 +709,8 @@ __global__ void __launch_bounds__(MB_THREADS, 1) k_mx4_bwd(const __grid_constant
         }
     } else {
         // ------------------------------------------------------------ widening, then the epilogue
-        const int w8 = warp - 2;
-        const int q = warp & 3, acc = w8 >> 2;     // TMEM lane quadrant; accumulator drained by this warp
+        const int w8 = (warp - 2) % MB_GROUP, turn = (warp - 2) / MB_GROUP;
+        const int q = warp & 3, acc = w8 >> 2;     // TMEM lane quadrant and accumulator drained by this warp
         const uint32_t lane_base = (uint32_t)(32 * q) << 16;
         uint32_t ki = 0, li = 0;
         bool ok = true;
@@ -621,8 +718,10 @@ __global__ void __launch_bounds__(MB_THREADS, 1) k_mx4_bwd(const __grid_constant
             const Item x = item_of(it, tbase, p.off, p.mat_of, p.n_mats, p.G, p.M, p.NTL, MB_M);
             if (x.mat >= 0) {
                 for (int kb = 0; ok && kb < KB; kb++, ki++) {
+                    if ((ki & 1u) != (uint32_t)turn) continue;
                     const int st = ki % MB_STAGES;
-                    if (!tc::mbar_wait(&full[st], (ki / MB_STAGES) & 1u, p.err, 96)) { ok = false; break; }
+                    ok = __all_sync(0xFFFFFFFFu, tc::mbar_wait(&full[st], (ki / MB_STAGES) & 1u, p.err, 96));
+                    if (!ok) break;
                     uint8_t *sb = smem + st * MB_STAGE + MB_A, *sw = sb + MB_B, *sf = sw + MB_W;
                     // a lane widens 32 codes of one W row: rows 8 w8 + (lane & 7), groups lane / 8 and
                     // 4 + lane / 8 (eight lanes touch eight rows: the swizzle spreads them over the banks)
@@ -659,7 +758,7 @@ __global__ void __launch_bounds__(MB_THREADS, 1) k_mx4_bwd(const __grid_constant
             const bool live = row < x.n;
             const bool full_warp = 128 * acc + 32 * q < x.n;     // warp-uniform
 #pragma unroll 1
-            for (int c0 = 0; c0 < MB_N; c0 += 32) {
+            for (int c0 = turn * (MB_N / 2); c0 < (turn + 1) * (MB_N / 2); c0 += 32) {
                 if (!full_warp) break;
                 uint32_t v[32];
                 if (x.mat >= 0) {
@@ -771,7 +870,7 @@ int check_items(const char *what, int64_t items) {
 int64_t most_tiles(int M, int n_groups, int tile) { return (int64_t)M / tile + (n_groups < M ? n_groups : M); }
 
 template <int NT>
-int launch_mm(const CUtensorMap &ma, const CUtensorMap &mw, MxArgs p, cudaStream_t s) {
+int launch_mm(const CUtensorMap &ma, const CUtensorMap &ma1, const CUtensorMap &mw, MxArgs p, cudaStream_t s) {
     static bool attr_of[64] = {};
     bool &attr = attr_of[cur_dev()];
     if (!attr) {
@@ -782,7 +881,7 @@ int launch_mm(const CUtensorMap &ma, const CUtensorMap &mw, MxArgs p, cudaStream
     const int64_t items = most_tiles(p.M, p.G, MM_M) * p.NTL;
     K3C_TRY(check_items("mxfp4_mm", items));
     const int grid = (int)(items < sm_count() ? items : sm_count());
-    K3C_TRY_CUDA(launch_pdl(k_mx4_mm<NT>, dim3(grid), dim3(MM_THREADS), MmCfg<NT>::BYTES, s, ma, mw, p));
+    K3C_TRY_CUDA(launch_pdl(k_mx4_mm<NT>, dim3(grid), dim3(MM_THREADS), MmCfg<NT>::BYTES, s, ma, ma1, mw, p));
     K3C_CHECK_LAUNCH();
     return K3C_OK;
 }
@@ -837,7 +936,8 @@ extern "C" int k3c_mxfp4_mm(void *y, int y_dtype, int64_t ldy, const uint8_t *a,
         return set_error(K3C_EINVAL, "mxfp4_mm: y_dtype=%d ldy=%lld rows=%d", y_dtype, (long long)ldy, W->rows);
     if (!M) return K3C_OK;
     if (!y || !a || !a_scales) return set_error(K3C_EINVAL, "mxfp4_mm: NULL array");
-    if (!al16(a)) return set_error(K3C_EINVAL, "mxfp4_mm: a must be 16-byte aligned");
+    if (!al16(a) || ((uintptr_t)a_scales & 3))
+        return set_error(K3C_EINVAL, "mxfp4_mm: a must be 16-byte aligned, a_scales 4-byte aligned");
     cudaStream_t s = (cudaStream_t)stream;
     MxArgs p = {};
     K3C_TRY(err_slot(&p.err));
@@ -860,12 +960,13 @@ extern "C" int k3c_mxfp4_mm(void *y, int y_dtype, int64_t ldy, const uint8_t *a,
     const int64_t tiles = off ? most_tiles(M, n_groups, MM_M) : (M + MM_M - 1) / MM_M;
     int nt = 256;
     while (nt > 64 && tiles * ((p.N + nt - 1) / nt) < sm_count()) nt /= 2;
-    CUtensorMap ma, mw;
-    K3C_TRY(make_map3(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, a, p.K / 2, M, 1, p.K / 2, (uint64_t)(p.K / 2) * M, 128, MM_ABOX));
+    CUtensorMap ma, ma1, mw;
+    K3C_TRY(make_map3(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, a, p.K / 2, M, 1, p.K / 2, (uint64_t)(p.K / 2) * M, 128, MM_M));
+    K3C_TRY(make_map3(&ma1, CU_TENSOR_MAP_DATA_TYPE_UINT8, a, p.K / 2, M, 1, p.K / 2, (uint64_t)(p.K / 2) * M, 128, MM_ABOX));
     K3C_TRY(map_weights(&mw, W, nt));
-    if (nt == 256) K3C_TRY(launch_mm<256>(ma, mw, p, s));
-    else if (nt == 128) K3C_TRY(launch_mm<128>(ma, mw, p, s));
-    else K3C_TRY(launch_mm<64>(ma, mw, p, s));
+    if (nt == 256) K3C_TRY(launch_mm<256>(ma, ma1, mw, p, s));
+    else if (nt == 128) K3C_TRY(launch_mm<128>(ma, ma1, mw, p, s));
+    else K3C_TRY(launch_mm<64>(ma, ma1, mw, p, s));
     return check_waits("mxfp4_mm", p.err, s);
 }
 
