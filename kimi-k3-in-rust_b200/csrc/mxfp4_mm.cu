@@ -568,20 +568,24 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant_
 }
 
 // ------------------------------------------------------------------ gradient of the activations
+// Three rings: packed W tiles (copied), widened W tiles (written by the widening warps) and dY
+// tiles (copied); the last two share their slots' numbers, and an MMA commit frees both. With
+// one ring for all three a slot was held through copy, widening and MMA, 3900 cycles for 1024
+// of MMAs: three slots' worth of them set the pace.
 constexpr int MB_M = 256;                        // rows per item: two accumulators share a widened W tile
 constexpr int MB_N = 256;                        // columns (W's in) per item
 constexpr int MB_KB = 64;                        // W rows per K block
 constexpr int MB_A = MB_M * 128;                 // dY: 256 rows x 64 bf16
 constexpr int MB_B = MB_N * MB_KB * 2;           // widened W: 4 blocks of 64 columns x 64 rows
 constexpr int MB_W = MB_KB * 128;                // packed W: 64 rows x 256 codes
-constexpr int MB_SF = 1024;                      // its two scale atoms
-constexpr int MB_STAGE = MB_A + MB_B + MB_W + MB_SF;
-constexpr int MB_STAGES = 3;
-constexpr int MB_GROUP = 8;                      // warps that widen one K block
-constexpr int MB_WARPS = 2 * MB_GROUP;           // two groups take K blocks in turn; all drain the accumulators
-constexpr int MB_THREADS = 64 + 32 * MB_WARPS;
-constexpr int MB_BYTES = 1024 + MB_STAGES * MB_STAGE + 256;
-static_assert(MB_STAGE % 1024 == 0, "stage bases stay 1024-byte aligned");
+constexpr int MB_R = MB_W + 1024;                // and its two scale atoms
+constexpr int MB_RING = 3;
+constexpr int MB_GROUP = 8;                      // warps that widen one K block; two groups take turns
+constexpr int MB_EPI = 8;
+constexpr int MB_WIDE0 = 3, MB_EPI0 = MB_WIDE0 + 2 * MB_GROUP;   // warps: dY, MMA, W, widening, epilogue
+constexpr int MB_THREADS = 32 * (MB_EPI0 + MB_EPI);
+constexpr int MB_BYTES = 1024 + MB_RING * (MB_A + MB_B + MB_R) + 256;
+static_assert(MB_A % 1024 == 0 && MB_B % 1024 == 0 && MB_R % 1024 == 0, "slots stay 1024-byte aligned");
 static_assert(MB_BYTES + (MX_GMAX + 1) * 4 + 128 <= 227 * 1024, "one CTA per SM");
 
 // kind::f16: bf16 A (K-major) and B (N-major: transpose bit 16), fp32 accumulator, M = 128.
@@ -605,37 +609,80 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
 }
-// Eight E2M1 codes to eight bf16 (element k in half k): table bytes through permutes, as
-// e2m1x8_to_f32, without the widening.
-__device__ __forceinline__ void e2m1x8_to_bf16(uint32_t w, uint32_t (&o)[4]) {
-    const uint32_t m = w & 0x77777777u, mh = m >> 16, w4 = w << 4;
-    const uint32_t lo_a = __byte_perm(0xC0800000u, 0xC0804000u, m), hi_a = __byte_perm(0x3F3F3F00u, 0x40404040u, m);
-    const uint32_t lo_b = __byte_perm(0xC0800000u, 0xC0804000u, mh), hi_b = __byte_perm(0x3F3F3F00u, 0x40404040u, mh);
-    o[0] = __byte_perm(lo_a, hi_a, 0x5140u) | (__byte_perm(w4, w, 0x4000u) & 0x80008000u);
-    o[1] = __byte_perm(lo_a, hi_a, 0x7362u) | (__byte_perm(w4, w, 0x5010u) & 0x80008000u);
-    o[2] = __byte_perm(lo_b, hi_b, 0x5140u) | (__byte_perm(w4, w, 0x6020u) & 0x80008000u);
-    o[3] = __byte_perm(lo_b, hi_b, 0x7362u) | (__byte_perm(w4, w, 0x7030u) & 0x80008000u);
+// Eight E2M1 codes to bf16: a code's exponent and mantissa bits at bits 8..6 of a bf16 are its
+// value times 2^-126, subnormals included, so f1 = 2^(byte-1) under both halves gives the scaled
+// value in one exact product. Codes j and j + 4 share word j, as they lie 16 bits apart.
+__device__ __forceinline__ void e2m1x8_widen(uint32_t w, uint32_t f1, uint32_t (&o)[4]) {
+    constexpr uint32_t mag = 0x01C001C0u, sign = 0x80008000u;
+    o[0] = mul_bf16x2(((w << 6) & mag) | ((w << 12) & sign), f1);
+    o[1] = mul_bf16x2(((w << 2) & mag) | ((w << 8) & sign), f1);
+    o[2] = mul_bf16x2(((w >> 2) & mag) | ((w << 4) & sign), f1);
+    o[3] = mul_bf16x2(((w >> 6) & mag) | (w & sign), f1);
+}
+
+// 16 rows x 32 fp32 columns of TMEM: lane l gets, of rows l/4 (v[4i], v[4i+1]) and l/4 + 8
+// (v[4i+2], v[4i+3]), columns 8i + 2(l%4) and the next, for i = 0..3.
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t addr, uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(addr));
+}
+
+// Eight neighbouring columns of one row, q[2i] and q[2i + 1] holding columns i and i + 4 (i = 0..3).
+__device__ __forceinline__ void put8(const MxArgs &p, int64_t row, int col, const uint32_t (&q)[8]) {
+    if (p.y_bf16) {
+        uint16_t *d = reinterpret_cast<uint16_t *>(p.y) + row * p.ldy + col;
+        const uint32_t o[4] = {f32x2_to_bf16x2(__uint_as_float(q[0]), __uint_as_float(q[2])),
+                               f32x2_to_bf16x2(__uint_as_float(q[4]), __uint_as_float(q[6])),
+                               f32x2_to_bf16x2(__uint_as_float(q[1]), __uint_as_float(q[3])),
+                               f32x2_to_bf16x2(__uint_as_float(q[5]), __uint_as_float(q[7]))};
+        if (p.vec) *reinterpret_cast<uint4 *>(d) = make_uint4(o[0], o[1], o[2], o[3]);
+        else
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                d[2 * i] = (uint16_t)o[i];
+                d[2 * i + 1] = (uint16_t)(o[i] >> 16);
+            }
+    } else {
+        uint32_t *d = reinterpret_cast<uint32_t *>(p.y) + row * p.ldy + col;
+        if (p.vec) {
+            reinterpret_cast<uint4 *>(d)[0] = make_uint4(q[0], q[2], q[4], q[6]);
+            reinterpret_cast<uint4 *>(d)[1] = make_uint4(q[1], q[3], q[5], q[7]);
+        } else
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                d[i] = q[2 * i];
+                d[4 + i] = q[2 * i + 1];
+            }
+    }
 }
 
 __global__ void __launch_bounds__(MB_THREADS, 1) k_mx4_bwd(const __grid_constant__ CUtensorMap tmD,
+                                                           const __grid_constant__ CUtensorMap tmD1,
                                                            const __grid_constant__ CUtensorMap tmW, MxArgs p) {
     extern __shared__ uint8_t mb_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)mb_raw + 1023) & ~(uintptr_t)1023);
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + MB_STAGES * MB_STAGE);
-    uint64_t *wide = full + MB_STAGES, *empty = wide + MB_STAGES, *tfull = empty + MB_STAGES, *tempty = tfull + 1;
+    uint8_t *s_a = smem, *s_b = s_a + MB_RING * MB_A, *s_r = s_b + MB_RING * MB_B;
+    uint64_t *afull = reinterpret_cast<uint64_t *>(s_r + MB_RING * MB_R);
+    uint64_t *wide = afull + MB_RING, *empty = wide + MB_RING, *rfull = empty + MB_RING, *rempty = rfull + MB_RING;
+    uint64_t *tfull = rempty + MB_RING, *tempty = tfull + 1;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tempty + 1);
     __shared__ int tbase[MX_GMAX + 1];
     __shared__ int warp_tot[MB_THREADS / 32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < MB_STAGES; i++) {
-            tc::mbar_init(&full[i], 1);
+        for (int i = 0; i < MB_RING; i++) {
+            tc::mbar_init(&afull[i], 1);
             tc::mbar_init(&wide[i], MB_GROUP);
             tc::mbar_init(&empty[i], 1);
+            tc::mbar_init(&rfull[i], 1);
+            tc::mbar_init(&rempty[i], MB_GROUP);
         }
         tc::mbar_init(tfull, 1);
-        tc::mbar_init(tempty, MB_WARPS);
+        tc::mbar_init(tempty, MB_EPI);
         tc::fence_mbar_init();
         tc::prefetch_tmap(&tmD);
         tc::prefetch_tmap(&tmW);
@@ -650,157 +697,201 @@ __global__ void __launch_bounds__(MB_THREADS, 1) k_mx4_bwd(const __grid_constant
     const int n_items = tiles * p.NTL;
     const int KB = (p.N + MB_KB - 1) / MB_KB;      // contracted: W's rows
     const int KA = (p.K + 127) / 128;
+    auto item = [&](int it) { return item_of(it, tbase, p.off, p.mat_of, p.n_mats, p.G, p.M, p.NTL, MB_M); };
 
     if (warp == 0) {
-        // ------------------------------------------------------------ copies
+        // ------------------------------------------------------------ dY copies
         if (elect_one()) {
             bool ok = tc::tc_check((tc::smem_u32(smem) & 1023) == 0, p.err, 90);
-            uint32_t ki = 0;
+            uint32_t st = 0, ph = 1, n = 0;
             for (int it = blockIdx.x; ok && it < n_items; it += gridDim.x) {
-                const Item x = item_of(it, tbase, p.off, p.mat_of, p.n_mats, p.G, p.M, p.NTL, MB_M);
+                const Item x = item(it);
                 if (x.mat < 0) continue;
                 const int boxes = (x.n + 31) / 32;
-                const uint32_t sfb = min(2, KA - 2 * x.nt) * 512;
-                const uint8_t *wsf = p.atoms + (size_t)x.mat * p.atom_stride + (size_t)(2 * x.nt) * 512;
-                for (int kb = 0; kb < KB; kb++, ki++) {
-                    const int st = ki % MB_STAGES;
-                    const uint32_t ph = (ki / MB_STAGES) & 1u;
-                    if (ki >= MB_STAGES && !tc::mbar_wait(&empty[st], ph ^ 1u, p.err, 91)) { ok = false; break; }
-                    uint8_t *sa = smem + st * MB_STAGE, *sw = sa + MB_A + MB_B;
-                    tc::mbar_expect_tx(&full[st], boxes * 32 * 128 + MB_W + sfb);
-                    tc::tma_load_3d(sw, &tmW, &full[st], x.nt * 128, kb * MB_KB, x.mat);
-                    tc::bulk_load(sw + MB_W, wsf + (size_t)(kb / 2) * KA * 512, sfb, &full[st]);
-                    for (int b = 0; b < boxes; b++)
-                        tc::tma_load_3d(sa + b * (32 * 128), &tmD, &full[st], kb * MB_KB, x.row0 + b * 32, 0);
+                for (int kb = 0; kb < KB; kb++, n++) {
+                    if (!tc::mbar_wait(&empty[st], ph, p.err, 91)) { ok = false; break; }
+                    uint8_t *sa = s_a + st * MB_A;
+                    tc::mbar_expect_tx(&afull[st], boxes * 32 * 128);
+                    if (boxes >= 4) tc::tma_load_3d(sa, &tmD, &afull[st], kb * MB_KB, x.row0, 0);
+                    if (boxes == 8) tc::tma_load_3d(sa + 128 * 128, &tmD, &afull[st], kb * MB_KB, x.row0 + 128, 0);
+                    else
+                        for (int b = boxes & 4; b < boxes; b++)
+                            tc::tma_load_3d(sa + b * (32 * 128), &tmD1, &afull[st], kb * MB_KB, x.row0 + b * 32, 0);
+                    if (++st == MB_RING) {
+                        st = 0;
+                        ph ^= 1u;
+                    }
                 }
             }
-            for (uint32_t i = ki > MB_STAGES ? ki - MB_STAGES : 0; i < ki; i++)
-                tc::mbar_wait(&full[i % MB_STAGES], (i / MB_STAGES) & 1u, p.err, 92);
+            // no copy may still be landing when the CTA exits
+            for (uint32_t i = n > MB_RING ? n - MB_RING : 0; i < n; i++)
+                tc::mbar_wait(&afull[i % MB_RING], (i / MB_RING) & 1u, p.err, 92);
+        }
+    } else if (warp == 2) {
+        // ------------------------------------------------------------ W copies
+        if (elect_one()) {
+            bool ok = true;
+            uint32_t st = 0, ph = 1, n = 0;
+            for (int it = blockIdx.x; ok && it < n_items; it += gridDim.x) {
+                const Item x = item(it);
+                if (x.mat < 0) continue;
+                const uint32_t sfb = min(2, KA - 2 * x.nt) * 512;
+                const uint8_t *wsf = p.atoms + (size_t)x.mat * p.atom_stride + (size_t)(2 * x.nt) * 512;
+                for (int kb = 0; kb < KB; kb++, n++) {
+                    if (!tc::mbar_wait(&rempty[st], ph, p.err, 93)) { ok = false; break; }
+                    uint8_t *sw = s_r + st * MB_R;
+                    tc::mbar_expect_tx(&rfull[st], MB_W + sfb);
+                    tc::tma_load_3d(sw, &tmW, &rfull[st], x.nt * 128, kb * MB_KB, x.mat);
+                    tc::bulk_load(sw + MB_W, wsf + (size_t)(kb / 2) * KA * 512, sfb, &rfull[st]);
+                    if (++st == MB_RING) {
+                        st = 0;
+                        ph ^= 1u;
+                    }
+                }
+            }
+            for (uint32_t i = n > MB_RING ? n - MB_RING : 0; i < n; i++)
+                tc::mbar_wait(&rfull[i % MB_RING], (i / MB_RING) & 1u, p.err, 94);
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA
         if (elect_one()) {
-            uint32_t ki = 0, li = 0;
+            uint32_t st = 0, ph = 0, tph = 1;
             bool ok = true;
             constexpr uint32_t idesc = idesc_bf16_tb(MB_N);
+            const uint64_t da0 = tc::desc_kmajor_sw128(tc::smem_u32(s_a)), db0 = desc_nmajor_sw128(tc::smem_u32(s_b));
             for (int it = blockIdx.x; ok && it < n_items; it += gridDim.x) {
-                const Item x = item_of(it, tbase, p.off, p.mat_of, p.n_mats, p.G, p.M, p.NTL, MB_M);
+                const Item x = item(it);
                 if (x.mat < 0) continue;
-                if (li >= 1 && !tc::mbar_wait(tempty, (li - 1) & 1u, p.err, 93)) { ok = false; break; }
-                li++;
+                if (!tc::mbar_wait(tempty, tph, p.err, 95)) { ok = false; break; }
+                tph ^= 1u;
                 tc::tc_fence_after();
-                for (int kb = 0; kb < KB; kb++, ki++) {
-                    const int st = ki % MB_STAGES;
-                    const uint32_t ph = (ki / MB_STAGES) & 1u;
-                    if (!tc::mbar_wait(&full[st], ph, p.err, 94) || !tc::mbar_wait(&wide[st], ph, p.err, 95)) { ok = false; break; }
+                const bool two = x.n > 128;
+                for (int kb = 0; kb < KB; kb++) {
+                    if (!tc::mbar_wait(&afull[st], ph, p.err, 96) || !tc::mbar_wait(&wide[st], ph, p.err, 97)) { ok = false; break; }
                     tc::tc_fence_after();
-                    const uint32_t sa = tc::smem_u32(smem + st * MB_STAGE), sb = sa + MB_A;
+                    const uint64_t da = da0 + st * (MB_A >> 4), db = db0 + st * (MB_B >> 4);
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const uint64_t db = desc_nmajor_sw128(sb + 2048 * k);
-                        tc_mma_bf16(tmem, tc::desc_kmajor_sw128(sa + 32 * k), db, idesc, (kb | k) != 0);
-                        if (x.n > 128)
-                            tc_mma_bf16(tmem + MB_N, tc::desc_kmajor_sw128(sa + 128 * 128 + 32 * k), db, idesc, (kb | k) != 0);
+                    for (int k = 0; k < 4; k++) tc_mma_bf16(tmem, da + 2 * k, db + 128 * k, idesc, (kb | k) != 0);
+                    if (two) {
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            tc_mma_bf16(tmem + MB_N, da + 1024 + 2 * k, db + 128 * k, idesc, (kb | k) != 0);
                     }
                     tc::tc_commit(&empty[st]);
+                    if (++st == MB_RING) {
+                        st = 0;
+                        ph ^= 1u;
+                    }
                 }
                 if (ok) tc::tc_commit(tfull);
             }
         }
-    } else {
-        // ------------------------------------------------------------ widening, then the epilogue
-        const int w8 = (warp - 2) % MB_GROUP, turn = (warp - 2) / MB_GROUP;
-        const int q = warp & 3, acc = w8 >> 2;     // TMEM lane quadrant and accumulator drained by this warp
-        const uint32_t lane_base = (uint32_t)(32 * q) << 16;
-        uint32_t ki = 0, li = 0;
+    } else if (warp >= MB_WIDE0 && warp < MB_EPI0) {
+        // ------------------------------------------------------------ widening
+        const int w4 = (warp - MB_WIDE0) % MB_GROUP;
+        const uint32_t turn = (warp - MB_WIDE0) / MB_GROUP;
+        uint32_t n = 0, st = 0, ph = 1;            // st, ph: both rings' slot and the parity of its last release
         bool ok = true;
-        for (int it = blockIdx.x; it < n_items; it += gridDim.x) {
-            const Item x = item_of(it, tbase, p.off, p.mat_of, p.n_mats, p.G, p.M, p.NTL, MB_M);
-            if (x.mat >= 0) {
-                for (int kb = 0; ok && kb < KB; kb++, ki++) {
-                    if ((ki & 1u) != (uint32_t)turn) continue;
-                    const int st = ki % MB_STAGES;
-                    ok = __all_sync(0xFFFFFFFFu, tc::mbar_wait(&full[st], (ki / MB_STAGES) & 1u, p.err, 96));
+        for (int it = blockIdx.x; ok && it < n_items; it += gridDim.x) {
+            const Item x = item(it);
+            if (x.mat < 0) continue;
+            for (int kb = 0; ok && kb < KB; kb++, n++) {
+                if ((n & 1u) == turn) {
+                    ok = __all_sync(0xFFFFFFFFu, tc::mbar_wait(&rfull[st], ph ^ 1u, p.err, 98));
                     if (!ok) break;
-                    uint8_t *sb = smem + st * MB_STAGE + MB_A, *sw = sb + MB_B, *sf = sw + MB_W;
-                    // a lane widens 32 codes of one W row: rows 8 w8 + (lane & 7), groups lane / 8 and
-                    // 4 + lane / 8 (eight lanes touch eight rows: the swizzle spreads them over the banks)
-                    const int n = 8 * w8 + (lane & 7), m = (kb & 1) * 64 + n;
+                    // a lane widens 2 x 32 codes: groups g and g + 4 of W row r (eight lanes touch
+                    // eight rows: the swizzle spreads them over the banks)
+                    const uint8_t *sw = s_r + st * MB_R;
+                    const int r = 8 * w4 + (lane & 7), g = lane >> 3;
+                    uint4 c[2];
+                    uint32_t s[2];
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const int g = 4 * h + (lane >> 3);
-                        const uint4 c = *reinterpret_cast<const uint4 *>(sw + n * 128 + 16 * (g ^ (n & 7)));
-                        const uint32_t s = sf[h * 512 + sf_byte(m, g & 3)];
-                        const uint32_t s16 = s ? s << 7 : 0x40u;    // 2^(s-127) in bf16
-                        const uint32_t s2 = s16 | (s16 << 16);
-                        const uint32_t cw[4] = {c.x, c.y, c.z, c.w};
-                        uint8_t *row = sb + (g >> 1) * (MB_KB * 128) + n * 128;
+                    for (int i = 0; i < 2; i++) {
+                        c[i] = *reinterpret_cast<const uint4 *>(sw + r * 128 + 16 * ((g + 4 * i) ^ (r & 7)));
+                        s[i] = sw[MB_W + i * 512 + sf_byte((kb & 1) * 64 + r, g)];
+                    }
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&rempty[st]);
+                    ok = __all_sync(0xFFFFFFFFu, tc::mbar_wait(&empty[st], ph, p.err, 99));
+                    if (!ok) break;
+                    uint8_t *sb = s_b + st * MB_B;
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            uint32_t o[4];
-                            e2m1x8_to_bf16(cw[k], o);
+                    for (int i = 0; i < 2; i++) {
+                        const uint32_t e = min(s[i], 128u) + 126u;    // 2^(min(byte, 128) - 1)
+                        const uint32_t f1 = e << 7 | e << 23;
+                        const uint32_t cw[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+                        uint32_t o[4][4];
 #pragma unroll
-                            for (int i = 0; i < 4; i++) o[i] = mul_bf16x2(o[i], s2);
-                            *reinterpret_cast<uint4 *>(row + 16 * (((g & 1) * 4 + k) ^ (n & 7))) =
-                                make_uint4(o[0], o[1], o[2], o[3]);
+                        for (int k = 0; k < 4; k++) e2m1x8_widen(cw[k], f1, o[k]);
+                        if (s[i] > 128) {                             // the rest of a scale above 2^1
+                            const uint32_t h = s[i] - 1u, f2 = h << 7 | h << 23;   // 2^(byte - 128)
+#pragma unroll
+                            for (int k = 0; k < 4; k++)
+#pragma unroll
+                                for (int q = 0; q < 4; q++) o[k][q] = mul_bf16x2(o[k][q], f2);
                         }
+                        // Column order within the 32: piece q holds codes q and q + 4 of each of the
+                        // four words, so that a lane of the epilogue's 16x256b loads, which gets
+                        // columns 2l and 2l + 1 of every piece, gets word l: eight neighbours.
+                        uint8_t *row = sb + ((g + 4 * i) >> 1) * (MB_KB * 128) + r * 128;
+#pragma unroll
+                        for (int q = 0; q < 4; q++)
+                            *reinterpret_cast<uint4 *>(row + 16 * (((g & 1) * 4 + q) ^ (r & 7))) =
+                                make_uint4(o[0][q], o[1][q], o[2][q], o[3][q]);
                     }
                     tc::fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(&wide[st]);
                 }
-                ok = ok && tc::mbar_wait(tfull, li & 1u, p.err, 97);
-                li++;
+                if (++st == MB_RING) {
+                    st = 0;
+                    ph ^= 1u;
+                }
+            }
+        }
+    } else if (warp >= MB_EPI0) {
+        // ------------------------------------------------------------ epilogue
+        // A store covers 8 rows x 64 bytes (bf16); with a row per lane it was 32 rows x 16, and
+        // the accumulators stayed taken for 12000 cycles an item instead of EPI_CYCLES.
+        const int q = warp & 3, acc = (warp - MB_EPI0) >> 2;   // TMEM lane quadrant, accumulator
+        const uint32_t taddr = tmem + ((uint32_t)(32 * q) << 16) + acc * MB_N;
+        uint32_t tph = 0;
+        bool alive = true;
+        for (int it = blockIdx.x; it < n_items; it += gridDim.x) {
+            const Item x = item(it);
+            const int r0 = 128 * acc + 32 * q;                         // the warp's first row
+            const int c0 = x.nt * MB_N, cols = min(MB_N, p.K - c0);    // a multiple of 32
+            const bool real = x.mat >= 0;
+            if (real) {
+                alive = alive && tc::mbar_wait(tfull, tph, p.err, 100);
+                tph ^= 1u;
                 __syncwarp();
                 tc::tc_fence_after();
             }
-            const int row = 128 * acc + 32 * q + lane;
-            const bool live = row < x.n;
-            const bool full_warp = 128 * acc + 32 * q < x.n;     // warp-uniform
-#pragma unroll 1
-            for (int c0 = turn * (MB_N / 2); c0 < (turn + 1) * (MB_N / 2); c0 += 32) {
-                if (!full_warp) break;
-                uint32_t v[32];
-                if (x.mat >= 0) {
-                    tc::tmem_ld32(tmem + lane_base + acc * MB_N + c0, v);
-                    tc::tmem_ld_wait();
-                } else {
+            if (r0 < x.n) {
+#pragma unroll 2
+                for (int c = 0; c < cols; c += 32) {
 #pragma unroll
-                    for (int i = 0; i < 32; i++) v[i] = 0;
-                }
-                const int col = x.nt * MB_N + c0;
-                if (!live || col >= p.K) continue;
-                if (x.mat >= 0 && !ok)
+                    for (int h = 0; h < 2; h++) {                      // rows r0 + 16h ..
+                        uint32_t v[16];
+                        if (real) {
+                            tmem_ld_16x32(taddr + ((uint32_t)(16 * h) << 16) + c, v);
+                            tc::tmem_ld_wait();
+                        }
+                        if (!real || !alive)
 #pragma unroll
-                    for (int i = 0; i < 32; i++) v[i] = 0x7FC00000u;
-                if (p.y_bf16) {
-                    uint16_t *d = reinterpret_cast<uint16_t *>(p.y) + (x.row0 + row) * p.ldy + col;
+                            for (int i = 0; i < 16; i++) v[i] = real ? 0x7FC00000u : 0u;
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        uint32_t o[4];
-#pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            o[k] = f32x2_to_bf16x2(__uint_as_float(v[8 * i + 2 * k]), __uint_as_float(v[8 * i + 2 * k + 1]));
-                        if (p.vec) reinterpret_cast<uint4 *>(d)[i] = make_uint4(o[0], o[1], o[2], o[3]);
-                        else
-#pragma unroll
-                            for (int k = 0; k < 4; k++) {
-                                d[8 * i + 2 * k] = (uint16_t)o[k];
-                                d[8 * i + 2 * k + 1] = (uint16_t)(o[k] >> 16);
-                            }
-                    }
-                } else {
-                    uint32_t *d = reinterpret_cast<uint32_t *>(p.y) + (x.row0 + row) * p.ldy + col;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        if (p.vec) reinterpret_cast<uint4 *>(d)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                        else
-#pragma unroll
-                            for (int k = 0; k < 4; k++) d[4 * i + k] = v[4 * i + k];
+                        for (int e = 0; e < 2; e++) {
+                            const int r = r0 + 16 * h + 8 * e + (lane >> 2);
+                            const uint32_t u[8] = {v[2 * e], v[2 * e + 1], v[4 + 2 * e], v[5 + 2 * e],
+                                                   v[8 + 2 * e], v[9 + 2 * e], v[12 + 2 * e], v[13 + 2 * e]};
+                            if (r < x.n) put8(p, x.row0 + r, c0 + c + 8 * (lane & 3), u);
+                        }
                     }
                 }
             }
-            if (x.mat >= 0) {
+            if (real) {
                 tc::tc_fence_before();
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(tempty);
@@ -997,8 +1088,9 @@ extern "C" int k3c_mxfp4_mm_bwd(void *da, int da_dtype, int64_t ldda, const void
     p.atoms = W->atoms;
     p.atom_stride = W->atom_stride;
     p.NTL = (p.K + MB_N - 1) / MB_N;
-    CUtensorMap md, mw;
-    K3C_TRY(make_map3(&md, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dy, p.N, M, 1, lddy * 2, (uint64_t)lddy * 2 * M, 64, 32));
+    CUtensorMap md, md1, mw;
+    K3C_TRY(make_map3(&md, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dy, p.N, M, 1, lddy * 2, (uint64_t)lddy * 2 * M, 64, 128));
+    K3C_TRY(make_map3(&md1, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dy, p.N, M, 1, lddy * 2, (uint64_t)lddy * 2 * M, 64, 32));
     K3C_TRY(map_weights(&mw, W, MB_KB));
     static bool attr_of[64] = {};
     bool &attr = attr_of[cur_dev()];
@@ -1009,7 +1101,7 @@ extern "C" int k3c_mxfp4_mm_bwd(void *da, int da_dtype, int64_t ldda, const void
     const int64_t items = most_tiles(M, n_groups, MB_M) * p.NTL;
     K3C_TRY(check_items("mxfp4_mm_bwd", items));
     const int grid = (int)(items < sm_count() ? items : sm_count());
-    K3C_TRY_CUDA(launch_pdl(k_mx4_bwd, dim3(grid), dim3(MB_THREADS), MB_BYTES, s, md, mw, p));
+    K3C_TRY_CUDA(launch_pdl(k_mx4_bwd, dim3(grid), dim3(MB_THREADS), MB_BYTES, s, md, md1, mw, p));
     K3C_CHECK_LAUNCH();
     return check_waits("mxfp4_mm_bwd", p.err, s);
 }
