@@ -29,7 +29,7 @@ namespace k3c {
 
 namespace {
 
-constexpr int MX_GMAX = 1024;   // groups of a product
+constexpr int MX_GMAX = 512;    // groups of a product
 
 static __device__ int g_mx_err;
 
@@ -102,56 +102,58 @@ __global__ void __launch_bounds__(256) k_mx4_pack(uint8_t *codes, uint8_t *__res
 }
 
 // ------------------------------------------------------------------ work items
-// Groups own consecutive rows; an item is one row tile of one group x one column tile. tbase[g]
-// (shared memory) is the number of row tiles before group g.
+// Groups own consecutive rows; an item is one row tile of one group x one column tile.
 struct Item {
     int mat;         // matrix index, -1: none (the rows' results are zeros)
     int row0, n;     // first row, rows of the tile
     int nt;          // column tile
 };
 
-__device__ __forceinline__ void group_rows(const int *off, int g, int M, int &lo, int &hi) {
-    if (!off) {
-        lo = 0;
-        hi = M;
-        return;
-    }
-    lo = min(max(__ldg(off + g), 0), M);   // offsets outside the rows cannot leave them
-    hi = min(max(__ldg(off + g + 1), lo), M);
-}
+// The groups' rows and tiles, in shared memory: group g has rows first[g] .. max(first[g],
+// first[g+1]) - 1 and row tiles tile[g] .. tile[g+1] - 1.
+struct Plan {
+    int first[MX_GMAX + 1], tile[MX_GMAX + 1], warp_tot[32];
+};
 
-// tbase[0..G] by all THREADS of the block; returns the number of row tiles.
+// Filled by all THREADS of the block; returns the number of row tiles.
 template <int THREADS>
-__device__ int plan_tiles(int *tbase, int *warp_tot, const int *off, int G, int M, int tile) {
+__device__ int plan_tiles(Plan &pl, const int *off, int G, int M, int rows) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (!off) {
+        const int n = (M + rows - 1) / rows;
+        if (tid == 0) {
+            pl.first[0] = pl.tile[0] = 0;
+            pl.first[1] = M;
+            pl.tile[1] = n;
+        }
+        __syncthreads();
+        return n;
+    }
+    for (int g = tid; g <= G; g += THREADS) pl.first[g] = min(max(__ldg(off + g), 0), M);   // offsets cannot leave the rows
+    __syncthreads();
     int run = 0;
     for (int g0 = 0; g0 < G; g0 += THREADS) {
         const int g = g0 + tid;
-        int n = 0;
-        if (g < G) {
-            int lo, hi;
-            group_rows(off, g, M, lo, hi);
-            n = (hi - lo + tile - 1) / tile;
-        }
+        const int n = g < G ? (max(pl.first[g + 1] - pl.first[g], 0) + rows - 1) / rows : 0;
         int inc = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += v;
         }
-        if (lane == 31) warp_tot[warp] = inc;
+        if (lane == 31) pl.warp_tot[warp] = inc;
         __syncthreads();
         int pre = 0, all = 0;
 #pragma unroll
         for (int w = 0; w < THREADS / 32; w++) {
-            pre += w < warp ? warp_tot[w] : 0;
-            all += warp_tot[w];
+            pre += w < warp ? pl.warp_tot[w] : 0;
+            all += pl.warp_tot[w];
         }
-        if (g < G) tbase[g] = run + pre + inc - n;
+        if (g < G) pl.tile[g] = run + pre + inc - n;
         run += all;
         __syncthreads();
     }
-    if (tid == 0) tbase[G] = run;
+    if (tid == 0) pl.tile[G] = run;
     __syncthreads();
     return run;
 }
@@ -159,25 +161,31 @@ __device__ int plan_tiles(int *tbase, int *warp_tot, const int *off, int G, int 
 // Items of a group run through its row tiles first, RB of them at a time, so that the CTAs
 // working side by side share W tiles and a bounded set of A rows in L2.
 constexpr int MX_RB = 16;
-__device__ __forceinline__ Item item_of(int it, const int *tbase, const int *off, const int *mat_of, int n_mats, int G,
-                                        int M, int NTL, int tile) {
-    const int tt = it / NTL;
-    int g = 0, h = G;   // tbase[g] <= tt < tbase[h]
-    while (h - g > 1) {
-        const int c = (g + h) >> 1;
-        if (tbase[c] <= tt) g = c;
-        else h = c;
+__device__ __forceinline__ Item item_of(int it, const Plan &pl, const int *mat_of, int n_mats, int G, int NTL, int rows) {
+    int g = 0;
+    if (G > 1) {
+        const int tt = it / NTL;
+        int h = G;   // tile[g] <= tt < tile[h]
+        while (h - g > 1) {
+            const int c = (g + h) >> 1;
+            if (pl.tile[c] <= tt) g = c;
+            else h = c;
+        }
     }
-    const int i = it - tbase[g] * NTL, mt = tbase[g + 1] - tbase[g];
-    const int b = i / (MX_RB * NTL), mb = min(MX_RB, mt - MX_RB * b), r = i - b * MX_RB * NTL;
-    int lo, hi;
-    group_rows(off, g, M, lo, hi);
+    const int t0 = pl.tile[g], mt = pl.tile[g + 1] - t0;
+    int i = it - t0 * NTL, m = 0, mb = mt;
+    if (mt > MX_RB) {
+        const int b = i / (MX_RB * NTL);
+        m = MX_RB * b;
+        mb = min(MX_RB, mt - m);
+        i -= m * NTL;
+    }
     Item x;
-    x.nt = r / mb;
-    const int m = MX_RB * b + r % mb;
-    x.row0 = lo + m * tile;
-    x.n = min(tile, hi - x.row0);
-    const int mat = mat_of ? __ldg(mat_of + g) : (off ? g : 0);
+    x.nt = i / mb;
+    m += i - x.nt * mb;
+    x.row0 = pl.first[g] + m * rows;
+    x.n = min(rows, pl.first[g + 1] - x.row0);
+    const int mat = mat_of ? __ldg(mat_of + g) : g;
     x.mat = mat >= 0 && mat < n_mats ? mat : -1;
     return x;
 }
@@ -306,10 +314,10 @@ struct MmCfg {
     static constexpr uint32_t SFW = 2 * (4 + 4 * NA);     // TMEM columns of a stage's scales
     static constexpr uint32_t SF_COL = NT * NACC;
     static constexpr int BAR = 256;
-    static constexpr int BYTES = 1024 + STAGES * STAGE + BAR + MM_EPI * 2048 + (MX_GMAX + 1) * 4 + 64;
+    static constexpr int BYTES = 1024 + STAGES * STAGE + BAR + MM_EPI * 2048;
     static_assert(STAGE % 1024 == 0, "stage bases stay 1024-byte aligned");
     static_assert(SF_COL + STAGES * SFW <= 512, "TMEM columns");
-    static_assert(BYTES <= 227 * 1024, "one CTA per SM");
+    static_assert(BYTES + sizeof(Plan) + 64 <= 227 * 1024, "one CTA per SM");
     static_assert((2 * STAGES + 2 * NACC) * 8 + 4 <= BAR, "barriers");
 };
 
@@ -324,8 +332,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant_
     uint64_t *empty = full + C::STAGES, *tfull = empty + C::STAGES, *tempty = tfull + C::NACC;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tempty + C::NACC);
     uint8_t *stg_all = smem + C::STAGES * C::STAGE + C::BAR;
-    int *tbase = reinterpret_cast<int *>(stg_all + MM_EPI * 2048);
-    __shared__ int warp_tot[MM_THREADS / 32];
+    __shared__ Plan plan;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
@@ -347,10 +354,11 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant_
     tc::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     grid_dep_wait();   // everything read from here on may come from the kernel before
-    const int tiles = plan_tiles<MM_THREADS>(tbase, warp_tot, p.off, p.G, p.M, MM_M);
+    const int tiles = plan_tiles<MM_THREADS>(plan, p.off, p.G, p.M, MM_M);
     const int n_items = tiles * p.NTL;
     const int KB = (p.K + 255) / 256;
     const int KA = (p.K + 127) / 128;              // scale atoms along K
+    auto item = [&](int it) { return item_of(it, plan, p.mat_of, p.n_mats, p.G, p.NTL, MM_M); };
 
     if (warp == 0) {
         // ------------------------------------------------------------ copies
@@ -358,7 +366,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant_
             bool ok = tc::tc_check((tc::smem_u32(smem) & 1023) == 0, p.err, 80);
             uint32_t ki = 0, st = 0, ph = 0;
             for (int it = blockIdx.x; ok && it < n_items; it += gridDim.x) {
-                const Item x = item_of(it, tbase, p.off, p.mat_of, p.n_mats, p.G, p.M, p.NTL, MM_M);
+                const Item x = item(it);
                 if (x.mat < 0) continue;
                 const int boxes = (x.n + MM_ABOX - 1) / MM_ABOX;
                 const int arow = NT >= 128 ? x.nt * C::NA : x.nt / 2;         // W's 128-row atom
@@ -396,7 +404,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant_
             const uint64_t da0 = tc::desc_kmajor_sw128(tc::smem_u32(smem)), db0 = tc::desc_kmajor_sw128(tc::smem_u32(smem) + MM_A);
             const uint64_t dsf0 = tc::desc_sf_atom(tc::smem_u32(smem) + MM_A + C::B);
             for (int it = blockIdx.x; ok && it < n_items; it += gridDim.x) {
-                const Item x = item_of(it, tbase, p.off, p.mat_of, p.n_mats, p.G, p.M, p.NTL, MM_M);
+                const Item x = item(it);
                 if (x.mat < 0) continue;
                 if (!tc::mbar_wait(&tempty[a], aph, p.err, 83)) { ok = false; break; }
                 tc::tc_fence_after();
@@ -460,7 +468,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant_
         bool ok = true;
         auto next_item = [&](int &it, Item &x) {   // the first item from `it` on that has a matrix
             for (; it < n_items; it += gridDim.x) {
-                x = item_of(it, tbase, p.off, p.mat_of, p.n_mats, p.G, p.M, p.NTL, MM_M);
+                x = item(it);
                 if (x.mat >= 0) return;
             }
         };
@@ -531,7 +539,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant_
         uint32_t li = 0;
         bool alive = true;   // false after a wait gave up: the remaining results are NaN
         for (int it = blockIdx.x; it < n_items; it += gridDim.x) {
-            const Item x = item_of(it, tbase, p.off, p.mat_of, p.n_mats, p.G, p.M, p.NTL, MM_M);
+            const Item x = item(it);
             const int rows = min(32, x.n - 32 * q);
             uint32_t v[NC][32];
             bool ok = true;   // zeros of a group without a matrix stay zeros
@@ -572,21 +580,31 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant_
 // tiles (copied); the last two share their slots' numbers, and an MMA commit frees both. With
 // one ring for all three a slot was held through copy, widening and MMA, 3900 cycles for 1024
 // of MMAs: three slots' worth of them set the pace.
-constexpr int MB_M = 256;                        // rows per item: two accumulators share a widened W tile
-constexpr int MB_N = 256;                        // columns (W's in) per item
 constexpr int MB_KB = 64;                        // W rows per K block
-constexpr int MB_A = MB_M * 128;                 // dY: 256 rows x 64 bf16
-constexpr int MB_B = MB_N * MB_KB * 2;           // widened W: 4 blocks of 64 columns x 64 rows
-constexpr int MB_W = MB_KB * 128;                // packed W: 64 rows x 256 codes
-constexpr int MB_R = MB_W + 1024;                // and its two scale atoms
-constexpr int MB_RING = 3;
 constexpr int MB_GROUP = 8;                      // warps that widen one K block; two groups take turns
 constexpr int MB_EPI = 8;
 constexpr int MB_WIDE0 = 3, MB_EPI0 = MB_WIDE0 + 2 * MB_GROUP;   // warps: dY, MMA, W, widening, epilogue
 constexpr int MB_THREADS = 32 * (MB_EPI0 + MB_EPI);
-constexpr int MB_BYTES = 1024 + MB_RING * (MB_A + MB_B + MB_R) + 256;
-static_assert(MB_A % 1024 == 0 && MB_B % 1024 == 0 && MB_R % 1024 == 0, "slots stay 1024-byte aligned");
-static_assert(MB_BYTES + (MX_GMAX + 1) * 4 + 128 <= 227 * 1024, "one CTA per SM");
+// MT rows x NT columns (W's in) per item. 256 x 256: two accumulators of 128 rows share a widened
+// W tile, 1024 cycles of MMAs for it. 128 x 256: for groups of few rows, whose time is W's way
+// through the SM; the room goes to packed tiles in flight and a second accumulator. 128 x 128:
+// more items, when there are too few for every SM.
+template <int MT, int NT>
+struct MbCfg {
+    static constexpr int A = MT * 128;                       // dY: MT rows x 64 bf16
+    static constexpr int B = NT * MB_KB * 2;                 // widened W: NT/64 blocks of 64 columns x 64 rows
+    static constexpr int WB = NT / 2;                        // bytes of a packed W row
+    static constexpr int W = MB_KB * WB;
+    static constexpr int R = (W + NT / 128 * 512 + 1023) / 1024 * 1024;   // and its scale atoms
+    static constexpr int RING = NT == 256 ? 3 : 4;           // slots of dY and widened W
+    static constexpr int RAW = MT == 256 ? 3 : NT == 256 ? 8 : 15;        // slots of packed W
+    static constexpr int ACC = MT / 128 * NT;                // TMEM columns of an item
+    static constexpr int NACC = 512 / ACC < 2 ? 1 : 2;
+    static constexpr int BYTES = 1024 + RING * (A + B) + RAW * R + 512;
+    static_assert(A % 1024 == 0 && B % 1024 == 0, "slots stay 1024-byte aligned");
+    static_assert((3 * RING + 2 * RAW + 2 * NACC) * 8 + 4 <= 512, "barriers");
+    static_assert(BYTES + sizeof(Plan) + 64 <= 227 * 1024, "one CTA per SM");
+};
 
 // kind::f16: bf16 A (K-major) and B (N-major: transpose bit 16), fp32 accumulator, M = 128.
 __host__ __device__ constexpr uint32_t idesc_bf16_tb(uint32_t n) {
@@ -659,30 +677,35 @@ __device__ __forceinline__ void put8(const MxArgs &p, int64_t row, int col, cons
     }
 }
 
+template <int MT, int NT>
 __global__ void __launch_bounds__(MB_THREADS, 1) k_mx4_bwd(const __grid_constant__ CUtensorMap tmD,
                                                            const __grid_constant__ CUtensorMap tmD1,
                                                            const __grid_constant__ CUtensorMap tmW, MxArgs p) {
+    using C = MbCfg<MT, NT>;
     extern __shared__ uint8_t mb_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)mb_raw + 1023) & ~(uintptr_t)1023);
-    uint8_t *s_a = smem, *s_b = s_a + MB_RING * MB_A, *s_r = s_b + MB_RING * MB_B;
-    uint64_t *afull = reinterpret_cast<uint64_t *>(s_r + MB_RING * MB_R);
-    uint64_t *wide = afull + MB_RING, *empty = wide + MB_RING, *rfull = empty + MB_RING, *rempty = rfull + MB_RING;
-    uint64_t *tfull = rempty + MB_RING, *tempty = tfull + 1;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tempty + 1);
-    __shared__ int tbase[MX_GMAX + 1];
-    __shared__ int warp_tot[MB_THREADS / 32];
+    uint8_t *s_a = smem, *s_b = s_a + C::RING * C::A, *s_r = s_b + C::RING * C::B;
+    uint64_t *afull = reinterpret_cast<uint64_t *>(s_r + C::RAW * C::R);
+    uint64_t *wide = afull + C::RING, *empty = wide + C::RING, *rfull = empty + C::RING, *rempty = rfull + C::RAW;
+    uint64_t *tfull = rempty + C::RAW, *tempty = tfull + C::NACC;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tempty + C::NACC);
+    __shared__ Plan plan;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < MB_RING; i++) {
+        for (int i = 0; i < C::RING; i++) {
             tc::mbar_init(&afull[i], 1);
             tc::mbar_init(&wide[i], MB_GROUP);
             tc::mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < C::RAW; i++) {
             tc::mbar_init(&rfull[i], 1);
             tc::mbar_init(&rempty[i], MB_GROUP);
         }
-        tc::mbar_init(tfull, 1);
-        tc::mbar_init(tempty, MB_EPI);
+        for (int i = 0; i < C::NACC; i++) {
+            tc::mbar_init(&tfull[i], 1);
+            tc::mbar_init(&tempty[i], MB_EPI);
+        }
         tc::fence_mbar_init();
         tc::prefetch_tmap(&tmD);
         tc::prefetch_tmap(&tmW);
@@ -693,11 +716,11 @@ __global__ void __launch_bounds__(MB_THREADS, 1) k_mx4_bwd(const __grid_constant
     tc::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     grid_dep_wait();
-    const int tiles = plan_tiles<MB_THREADS>(tbase, warp_tot, p.off, p.G, p.M, MB_M);
+    const int tiles = plan_tiles<MB_THREADS>(plan, p.off, p.G, p.M, MT);
     const int n_items = tiles * p.NTL;
     const int KB = (p.N + MB_KB - 1) / MB_KB;      // contracted: W's rows
     const int KA = (p.K + 127) / 128;
-    auto item = [&](int it) { return item_of(it, tbase, p.off, p.mat_of, p.n_mats, p.G, p.M, p.NTL, MB_M); };
+    auto item = [&](int it) { return item_of(it, plan, p.mat_of, p.n_mats, p.G, p.NTL, MT); };
 
     if (warp == 0) {
         // ------------------------------------------------------------ dY copies
@@ -710,22 +733,22 @@ __global__ void __launch_bounds__(MB_THREADS, 1) k_mx4_bwd(const __grid_constant
                 const int boxes = (x.n + 31) / 32;
                 for (int kb = 0; kb < KB; kb++, n++) {
                     if (!tc::mbar_wait(&empty[st], ph, p.err, 91)) { ok = false; break; }
-                    uint8_t *sa = s_a + st * MB_A;
+                    uint8_t *sa = s_a + st * C::A;
                     tc::mbar_expect_tx(&afull[st], boxes * 32 * 128);
                     if (boxes >= 4) tc::tma_load_3d(sa, &tmD, &afull[st], kb * MB_KB, x.row0, 0);
-                    if (boxes == 8) tc::tma_load_3d(sa + 128 * 128, &tmD, &afull[st], kb * MB_KB, x.row0 + 128, 0);
+                    if (MT == 256 && boxes == 8) tc::tma_load_3d(sa + 128 * 128, &tmD, &afull[st], kb * MB_KB, x.row0 + 128, 0);
                     else
-                        for (int b = boxes & 4; b < boxes; b++)
+                        for (int b = boxes & 4; b < boxes; b++)   // the rest of a short tile
                             tc::tma_load_3d(sa + b * (32 * 128), &tmD1, &afull[st], kb * MB_KB, x.row0 + b * 32, 0);
-                    if (++st == MB_RING) {
+                    if (++st == C::RING) {
                         st = 0;
                         ph ^= 1u;
                     }
                 }
             }
             // no copy may still be landing when the CTA exits
-            for (uint32_t i = n > MB_RING ? n - MB_RING : 0; i < n; i++)
-                tc::mbar_wait(&afull[i % MB_RING], (i / MB_RING) & 1u, p.err, 92);
+            for (uint32_t i = n > C::RING ? n - C::RING : 0; i < n; i++)
+                tc::mbar_wait(&afull[i % C::RING], (i / C::RING) & 1u, p.err, 92);
         }
     } else if (warp == 2) {
         // ------------------------------------------------------------ W copies
@@ -735,88 +758,93 @@ __global__ void __launch_bounds__(MB_THREADS, 1) k_mx4_bwd(const __grid_constant
             for (int it = blockIdx.x; ok && it < n_items; it += gridDim.x) {
                 const Item x = item(it);
                 if (x.mat < 0) continue;
-                const uint32_t sfb = min(2, KA - 2 * x.nt) * 512;
-                const uint8_t *wsf = p.atoms + (size_t)x.mat * p.atom_stride + (size_t)(2 * x.nt) * 512;
+                const uint32_t sfb = min(NT / 128, KA - NT / 128 * x.nt) * 512;
+                const uint8_t *wsf = p.atoms + (size_t)x.mat * p.atom_stride + (size_t)(NT / 128 * x.nt) * 512;
                 for (int kb = 0; kb < KB; kb++, n++) {
                     if (!tc::mbar_wait(&rempty[st], ph, p.err, 93)) { ok = false; break; }
-                    uint8_t *sw = s_r + st * MB_R;
-                    tc::mbar_expect_tx(&rfull[st], MB_W + sfb);
-                    tc::tma_load_3d(sw, &tmW, &rfull[st], x.nt * 128, kb * MB_KB, x.mat);
-                    tc::bulk_load(sw + MB_W, wsf + (size_t)(kb / 2) * KA * 512, sfb, &rfull[st]);
-                    if (++st == MB_RING) {
+                    uint8_t *sw = s_r + st * C::R;
+                    tc::mbar_expect_tx(&rfull[st], C::W + sfb);
+                    tc::tma_load_3d(sw, &tmW, &rfull[st], x.nt * C::WB, kb * MB_KB, x.mat);
+                    tc::bulk_load(sw + C::W, wsf + (size_t)(kb / 2) * KA * 512, sfb, &rfull[st]);
+                    if (++st == C::RAW) {
                         st = 0;
                         ph ^= 1u;
                     }
                 }
             }
-            for (uint32_t i = n > MB_RING ? n - MB_RING : 0; i < n; i++)
-                tc::mbar_wait(&rfull[i % MB_RING], (i / MB_RING) & 1u, p.err, 94);
+            for (uint32_t i = n > C::RAW ? n - C::RAW : 0; i < n; i++)
+                tc::mbar_wait(&rfull[i % C::RAW], (i / C::RAW) & 1u, p.err, 94);
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA
         if (elect_one()) {
-            uint32_t st = 0, ph = 0, tph = 1;
+            uint32_t st = 0, ph = 0, a = 0, aph = 1;
             bool ok = true;
-            constexpr uint32_t idesc = idesc_bf16_tb(MB_N);
+            constexpr uint32_t idesc = idesc_bf16_tb(NT);
             const uint64_t da0 = tc::desc_kmajor_sw128(tc::smem_u32(s_a)), db0 = desc_nmajor_sw128(tc::smem_u32(s_b));
             for (int it = blockIdx.x; ok && it < n_items; it += gridDim.x) {
                 const Item x = item(it);
                 if (x.mat < 0) continue;
-                if (!tc::mbar_wait(tempty, tph, p.err, 95)) { ok = false; break; }
-                tph ^= 1u;
+                if (!tc::mbar_wait(&tempty[a], aph, p.err, 95)) { ok = false; break; }
                 tc::tc_fence_after();
-                const bool two = x.n > 128;
+                const bool two = MT == 256 && x.n > 128;
+                const uint32_t d = tmem + a * C::ACC;
                 for (int kb = 0; kb < KB; kb++) {
                     if (!tc::mbar_wait(&afull[st], ph, p.err, 96) || !tc::mbar_wait(&wide[st], ph, p.err, 97)) { ok = false; break; }
                     tc::tc_fence_after();
-                    const uint64_t da = da0 + st * (MB_A >> 4), db = db0 + st * (MB_B >> 4);
+                    const uint64_t da = da0 + st * (C::A >> 4), db = db0 + st * (C::B >> 4);
 #pragma unroll
-                    for (int k = 0; k < 4; k++) tc_mma_bf16(tmem, da + 2 * k, db + 128 * k, idesc, (kb | k) != 0);
+                    for (int k = 0; k < 4; k++) tc_mma_bf16(d, da + 2 * k, db + 128 * k, idesc, (kb | k) != 0);
                     if (two) {
 #pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            tc_mma_bf16(tmem + MB_N, da + 1024 + 2 * k, db + 128 * k, idesc, (kb | k) != 0);
+                        for (int k = 0; k < 4; k++) tc_mma_bf16(d + NT, da + 1024 + 2 * k, db + 128 * k, idesc, (kb | k) != 0);
                     }
                     tc::tc_commit(&empty[st]);
-                    if (++st == MB_RING) {
+                    if (++st == C::RING) {
                         st = 0;
                         ph ^= 1u;
                     }
                 }
-                if (ok) tc::tc_commit(tfull);
+                if (ok) tc::tc_commit(&tfull[a]);
+                if (++a == C::NACC) {
+                    a = 0;
+                    aph ^= 1u;
+                }
             }
         }
     } else if (warp >= MB_WIDE0 && warp < MB_EPI0) {
         // ------------------------------------------------------------ widening
         const int w4 = (warp - MB_WIDE0) % MB_GROUP;
         const uint32_t turn = (warp - MB_WIDE0) / MB_GROUP;
-        uint32_t n = 0, st = 0, ph = 1;            // st, ph: both rings' slot and the parity of its last release
+        uint32_t n = 0, st = 0, ph = 1, rt = 0, rph = 0;   // slot and awaited parity of the two rings
         bool ok = true;
         for (int it = blockIdx.x; ok && it < n_items; it += gridDim.x) {
             const Item x = item(it);
             if (x.mat < 0) continue;
             for (int kb = 0; ok && kb < KB; kb++, n++) {
                 if ((n & 1u) == turn) {
-                    ok = __all_sync(0xFFFFFFFFu, tc::mbar_wait(&rfull[st], ph ^ 1u, p.err, 98));
+                    ok = __all_sync(0xFFFFFFFFu, tc::mbar_wait(&rfull[rt], rph, p.err, 98));
                     if (!ok) break;
-                    // a lane widens 2 x 32 codes: groups g and g + 4 of W row r (eight lanes touch
-                    // eight rows: the swizzle spreads them over the banks)
-                    const uint8_t *sw = s_r + st * MB_R;
+                    // a lane widens 32 codes of W row r in each 128 columns: groups g and g + 4 (eight
+                    // lanes touch eight rows: the swizzle spreads them over the banks)
+                    constexpr int GH = NT / 128;
+                    const uint8_t *sw = s_r + rt * C::R;
                     const int r = 8 * w4 + (lane & 7), g = lane >> 3;
-                    uint4 c[2];
-                    uint32_t s[2];
+                    uint4 c[GH];
+                    uint32_t s[GH];
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        c[i] = *reinterpret_cast<const uint4 *>(sw + r * 128 + 16 * ((g + 4 * i) ^ (r & 7)));
-                        s[i] = sw[MB_W + i * 512 + sf_byte((kb & 1) * 64 + r, g)];
+                    for (int i = 0; i < GH; i++) {
+                        const int at = NT == 256 ? (g + 4 * i) ^ (r & 7) : g ^ ((r >> 1) & 3);   // 128- and 64-byte swizzle
+                        c[i] = *reinterpret_cast<const uint4 *>(sw + r * C::WB + 16 * at);
+                        s[i] = sw[C::W + i * 512 + sf_byte((kb & 1) * 64 + r, g)];
                     }
                     __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(&rempty[st]);
+                    if (lane == 0) tc::mbar_arrive(&rempty[rt]);
                     ok = __all_sync(0xFFFFFFFFu, tc::mbar_wait(&empty[st], ph, p.err, 99));
                     if (!ok) break;
-                    uint8_t *sb = s_b + st * MB_B;
+                    uint8_t *sb = s_b + st * C::B;
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
+                    for (int i = 0; i < GH; i++) {
                         const uint32_t e = min(s[i], 128u) + 126u;    // 2^(min(byte, 128) - 1)
                         const uint32_t f1 = e << 7 | e << 23;
                         const uint32_t cw[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
@@ -843,9 +871,13 @@ __global__ void __launch_bounds__(MB_THREADS, 1) k_mx4_bwd(const __grid_constant
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(&wide[st]);
                 }
-                if (++st == MB_RING) {
+                if (++st == C::RING) {
                     st = 0;
                     ph ^= 1u;
+                }
+                if (++rt == C::RAW) {
+                    rt = 0;
+                    rph ^= 1u;
                 }
             }
         }
@@ -853,24 +885,25 @@ __global__ void __launch_bounds__(MB_THREADS, 1) k_mx4_bwd(const __grid_constant
         // ------------------------------------------------------------ epilogue
         // A store covers 8 rows x 64 bytes (bf16); with a row per lane it was 32 rows x 16, and
         // the accumulators stayed taken for 12000 cycles an item instead of EPI_CYCLES.
-        const int q = warp & 3, acc = (warp - MB_EPI0) >> 2;   // TMEM lane quadrant, accumulator
-        const uint32_t taddr = tmem + ((uint32_t)(32 * q) << 16) + acc * MB_N;
-        uint32_t tph = 0;
+        const int q = warp & 3, half = (warp - MB_EPI0) >> 2;   // TMEM lane quadrant; accumulator or half of the columns
+        const uint32_t lanes = (uint32_t)(32 * q) << 16;
+        uint32_t a = 0, aph = 0;
         bool alive = true;
         for (int it = blockIdx.x; it < n_items; it += gridDim.x) {
             const Item x = item(it);
-            const int r0 = 128 * acc + 32 * q;                         // the warp's first row
-            const int c0 = x.nt * MB_N, cols = min(MB_N, p.K - c0);    // a multiple of 32
+            const int r0 = (MT == 256 ? 128 * half : 0) + 32 * q;              // the warp's first row
+            const int first = MT == 256 ? 0 : half * (NT / 2);                 // and its columns of the tile
+            const int c0 = x.nt * NT, last = min(MT == 256 ? NT : first + NT / 2, p.K - c0);   // a multiple of 32
+            const uint32_t taddr = tmem + lanes + a * C::ACC + (MT == 256 ? half * NT : 0);
             const bool real = x.mat >= 0;
             if (real) {
-                alive = alive && tc::mbar_wait(tfull, tph, p.err, 100);
-                tph ^= 1u;
+                alive = alive && tc::mbar_wait(&tfull[a], aph, p.err, 100);
                 __syncwarp();
                 tc::tc_fence_after();
             }
             if (r0 < x.n) {
 #pragma unroll 2
-                for (int c = 0; c < cols; c += 32) {
+                for (int c = first; c < last; c += 32) {
 #pragma unroll
                     for (int h = 0; h < 2; h++) {                      // rows r0 + 16h ..
                         uint32_t v[16];
@@ -894,7 +927,11 @@ __global__ void __launch_bounds__(MB_THREADS, 1) k_mx4_bwd(const __grid_constant
             if (real) {
                 tc::tc_fence_before();
                 __syncwarp();
-                if (lane == 0) tc::mbar_arrive(tempty);
+                if (lane == 0) tc::mbar_arrive(&tempty[a]);
+                if (++a == C::NACC) {
+                    a = 0;
+                    aph ^= 1u;
+                }
             }
         }
     }
@@ -925,10 +962,19 @@ int check_mat(const char *what, const k3c_mxfp4_mat *W, int M, const int *off, i
     return K3C_OK;
 }
 
-int map_weights(CUtensorMap *m, const k3c_mxfp4_mat *W, int box_rows) {
+// Boxes of box_bytes (128 or 64: the swizzle) x box_rows of the packed matrices.
+int map_weights(CUtensorMap *m, const k3c_mxfp4_mat *W, int box_bytes, int box_rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return set_error(K3C_ECUDA, "mxfp4: cuTensorMapEncodeTiled unavailable");
     const size_t stride = W->n_mats > 1 ? W->code_stride : (size_t)W->rows * (W->in / 2);
-    return make_map3(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, W->codes, W->in / 2, W->rows, W->n_mats, W->in / 2,
-                     (stride + 15) / 16 * 16, 128, box_rows);
+    cuuint64_t dims[3] = {(cuuint64_t)W->in / 2, (cuuint64_t)W->rows, (cuuint64_t)W->n_mats};
+    cuuint64_t strides[2] = {(cuuint64_t)W->in / 2, (cuuint64_t)stride};
+    cuuint32_t box[3] = {(cuuint32_t)box_bytes, (cuuint32_t)box_rows, 1}, es[3] = {1, 1, 1};
+    CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t *>(W->codes), dims, strides, box, es,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(K3C_ECUDA, "mxfp4: tensor map encode failed (%d)", (int)r);
+    return K3C_OK;
 }
 
 int err_slot(int **err) {
@@ -973,6 +1019,28 @@ int launch_mm(const CUtensorMap &ma, const CUtensorMap &ma1, const CUtensorMap &
     K3C_TRY(check_items("mxfp4_mm", items));
     const int grid = (int)(items < sm_count() ? items : sm_count());
     K3C_TRY_CUDA(launch_pdl(k_mx4_mm<NT>, dim3(grid), dim3(MM_THREADS), MmCfg<NT>::BYTES, s, ma, ma1, mw, p));
+    K3C_CHECK_LAUNCH();
+    return K3C_OK;
+}
+
+template <int MT, int NT>
+int launch_bwd(MxArgs p, const k3c_mxfp4_mat *W, const void *dy, int64_t lddy, cudaStream_t s) {
+    using C = MbCfg<MT, NT>;
+    CUtensorMap md, md1, mw;
+    K3C_TRY(make_map3(&md, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dy, p.N, p.M, 1, lddy * 2, (uint64_t)lddy * 2 * p.M, 64, 128));
+    K3C_TRY(make_map3(&md1, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dy, p.N, p.M, 1, lddy * 2, (uint64_t)lddy * 2 * p.M, 64, 32));
+    K3C_TRY(map_weights(&mw, W, C::WB, MB_KB));
+    static bool attr_of[64] = {};
+    bool &attr = attr_of[cur_dev()];
+    if (!attr) {
+        K3C_TRY_CUDA(cudaFuncSetAttribute(k_mx4_bwd<MT, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES));
+        attr = true;
+    }
+    p.NTL = (p.K + NT - 1) / NT;
+    const int64_t items = most_tiles(p.M, p.G, MT) * p.NTL;
+    K3C_TRY(check_items("mxfp4_mm_bwd", items));
+    const int grid = (int)(items < sm_count() ? items : sm_count());
+    K3C_TRY_CUDA(launch_pdl(k_mx4_bwd<MT, NT>, dim3(grid), dim3(MB_THREADS), C::BYTES, s, md, md1, mw, p));
     K3C_CHECK_LAUNCH();
     return K3C_OK;
 }
@@ -1054,7 +1122,7 @@ extern "C" int k3c_mxfp4_mm(void *y, int y_dtype, int64_t ldy, const uint8_t *a,
     CUtensorMap ma, ma1, mw;
     K3C_TRY(make_map3(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, a, p.K / 2, M, 1, p.K / 2, (uint64_t)(p.K / 2) * M, 128, MM_M));
     K3C_TRY(make_map3(&ma1, CU_TENSOR_MAP_DATA_TYPE_UINT8, a, p.K / 2, M, 1, p.K / 2, (uint64_t)(p.K / 2) * M, 128, MM_ABOX));
-    K3C_TRY(map_weights(&mw, W, nt));
+    K3C_TRY(map_weights(&mw, W, 128, nt));
     if (nt == 256) K3C_TRY(launch_mm<256>(ma, ma1, mw, p, s));
     else if (nt == 128) K3C_TRY(launch_mm<128>(ma, ma1, mw, p, s));
     else K3C_TRY(launch_mm<64>(ma, ma1, mw, p, s));
@@ -1087,21 +1155,13 @@ extern "C" int k3c_mxfp4_mm_bwd(void *da, int da_dtype, int64_t ldda, const void
     p.n_mats = W->n_mats;
     p.atoms = W->atoms;
     p.atom_stride = W->atom_stride;
-    p.NTL = (p.K + MB_N - 1) / MB_N;
-    CUtensorMap md, md1, mw;
-    K3C_TRY(make_map3(&md, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dy, p.N, M, 1, lddy * 2, (uint64_t)lddy * 2 * M, 64, 128));
-    K3C_TRY(make_map3(&md1, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dy, p.N, M, 1, lddy * 2, (uint64_t)lddy * 2 * M, 64, 32));
-    K3C_TRY(map_weights(&mw, W, MB_KB));
-    static bool attr_of[64] = {};
-    bool &attr = attr_of[cur_dev()];
-    if (!attr) {
-        K3C_TRY_CUDA(cudaFuncSetAttribute(k_mx4_bwd, cudaFuncAttributeMaxDynamicSharedMemorySize, MB_BYTES));
-        attr = true;
-    }
-    const int64_t items = most_tiles(M, n_groups, MB_M) * p.NTL;
-    K3C_TRY(check_items("mxfp4_mm_bwd", items));
-    const int grid = (int)(items < sm_count() ? items : sm_count());
-    K3C_TRY_CUDA(launch_pdl(k_mx4_bwd, dim3(grid), dim3(MB_THREADS), MB_BYTES, s, md, md1, mw, p));
-    K3C_CHECK_LAUNCH();
+    // The largest tile whose items still give every SM one; 256 rows only if the groups have more
+    // than 128 on average.
+    auto enough = [&](int mt, int nt) {
+        return (off ? most_tiles(M, n_groups, mt) : (M + mt - 1) / mt) * ((p.K + nt - 1) / nt) >= sm_count();
+    };
+    if (M / n_groups > 128 && enough(256, 256)) K3C_TRY((launch_bwd<256, 256>(p, W, dy, lddy, s)));
+    else if (enough(128, 256)) K3C_TRY((launch_bwd<128, 256>(p, W, dy, lddy, s)));
+    else K3C_TRY((launch_bwd<128, 128>(p, W, dy, lddy, s)));
     return check_waits("mxfp4_mm_bwd", p.err, s);
 }

@@ -163,7 +163,8 @@ def test_mm(k3, dev, M, N, K, out):
 
 
 @pytest.mark.parametrize("out", ["f32", "bf16"])
-@pytest.mark.parametrize("M,N,K", [m for m in DENSE if m[1] % 8 == 0])
+@pytest.mark.parametrize("M,N,K", [m for m in DENSE if m[1] % 8 == 0]
+                         + [(4000, 72, 2592), (100, 200, 37920), (300, 136, 19232), (2200, 4096, 64)])
 def test_mm_bwd(k3, dev, M, N, K, out):
     import torch
     W, w = matrices(k3, dev, 7, 1, N, K)
@@ -178,11 +179,11 @@ def test_mm_bwd(k3, dev, M, N, K, out):
 
 # rows per group: empty groups at both ends and in the middle, groups that end inside a tile, one
 # row, several tiles
-GROUPS = [[0], [1], [0, 0, 5, 0], [1] * 9, [130, 0, 1, 257, 32], [0, 40, 33, 128, 129, 1, 0, 300, 0], [2300, 1]]
+GROUPS = [[700, 0, 900, 1300] + [300] * 30, [0], [1], [0, 0, 5, 0], [1] * 9, [130, 0, 1, 257, 32], [0, 40, 33, 128, 129, 1, 0, 300, 0], [2300, 1]]
 
 
 @pytest.mark.parametrize("N,K", [(64, 32), (200, 416), (520, 1056)])
-@pytest.mark.parametrize("sizes", GROUPS, ids=lambda s: "-".join(map(str, s)))
+@pytest.mark.parametrize("sizes", GROUPS, ids=lambda s: "-".join(map(str, s[:8])))
 def test_grouped_products(k3, dev, sizes, N, K):
     """Both products over ragged groups; rows behind the last group stay as they were."""
     import torch
