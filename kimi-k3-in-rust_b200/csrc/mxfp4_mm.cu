@@ -321,6 +321,90 @@ struct MmCfg {
     static_assert((2 * STAGES + 2 * NACC) * 8 + 4 <= BAR, "barriers");
 };
 
+// A's scales of every K block of this CTA's items, by one warp. Lane i fetches the bytes of rows i,
+// 32+i, 64+i and 96+i and stores the four rows' words of each atom as one 16-byte piece (sf_byte's
+// order). MM_KS K blocks are fetched at a time, while the MM_KS before them are stored, across
+// items. The stores become visible to tcgen05.cp by a proxy fence of the thread that waits on
+// `full`: one here would wait for the fetches in flight. sf: the scales' place in stage 0; item(it)
+// gives the rows of this CTA.
+template <int STAGES, typename ItemFn>
+__device__ __forceinline__ void a_scales(const MxArgs &p, int n_items, const ItemFn &item, uint8_t *sf0, int stage_bytes,
+                                         uint64_t *full, uint64_t *empty, int KB, int it0, int step) {
+    const int lane = threadIdx.x & 31;
+    const int SR = p.K / 32;
+    const int wide = SR % 16 == 0 && ((uintptr_t)p.as & 15) == 0;
+    const uint8_t *as_end = p.as + (size_t)p.M * SR;
+    uint32_t tail = 0;   // the bytes of the array's last word, if it is no whole one
+    for (const uint8_t *c = reinterpret_cast<const uint8_t *>((uintptr_t)as_end & ~(uintptr_t)3); c < as_end; c++)
+        tail |= (uint32_t)__ldg(c) << (8 * ((uintptr_t)c & 3));
+    uint32_t st = 0, ph = 1, w[4][2 * MM_KS];
+    bool ok = true;
+    auto next_item = [&](int &it, Item &x) {   // the first item from `it` on that has a matrix
+        for (; it < n_items; it += step) {
+            x = item(it);
+            if (x.mat >= 0) return;
+        }
+    };
+    auto fetch = [&](uint32_t (&v)[4][2 * MM_KS], const Item &x, int k0) {
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+#pragma unroll
+            for (int i = 0; i < 2 * MM_KS; i++) v[q][i] = 0x7F7F7F7Fu;   // rows past the tile, groups past K: scale 1
+            if (32 * q + lane < x.n) {
+                const uint8_t *s = p.as + (size_t)(x.row0 + 32 * q + lane) * SR + 8 * k0;
+                if (wide) {   // SR is a multiple of 16: two K blocks at a time, all of them inside the row
+#pragma unroll
+                    for (int h = 0; h < MM_KS / 2; h++)
+                        if (k0 + 2 * h < KB) {
+                            const uint4 u = __ldg(reinterpret_cast<const uint4 *>(s + 16 * h));
+                            v[q][4 * h] = u.x;
+                            v[q][4 * h + 1] = u.y;
+                            v[q][4 * h + 2] = u.z;
+                            v[q][4 * h + 3] = u.w;
+                        }
+                } else {
+                    scales_at<2 * MM_KS>(v[q], s, SR - 8 * k0, p.atoms, as_end, tail);
+                }
+            }
+        }
+    };
+    int it = it0, k0 = 0;
+    Item x = {};
+    next_item(it, x);
+    if (it < n_items) fetch(w, x, 0);
+    while (ok && it < n_items) {
+        uint32_t nx[4][2 * MM_KS] = {};
+        const int kn = min(MM_KS, KB - k0);
+        k0 += MM_KS;
+        if (k0 >= KB) {
+            k0 = 0;
+            it += step;
+            next_item(it, x);
+        }
+        if (it < n_items) fetch(nx, x, k0);
+#pragma unroll
+        for (int e = 0; e < MM_KS; e++) {
+            if (!ok || e >= kn) continue;
+            ok = __all_sync(0xFFFFFFFFu, tc::mbar_wait(&empty[st], ph, p.err, 85));   // the warp gives up together
+            if (!ok) continue;
+            uint8_t *sf = sf0 + st * stage_bytes;
+            *reinterpret_cast<uint4 *>(sf + 16 * lane) = make_uint4(w[0][2 * e], w[1][2 * e], w[2][2 * e], w[3][2 * e]);
+            *reinterpret_cast<uint4 *>(sf + 512 + 16 * lane) =
+                make_uint4(w[0][2 * e + 1], w[1][2 * e + 1], w[2][2 * e + 1], w[3][2 * e + 1]);
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&full[st]);
+            if (++st == STAGES) {
+                st = 0;
+                ph ^= 1u;
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+#pragma unroll
+            for (int i = 0; i < 2 * MM_KS; i++) w[q][i] = nx[q][i];
+    }
+}
+
 template <int NT>
 __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant__ CUtensorMap tmA,
                                                           const __grid_constant__ CUtensorMap tmA1,
@@ -452,84 +536,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant_
             }
         }
     } else if (warp == 2) {
-        // ------------------------------------------------------------ A's scales
-        // Lane i fetches the scale bytes of rows i, 32+i, 64+i and 96+i and stores the four rows'
-        // words of each atom as one 16-byte piece (sf_byte's order). MM_KS K blocks are fetched
-        // at a time, while the MM_KS before them are stored, across items. The stores become
-        // visible to tcgen05.cp by the MMA thread's proxy fence: one here would wait for the
-        // fetches in flight.
-        const int SR = p.K / 32;
-        const int wide = SR % 16 == 0 && ((uintptr_t)p.as & 15) == 0;
-        const uint8_t *as_end = p.as + (size_t)p.M * SR;
-        uint32_t tail = 0;   // the bytes of the array's last word, if it is no whole one
-        for (const uint8_t *c = reinterpret_cast<const uint8_t *>((uintptr_t)as_end & ~(uintptr_t)3); c < as_end; c++)
-            tail |= (uint32_t)__ldg(c) << (8 * ((uintptr_t)c & 3));
-        uint32_t st = 0, ph = 1, w[4][2 * MM_KS];
-        bool ok = true;
-        auto next_item = [&](int &it, Item &x) {   // the first item from `it` on that has a matrix
-            for (; it < n_items; it += gridDim.x) {
-                x = item(it);
-                if (x.mat >= 0) return;
-            }
-        };
-        auto fetch = [&](uint32_t (&v)[4][2 * MM_KS], const Item &x, int k0) {
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-#pragma unroll
-                for (int i = 0; i < 2 * MM_KS; i++) v[q][i] = 0x7F7F7F7Fu;   // rows past the tile, groups past K: scale 1
-                if (32 * q + lane < x.n) {
-                    const uint8_t *s = p.as + (size_t)(x.row0 + 32 * q + lane) * SR + 8 * k0;
-                    if (wide) {   // SR is a multiple of 16: two K blocks at a time, all of them inside the row
-#pragma unroll
-                        for (int h = 0; h < MM_KS / 2; h++)
-                            if (k0 + 2 * h < KB) {
-                                const uint4 u = __ldg(reinterpret_cast<const uint4 *>(s + 16 * h));
-                                v[q][4 * h] = u.x;
-                                v[q][4 * h + 1] = u.y;
-                                v[q][4 * h + 2] = u.z;
-                                v[q][4 * h + 3] = u.w;
-                            }
-                    } else {
-                        scales_at<2 * MM_KS>(v[q], s, SR - 8 * k0, p.atoms, as_end, tail);
-                    }
-                }
-            }
-        };
-        int it = blockIdx.x, k0 = 0;
-        Item x = {};
-        next_item(it, x);
-        if (it < n_items) fetch(w, x, 0);
-        while (ok && it < n_items) {
-            uint32_t nx[4][2 * MM_KS] = {};
-            const int kn = min(MM_KS, KB - k0);
-            k0 += MM_KS;
-            if (k0 >= KB) {
-                k0 = 0;
-                it += gridDim.x;
-                next_item(it, x);
-            }
-            if (it < n_items) fetch(nx, x, k0);
-#pragma unroll
-            for (int e = 0; e < MM_KS; e++) {
-                if (!ok || e >= kn) continue;
-                ok = __all_sync(0xFFFFFFFFu, tc::mbar_wait(&empty[st], ph, p.err, 85));   // the warp gives up together
-                if (!ok) continue;
-                uint8_t *sf = smem + st * C::STAGE + MM_A + C::B;
-                *reinterpret_cast<uint4 *>(sf + 16 * lane) = make_uint4(w[0][2 * e], w[1][2 * e], w[2][2 * e], w[3][2 * e]);
-                *reinterpret_cast<uint4 *>(sf + 512 + 16 * lane) =
-                    make_uint4(w[0][2 * e + 1], w[1][2 * e + 1], w[2][2 * e + 1], w[3][2 * e + 1]);
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&full[st]);
-                if (++st == C::STAGES) {
-                    st = 0;
-                    ph ^= 1u;
-                }
-            }
-#pragma unroll
-            for (int q = 0; q < 4; q++)
-#pragma unroll
-                for (int i = 0; i < 2 * MM_KS; i++) w[q][i] = nx[q][i];
-        }
+        a_scales<C::STAGES>(p, n_items, item, smem + MM_A + C::B, C::STAGE, full, empty, KB, blockIdx.x, gridDim.x);
     } else if (warp >= 4) {
         // ------------------------------------------------------------ epilogue
         const int q = warp & 3, half = (warp - 4) >> 2;   // TMEM lane quadrant, half of the columns
@@ -573,6 +580,251 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant_
     __syncthreads();
     tc::tc_fence_after();
     if (warp == 1) tc::tmem_dealloc(tmem, 512);
+}
+
+// ------------------------------------------------------------------ two CTAs on one tile
+// k_mx4_mm on 256 rows x 256 columns per pair of CTAs (cta_group::2): each holds its 128 rows of A
+// and its 128 rows of W, and the MMA reads both halves of W, so an SM fetches 32 KB of codes per
+// 256 x 256 x 128 products instead of 48: at 8192 x 7168 x 7168 those fetches from L2 set the
+// one-CTA kernel's pace (PAIR_FIGURES). W's scales of all 256 columns are in both CTAs.
+// The pair's first CTA issues all MMAs. Its partner's warp 1 passes each filled stage on: it waits
+// for the local copies, fences A's scales and arrives on pfull in the first CTA. MMA commits free
+// the stage in both.
+struct PrCfg {
+    static constexpr int B = 128 * 128;
+    static constexpr int SF = 1024 + 2048;
+    static constexpr int STAGE = MM_A + B + SF;
+    static constexpr int STAGES = 5;
+    static constexpr uint32_t SFW = 24, SF_COL = 256;
+    static constexpr int BYTES = 1024 + STAGES * STAGE + 256 + MM_EPI * 2048;
+    static_assert(STAGE % 1024 == 0, "stage bases stay 1024-byte aligned");
+    static_assert(SF_COL + STAGES * SFW <= 512, "TMEM columns");
+    static_assert(BYTES + sizeof(Plan) + 64 <= 227 * 1024, "one CTA per SM");
+};
+
+__device__ __forceinline__ void mbar_arrive_cta(uint64_t *bar, uint32_t cta) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(tc::dsmem_addr(tc::smem_u32(bar), cta))
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t *slot, uint32_t ncols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(slot)), "r"(ncols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t base, uint32_t ncols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(ncols) : "memory");
+}
+// Arrives on *bar of both CTAs once this thread's earlier tcgen05 operations have completed.
+__device__ __forceinline__ void tc_commit_pair(uint64_t *bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            tc::smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+__device__ __forceinline__ void tc_cp_sf_pair(uint32_t col, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(col), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void tc_mma_mx4_pair(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sfa,
+                                                uint32_t sfb, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d),
+        "l"(da), "l"(db), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)
+        : "memory");
+}
+// idesc_mxf4 with M = 256 (the pair's rows).
+__host__ __device__ constexpr uint32_t idesc_mxf4_pair(uint32_t n, uint32_t sf_id) {
+    return (sf_id << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((256u >> 4) << 24) | (sf_id << 29);
+}
+
+__global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm_pair(const __grid_constant__ CUtensorMap tmA,
+                                                               const __grid_constant__ CUtensorMap tmA1,
+                                                               const __grid_constant__ CUtensorMap tmW, MxArgs p) {
+    using C = PrCfg;
+    extern __shared__ uint8_t pr_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)pr_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::STAGES * C::STAGE);
+    uint64_t *pfull = full + C::STAGES, *empty = pfull + C::STAGES, *tfull = empty + C::STAGES, *tempty = tfull + 1;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tempty + 1);
+    uint8_t *stg_all = smem + C::STAGES * C::STAGE + 256;
+    __shared__ Plan plan;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = tc::cluster_ctarank();
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::STAGES; i++) {
+            tc::mbar_init(&full[i], 2);
+            tc::mbar_init(&pfull[i], 1);
+            tc::mbar_init(&empty[i], 1);
+        }
+        tc::mbar_init(tfull, 1);
+        tc::mbar_init(tempty, 2 * MM_EPI);
+        tc::fence_mbar_init();
+        tc::prefetch_tmap(&tmA);
+        tc::prefetch_tmap(&tmW);
+    }
+    if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::cluster_sync();   // both CTAs' barriers and TMEM are there
+    tc::tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    grid_dep_wait();
+    const int tiles = plan_tiles<MM_THREADS>(plan, p.off, p.G, p.M, 2 * MM_M);
+    const int n_items = tiles * p.NTL;
+    const int KB = (p.K + 255) / 256, KA = (p.K + 127) / 128;
+    const int it0 = blockIdx.x >> 1, step = gridDim.x >> 1;
+    auto pair_item = [&](int it) { return item_of(it, plan, p.mat_of, p.n_mats, p.G, p.NTL, 2 * MM_M); };
+    auto item = [&](int it) {   // this CTA's rows of the pair's item
+        Item x = pair_item(it);
+        x.row0 += rank * MM_M;
+        x.n = min(max(x.n - (int)rank * MM_M, 0), MM_M);
+        return x;
+    };
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ copies
+        if (elect_one()) {
+            bool ok = tc::tc_check((tc::smem_u32(smem) & 1023) == 0, p.err, 110);
+            uint32_t ki = 0, st = 0, ph = 1;
+            for (int it = it0; ok && it < n_items; it += step) {
+                const Item x = item(it);
+                if (x.mat < 0) continue;
+                const int boxes = (x.n + MM_ABOX - 1) / MM_ABOX;
+                const int atoms = min(2, (p.N + 127) / 128 - 2 * x.nt);
+                const uint8_t *wsf = p.atoms + (size_t)x.mat * p.atom_stride + (size_t)(2 * x.nt) * KA * 512;
+                for (int kb = 0; kb < KB; kb++, ki++) {
+                    if (!tc::mbar_wait(&empty[st], ph, p.err, 111)) { ok = false; break; }
+                    uint8_t *sa = smem + st * C::STAGE, *sb = sa + MM_A, *sf = sb + C::B + 1024;
+                    const uint32_t sfb = min(2, KA - 2 * kb) * 512;
+                    tc::mbar_expect_tx(&full[st], boxes * MM_ABOX * 128 + C::B + atoms * sfb);
+                    tc::tma_load_3d(sb, &tmW, &full[st], kb * 128, x.nt * 256 + rank * 128, x.mat);
+                    for (int a = 0; a < atoms; a++)
+                        tc::bulk_load(sf + a * 1024, wsf + ((size_t)a * KA + 2 * kb) * 512, sfb, &full[st]);
+                    if (boxes == MM_M / MM_ABOX) tc::tma_load_3d(sa, &tmA, &full[st], kb * 128, x.row0, 0);
+                    else
+                        for (int b = 0; b < boxes; b++)
+                            tc::tma_load_3d(sa + b * (MM_ABOX * 128), &tmA1, &full[st], kb * 128, x.row0 + b * MM_ABOX, 0);
+                    if (++st == C::STAGES) {
+                        st = 0;
+                        ph ^= 1u;
+                    }
+                }
+            }
+            for (uint32_t i = ki > C::STAGES ? ki - C::STAGES : 0; i < ki; i++)
+                tc::mbar_wait(&full[i % C::STAGES], (i / C::STAGES) & 1u, p.err, 112);
+        }
+    } else if (warp == 1 && rank != 0) {
+        // ------------------------------------------------------------ filled stages to the first CTA
+        if (elect_one()) {
+            uint32_t st = 0, ph = 0;
+            bool ok = true;
+            for (int it = it0; ok && it < n_items; it += step) {
+                if (pair_item(it).mat < 0) continue;
+                for (int kb = 0; kb < KB; kb++) {
+                    if (!tc::mbar_wait(&full[st], ph, p.err, 113)) { ok = false; break; }
+                    tc::fence_proxy_async_smem();
+                    mbar_arrive_cta(&pfull[st], 0);
+                    if (++st == C::STAGES) {
+                        st = 0;
+                        ph ^= 1u;
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA
+        if (elect_one()) {
+            uint32_t st = 0, ph = 0, tph = 1;
+            bool ok = true;
+            const uint64_t da0 = tc::desc_kmajor_sw128(tc::smem_u32(smem)), db0 = tc::desc_kmajor_sw128(tc::smem_u32(smem) + MM_A);
+            const uint64_t dsf0 = tc::desc_sf_atom(tc::smem_u32(smem) + MM_A + C::B);
+            for (int it = it0; ok && it < n_items; it += step) {
+                if (pair_item(it).mat < 0) continue;
+                if (!tc::mbar_wait(tempty, tph, p.err, 114)) { ok = false; break; }
+                tph ^= 1u;
+                tc::tc_fence_after();
+                for (int kb = 0; kb < KB; kb++) {
+                    if (!tc::mbar_wait(&full[st], ph, p.err, 115) || !tc::mbar_wait(&pfull[st], ph, p.err, 116)) { ok = false; break; }
+                    tc::fence_proxy_async_smem();
+                    tc::tc_fence_after();
+                    const uint64_t so = (uint64_t)(st * (C::STAGE >> 4));
+                    const uint64_t da = da0 + so, db = db0 + so, dsf = dsf0 + so;
+                    const uint32_t col = tmem + C::SF_COL + st * C::SFW;
+                    auto scales = [&](int j) {
+                        tc_cp_sf_pair(col + j * 12, dsf + j * 32);
+                        tc_cp_sf_pair(col + j * 12 + 4, dsf + 64 + j * 32);
+                        tc_cp_sf_pair(col + j * 12 + 8, dsf + 128 + j * 32);
+                    };
+                    auto mma = [&](int k, uint32_t acc) {
+                        const uint32_t id = 2u * (k & 1), sfa = col + (k >> 1) * 12;
+                        tc_mma_mx4_pair(tmem, da + 2 * k, db + 2 * k, idesc_mxf4_pair(256, id), sfa | (id << 30), (sfa + 4) | (id << 30), acc);
+                    };
+                    const int left = p.K - 256 * kb;
+                    scales(0);
+                    if (left >= 256) {
+                        scales(1);
+                        mma(0, kb != 0);
+#pragma unroll
+                        for (int k = 1; k < 4; k++) mma(k, 1);
+                    } else {
+                        if (left > 128) scales(1);
+                        for (int k = 0; 64 * k < left; k++) mma(k, (kb | k) != 0);
+                    }
+                    tc_commit_pair(&empty[st]);
+                    if (++st == C::STAGES) {
+                        st = 0;
+                        ph ^= 1u;
+                    }
+                }
+                if (ok) tc_commit_pair(tfull);
+            }
+        }
+    } else if (warp == 2) {
+        a_scales<C::STAGES>(p, n_items, item, smem + MM_A + C::B, C::STAGE, full, empty, KB, it0, step);
+    } else if (warp >= 4) {
+        // ------------------------------------------------------------ epilogue
+        const int q = warp & 3, half = (warp - 4) >> 2;
+        const uint32_t lane_base = (uint32_t)(32 * q) << 16;
+        uint8_t *stg = stg_all + (warp - 4) * 2048;
+        uint32_t tph = 0;
+        bool alive = true;
+        for (int it = it0; it < n_items; it += step) {
+            const Item x = item(it);
+            const int rows = min(32, x.n - 32 * q);
+            uint32_t v[4][32];
+            bool ok = true;
+            if (x.mat < 0) {
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+#pragma unroll
+                    for (int i = 0; i < 32; i++) v[c][i] = 0;
+            } else {
+                ok = alive = alive && tc::mbar_wait(tfull, tph, p.err, 117);
+                tph ^= 1u;
+                __syncwarp();
+                tc::tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < 4; c++) tc::tmem_ld32(tmem + lane_base + 32u * (half * 4 + c), v[c]);
+                tc::tmem_ld_wait();
+                tc::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cta(tempty, 0);
+            }
+            if (rows > 0) {
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+                    store_rows(stg, v[c], p, x.row0 + 32 * q, rows, x.nt * 256 + 32 * (half * 4 + c), p.N, ok);
+            }
+        }
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::cluster_sync();   // the partner's MMAs, commits and arrivals reach this CTA's memory until here
+    tc::tc_fence_after();
+    if (warp == 1) tmem_dealloc_pair(tmem, 512);
 }
 
 // ------------------------------------------------------------------ gradient of the activations
@@ -1023,6 +1275,41 @@ int launch_mm(const CUtensorMap &ma, const CUtensorMap &ma1, const CUtensorMap &
     return K3C_OK;
 }
 
+// A kernel of CTA pairs, as a programmatic dependent.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_pairs(void (*kernel)(KArgs...), int grid, int block, size_t smem, cudaStream_t s, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = 2;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
+int launch_mm_pair(const CUtensorMap &ma, const CUtensorMap &ma1, const CUtensorMap &mw, MxArgs p, cudaStream_t s) {
+    static bool attr_of[64] = {};
+    bool &attr = attr_of[cur_dev()];
+    if (!attr) {
+        K3C_TRY_CUDA(cudaFuncSetAttribute(k_mx4_mm_pair, cudaFuncAttributeMaxDynamicSharedMemorySize, PrCfg::BYTES));
+        attr = true;
+    }
+    p.NTL = (p.N + 255) / 256;
+    const int64_t items = most_tiles(p.M, p.G, 2 * MM_M) * p.NTL;
+    K3C_TRY(check_items("mxfp4_mm", items));
+    const int grid = 2 * (int)(items < sm_count() / 2 ? items : sm_count() / 2);
+    K3C_TRY_CUDA(launch_pairs(k_mx4_mm_pair, grid, MM_THREADS, PrCfg::BYTES, s, ma, ma1, mw, p));
+    K3C_CHECK_LAUNCH();
+    return K3C_OK;
+}
+
 template <int MT, int NT>
 int launch_bwd(MxArgs p, const k3c_mxfp4_mat *W, const void *dy, int64_t lddy, cudaStream_t s) {
     using C = MbCfg<MT, NT>;
@@ -1114,16 +1401,19 @@ extern "C" int k3c_mxfp4_mm(void *y, int y_dtype, int64_t ldy, const uint8_t *a,
     p.as = a_scales;
     p.atoms = W->atoms;
     p.atom_stride = W->atom_stride;
-    // Column tile: the widest that still gives every SM an item; with fewer items a narrower
-    // tile spreads W's bytes over more SMs.
-    const int64_t tiles = off ? most_tiles(M, n_groups, MM_M) : (M + MM_M - 1) / MM_M;
+    // CTA pairs on 256 x 256 tiles where the groups have more than 128 rows on average and there
+    // is an item for every pair. Else the widest column tile that still gives every SM an item; with
+    // fewer items a narrower tile spreads W's bytes over more SMs.
+    auto tiles = [&](int mt) { return off ? most_tiles(M, n_groups, mt) : (int64_t)(M + mt - 1) / mt; };
+    const bool pairs = M / n_groups > 128 && tiles(256) * ((p.N + 255) / 256) >= sm_count() / 2;
     int nt = 256;
-    while (nt > 64 && tiles * ((p.N + nt - 1) / nt) < sm_count()) nt /= 2;
+    while (!pairs && nt > 64 && tiles(MM_M) * ((p.N + nt - 1) / nt) < sm_count()) nt /= 2;
     CUtensorMap ma, ma1, mw;
     K3C_TRY(make_map3(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, a, p.K / 2, M, 1, p.K / 2, (uint64_t)(p.K / 2) * M, 128, MM_M));
     K3C_TRY(make_map3(&ma1, CU_TENSOR_MAP_DATA_TYPE_UINT8, a, p.K / 2, M, 1, p.K / 2, (uint64_t)(p.K / 2) * M, 128, MM_ABOX));
-    K3C_TRY(map_weights(&mw, W, 128, nt));
-    if (nt == 256) K3C_TRY(launch_mm<256>(ma, ma1, mw, p, s));
+    K3C_TRY(map_weights(&mw, W, 128, pairs ? 128 : nt));
+    if (pairs) K3C_TRY(launch_mm_pair(ma, ma1, mw, p, s));
+    else if (nt == 256) K3C_TRY(launch_mm<256>(ma, ma1, mw, p, s));
     else if (nt == 128) K3C_TRY(launch_mm<128>(ma, ma1, mw, p, s));
     else K3C_TRY(launch_mm<64>(ma, ma1, mw, p, s));
     return check_waits("mxfp4_mm", p.err, s);
