@@ -158,37 +158,50 @@ __device__ int plan_tiles(Plan &pl, const int *off, int G, int M, int rows) {
     return run;
 }
 
-// Items of a group run through its row tiles first, RB of them at a time, so that the CTAs
-// working side by side share W tiles and a bounded set of A rows in L2.
+// Items of a group run through its row tiles first, MX_RB of them at a time, so that the CTAs
+// working side by side share W tiles and a bounded set of A rows in L2. A Walk turns ascending
+// item numbers into items; it keeps the group at hand, since a search with its divisions (1500
+// cycles for one thread) at every item left the copies that far behind.
 constexpr int MX_RB = 16;
-__device__ __forceinline__ Item item_of(int it, const Plan &pl, const int *mat_of, int n_mats, int G, int NTL, int rows) {
-    int g = 0;
-    if (G > 1) {
-        const int tt = it / NTL;
-        int h = G;   // tile[g] <= tt < tile[h]
-        while (h - g > 1) {
-            const int c = (g + h) >> 1;
-            if (pl.tile[c] <= tt) g = c;
-            else h = c;
+struct Walk {
+    const Plan &pl;
+    const int *mat_of;
+    int n_mats, G, NTL, rows;
+    int g = -1, lo = 0, hi = 0;    // items lo .. hi - 1 belong to group g
+    int mt = 0, f0 = 0, f1 = 0, mat = -1;
+    __device__ __forceinline__ Item at(int it) {
+        if (it >= hi) {
+            int a = g + 1, b = G;   // tile[a] * NTL <= it < tile[b] * NTL
+            while (b - a > 1) {
+                const int c = (a + b) >> 1;
+                if (pl.tile[c] * NTL <= it) a = c;
+                else b = c;
+            }
+            g = a;
+            mt = pl.tile[g + 1] - pl.tile[g];
+            lo = pl.tile[g] * NTL;
+            hi = pl.tile[g + 1] * NTL;
+            f0 = pl.first[g];
+            f1 = pl.first[g + 1];
+            mat = mat_of ? __ldg(mat_of + g) : g;
+            if (mat < 0 || mat >= n_mats) mat = -1;
         }
+        int i = it - lo, m = 0, mb = mt;
+        if (mt > MX_RB) {
+            const int b = i / (MX_RB * NTL);
+            m = MX_RB * b;
+            mb = min(MX_RB, mt - m);
+            i -= m * NTL;
+        }
+        Item x;
+        x.mat = mat;
+        x.nt = mb == 1 ? i : i / mb;
+        m += i - x.nt * mb;
+        x.row0 = f0 + m * rows;
+        x.n = min(rows, f1 - x.row0);
+        return x;
     }
-    const int t0 = pl.tile[g], mt = pl.tile[g + 1] - t0;
-    int i = it - t0 * NTL, m = 0, mb = mt;
-    if (mt > MX_RB) {
-        const int b = i / (MX_RB * NTL);
-        m = MX_RB * b;
-        mb = min(MX_RB, mt - m);
-        i -= m * NTL;
-    }
-    Item x;
-    x.nt = i / mb;
-    m += i - x.nt * mb;
-    x.row0 = pl.first[g] + m * rows;
-    x.n = min(rows, pl.first[g + 1] - x.row0);
-    const int mat = mat_of ? __ldg(mat_of + g) : g;
-    x.mat = mat >= 0 && mat < n_mats ? mat : -1;
-    return x;
-}
+};
 
 struct MxArgs {
     void *y;
@@ -300,7 +313,7 @@ __device__ __forceinline__ void tc_mma_mx4(uint32_t d, uint64_t da, uint64_t db,
 constexpr int MM_M = 128;
 constexpr int MM_ABOX = 32;                      // rows per A copy of a short tile; a full one takes one copy
 constexpr int MM_A = MM_M * 128;                 // 128 rows x 256 codes
-constexpr int MM_THREADS = 384;                  // copies, MMA, A scales, (idle), 8 epilogue warps
+constexpr int MM_THREADS = 384;                  // warps: W copies, MMA, A scales, A copies, 8 of epilogue
 constexpr int MM_EPI = 8;
 constexpr int MM_KS = 4;                         // K blocks per fetch of A scales: one 32-byte sector a row
 template <int NT>
@@ -320,6 +333,37 @@ struct MmCfg {
     static_assert(BYTES + sizeof(Plan) + 64 <= 227 * 1024, "one CTA per SM");
     static_assert((2 * STAGES + 2 * NACC) * 8 + 4 <= BAR, "barriers");
 };
+
+// A's codes of every K block of this CTA's items, by one thread, to sa0 in stage 0; item(it) gives
+// the rows of this CTA. (With W's copies in the same thread a stage took 440 cycles to issue, as
+// long as its MMAs: after a stall the copies never got ahead again.)
+template <int STAGES, typename ItemFn>
+__device__ __forceinline__ void copy_a(const MxArgs &p, int n_items, const ItemFn &item, const CUtensorMap &tmA,
+                                       const CUtensorMap &tmA1, uint8_t *sa0, int stage_bytes, uint64_t *full,
+                                       uint64_t *empty, int KB, int it0, int step) {
+    uint32_t n = 0, st = 0, ph = 1;
+    bool ok = true;
+    for (int it = it0; ok && it < n_items; it += step) {
+        const Item x = item(it);
+        if (x.mat < 0) continue;
+        const int boxes = (x.n + MM_ABOX - 1) / MM_ABOX;
+        for (int kb = 0; kb < KB; kb++, n++) {
+            if (!tc::mbar_wait(&empty[st], ph, p.err, 87)) { ok = false; break; }
+            uint8_t *sa = sa0 + st * stage_bytes;
+            tc::mbar_expect_tx(&full[st], boxes * MM_ABOX * 128);
+            if (boxes == MM_M / MM_ABOX) tc::tma_load_3d(sa, &tmA, &full[st], kb * 128, x.row0, 0);
+            else
+                for (int b = 0; b < boxes; b++)
+                    tc::tma_load_3d(sa + b * (MM_ABOX * 128), &tmA1, &full[st], kb * 128, x.row0 + b * MM_ABOX, 0);
+            if (++st == STAGES) {
+                st = 0;
+                ph ^= 1u;
+            }
+        }
+    }
+    for (uint32_t i = n > STAGES ? n - STAGES : 0; i < n; i++)
+        tc::mbar_wait(&full[i % STAGES], (i / STAGES) & 1u, p.err, 88);
+}
 
 // A's scales of every K block of this CTA's items, by one warp. Lane i fetches the bytes of rows i,
 // 32+i, 64+i and 96+i and stores the four rows' words of each atom as one 16-byte piece (sf_byte's
@@ -421,7 +465,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant_
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::STAGES; i++) {
-            tc::mbar_init(&full[i], 2);     // the copies' thread and the A scales' warp
+            tc::mbar_init(&full[i], 3);     // W's thread, A's thread and the A scales' warp
             tc::mbar_init(&empty[i], 1);
         }
         for (int i = 0; i < C::NACC; i++) {
@@ -442,33 +486,28 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant_
     const int n_items = tiles * p.NTL;
     const int KB = (p.K + 255) / 256;
     const int KA = (p.K + 127) / 128;              // scale atoms along K
-    auto item = [&](int it) { return item_of(it, plan, p.mat_of, p.n_mats, p.G, p.NTL, MM_M); };
+    Walk walk{plan, p.mat_of, p.n_mats, p.G, p.NTL, MM_M};
+    auto item = [&](int it) { return walk.at(it); };   // a thread takes one role
 
     if (warp == 0) {
-        // ------------------------------------------------------------ copies
+        // ------------------------------------------------------------ W's codes and scales
         if (elect_one()) {
             bool ok = tc::tc_check((tc::smem_u32(smem) & 1023) == 0, p.err, 80);
-            uint32_t ki = 0, st = 0, ph = 0;
+            uint32_t n = 0, st = 0, ph = 1;
             for (int it = blockIdx.x; ok && it < n_items; it += gridDim.x) {
                 const Item x = item(it);
                 if (x.mat < 0) continue;
-                const int boxes = (x.n + MM_ABOX - 1) / MM_ABOX;
                 const int arow = NT >= 128 ? x.nt * C::NA : x.nt / 2;         // W's 128-row atom
                 const int atoms = min(C::NA, (p.N + 127) / 128 - arow);        // the last tile may end early
                 const uint8_t *wsf = p.atoms + (size_t)x.mat * p.atom_stride + (size_t)arow * KA * 512;
-                for (int kb = 0; kb < KB; kb++, ki++) {
-                    if (ki >= C::STAGES && !tc::mbar_wait(&empty[st], ph ^ 1u, p.err, 81)) { ok = false; break; }
-                    uint8_t *sa = smem + st * C::STAGE, *sb = sa + MM_A, *sf = sb + C::B + 1024;
-                    const uint32_t sfb = min(2, KA - 2 * kb) * 512;            // W's scales of this K block
-                    tc::mbar_expect_tx(&full[st], boxes * MM_ABOX * 128 + C::B + atoms * sfb);
+                for (int kb = 0; kb < KB; kb++, n++) {
+                    if (!tc::mbar_wait(&empty[st], ph, p.err, 81)) { ok = false; break; }
+                    uint8_t *sb = smem + st * C::STAGE + MM_A, *sf = sb + C::B + 1024;
+                    const uint32_t sfb = min(2, KA - 2 * kb) * 512;            // of this K block
+                    tc::mbar_expect_tx(&full[st], C::B + atoms * sfb);
                     tc::tma_load_3d(sb, &tmW, &full[st], kb * 128, x.nt * NT, x.mat);
                     for (int a = 0; a < atoms; a++)
                         tc::bulk_load(sf + a * 1024, wsf + ((size_t)a * KA + 2 * kb) * 512, sfb, &full[st]);
-                    if (boxes == MM_M / MM_ABOX)
-                        tc::tma_load_3d(sa, &tmA, &full[st], kb * 128, x.row0, 0);
-                    else
-                        for (int b = 0; b < boxes; b++)
-                            tc::tma_load_3d(sa + b * (MM_ABOX * 128), &tmA1, &full[st], kb * 128, x.row0 + b * MM_ABOX, 0);
                     if (++st == C::STAGES) {
                         st = 0;
                         ph ^= 1u;
@@ -476,9 +515,12 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant_
                 }
             }
             // no copy may still be landing when the CTA exits
-            for (uint32_t i = ki > C::STAGES ? ki - C::STAGES : 0; i < ki; i++)
+            for (uint32_t i = n > C::STAGES ? n - C::STAGES : 0; i < n; i++)
                 tc::mbar_wait(&full[i % C::STAGES], (i / C::STAGES) & 1u, p.err, 82);
         }
+    } else if (warp == 3) {
+        // ------------------------------------------------------------ A's codes
+        if (elect_one()) copy_a<C::STAGES>(p, n_items, item, tmA, tmA1, smem, C::STAGE, full, empty, KB, blockIdx.x, gridDim.x);
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA
         if (elect_one()) {
@@ -655,7 +697,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm_pair(const __grid_cons
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::STAGES; i++) {
-            tc::mbar_init(&full[i], 2);
+            tc::mbar_init(&full[i], 3);
             tc::mbar_init(&pfull[i], 1);
             tc::mbar_init(&empty[i], 1);
         }
@@ -676,7 +718,8 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm_pair(const __grid_cons
     const int n_items = tiles * p.NTL;
     const int KB = (p.K + 255) / 256, KA = (p.K + 127) / 128;
     const int it0 = blockIdx.x >> 1, step = gridDim.x >> 1;
-    auto pair_item = [&](int it) { return item_of(it, plan, p.mat_of, p.n_mats, p.G, p.NTL, 2 * MM_M); };
+    Walk walk{plan, p.mat_of, p.n_mats, p.G, p.NTL, 2 * MM_M};
+    auto pair_item = [&](int it) { return walk.at(it); };   // a thread takes one role
     auto item = [&](int it) {   // this CTA's rows of the pair's item
         Item x = pair_item(it);
         x.row0 += rank * MM_M;
@@ -685,37 +728,35 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm_pair(const __grid_cons
     };
 
     if (warp == 0) {
-        // ------------------------------------------------------------ copies
+        // ------------------------------------------------------------ W's codes and scales
         if (elect_one()) {
             bool ok = tc::tc_check((tc::smem_u32(smem) & 1023) == 0, p.err, 110);
-            uint32_t ki = 0, st = 0, ph = 1;
+            uint32_t n = 0, st = 0, ph = 1;
             for (int it = it0; ok && it < n_items; it += step) {
-                const Item x = item(it);
+                const Item x = pair_item(it);
                 if (x.mat < 0) continue;
-                const int boxes = (x.n + MM_ABOX - 1) / MM_ABOX;
                 const int atoms = min(2, (p.N + 127) / 128 - 2 * x.nt);
                 const uint8_t *wsf = p.atoms + (size_t)x.mat * p.atom_stride + (size_t)(2 * x.nt) * KA * 512;
-                for (int kb = 0; kb < KB; kb++, ki++) {
+                for (int kb = 0; kb < KB; kb++, n++) {
                     if (!tc::mbar_wait(&empty[st], ph, p.err, 111)) { ok = false; break; }
-                    uint8_t *sa = smem + st * C::STAGE, *sb = sa + MM_A, *sf = sb + C::B + 1024;
+                    uint8_t *sb = smem + st * C::STAGE + MM_A, *sf = sb + C::B + 1024;
                     const uint32_t sfb = min(2, KA - 2 * kb) * 512;
-                    tc::mbar_expect_tx(&full[st], boxes * MM_ABOX * 128 + C::B + atoms * sfb);
+                    tc::mbar_expect_tx(&full[st], C::B + atoms * sfb);
                     tc::tma_load_3d(sb, &tmW, &full[st], kb * 128, x.nt * 256 + rank * 128, x.mat);
                     for (int a = 0; a < atoms; a++)
                         tc::bulk_load(sf + a * 1024, wsf + ((size_t)a * KA + 2 * kb) * 512, sfb, &full[st]);
-                    if (boxes == MM_M / MM_ABOX) tc::tma_load_3d(sa, &tmA, &full[st], kb * 128, x.row0, 0);
-                    else
-                        for (int b = 0; b < boxes; b++)
-                            tc::tma_load_3d(sa + b * (MM_ABOX * 128), &tmA1, &full[st], kb * 128, x.row0 + b * MM_ABOX, 0);
                     if (++st == C::STAGES) {
                         st = 0;
                         ph ^= 1u;
                     }
                 }
             }
-            for (uint32_t i = ki > C::STAGES ? ki - C::STAGES : 0; i < ki; i++)
+            for (uint32_t i = n > C::STAGES ? n - C::STAGES : 0; i < n; i++)
                 tc::mbar_wait(&full[i % C::STAGES], (i / C::STAGES) & 1u, p.err, 112);
         }
+    } else if (warp == 3) {
+        // ------------------------------------------------------------ A's codes
+        if (elect_one()) copy_a<C::STAGES>(p, n_items, item, tmA, tmA1, smem, C::STAGE, full, empty, KB, it0, step);
     } else if (warp == 1 && rank != 0) {
         // ------------------------------------------------------------ filled stages to the first CTA
         if (elect_one()) {
@@ -972,7 +1013,8 @@ __global__ void __launch_bounds__(MB_THREADS, 1) k_mx4_bwd(const __grid_constant
     const int n_items = tiles * p.NTL;
     const int KB = (p.N + MB_KB - 1) / MB_KB;      // contracted: W's rows
     const int KA = (p.K + 127) / 128;
-    auto item = [&](int it) { return item_of(it, plan, p.mat_of, p.n_mats, p.G, p.NTL, MT); };
+    Walk walk{plan, p.mat_of, p.n_mats, p.G, p.NTL, MT};
+    auto item = [&](int it) { return walk.at(it); };   // a thread takes one role
 
     if (warp == 0) {
         // ------------------------------------------------------------ dY copies
