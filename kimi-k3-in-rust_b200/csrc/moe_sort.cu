@@ -25,8 +25,9 @@ namespace {
 // ------------------------------------------------------------------ sort
 constexpr int SORT_TH = 1024;
 constexpr int SORT_WARPS = SORT_TH / 32;
-constexpr int SORT_SUB = 4096;                    // pairs placed per pass of a block
-constexpr int SORT_ROUNDS = SORT_SUB / SORT_TH;   // 32-pair rounds per warp and pass
+constexpr int SORT_ONE = 8;                       // rounds of 32 pairs a warp, when one block takes all pairs
+constexpr int SORT_MANY = 2;                      // and when several do, per pass
+constexpr int SORT_SUB = SORT_MANY * SORT_TH;     // pairs of a pass
 constexpr int SORT_BLOCKS = 128;                  // blocks at most: every one reads all blocks' counts
 constexpr int SORT_EMAX = 2048;
 
@@ -36,9 +37,113 @@ __device__ __forceinline__ int expert_of(const int *idx, int p, int P, int E) {
     return (unsigned)e < (unsigned)E ? e : -1;
 }
 
+// Exclusive prefix sums of v over the block's threads; all: their total. warp_tot: SORT_WARPS ints.
+__device__ __forceinline__ int block_prefix(int v, int &all, int *warp_tot) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += u;
+    }
+    if (lane == 31) warp_tot[warp] = inc;
+    __syncthreads();
+    const int t = warp_tot[lane];                 // every warp sums the warps' totals itself
+    int ti = t;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, ti, o);
+        if (lane >= o) ti += u;
+    }
+    all = __shfl_sync(0xffffffffu, ti, 31);
+    const int pre = __shfl_sync(0xffffffffu, ti - t, warp);
+    __syncthreads();                              // warp_tot may be written again
+    return pre + inc - v;
+}
+
+// A warp's pairs of one pass: 32 * R of them side by side from p0 on. count() adds the warp's counts
+// per expert into its own row `mine` of the table; after the table's columns have been turned
+// into first ranks, place() gives each pair its rank: earlier rounds through `mine`, lower lanes
+// with the same expert by one match per round. No atomics, and a stable order.
+template <int R>
+struct WarpPairs {
+    int ex[R];
+    uint32_t same[R];
+    __device__ __forceinline__ void count(uint16_t *mine, const int *idx, int p0, int hi, int E) {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int r = 0; r < R; r++) ex[r] = expert_of(idx, p0 + 32 * r + lane, hi, E);
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            same[r] = __match_any_sync(0xffffffffu, ex[r]);
+            if (ex[r] >= 0 && (same[r] & ((1u << lane) - 1u)) == 0) mine[ex[r]] += (uint16_t)__popc(same[r]);
+            __syncwarp();
+        }
+    }
+    __device__ __forceinline__ void place(uint16_t *mine, const int *base, int *pos, int *pair, int p0, int hi) {
+        const int lane = threadIdx.x & 31;
+        const uint32_t below = (1u << lane) - 1u;
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const int p = p0 + 32 * r + lane;
+            int row = -1;
+            if (ex[r] >= 0) row = base[ex[r]] + mine[ex[r]] + __popc(same[r] & below);
+            __syncwarp();
+            if (ex[r] >= 0 && (same[r] & below) == 0) mine[ex[r]] += (uint16_t)__popc(same[r]);
+            __syncwarp();
+            if (p < hi) {
+                pos[p] = row;
+                if (row >= 0) pair[row] = p;
+            }
+        }
+    }
+};
+
+// Column e of the table [warps][E] from counts to first ranks; returns its sum.
+__device__ __forceinline__ int column_ranks(uint16_t *wh, int warps, int E, int e) {
+    int at = 0;
+#pragma unroll 4
+    for (int w = 0; w < warps; w++) {
+        const int c = wh[w * E + e];
+        wh[w * E + e] = (uint16_t)at;
+        at += c;
+    }
+    return at;
+}
+
+// All pairs in one block (at most SORT_ONE * SORT_TH): warps = those that have any.
+__global__ void __launch_bounds__(SORT_TH) k_sort_one(int *__restrict__ pos, int *__restrict__ pair, int *__restrict__ off,
+                                                      const int *__restrict__ idx, int P, int E, int warps) {
+    extern __shared__ int sort_sm[];
+    int *base = sort_sm;                                       // [E] first row of each expert
+    uint16_t *wh = reinterpret_cast<uint16_t *>(base + E);     // [warps][E]
+    __shared__ int warp_tot[SORT_WARPS];
+    const int tid = threadIdx.x, warp = tid >> 5;
+    for (int i = tid; i < (warps * E + 1) / 2; i += SORT_TH) reinterpret_cast<uint32_t *>(wh)[i] = 0;
+    __syncthreads();
+    WarpPairs<SORT_ONE> mine;
+    uint16_t *row = wh + warp * E;
+    const int p0 = warp * (SORT_ONE * 32);
+    if (warp < warps) mine.count(row, idx, p0, P, E);
+    __syncthreads();
+    int run = 0;
+    for (int e0 = 0; e0 < E; e0 += SORT_TH) {
+        const int e = e0 + tid, n = e < E ? column_ranks(wh, warps, E, e) : 0;
+        int all;
+        const int first = run + block_prefix(n, all, warp_tot);
+        if (e < E) base[e] = off[e] = first;
+        run += all;
+    }
+    if (tid == 0) off[E] = run;
+    for (int r = run + tid; r < P; r += SORT_TH) pair[r] = -1;   // rows behind the last pair
+    __syncthreads();
+    if (warp < warps) mine.place(row, base, pos, pair, p0, P);
+}
+
 // Counts of a block's pairs per expert: cnt[block][E].
 __global__ void __launch_bounds__(SORT_TH) k_sort_count(int *__restrict__ cnt, const int *__restrict__ idx, int P,
                                                         int E, int chunk) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     extern __shared__ int sort_sm[];
     for (int e = threadIdx.x; e < E; e += SORT_TH) sort_sm[e] = 0;
     __syncthreads();
@@ -51,109 +156,59 @@ __global__ void __launch_bounds__(SORT_TH) k_sort_count(int *__restrict__ cnt, c
     for (int e = threadIdx.x; e < E; e += SORT_TH) cnt[(size_t)blockIdx.x * E + e] = sort_sm[e];
 }
 
-// Each block finds its experts' first rows from all blocks' counts (nblk == 1: from its own
-// pairs) and places its chunk, SORT_SUB pairs at a time. A warp owns 128 consecutive pairs of
-// a pass, so a pair's rank is (earlier passes) + (earlier warps) + (earlier rounds of the warp)
-// + (lower lanes with the same expert, from one match per round): no atomics, and a stable order.
+// Each block finds its experts' next free rows from all blocks' counts and places its chunk,
+// SORT_SUB pairs at a time. A programmatic dependent of k_sort_count: the first pass's matching
+// needs only idx, which was there before that kernel began.
 __global__ void __launch_bounds__(SORT_TH) k_sort_place(int *__restrict__ pos, int *__restrict__ pair,
                                                         int *__restrict__ off, const int *__restrict__ idx,
-                                                        const int *__restrict__ cnt, int P, int E, int chunk, int nblk) {
+                                                        const int *cnt, int P, int E, int chunk) {
     extern __shared__ int sort_sm[];
     int *base = sort_sm;                                       // [E] next free row of each expert
-    uint16_t *wh = reinterpret_cast<uint16_t *>(base + E);     // [warps][E] counts, then ranks, of a pass
+    uint16_t *wh = reinterpret_cast<uint16_t *>(base + E);     // [SORT_WARPS][E]
     __shared__ int warp_tot[SORT_WARPS];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = tid >> 5, nblk = gridDim.x;
     const int lo = blockIdx.x * chunk, hi = min(P - lo, chunk) + lo;
-
-    if (nblk == 1) {
-        for (int e = tid; e < E; e += SORT_TH) base[e] = 0;
+    uint16_t *row = wh + warp * E;
+    WarpPairs<SORT_MANY> mine;
+    auto first_half = [&](int s0) {
+        for (int i = tid; i < SORT_WARPS * E / 2; i += SORT_TH) reinterpret_cast<uint32_t *>(wh)[i] = 0;
         __syncthreads();
-        for (int p = lo + tid; p < hi; p += SORT_TH) {
-            const int e = expert_of(idx, p, P, E);
-            if (e >= 0) atomicAdd(&base[e], 1);
-        }
-        __syncthreads();
-    }
-    int run = 0;   // pairs of the experts before this round of the scan
+        mine.count(row, idx, s0 + warp * (SORT_MANY * 32), hi, E);
+    };
+    first_half(lo);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    int run = 0;
     for (int e0 = 0; e0 < E; e0 += SORT_TH) {
         const int e = e0 + tid;
-        int tot = 0, before = 0;
+        int n = 0, before = 0;
         if (e < E) {
-            if (nblk == 1) tot = base[e];
-            else
-                for (int b = 0; b < nblk; b++) {
-                    const int c = cnt[(size_t)b * E + e];
-                    before += b < (int)blockIdx.x ? c : 0;
-                    tot += c;
-                }
+#pragma unroll 8
+            for (int b = 0; b < nblk; b++) {
+                const int c = __ldcg(cnt + (size_t)b * E + e);
+                before += b < (int)blockIdx.x ? c : 0;
+                n += c;
+            }
         }
-        int inc = tot;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += v;
-        }
-        if (lane == 31) warp_tot[warp] = inc;
-        __syncthreads();
-        int pre = 0, all = 0;
-        for (int w = 0; w < SORT_WARPS; w++) {
-            const int v = warp_tot[w];
-            pre += w < warp ? v : 0;
-            all += v;
-        }
+        int all;
+        const int first = run + block_prefix(n, all, warp_tot);
         if (e < E) {
-            const int first = run + pre + inc - tot;
             base[e] = first + before;
             if (blockIdx.x == 0) off[e] = first;
         }
         run += all;
-        __syncthreads();
     }
     if (blockIdx.x == 0 && tid == 0) off[E] = run;
     for (int r = lo + tid; r < hi; r += SORT_TH)   // rows behind the last pair
         if (r >= run) pair[r] = -1;
-
-    uint16_t *mine = wh + (size_t)warp * E;
-    const uint32_t below = (1u << lane) - 1u;
     for (int s0 = lo; s0 < hi; s0 += SORT_SUB) {
-        for (int i = tid; i < SORT_WARPS * E; i += SORT_TH) wh[i] = 0;
+        if (s0 != lo) first_half(s0);
         __syncthreads();
-        int ex[SORT_ROUNDS];
-        uint32_t same[SORT_ROUNDS];
-        const int w0 = s0 + warp * (SORT_ROUNDS * 32) + lane;
-#pragma unroll
-        for (int r = 0; r < SORT_ROUNDS; r++) {
-            ex[r] = expert_of(idx, w0 + 32 * r, hi, E);
-            same[r] = __match_any_sync(0xffffffffu, ex[r]);
-            if (ex[r] >= 0 && (same[r] & below) == 0) mine[ex[r]] += (uint16_t)__popc(same[r]);
-            __syncwarp();
-        }
+        for (int e = tid; e < E; e += SORT_TH) column_ranks(wh, SORT_WARPS, E, e);
         __syncthreads();
-        for (int e = tid; e < E; e += SORT_TH) {
-            int at = 0;
-            for (int w = 0; w < SORT_WARPS; w++) {
-                const int c = wh[(size_t)w * E + e];
-                wh[(size_t)w * E + e] = (uint16_t)at;
-                at += c;
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < SORT_ROUNDS; r++) {
-            const int p = w0 + 32 * r;
-            int row = -1;
-            if (ex[r] >= 0) row = base[ex[r]] + mine[ex[r]] + __popc(same[r] & below);
-            __syncwarp();
-            if (ex[r] >= 0 && (same[r] & below) == 0) mine[ex[r]] += (uint16_t)__popc(same[r]);
-            __syncwarp();
-            if (p < hi) {
-                pos[p] = row;
-                if (row >= 0) pair[row] = p;
-            }
-        }
+        mine.place(row, base, pos, pair, s0 + warp * (SORT_MANY * 32), hi);
         __syncthreads();
         // the last warp's running ranks are the pass's counts
-        for (int e = tid; e < E; e += SORT_TH) base[e] += wh[(size_t)(SORT_WARPS - 1) * E + e];
+        for (int e = tid; e < E; e += SORT_TH) base[e] += wh[(SORT_WARPS - 1) * E + e];
         __syncthreads();
     }
 }
@@ -200,82 +255,111 @@ __device__ __forceinline__ uint4 ld16(const void *p) { return ldg_nc_v4(p); }
 // Rows are written once and read by a later kernel: streaming stores keep x and pos in L2.
 __device__ __forceinline__ void st16(void *p, const uint4 &v) { __stcs(reinterpret_cast<uint4 *>(p), v); }
 
-// The row of pair (t, j): -1 for a dropped pair or anything outside [0, P).
-__device__ __forceinline__ int row_of(const int *__restrict__ pos, size_t p, int P) {
-    const int r = __ldg(pos + p);
-    return (unsigned)r < (unsigned)P ? r : -1;
-}
-
 constexpr int PM_TH = 256;
 
+// A token's pairs that have a row, in the order of j: rows, j and weights in shared memory, so that
+// the loops below run over those pairs alone with several loads in flight (an expert-parallel
+// rank holds one pair in eight). A row outside [0, P) counts as none.
+struct TokenRows {
+    int row[K3_MAX_TOPK], j[K3_MAX_TOPK];
+    float w[K3_MAX_TOPK];
+    int n;
+};
+__device__ __forceinline__ int token_rows(TokenRows &s, const int *__restrict__ pos, const float *__restrict__ wt,
+                                          size_t p0, int P, int topk) {
+    if (threadIdx.x < 32) {
+        const int lane = threadIdx.x;
+        int n = 0;
+        for (int j0 = 0; j0 < topk; j0 += 32) {
+            const int j = j0 + lane, r = j < topk ? __ldg(pos + p0 + j) : -1;
+            const float w = wt && j < topk ? __ldg(wt + p0 + j) : 1.0f;
+            const bool on = (unsigned)r < (unsigned)P;
+            const uint32_t m = __ballot_sync(0xffffffffu, on);
+            if (on) {
+                const int at = n + __popc(m & ((1u << lane) - 1u));
+                s.row[at] = r;
+                s.j[at] = j;
+                s.w[at] = w;
+            }
+            n += __popc(m);
+        }
+        if (lane == 0) s.n = n;
+    }
+    __syncthreads();
+    return s.n;
+}
+
 // ------------------------------------------------------------------ permute
-// Block (t, h): 16-byte chunks h*PM_TH.. of token t, read once and stored into the token's rows.
+// Block (t, h): 16-byte chunks of token t, read once and stored into the token's rows.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(PM_TH) k_permute(T *__restrict__ rows, const T *__restrict__ x, int64_t ldx,
                                                    const int *__restrict__ pos, int P, int topk, int H) {
+    __shared__ TokenRows s;
     const int t = blockIdx.x;
     const T *xr = x + (size_t)t * ldx;
-    const int *pt = pos + (size_t)t * topk;
-    if constexpr (VEC) {
-        const int n = H / Vec<T>::V, stride = gridDim.y * PM_TH;
-        for (int c = blockIdx.y * PM_TH + threadIdx.x; c < n; c += stride) {
-            const uint4 v = ld16(xr + (size_t)c * Vec<T>::V);
-            for (int j = 0; j < topk; j++) {
-                const int r = row_of(pt, j, P);
-                if (r >= 0) st16(rows + (size_t)r * H + (size_t)c * Vec<T>::V, v);
-            }
-        }
-    } else {
-        for (int i = blockIdx.y * PM_TH + threadIdx.x; i < H; i += gridDim.y * PM_TH) {
-            const T v = xr[i];
-            for (int j = 0; j < topk; j++) {
-                const int r = row_of(pt, j, P);
-                if (r >= 0) rows[(size_t)r * H + i] = v;
-            }
+    constexpr int V = VEC ? Vec<T>::V : 1;
+    const int n = H / V, stride = gridDim.y * PM_TH;
+    const int m = token_rows(s, pos, nullptr, (size_t)t * topk, P, topk);
+    if (!m) return;
+    for (int c = blockIdx.y * PM_TH + threadIdx.x; c < n; c += stride) {
+        if constexpr (VEC) {
+            const uint4 v = ld16(xr + (size_t)c * V);
+#pragma unroll 4
+            for (int j = 0; j < m; j++) st16(rows + (size_t)s.row[j] * H + (size_t)c * V, v);
+        } else {
+            const T v = xr[c];
+#pragma unroll 4
+            for (int j = 0; j < m; j++) rows[(size_t)s.row[j] * H + c] = v;
         }
     }
 }
 
 // ------------------------------------------------------------------ sums back per token
-// out[t] = sum_j w_j y[pos[t][j]]; wt NULL: w_j = 1 (the gradient of the permute). Four rows'
+// out[t] = sum_j w_j y[pos[t][j]]; wt NULL: w_j = 1 (the gradient of the permute). Eight rows'
 // loads are in flight before the first is added; the additions keep the order of j.
+constexpr int GS_JB = 8;
 template <typename T, typename O, bool VEC>
 __global__ void __launch_bounds__(PM_TH) k_gather_sum(O *__restrict__ out, const T *__restrict__ y,
                                                       const float *__restrict__ wt, const int *__restrict__ pos, int P,
                                                       int topk, int H) {
+    __shared__ TokenRows s;
     const int t = blockIdx.x;
-    const size_t p0 = (size_t)t * topk;
-    if constexpr (VEC) {
-        constexpr int V = Vec<T>::V;
-        const int n = H / V, stride = gridDim.y * PM_TH;
-        for (int c = blockIdx.y * PM_TH + threadIdx.x; c < n; c += stride) {
-            float acc[V];
+    const int m = token_rows(s, pos, wt, (size_t)t * topk, P, topk);
+    constexpr int V = VEC ? Vec<T>::V : 1;
+    const int n = H / V, stride = gridDim.y * PM_TH;
+    for (int c = blockIdx.y * PM_TH + threadIdx.x; c < n; c += stride) {
+        float acc[V];
 #pragma unroll
-            for (int i = 0; i < V; i++) acc[i] = 0.0f;
-            for (int j0 = 0; j0 < topk; j0 += 4) {
-                uint4 u[4];
-                float w[4];
-                bool on[4];
+        for (int i = 0; i < V; i++) acc[i] = 0.0f;
+        for (int j0 = 0; j0 < m; j0 += GS_JB) {
+            if constexpr (VEC) {
+                uint4 u[GS_JB];
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const int j = j0 + q;
-                    const int r = j < topk ? row_of(pos, p0 + j, P) : -1;
-                    on[q] = r >= 0;
-                    if (on[q]) {
-                        u[q] = ld16(y + (size_t)r * H + (size_t)c * V);
-                        w[q] = wt ? __ldg(wt + p0 + j) : 1.0f;
-                    }
-                }
+                for (int q = 0; q < GS_JB; q++)
+                    if (j0 + q < m) u[q] = ld16(y + (size_t)s.row[j0 + q] * H + (size_t)c * V);
 #pragma unroll
-                for (int q = 0; q < 4; q++)
-                    if (on[q]) {
+                for (int q = 0; q < GS_JB; q++)
+                    if (j0 + q < m) {
+                        const float w = s.w[j0 + q];
                         float f[V];
                         Vec<T>::get(u[q], f);
 #pragma unroll
-                        for (int i = 0; i < V; i++) acc[i] = __fadd_rn(acc[i], __fmul_rn(w[q], f[i]));
+                        for (int i = 0; i < V; i++) acc[i] = __fadd_rn(acc[i], __fmul_rn(w, f[i]));
                     }
+            } else {
+                float f[GS_JB];
+#pragma unroll
+                for (int q = 0; q < GS_JB; q++)
+                    if (j0 + q < m) f[q] = Vec<T>::one(y[(size_t)s.row[j0 + q] * H + c]);
+#pragma unroll
+                for (int q = 0; q < GS_JB; q++)
+                    if (j0 + q < m) acc[0] = __fadd_rn(acc[0], __fmul_rn(s.w[j0 + q], f[q]));
             }
-            O *o = out + (size_t)t * H + (size_t)c * V;
+        }
+        O *o = out + (size_t)t * H + (size_t)c * V;
+        if constexpr (!VEC) {
+            *o = Vec<O>::back(acc[0]);
+        } else {
             constexpr int VO = Vec<O>::V;
             if constexpr (VO == V) {
                 st16(o, Vec<O>::put(acc));
@@ -291,21 +375,11 @@ __global__ void __launch_bounds__(PM_TH) k_gather_sum(O *__restrict__ out, const
                 *reinterpret_cast<uint2 *>(o) = make_uint2(f32x2_to_bf16x2(acc[0], acc[1]), f32x2_to_bf16x2(acc[2], acc[3]));
             }
         }
-    } else {
-        for (int i = blockIdx.y * PM_TH + threadIdx.x; i < H; i += gridDim.y * PM_TH) {
-            float acc = 0.0f;
-            for (int j = 0; j < topk; j++) {
-                const int r = row_of(pos, p0 + j, P);
-                if (r >= 0)
-                    acc = __fadd_rn(acc, __fmul_rn(wt ? __ldg(wt + p0 + j) : 1.0f, Vec<T>::one(y[(size_t)r * H + i])));
-            }
-            out[(size_t)t * H + i] = Vec<O>::back(acc);
-        }
     }
 }
 
 // ------------------------------------------------------------------ unpermute's gradients
-// One block per token: dout[t] is read once per batch of JB pairs, each pair's y row once; the
+// One block per token: dout[t] is read once per batch of UB_JB pairs, each pair's y row once; the
 // products for dwt are summed per thread in fp32, then across the block in a fixed tree.
 constexpr int UB_JB = 8;
 template <typename T, typename D, bool VEC>
@@ -314,33 +388,35 @@ __global__ void __launch_bounds__(PM_TH) k_unpermute_bwd(T *__restrict__ dy, flo
                                                          const float *__restrict__ wt, const int *__restrict__ pos,
                                                          int P, int topk, int H) {
     __shared__ float part[PM_TH / 32][UB_JB];
+    __shared__ TokenRows s;
     const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const size_t p0 = (size_t)t * topk;
     const D *dr = dout + (size_t)t * H;
-    for (int j0 = 0; j0 < topk; j0 += UB_JB) {
-        int r[UB_JB];
-        float w[UB_JB], dot[UB_JB];
-#pragma unroll
-        for (int q = 0; q < UB_JB; q++) {
-            r[q] = j0 + q < topk ? row_of(pos, p0 + j0 + q, P) : -1;
-            w[q] = r[q] >= 0 ? __ldg(wt + p0 + j0 + q) : 0.0f;
-            dot[q] = 0.0f;
+    const int m = token_rows(s, pos, wt, p0, P, topk);
+    // pairs without a row: their products are all absent
+    if (dwt)
+        for (int j = threadIdx.x; j < topk; j += PM_TH) {
+            const int r = __ldg(pos + p0 + j);
+            if ((unsigned)r >= (unsigned)P) dwt[p0 + j] = 0.0f;
         }
+    for (int j0 = 0; j0 < m; j0 += UB_JB) {
+        const int jn = min(UB_JB, m - j0);
+        float dot[UB_JB];
+#pragma unroll
+        for (int q = 0; q < UB_JB; q++) dot[q] = 0.0f;
         if constexpr (VEC) {
             constexpr int V = Vec<T>::V, VD = Vec<D>::V;
             for (int c = threadIdx.x; c < H / V; c += PM_TH) {
                 float d[V];
-                if constexpr (VD >= V) {
-                    if constexpr (VD == V) {
-                        Vec<D>::get(ld16(dr + (size_t)c * V), d);
-                    } else {   // bf16 dout, fp32 rows: half a load
-                        const uint2 u = *reinterpret_cast<const uint2 *>(dr + (size_t)c * V);
-                        d[0] = __uint_as_float(u.x << 16);
-                        d[1] = __uint_as_float(u.x & 0xFFFF0000u);
-                        d[2] = __uint_as_float(u.y << 16);
-                        d[3] = __uint_as_float(u.y & 0xFFFF0000u);
-                    }
-                } else {       // fp32 dout, bf16 rows: two loads
+                if constexpr (VD == V) {
+                    Vec<D>::get(ld16(dr + (size_t)c * V), d);
+                } else if constexpr (VD > V) {   // bf16 dout, fp32 rows: half a load
+                    const uint2 u = *reinterpret_cast<const uint2 *>(dr + (size_t)c * V);
+                    d[0] = __uint_as_float(u.x << 16);
+                    d[1] = __uint_as_float(u.x & 0xFFFF0000u);
+                    d[2] = __uint_as_float(u.y << 16);
+                    d[3] = __uint_as_float(u.y & 0xFFFF0000u);
+                } else {                         // fp32 dout, bf16 rows: two loads
 #pragma unroll
                     for (int h = 0; h < V / VD; h++) {
                         float g[VD];
@@ -355,23 +431,23 @@ __global__ void __launch_bounds__(PM_TH) k_unpermute_bwd(T *__restrict__ dy, flo
                     if (dwt) {
 #pragma unroll
                         for (int q = 0; q < 4; q++)
-                            if (r[q0 + q] >= 0) u[q] = ld16(y + (size_t)r[q0 + q] * H + (size_t)c * V);
+                            if (q0 + q < jn) u[q] = ld16(y + (size_t)s.row[j0 + q0 + q] * H + (size_t)c * V);
                     }
 #pragma unroll
                     for (int q = 0; q < 4; q++) {
                         const int a = q0 + q;
-                        if (r[a] < 0) continue;
+                        if (a >= jn) continue;
+                        float f[V];
                         if (dwt) {
-                            float f[V];
                             Vec<T>::get(u[q], f);
 #pragma unroll
                             for (int i = 0; i < V; i++) dot[a] = fmaf(d[i], f[i], dot[a]);
                         }
                         if (dy) {
-                            float f[V];
+                            const float w = s.w[j0 + a];
 #pragma unroll
-                            for (int i = 0; i < V; i++) f[i] = w[a] * d[i];
-                            st16(dy + (size_t)r[a] * H + (size_t)c * V, Vec<T>::put(f));
+                            for (int i = 0; i < V; i++) f[i] = w * d[i];
+                            st16(dy + (size_t)s.row[j0 + a] * H + (size_t)c * V, Vec<T>::put(f));
                         }
                     }
                 }
@@ -379,27 +455,30 @@ __global__ void __launch_bounds__(PM_TH) k_unpermute_bwd(T *__restrict__ dy, flo
         } else {
             for (int i = threadIdx.x; i < H; i += PM_TH) {
                 const float d = Vec<D>::one(dr[i]);
+                float f[UB_JB];
+#pragma unroll
+                for (int q = 0; q < UB_JB; q++)
+                    if (dwt && q < jn) f[q] = Vec<T>::one(y[(size_t)s.row[j0 + q] * H + i]);
 #pragma unroll
                 for (int q = 0; q < UB_JB; q++) {
-                    if (r[q] < 0) continue;
-                    const size_t at = (size_t)r[q] * H + i;
-                    if (dwt) dot[q] = fmaf(d, Vec<T>::one(y[at]), dot[q]);
-                    if (dy) dy[at] = Vec<T>::back(w[q] * d);
+                    if (q >= jn) continue;
+                    if (dwt) dot[q] = fmaf(d, f[q], dot[q]);
+                    if (dy) dy[(size_t)s.row[j0 + q] * H + i] = Vec<T>::back(s.w[j0 + q] * d);
                 }
             }
         }
         if (dwt) {
 #pragma unroll
             for (int q = 0; q < UB_JB; q++) {
-                const float s = warp_sum(dot[q]);
-                if (lane == 0) part[warp][q] = s;
+                const float v = warp_sum(dot[q]);
+                if (lane == 0) part[warp][q] = v;
             }
             __syncthreads();
-            if (threadIdx.x < UB_JB && j0 + (int)threadIdx.x < topk) {
-                float s = 0.0f;
+            if ((int)threadIdx.x < jn) {
+                float v = 0.0f;
 #pragma unroll
-                for (int w2 = 0; w2 < PM_TH / 32; w2++) s += part[w2][threadIdx.x];
-                dwt[p0 + j0 + threadIdx.x] = s;   // a dropped pair's products are all absent: 0
+                for (int w2 = 0; w2 < PM_TH / 32; w2++) v += part[w2][threadIdx.x];
+                dwt[p0 + s.j[j0 + threadIdx.x]] = v;
             }
             __syncthreads();
         }
@@ -413,15 +492,18 @@ template <typename T>
 __global__ void __launch_bounds__(PM_TH) k_permute_mx4(uint8_t *__restrict__ packed, uint8_t *__restrict__ scales,
                                                        const T *__restrict__ x, int64_t ldx,
                                                        const int *__restrict__ pos, int P, int topk, int H, int vec) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    __shared__ TokenRows s;
     const int t = blockIdx.x, G = H / 32;
+    const int m = token_rows(s, pos, nullptr, (size_t)t * topk, P, topk);
+    if (!m) return;
     for (int g = blockIdx.y * PM_TH + threadIdx.x; g < G; g += gridDim.y * PM_TH) {
         float v[32];
         mx4_load32(v, x + (size_t)t * ldx + (size_t)g * 32, 32, vec);
         uint4 codes;
         const uint8_t sb = mx4_quant32(v, codes);
-        for (int j = 0; j < topk; j++) {
-            const int r = row_of(pos, (size_t)t * topk + j, P);
-            if (r < 0) continue;
+        for (int j = 0; j < m; j++) {
+            const int r = s.row[j];
             *reinterpret_cast<uint4 *>(packed + (size_t)r * (H / 2) + (size_t)g * 16) = codes;
             scales[(size_t)r * G + g] = sb;
         }
@@ -449,10 +531,12 @@ int check_pairs(const char *what, int ntok, int topk, int hidden) {
     return K3C_OK;
 }
 
+// One block as far as its warps' registers reach: a second launch costs more than the other SMs
+// save. Beyond that, blocks of one pass or more.
 int sort_blocks(int64_t P) {
-    // One block up to two passes: a second launch costs more than the passes it saves.
+    if (P <= SORT_ONE * SORT_TH) return 1;
     const int64_t n = (P + SORT_SUB - 1) / SORT_SUB;
-    return n <= 2 ? 1 : (int)(n < SORT_BLOCKS ? n : SORT_BLOCKS);
+    return (int)(n < SORT_BLOCKS ? n : SORT_BLOCKS);
 }
 
 template <typename T, typename O>
@@ -498,21 +582,27 @@ extern "C" int k3c_moe_sort(int *pos, int *pair, int *off, const int *idx, int n
         return set_error(K3C_EINVAL, "moe_sort: scratch of %zu bytes, %zu needed (4-byte aligned)", scratch_bytes, need);
     cudaStream_t s = (cudaStream_t)stream;
     const int P = ntok * topk, nblk = sort_blocks(P);
-    const int64_t n = ((int64_t)P + SORT_SUB - 1) / SORT_SUB;
-    const int chunk = (int)((n + nblk - 1) / nblk) * SORT_SUB;
-    const size_t sm = (size_t)n_experts * (sizeof(int) + SORT_WARPS * sizeof(uint16_t));
     static bool attr_of[64] = {};
     bool &attr = attr_of[cur_dev()];
     if (!attr) {
-        K3C_TRY_CUDA(cudaFuncSetAttribute(k_sort_place, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                          SORT_EMAX * (int)(sizeof(int) + SORT_WARPS * sizeof(uint16_t))));
+        const int most = SORT_EMAX * (int)(sizeof(int) + SORT_WARPS * sizeof(uint16_t));
+        K3C_TRY_CUDA(cudaFuncSetAttribute(k_sort_one, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+        K3C_TRY_CUDA(cudaFuncSetAttribute(k_sort_place, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
         attr = true;
     }
-    if (nblk > 1) {
-        k_sort_count<<<nblk, SORT_TH, n_experts * sizeof(int), s>>>((int *)scratch, idx, P, n_experts, chunk);
+    auto table = [&](int warps) { return (size_t)n_experts * sizeof(int) + ((size_t)n_experts * warps + 1) / 2 * 4; };
+    if (nblk == 1) {
+        const int warps = (P + SORT_ONE * 32 - 1) / (SORT_ONE * 32);
+        k_sort_one<<<1, SORT_TH, table(warps), s>>>(pos, pair, off, idx, P, n_experts, warps);
         K3C_CHECK_LAUNCH();
+        return K3C_OK;
     }
-    k_sort_place<<<nblk, SORT_TH, sm, s>>>(pos, pair, off, idx, (const int *)scratch, P, n_experts, chunk, nblk);
+    const int64_t n = ((int64_t)P + SORT_SUB - 1) / SORT_SUB;
+    const int chunk = (int)((n + nblk - 1) / nblk) * SORT_SUB;
+    k_sort_count<<<nblk, SORT_TH, n_experts * sizeof(int), s>>>((int *)scratch, idx, P, n_experts, chunk);
+    K3C_CHECK_LAUNCH();
+    K3C_TRY_CUDA(launch_pdl(k_sort_place, dim3(nblk), dim3(SORT_TH), table(SORT_WARPS), s, pos, pair, off, idx,
+                            (const int *)scratch, P, n_experts, chunk));
     K3C_CHECK_LAUNCH();
     return K3C_OK;
 }

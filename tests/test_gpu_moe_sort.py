@@ -64,7 +64,8 @@ def routing(T, K, E, kind, seed):
 
 @pytest.mark.parametrize("kind", ["distinct", "repeats", "one", "none", "holes"])
 @pytest.mark.parametrize("T,K,E", [(1, 1, 1), (1, 8, 384), (3, 5, 7), (128, 8, 32), (129, 8, 33), (512, 8, 384),
-                                   (1024, 8, 384), (1025, 8, 384), (2053, 6, 1500), (5000, 1, 2048), (9001, 7, 13)])
+                                   (1024, 8, 384), (1025, 8, 384), (2053, 6, 1500), (5000, 1, 2048), (9001, 7, 13),
+                                   (513, 64, 7), (1000, 64, 383)])
 def test_sort(k3, dev, T, K, E, kind):
     import torch
     idx = routing(T, K, E, kind, T + K + E)

@@ -33,7 +33,8 @@ def test_sort_refusals(k3):
                        ((BUF, BUF, BUF, BUF, 4096, 8, 4, BUF + 1, 1 << 20, None), "scratch")):
         assert L.k3c_moe_sort(*args) == -1 and word in err(k3), (args, err(k3))
     assert L.k3c_moe_sort_scratch(16, 8, 384) == 0
-    assert L.k3c_moe_sort_scratch(4096, 8, 384) == 8 * 384 * 4
+    assert L.k3c_moe_sort_scratch(1024, 8, 384) == 0
+    assert L.k3c_moe_sort_scratch(4096, 8, 384) == 16 * 384 * 4
     assert L.k3c_moe_sort_scratch(-1, 8, 384) == 0
 
 
