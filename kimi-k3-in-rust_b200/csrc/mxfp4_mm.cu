@@ -874,10 +874,9 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm_pair(const __grid_cons
 // one ring for all three a slot was held through copy, widening and MMA, 3900 cycles for 1024
 // of MMAs: three slots' worth of them set the pace.
 constexpr int MB_KB = 64;                        // W rows per K block
-constexpr int MB_GROUP = 8;                      // warps that widen one K block; two groups take turns
+constexpr int MB_GROUP = 4;                      // warps that widen one K block; groups take turns
 constexpr int MB_EPI = 8;
-constexpr int MB_WIDE0 = 3, MB_EPI0 = MB_WIDE0 + 2 * MB_GROUP;   // warps: dY, MMA, W, widening, epilogue
-constexpr int MB_THREADS = 32 * (MB_EPI0 + MB_EPI);
+constexpr int MB_WIDE0 = 3;                      // warps: dY, MMA, W, widening, epilogue
 // MT rows x NT columns (W's in) per item. 256 x 256: two accumulators of 128 rows share a widened
 // W tile, 1024 cycles of MMAs for it. 128 x 256: for groups of few rows, whose time is W's way
 // through the SM; the room goes to packed tiles in flight and a second accumulator. 128 x 128:
@@ -890,11 +889,17 @@ struct MbCfg {
     static constexpr int W = MB_KB * WB;
     static constexpr int R = (W + NT / 128 * 512 + 1023) / 1024 * 1024;   // and its scale atoms
     static constexpr int RING = NT == 256 ? 3 : 4;           // slots of dY and widened W
-    static constexpr int RAW = MT == 256 ? 3 : NT == 256 ? 8 : 15;        // slots of packed W
+    static constexpr int RAW = MT == 256 ? 3 : NT == 256 ? 6 : 12;        // slots of packed W
+    // Groups of widening warps. Both rings hold a multiple of TURNS, so a slot is always the same
+    // group's, which then awaits each of the slot's phases in turn: a group that skipped a phase
+    // could take the one before it, of the same parity, for the one it needs.
+    static constexpr int TURNS = RING;
+    static constexpr int EPI0 = MB_WIDE0 + TURNS * MB_GROUP, THREADS = 32 * (EPI0 + MB_EPI);
     static constexpr int ACC = MT / 128 * NT;                // TMEM columns of an item
     static constexpr int NACC = 512 / ACC < 2 ? 1 : 2;
     static constexpr int BYTES = 1024 + RING * (A + B) + RAW * R + 512;
     static_assert(A % 1024 == 0 && B % 1024 == 0, "slots stay 1024-byte aligned");
+    static_assert(RING % TURNS == 0 && RAW % TURNS == 0, "a slot belongs to one group");
     static_assert((3 * RING + 2 * RAW + 2 * NACC) * 8 + 4 <= 512, "barriers");
     static_assert(BYTES + sizeof(Plan) + 64 <= 227 * 1024, "one CTA per SM");
 };
@@ -971,7 +976,7 @@ __device__ __forceinline__ void put8(const MxArgs &p, int64_t row, int col, cons
 }
 
 template <int MT, int NT>
-__global__ void __launch_bounds__(MB_THREADS, 1) k_mx4_bwd(const __grid_constant__ CUtensorMap tmD,
+__global__ void __launch_bounds__(MbCfg<MT, NT>::THREADS, 1) k_mx4_bwd(const __grid_constant__ CUtensorMap tmD,
                                                            const __grid_constant__ CUtensorMap tmD1,
                                                            const __grid_constant__ CUtensorMap tmW, MxArgs p) {
     using C = MbCfg<MT, NT>;
@@ -1009,7 +1014,7 @@ __global__ void __launch_bounds__(MB_THREADS, 1) k_mx4_bwd(const __grid_constant
     tc::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     grid_dep_wait();
-    const int tiles = plan_tiles<MB_THREADS>(plan, p.off, p.G, p.M, MT);
+    const int tiles = plan_tiles<C::THREADS>(plan, p.off, p.G, p.M, MT);
     const int n_items = tiles * p.NTL;
     const int KB = (p.N + MB_KB - 1) / MB_KB;      // contracted: W's rows
     const int KA = (p.K + 127) / 128;
@@ -1106,7 +1111,7 @@ __global__ void __launch_bounds__(MB_THREADS, 1) k_mx4_bwd(const __grid_constant
                 }
             }
         }
-    } else if (warp >= MB_WIDE0 && warp < MB_EPI0) {
+    } else if (warp >= MB_WIDE0 && warp < C::EPI0) {
         // ------------------------------------------------------------ widening
         const int w4 = (warp - MB_WIDE0) % MB_GROUP;
         const uint32_t turn = (warp - MB_WIDE0) / MB_GROUP;
@@ -1116,51 +1121,57 @@ __global__ void __launch_bounds__(MB_THREADS, 1) k_mx4_bwd(const __grid_constant
             const Item x = item(it);
             if (x.mat < 0) continue;
             for (int kb = 0; ok && kb < KB; kb++, n++) {
-                if ((n & 1u) == turn) {
+                if (n % C::TURNS == turn) {
                     ok = __all_sync(0xFFFFFFFFu, tc::mbar_wait(&rfull[rt], rph, p.err, 98));
                     if (!ok) break;
-                    // a lane widens 32 codes of W row r in each 128 columns: groups g and g + 4 (eight
-                    // lanes touch eight rows: the swizzle spreads them over the banks)
-                    constexpr int GH = NT / 128;
+                    // a lane widens 32 codes of MB_RJ W rows in each 128 columns: groups g and g + 4
+                    // (eight lanes touch eight rows: the swizzle spreads them over the banks)
+                    constexpr int GH = NT / 128, RJ = 8 / MB_GROUP;
                     const uint8_t *sw = s_r + rt * C::R;
-                    const int r = 8 * w4 + (lane & 7), g = lane >> 3;
-                    uint4 c[GH];
-                    uint32_t s[GH];
+                    const int r0 = 8 * RJ * w4 + (lane & 7), g = lane >> 3;
+                    uint4 c[RJ][GH];
+                    uint32_t s[RJ][GH];
 #pragma unroll
-                    for (int i = 0; i < GH; i++) {
-                        const int at = NT == 256 ? (g + 4 * i) ^ (r & 7) : g ^ ((r >> 1) & 3);   // 128- and 64-byte swizzle
-                        c[i] = *reinterpret_cast<const uint4 *>(sw + r * C::WB + 16 * at);
-                        s[i] = sw[C::W + i * 512 + sf_byte((kb & 1) * 64 + r, g)];
-                    }
+                    for (int j = 0; j < RJ; j++)
+#pragma unroll
+                        for (int i = 0; i < GH; i++) {
+                            const int r = r0 + 8 * j;
+                            const int at = NT == 256 ? (g + 4 * i) ^ (r & 7) : g ^ ((r >> 1) & 3);   // 128- and 64-byte swizzle
+                            c[j][i] = *reinterpret_cast<const uint4 *>(sw + r * C::WB + 16 * at);
+                            s[j][i] = sw[C::W + i * 512 + sf_byte((kb & 1) * 64 + r, g)];
+                        }
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(&rempty[rt]);
                     ok = __all_sync(0xFFFFFFFFu, tc::mbar_wait(&empty[st], ph, p.err, 99));
                     if (!ok) break;
                     uint8_t *sb = s_b + st * C::B;
 #pragma unroll
-                    for (int i = 0; i < GH; i++) {
-                        const uint32_t e = min(s[i], 128u) + 126u;    // 2^(min(byte, 128) - 1)
-                        const uint32_t f1 = e << 7 | e << 23;
-                        const uint32_t cw[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
-                        uint32_t o[4][4];
+                    for (int j = 0; j < RJ; j++)
 #pragma unroll
-                        for (int k = 0; k < 4; k++) e2m1x8_widen(cw[k], f1, o[k]);
-                        if (s[i] > 128) {                             // the rest of a scale above 2^1
-                            const uint32_t h = s[i] - 1u, f2 = h << 7 | h << 23;   // 2^(byte - 128)
+                        for (int i = 0; i < GH; i++) {
+                            const int r = r0 + 8 * j;
+                            const uint32_t e = min(s[j][i], 128u) + 126u;    // 2^(min(byte, 128) - 1)
+                            const uint32_t f1 = e << 7 | e << 23;
+                            const uint32_t cw[4] = {c[j][i].x, c[j][i].y, c[j][i].z, c[j][i].w};
+                            uint32_t o[4][4];
 #pragma unroll
-                            for (int k = 0; k < 4; k++)
+                            for (int k = 0; k < 4; k++) e2m1x8_widen(cw[k], f1, o[k]);
+                            if (s[j][i] > 128) {                             // the rest of a scale above 2^1
+                                const uint32_t h = s[j][i] - 1u, f2 = h << 7 | h << 23;   // 2^(byte - 128)
 #pragma unroll
-                                for (int q = 0; q < 4; q++) o[k][q] = mul_bf16x2(o[k][q], f2);
+                                for (int k = 0; k < 4; k++)
+#pragma unroll
+                                    for (int q = 0; q < 4; q++) o[k][q] = mul_bf16x2(o[k][q], f2);
+                            }
+                            // Column order within the 32: piece q holds codes q and q + 4 of each of
+                            // the four words, so that a lane of the epilogue's 16x256b loads, which
+                            // gets columns 2l and 2l + 1 of every piece, gets word l: eight neighbours.
+                            uint8_t *row = sb + ((g + 4 * i) >> 1) * (MB_KB * 128) + r * 128;
+#pragma unroll
+                            for (int q = 0; q < 4; q++)
+                                *reinterpret_cast<uint4 *>(row + 16 * (((g & 1) * 4 + q) ^ (r & 7))) =
+                                    make_uint4(o[0][q], o[1][q], o[2][q], o[3][q]);
                         }
-                        // Column order within the 32: piece q holds codes q and q + 4 of each of the
-                        // four words, so that a lane of the epilogue's 16x256b loads, which gets
-                        // columns 2l and 2l + 1 of every piece, gets word l: eight neighbours.
-                        uint8_t *row = sb + ((g + 4 * i) >> 1) * (MB_KB * 128) + r * 128;
-#pragma unroll
-                        for (int q = 0; q < 4; q++)
-                            *reinterpret_cast<uint4 *>(row + 16 * (((g & 1) * 4 + q) ^ (r & 7))) =
-                                make_uint4(o[0][q], o[1][q], o[2][q], o[3][q]);
-                    }
                     tc::fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(&wide[st]);
@@ -1175,11 +1186,11 @@ __global__ void __launch_bounds__(MB_THREADS, 1) k_mx4_bwd(const __grid_constant
                 }
             }
         }
-    } else if (warp >= MB_EPI0) {
+    } else if (warp >= C::EPI0) {
         // ------------------------------------------------------------ epilogue
         // A store covers 8 rows x 64 bytes (bf16); with a row per lane it was 32 rows x 16, and
         // the accumulators stayed taken for 12000 cycles an item instead of EPI_CYCLES.
-        const int q = warp & 3, half = (warp - MB_EPI0) >> 2;   // TMEM lane quadrant; accumulator or half of the columns
+        const int q = warp & 3, half = (warp - C::EPI0) >> 2;   // TMEM lane quadrant; accumulator or half of the columns
         const uint32_t lanes = (uint32_t)(32 * q) << 16;
         uint32_t a = 0, aph = 0;
         bool alive = true;
@@ -1369,7 +1380,7 @@ int launch_bwd(MxArgs p, const k3c_mxfp4_mat *W, const void *dy, int64_t lddy, c
     const int64_t items = most_tiles(p.M, p.G, MT) * p.NTL;
     K3C_TRY(check_items("mxfp4_mm_bwd", items));
     const int grid = (int)(items < sm_count() ? items : sm_count());
-    K3C_TRY_CUDA(launch_pdl(k_mx4_bwd<MT, NT>, dim3(grid), dim3(MB_THREADS), C::BYTES, s, md, md1, mw, p));
+    K3C_TRY_CUDA(launch_pdl(k_mx4_bwd<MT, NT>, dim3(grid), dim3(C::THREADS), C::BYTES, s, md, md1, mw, p));
     K3C_CHECK_LAUNCH();
     return K3C_OK;
 }
