@@ -877,44 +877,54 @@ constexpr int MB_KB = 64;                        // W rows per K block
 constexpr int MB_GROUP = 4;                      // warps that widen one K block; groups take turns
 constexpr int MB_EPI = 8;
 constexpr int MB_WIDE0 = 3;                      // warps: dY, MMA, W, widening, epilogue
-// MT rows x NT columns (W's in) per item. 256 x 256: two accumulators of 128 rows share a widened
-// W tile, 1024 cycles of MMAs for it. 128 x 256: for groups of few rows, whose time is W's way
-// through the SM; the room goes to packed tiles in flight and a second accumulator. 128 x 128:
-// more items, when there are too few for every SM.
-template <int MT, int NT>
+// 128 rows x NT columns (W's in) per CTA and item; columns narrower than 256 make more items where
+// there are too few for every SM. PAIR: two CTAs with 128 rows each on the same 2 * NT columns
+// (cta_group::2); each widens NT of them and the MMA reads both CTAs' halves. Shared memory's
+// bandwidth bounds these kernels: a K block of 128 x 256 takes one CTA 121 KB through it (copies
+// in, packed tile out, widened tile in, both operands out), 950 cycles at 128 bytes a cycle, for
+// 512 cycles of MMAs; a pair's CTA 73 KB, 580 cycles.
+template <int NT, bool PAIR>
 struct MbCfg {
-    static constexpr int A = MT * 128;                       // dY: MT rows x 64 bf16
+    static constexpr int TN = PAIR ? 2 * NT : NT;            // columns of an item
+    static constexpr int A = 128 * 128;                      // dY: 128 rows x 64 bf16
     static constexpr int B = NT * MB_KB * 2;                 // widened W: NT/64 blocks of 64 columns x 64 rows
     static constexpr int WB = NT / 2;                        // bytes of a packed W row
     static constexpr int W = MB_KB * WB;
     static constexpr int R = (W + NT / 128 * 512 + 1023) / 1024 * 1024;   // and its scale atoms
     static constexpr int RING = NT == 256 ? 3 : 4;           // slots of dY and widened W
-    static constexpr int RAW = MT == 256 ? 3 : NT == 256 ? 6 : 12;        // slots of packed W
+    static constexpr int RAW = NT == 256 ? 6 : 12;           // slots of packed W
     // Groups of widening warps. Both rings hold a multiple of TURNS, so a slot is always the same
     // group's, which then awaits each of the slot's phases in turn: a group that skipped a phase
     // could take the one before it, of the same parity, for the one it needs.
     static constexpr int TURNS = RING;
     static constexpr int EPI0 = MB_WIDE0 + TURNS * MB_GROUP, THREADS = 32 * (EPI0 + MB_EPI);
-    static constexpr int ACC = MT / 128 * NT;                // TMEM columns of an item
-    static constexpr int NACC = 512 / ACC < 2 ? 1 : 2;
     static constexpr int BYTES = 1024 + RING * (A + B) + RAW * R + 512;
-    static_assert(A % 1024 == 0 && B % 1024 == 0, "slots stay 1024-byte aligned");
+    static_assert(B % 1024 == 0, "slots stay 1024-byte aligned");
     static_assert(RING % TURNS == 0 && RAW % TURNS == 0, "a slot belongs to one group");
-    static_assert((3 * RING + 2 * RAW + 2 * NACC) * 8 + 4 <= 512, "barriers");
+    static_assert((4 * RING + 2 * RAW + 4) * 8 + 4 <= 512, "barriers");
     static_assert(BYTES + sizeof(Plan) + 64 <= 227 * 1024, "one CTA per SM");
 };
 
-// kind::f16: bf16 A (K-major) and B (N-major: transpose bit 16), fp32 accumulator, M = 128.
-__host__ __device__ constexpr uint32_t idesc_bf16_tb(uint32_t n) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+// kind::f16: bf16 A (K-major) and B (N-major: transpose bit 16), fp32 accumulator.
+__host__ __device__ constexpr uint32_t idesc_bf16_tb(uint32_t m, uint32_t n) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
+template <bool PAIR>
 __device__ __forceinline__ void tc_mma_bf16(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
-        : "memory");
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+            : "memory");
 }
 // N-major operand, 128-byte swizzle: rows of 64 N-elements, 8 of the contracted index per 1024
 // bytes (SBO), blocks of 64 N-elements MB_KB * 128 bytes apart (LBO).
@@ -975,58 +985,73 @@ __device__ __forceinline__ void put8(const MxArgs &p, int64_t row, int col, cons
     }
 }
 
-template <int MT, int NT>
-__global__ void __launch_bounds__(MbCfg<MT, NT>::THREADS, 1) k_mx4_bwd(const __grid_constant__ CUtensorMap tmD,
+template <int NT, bool PAIR>
+__global__ void __launch_bounds__(MbCfg<NT, PAIR>::THREADS, 1) k_mx4_bwd(const __grid_constant__ CUtensorMap tmD,
                                                            const __grid_constant__ CUtensorMap tmD1,
                                                            const __grid_constant__ CUtensorMap tmW, MxArgs p) {
-    using C = MbCfg<MT, NT>;
+    using C = MbCfg<NT, PAIR>;
     extern __shared__ uint8_t mb_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)mb_raw + 1023) & ~(uintptr_t)1023);
     uint8_t *s_a = smem, *s_b = s_a + C::RING * C::A, *s_r = s_b + C::RING * C::B;
     uint64_t *afull = reinterpret_cast<uint64_t *>(s_r + C::RAW * C::R);
-    uint64_t *wide = afull + C::RING, *empty = wide + C::RING, *rfull = empty + C::RING, *rempty = rfull + C::RAW;
-    uint64_t *tfull = rempty + C::RAW, *tempty = tfull + C::NACC;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tempty + C::NACC);
+    uint64_t *wide = afull + C::RING, *empty = wide + C::RING, *pfull = empty + C::RING;
+    uint64_t *rfull = pfull + C::RING, *rempty = rfull + C::RAW;
+    uint64_t *tfull = rempty + C::RAW, *tempty = tfull + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tempty + 2);
     __shared__ Plan plan;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = PAIR ? tc::cluster_ctarank() : 0u;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::RING; i++) {
             tc::mbar_init(&afull[i], 1);
             tc::mbar_init(&wide[i], MB_GROUP);
             tc::mbar_init(&empty[i], 1);
+            tc::mbar_init(&pfull[i], 1);
         }
         for (int i = 0; i < C::RAW; i++) {
             tc::mbar_init(&rfull[i], 1);
             tc::mbar_init(&rempty[i], MB_GROUP);
         }
-        for (int i = 0; i < C::NACC; i++) {
+        for (int i = 0; i < 2; i++) {
             tc::mbar_init(&tfull[i], 1);
-            tc::mbar_init(&tempty[i], MB_EPI);
+            tc::mbar_init(&tempty[i], (PAIR ? 2 : 1) * MB_EPI);
         }
         tc::fence_mbar_init();
         tc::prefetch_tmap(&tmD);
         tc::prefetch_tmap(&tmW);
     }
-    if (warp == 1) tc::tmem_alloc(tmem_slot, 512);
+    if (warp == 1) {
+        if constexpr (PAIR) tmem_alloc_pair(tmem_slot, 512);
+        else tc::tmem_alloc(tmem_slot, 512);
+    }
     tc::tc_fence_before();
     __syncthreads();
+    if constexpr (PAIR) tc::cluster_sync();   // both CTAs' barriers and TMEM are there
     tc::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     grid_dep_wait();
-    const int tiles = plan_tiles<C::THREADS>(plan, p.off, p.G, p.M, MT);
+    const int tiles = plan_tiles<C::THREADS>(plan, p.off, p.G, p.M, PAIR ? 256 : 128);
     const int n_items = tiles * p.NTL;
     const int KB = (p.N + MB_KB - 1) / MB_KB;      // contracted: W's rows
     const int KA = (p.K + 127) / 128;
-    Walk walk{plan, p.mat_of, p.n_mats, p.G, p.NTL, MT};
-    auto item = [&](int it) { return walk.at(it); };   // a thread takes one role
+    const int it0 = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
+    Walk walk{plan, p.mat_of, p.n_mats, p.G, p.NTL, PAIR ? 256 : 128};
+    auto item = [&](int it) {   // this CTA's rows of an item; a thread takes one role
+        Item x = walk.at(it);
+        if constexpr (PAIR) {
+            x.row0 += rank * 128;
+            x.n = min(max(x.n - (int)rank * 128, 0), 128);
+        }
+        return x;
+    };
 
     if (warp == 0) {
         // ------------------------------------------------------------ dY copies
         if (elect_one()) {
             bool ok = tc::tc_check((tc::smem_u32(smem) & 1023) == 0, p.err, 90);
             uint32_t st = 0, ph = 1, n = 0;
-            for (int it = blockIdx.x; ok && it < n_items; it += gridDim.x) {
+            for (int it = it0; ok && it < n_items; it += step) {
                 const Item x = item(it);
                 if (x.mat < 0) continue;
                 const int boxes = (x.n + 31) / 32;
@@ -1034,10 +1059,9 @@ __global__ void __launch_bounds__(MbCfg<MT, NT>::THREADS, 1) k_mx4_bwd(const __g
                     if (!tc::mbar_wait(&empty[st], ph, p.err, 91)) { ok = false; break; }
                     uint8_t *sa = s_a + st * C::A;
                     tc::mbar_expect_tx(&afull[st], boxes * 32 * 128);
-                    if (boxes >= 4) tc::tma_load_3d(sa, &tmD, &afull[st], kb * MB_KB, x.row0, 0);
-                    if (MT == 256 && boxes == 8) tc::tma_load_3d(sa + 128 * 128, &tmD, &afull[st], kb * MB_KB, x.row0 + 128, 0);
+                    if (boxes == 4) tc::tma_load_3d(sa, &tmD, &afull[st], kb * MB_KB, x.row0, 0);
                     else
-                        for (int b = boxes & 4; b < boxes; b++)   // the rest of a short tile
+                        for (int b = 0; b < boxes; b++)
                             tc::tma_load_3d(sa + b * (32 * 128), &tmD1, &afull[st], kb * MB_KB, x.row0 + b * 32, 0);
                     if (++st == C::RING) {
                         st = 0;
@@ -1054,17 +1078,18 @@ __global__ void __launch_bounds__(MbCfg<MT, NT>::THREADS, 1) k_mx4_bwd(const __g
         if (elect_one()) {
             bool ok = true;
             uint32_t st = 0, ph = 1, n = 0;
-            for (int it = blockIdx.x; ok && it < n_items; it += gridDim.x) {
+            for (int it = it0; ok && it < n_items; it += step) {
                 const Item x = item(it);
                 if (x.mat < 0) continue;
-                const uint32_t sfb = min(NT / 128, KA - NT / 128 * x.nt) * 512;
-                const uint8_t *wsf = p.atoms + (size_t)x.mat * p.atom_stride + (size_t)(NT / 128 * x.nt) * 512;
+                const int col = x.nt * C::TN + (int)rank * NT;                   // the CTA's first column
+                const uint32_t sfb = min(NT / 128, max(KA - col / 128, 0)) * 512;   // none past W's columns
+                const uint8_t *wsf = p.atoms + (size_t)x.mat * p.atom_stride + (size_t)(col / 128) * 512;
                 for (int kb = 0; kb < KB; kb++, n++) {
                     if (!tc::mbar_wait(&rempty[st], ph, p.err, 93)) { ok = false; break; }
                     uint8_t *sw = s_r + st * C::R;
                     tc::mbar_expect_tx(&rfull[st], C::W + sfb);
-                    tc::tma_load_3d(sw, &tmW, &rfull[st], x.nt * C::WB, kb * MB_KB, x.mat);
-                    tc::bulk_load(sw + C::W, wsf + (size_t)(kb / 2) * KA * 512, sfb, &rfull[st]);
+                    tc::tma_load_3d(sw, &tmW, &rfull[st], col / 2, kb * MB_KB, x.mat);
+                    if (sfb) tc::bulk_load(sw + C::W, wsf + (size_t)(kb / 2) * KA * 512, sfb, &rfull[st]);
                     if (++st == C::RAW) {
                         st = 0;
                         ph ^= 1u;
@@ -1074,38 +1099,55 @@ __global__ void __launch_bounds__(MbCfg<MT, NT>::THREADS, 1) k_mx4_bwd(const __g
             for (uint32_t i = n > C::RAW ? n - C::RAW : 0; i < n; i++)
                 tc::mbar_wait(&rfull[i % C::RAW], (i / C::RAW) & 1u, p.err, 94);
         }
-    } else if (warp == 1) {
-        // ------------------------------------------------------------ MMA
+    } else if (PAIR && warp == 1 && rank != 0) {
+        // ------------------------------------------------------------ filled slots to the first CTA
         if (elect_one()) {
-            uint32_t st = 0, ph = 0, a = 0, aph = 1;
+            uint32_t st = 0, ph = 0;
             bool ok = true;
-            constexpr uint32_t idesc = idesc_bf16_tb(NT);
-            const uint64_t da0 = tc::desc_kmajor_sw128(tc::smem_u32(s_a)), db0 = desc_nmajor_sw128(tc::smem_u32(s_b));
-            for (int it = blockIdx.x; ok && it < n_items; it += gridDim.x) {
-                const Item x = item(it);
-                if (x.mat < 0) continue;
-                if (!tc::mbar_wait(&tempty[a], aph, p.err, 95)) { ok = false; break; }
-                tc::tc_fence_after();
-                const bool two = MT == 256 && x.n > 128;
-                const uint32_t d = tmem + a * C::ACC;
+            for (int it = it0; ok && it < n_items; it += step) {
+                if (item(it).mat < 0) continue;
                 for (int kb = 0; kb < KB; kb++) {
-                    if (!tc::mbar_wait(&afull[st], ph, p.err, 96) || !tc::mbar_wait(&wide[st], ph, p.err, 97)) { ok = false; break; }
-                    tc::tc_fence_after();
-                    const uint64_t da = da0 + st * (C::A >> 4), db = db0 + st * (C::B >> 4);
-#pragma unroll
-                    for (int k = 0; k < 4; k++) tc_mma_bf16(d, da + 2 * k, db + 128 * k, idesc, (kb | k) != 0);
-                    if (two) {
-#pragma unroll
-                        for (int k = 0; k < 4; k++) tc_mma_bf16(d + NT, da + 1024 + 2 * k, db + 128 * k, idesc, (kb | k) != 0);
-                    }
-                    tc::tc_commit(&empty[st]);
+                    if (!tc::mbar_wait(&afull[st], ph, p.err, 101) || !tc::mbar_wait(&wide[st], ph, p.err, 102)) { ok = false; break; }
+                    mbar_arrive_cta(&pfull[st], 0);
                     if (++st == C::RING) {
                         st = 0;
                         ph ^= 1u;
                     }
                 }
-                if (ok) tc::tc_commit(&tfull[a]);
-                if (++a == C::NACC) {
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA
+        if (elect_one()) {
+            uint32_t st = 0, ph = 0, a = 0, aph = 1;
+            bool ok = true;
+            constexpr uint32_t idesc = idesc_bf16_tb(PAIR ? 256 : 128, C::TN);
+            const uint64_t da0 = tc::desc_kmajor_sw128(tc::smem_u32(s_a)), db0 = desc_nmajor_sw128(tc::smem_u32(s_b));
+            for (int it = it0; ok && it < n_items; it += step) {
+                const Item x = item(it);
+                if (x.mat < 0) continue;
+                if (!tc::mbar_wait(&tempty[a], aph, p.err, 95)) { ok = false; break; }
+                tc::tc_fence_after();
+                const uint32_t d = tmem + a * C::TN;
+                for (int kb = 0; kb < KB; kb++) {
+                    if (!tc::mbar_wait(&afull[st], ph, p.err, 96) || !tc::mbar_wait(&wide[st], ph, p.err, 97)) { ok = false; break; }
+                    if (PAIR && !tc::mbar_wait(&pfull[st], ph, p.err, 103)) { ok = false; break; }
+                    tc::tc_fence_after();
+                    const uint64_t da = da0 + st * (C::A >> 4), db = db0 + st * (C::B >> 4);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) tc_mma_bf16<PAIR>(d, da + 2 * k, db + 128 * k, idesc, (kb | k) != 0);
+                    if constexpr (PAIR) tc_commit_pair(&empty[st]);
+                    else tc::tc_commit(&empty[st]);
+                    if (++st == C::RING) {
+                        st = 0;
+                        ph ^= 1u;
+                    }
+                }
+                if (ok) {
+                    if constexpr (PAIR) tc_commit_pair(&tfull[a]);
+                    else tc::tc_commit(&tfull[a]);
+                }
+                if (++a == 2) {
                     a = 0;
                     aph ^= 1u;
                 }
@@ -1117,7 +1159,7 @@ __global__ void __launch_bounds__(MbCfg<MT, NT>::THREADS, 1) k_mx4_bwd(const __g
         const uint32_t turn = (warp - MB_WIDE0) / MB_GROUP;
         uint32_t n = 0, st = 0, ph = 1, rt = 0, rph = 0;   // slot and awaited parity of the two rings
         bool ok = true;
-        for (int it = blockIdx.x; ok && it < n_items; it += gridDim.x) {
+        for (int it = it0; ok && it < n_items; it += step) {
             const Item x = item(it);
             if (x.mat < 0) continue;
             for (int kb = 0; ok && kb < KB; kb++, n++) {
@@ -1190,16 +1232,16 @@ __global__ void __launch_bounds__(MbCfg<MT, NT>::THREADS, 1) k_mx4_bwd(const __g
         // ------------------------------------------------------------ epilogue
         // A store covers 8 rows x 64 bytes (bf16); with a row per lane it was 32 rows x 16, and
         // the accumulators stayed taken for 12000 cycles an item instead of EPI_CYCLES.
-        const int q = warp & 3, half = (warp - C::EPI0) >> 2;   // TMEM lane quadrant; accumulator or half of the columns
+        const int q = warp & 3, half = (warp - C::EPI0) >> 2;   // TMEM lane quadrant, half of the columns
         const uint32_t lanes = (uint32_t)(32 * q) << 16;
         uint32_t a = 0, aph = 0;
         bool alive = true;
-        for (int it = blockIdx.x; it < n_items; it += gridDim.x) {
+        for (int it = it0; it < n_items; it += step) {
             const Item x = item(it);
-            const int r0 = (MT == 256 ? 128 * half : 0) + 32 * q;              // the warp's first row
-            const int first = MT == 256 ? 0 : half * (NT / 2);                 // and its columns of the tile
-            const int c0 = x.nt * NT, last = min(MT == 256 ? NT : first + NT / 2, p.K - c0);   // a multiple of 32
-            const uint32_t taddr = tmem + lanes + a * C::ACC + (MT == 256 ? half * NT : 0);
+            const int r0 = 32 * q;                                             // the warp's first row
+            const int first = half * (C::TN / 2);                              // and its columns of the tile
+            const int c0 = x.nt * C::TN, last = min(first + C::TN / 2, p.K - c0);   // a multiple of 32
+            const uint32_t taddr = tmem + lanes + a * C::TN;
             const bool real = x.mat >= 0;
             if (real) {
                 alive = alive && tc::mbar_wait(&tfull[a], aph, p.err, 100);
@@ -1232,8 +1274,11 @@ __global__ void __launch_bounds__(MbCfg<MT, NT>::THREADS, 1) k_mx4_bwd(const __g
             if (real) {
                 tc::tc_fence_before();
                 __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&tempty[a]);
-                if (++a == C::NACC) {
+                if (lane == 0) {
+                    if constexpr (PAIR) mbar_arrive_cta(&tempty[a], 0);
+                    else tc::mbar_arrive(&tempty[a]);
+                }
+                if (++a == 2) {
                     a = 0;
                     aph ^= 1u;
                 }
@@ -1242,8 +1287,12 @@ __global__ void __launch_bounds__(MbCfg<MT, NT>::THREADS, 1) k_mx4_bwd(const __g
     }
     tc::tc_fence_before();
     __syncthreads();
+    if constexpr (PAIR) tc::cluster_sync();   // the partner's MMAs, commits and arrivals end before this CTA's memory does
     tc::tc_fence_after();
-    if (warp == 1) tc::tmem_dealloc(tmem, 512);
+    if (warp == 1) {
+        if constexpr (PAIR) tmem_dealloc_pair(tmem, 512);
+        else tc::tmem_dealloc(tmem, 512);
+    }
 }
 
 // ------------------------------------------------------------------ host side
@@ -1311,6 +1360,35 @@ int check_items(const char *what, int64_t items) {
 // Row tiles of at most `tile` rows that n_groups groups of M rows can have together.
 int64_t most_tiles(int M, int n_groups, int tile) { return (int64_t)M / tile + (n_groups < M ? n_groups : M); }
 
+// A kernel's tile and what it costs: a launch takes about fixed + waves * (K blocks * block + item)
+// ns, a wave being one item on every SM (or pair of SMs). Fitted to measured launches of M = 1 to
+// 4096 rows, dense and in 48 groups (e.g. 8 K blocks of k3c_mxfp4_mm, 4096 x 7168: pair 33.5 us,
+// 256 columns 33.7, 128 38.8, 64 62; 1 x 7168: 9.5, 7.8, 6.4, 6.7).
+struct TileCost {
+    int rows, cols, ctas, block, item, fixed;
+};
+// The cheapest of n kernels for M rows in n_groups groups (grouped: their sizes are on the device;
+// each is taken to waste half a tile) and `cols` columns, kb K blocks. Ties go to the first.
+int cheapest(const TileCost *t, int n, int M, int n_groups, bool grouped, int cols, int kb) {
+    int best = 0;
+    double least = 0;
+    for (int i = 0; i < n; i++) {
+        double tiles = (M + t[i].rows - 1) / t[i].rows;
+        if (grouped) {
+            const double half = (double)M / t[i].rows + 0.5 * n_groups, few = n_groups < M ? n_groups : M;
+            tiles = half > few ? half : few;
+        }
+        const double items = tiles * ((cols + t[i].cols - 1) / t[i].cols), at_once = sm_count() / t[i].ctas;
+        const double waves = items <= at_once ? 1 : (double)(int64_t)((items + at_once - 1) / at_once);
+        const double ns = t[i].fixed + waves * ((double)kb * t[i].block + t[i].item);
+        if (!i || ns < least) {
+            best = i;
+            least = ns;
+        }
+    }
+    return best;
+}
+
 template <int NT>
 int launch_mm(const CUtensorMap &ma, const CUtensorMap &ma1, const CUtensorMap &mw, MxArgs p, cudaStream_t s) {
     static bool attr_of[64] = {};
@@ -1363,9 +1441,9 @@ int launch_mm_pair(const CUtensorMap &ma, const CUtensorMap &ma1, const CUtensor
     return K3C_OK;
 }
 
-template <int MT, int NT>
+template <int NT, bool PAIR>
 int launch_bwd(MxArgs p, const k3c_mxfp4_mat *W, const void *dy, int64_t lddy, cudaStream_t s) {
-    using C = MbCfg<MT, NT>;
+    using C = MbCfg<NT, PAIR>;
     CUtensorMap md, md1, mw;
     K3C_TRY(make_map3(&md, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dy, p.N, p.M, 1, lddy * 2, (uint64_t)lddy * 2 * p.M, 64, 128));
     K3C_TRY(make_map3(&md1, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dy, p.N, p.M, 1, lddy * 2, (uint64_t)lddy * 2 * p.M, 64, 32));
@@ -1373,14 +1451,19 @@ int launch_bwd(MxArgs p, const k3c_mxfp4_mat *W, const void *dy, int64_t lddy, c
     static bool attr_of[64] = {};
     bool &attr = attr_of[cur_dev()];
     if (!attr) {
-        K3C_TRY_CUDA(cudaFuncSetAttribute(k_mx4_bwd<MT, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES));
+        K3C_TRY_CUDA(cudaFuncSetAttribute(k_mx4_bwd<NT, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES));
         attr = true;
     }
-    p.NTL = (p.K + NT - 1) / NT;
-    const int64_t items = most_tiles(p.M, p.G, MT) * p.NTL;
+    p.NTL = (p.K + C::TN - 1) / C::TN;
+    const int64_t items = most_tiles(p.M, p.G, PAIR ? 256 : 128) * p.NTL;
     K3C_TRY(check_items("mxfp4_mm_bwd", items));
-    const int grid = (int)(items < sm_count() ? items : sm_count());
-    K3C_TRY_CUDA(launch_pdl(k_mx4_bwd<MT, NT>, dim3(grid), dim3(C::THREADS), C::BYTES, s, md, md1, mw, p));
+    if constexpr (PAIR) {
+        const int grid = 2 * (int)(items < sm_count() / 2 ? items : sm_count() / 2);
+        K3C_TRY_CUDA(launch_pairs(k_mx4_bwd<NT, PAIR>, grid, C::THREADS, C::BYTES, s, md, md1, mw, p));
+    } else {
+        const int grid = (int)(items < sm_count() ? items : sm_count());
+        K3C_TRY_CUDA(launch_pdl(k_mx4_bwd<NT, PAIR>, dim3(grid), dim3(C::THREADS), C::BYTES, s, md, md1, mw, p));
+    }
     K3C_CHECK_LAUNCH();
     return K3C_OK;
 }
@@ -1454,20 +1537,18 @@ extern "C" int k3c_mxfp4_mm(void *y, int y_dtype, int64_t ldy, const uint8_t *a,
     p.as = a_scales;
     p.atoms = W->atoms;
     p.atom_stride = W->atom_stride;
-    // CTA pairs on 256 x 256 tiles where the groups have more than 128 rows on average and there
-    // is an item for every pair. Else the widest column tile that still gives every SM an item; with
-    // fewer items a narrower tile spreads W's bytes over more SMs.
-    auto tiles = [&](int mt) { return off ? most_tiles(M, n_groups, mt) : (int64_t)(M + mt - 1) / mt; };
-    const bool pairs = M / n_groups > 128 && tiles(256) * ((p.N + 255) / 256) >= sm_count() / 2;
-    int nt = 256;
-    while (!pairs && nt > 64 && tiles(MM_M) * ((p.N + nt - 1) / nt) < sm_count()) nt /= 2;
+    static const TileCost kinds[] = {{256, 256, 2, 380, 700, 5400},
+                                     {128, 256, 1, 410, 1000, 3950},
+                                     {128, 128, 1, 270, 500, 3650},
+                                     {128, 64, 1, 240, 400, 3400}};
+    const int kind = cheapest(kinds, 4, M, n_groups, off != nullptr, p.N, (p.K + 255) / 256);
     CUtensorMap ma, ma1, mw;
     K3C_TRY(make_map3(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, a, p.K / 2, M, 1, p.K / 2, (uint64_t)(p.K / 2) * M, 128, MM_M));
     K3C_TRY(make_map3(&ma1, CU_TENSOR_MAP_DATA_TYPE_UINT8, a, p.K / 2, M, 1, p.K / 2, (uint64_t)(p.K / 2) * M, 128, MM_ABOX));
-    K3C_TRY(map_weights(&mw, W, 128, pairs ? 128 : nt));
-    if (pairs) K3C_TRY(launch_mm_pair(ma, ma1, mw, p, s));
-    else if (nt == 256) K3C_TRY(launch_mm<256>(ma, ma1, mw, p, s));
-    else if (nt == 128) K3C_TRY(launch_mm<128>(ma, ma1, mw, p, s));
+    K3C_TRY(map_weights(&mw, W, 128, kind == 0 ? 128 : kinds[kind].cols));   // a pair's CTAs copy half the columns each
+    if (kind == 0) K3C_TRY(launch_mm_pair(ma, ma1, mw, p, s));
+    else if (kind == 1) K3C_TRY(launch_mm<256>(ma, ma1, mw, p, s));
+    else if (kind == 2) K3C_TRY(launch_mm<128>(ma, ma1, mw, p, s));
     else K3C_TRY(launch_mm<64>(ma, ma1, mw, p, s));
     return check_waits("mxfp4_mm", p.err, s);
 }
@@ -1498,13 +1579,13 @@ extern "C" int k3c_mxfp4_mm_bwd(void *da, int da_dtype, int64_t ldda, const void
     p.n_mats = W->n_mats;
     p.atoms = W->atoms;
     p.atom_stride = W->atom_stride;
-    // The largest tile whose items still give every SM one; 256 rows only if the groups have more
-    // than 128 on average.
-    auto enough = [&](int mt, int nt) {
-        return (off ? most_tiles(M, n_groups, mt) : (M + mt - 1) / mt) * ((p.K + nt - 1) / nt) >= sm_count();
-    };
-    if (M / n_groups > 128 && enough(256, 256)) K3C_TRY((launch_bwd<256, 256>(p, W, dy, lddy, s)));
-    else if (enough(128, 256)) K3C_TRY((launch_bwd<128, 256>(p, W, dy, lddy, s)));
-    else K3C_TRY((launch_bwd<128, 128>(p, W, dy, lddy, s)));
+    // (112 K blocks: pair 43.8 us at 512 x 7168, 256 columns 69, 128 78; at 64 x 7168 42, 68, 41)
+    static const TileCost kinds[] = {{256, 256, 2, 335, 300, 6300},
+                                     {128, 256, 1, 555, 500, 5900},
+                                     {128, 128, 1, 320, 400, 4800}};
+    const int kind = cheapest(kinds, 3, M, n_groups, off != nullptr, p.K, (p.N + MB_KB - 1) / MB_KB);
+    if (kind == 0) K3C_TRY((launch_bwd<128, true>(p, W, dy, lddy, s)));
+    else if (kind == 1) K3C_TRY((launch_bwd<256, false>(p, W, dy, lddy, s)));
+    else K3C_TRY((launch_bwd<128, false>(p, W, dy, lddy, s)));
     return check_waits("mxfp4_mm_bwd", p.err, s);
 }

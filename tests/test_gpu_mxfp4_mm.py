@@ -145,7 +145,7 @@ def matrices(k3, dev, seed, n, rows, in_):
 
 DENSE = [(1, 1, 32), (1, 64, 64), (2, 65, 96), (1, 7168, 2048), (31, 130, 160), (33, 200, 256), (127, 384, 288),
          (128, 128, 512), (129, 257, 1056), (300, 1000, 3616), (64, 7168, 7168), (1000, 640, 352), (2200, 4100, 64),
-         (5000, 1300, 608), (2100, 2304, 1056), (256, 19000, 256)]
+         (2100, 2304, 1056), (256, 19000, 256), (900, 4100, 4128), (4300, 4100, 1312)]
 
 
 @pytest.mark.parametrize("out", ["f32", "bf16"])
@@ -165,7 +165,7 @@ def test_mm(k3, dev, M, N, K, out):
 
 @pytest.mark.parametrize("out", ["f32", "bf16"])
 @pytest.mark.parametrize("M,N,K", [m for m in DENSE if m[1] % 8 == 0]
-                         + [(4000, 72, 2592), (100, 200, 37920), (300, 136, 19232), (2200, 4096, 64)])
+                         + [(4000, 72, 2592), (128, 200, 60000), (300, 136, 19232), (2200, 4096, 64)])
 def test_mm_bwd(k3, dev, M, N, K, out):
     import torch
     W, w = matrices(k3, dev, 7, 1, N, K)
@@ -180,11 +180,14 @@ def test_mm_bwd(k3, dev, M, N, K, out):
 
 # rows per group: empty groups at both ends and in the middle, groups that end inside a tile, one
 # row, several tiles
-GROUPS = [[700, 0, 900, 1300] + [300] * 30, [0], [1], [0, 0, 5, 0], [1] * 9, [130, 0, 1, 257, 32], [0, 40, 33, 128, 129, 1, 0, 300, 0], [2300, 1]]
+GROUPS = [[0], [1], [0, 0, 5, 0], [1] * 9, [130, 0, 1, 257, 32], [0, 40, 33, 128, 129, 1, 0, 300, 0], [2300, 1]]
+# and sizes that reach every tile shape of both products
+SHAPES = [(g, N, K) for g in GROUPS for N, K in ((64, 32), (200, 416), (520, 1056))] + [
+    ([700, 0, 900, 1300] + [300] * 30, 1304, 1312), ([1000, 0] + [1000] * 7, 2104, 1312), ([9] * 100, 200, 2080),
+    ([100] * 100, 72, 1056)]
 
 
-@pytest.mark.parametrize("N,K", [(64, 32), (200, 416), (520, 1056)])
-@pytest.mark.parametrize("sizes", GROUPS, ids=lambda s: "-".join(map(str, s[:8])))
+@pytest.mark.parametrize("sizes,N,K", SHAPES, ids=lambda v: "-".join(map(str, v[:8])) if isinstance(v, list) else str(v))
 def test_grouped_products(k3, dev, sizes, N, K):
     """Both products over ragged groups; rows behind the last group stay as they were."""
     import torch
