@@ -9,6 +9,7 @@ binding fails loudly when the library is missing.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 
 import numpy as np
@@ -1077,6 +1078,11 @@ def _rows_arg(t, name, dev, dtypes):
     return rows, n, ld
 
 
+@functools.lru_cache(maxsize=256)
+def _sort_scratch(T, K, n_experts):
+    return int(lib().k3c_moe_sort_scratch(T, K, n_experts))
+
+
 def moe_sort(idx, n_experts):
     """Stable sort of a routing's pairs by expert: idx [T][topk] int32 -> (pos [T][topk], pair
     [T * topk], off [n_experts + 1]) int32. pos is a pair's row, -1 for ids outside
@@ -1084,7 +1090,7 @@ def moe_sort(idx, n_experts):
     rt = _runtime(idx)
     dev = idx.get_device()
     T, K = _mat_arg(idx, "idx", dev, (rt.i32,))
-    n = rt.lib.k3c_moe_sort_scratch(T, K, n_experts)
+    n = _sort_scratch(T, K, n_experts)
     pos, pair, off = rt.torch.empty_like(idx), idx.new_empty(T * K), idx.new_empty(max(n_experts, 0) + 1)
     ws = idx.new_empty(n // 4) if n else None
     _launch(rt, "k3c_moe_sort", dev, pos.data_ptr(), pair.data_ptr(), off.data_ptr(), idx.data_ptr(), T, K, n_experts,
@@ -1101,7 +1107,7 @@ def moe_permute(x, pos, out=None):
     T, H, ld = _rows_arg(x, "x", dev, rt.floats)
     K = _mat_arg(pos, "pos", dev, (rt.i32,), T)[1]
     if out is None:
-        out = x.new_empty((T * K, H))
+        out = x.new_empty(T * K, H)
     else:
         _mat_arg(out, "out", dev, (x.dtype,), T * K, H)
     _launch(rt, "k3c_moe_permute", dev, out.data_ptr(), x.data_ptr(), rt.code[x.dtype], ld, pos.data_ptr(), T, K, H)
@@ -1115,7 +1121,7 @@ def moe_permute_bwd(drows, pos, out=None):
     T, K = _mat_arg(pos, "pos", dev, (rt.i32,))
     H = _mat_arg(drows, "drows", dev, rt.floats, T * K)[1]
     if out is None:
-        out = drows.new_empty((T, H))
+        out = drows.new_empty(T, H)
     else:
         _mat_arg(out, "out", dev, (drows.dtype,), T, H)
     _launch(rt, "k3c_moe_permute_bwd", dev, out.data_ptr(), drows.data_ptr(), rt.code[drows.dtype], pos.data_ptr(), T, K, H)
@@ -1129,7 +1135,7 @@ def moe_permute_mxfp4(x, pos):
     dev = x.get_device()
     T, H, ld = _rows_arg(x, "x", dev, rt.floats)
     K = _mat_arg(pos, "pos", dev, (rt.i32,), T)[1]
-    packed, scales = pos.new_empty((T * K, H // 2), dtype=rt.u8), pos.new_empty((T * K, H // 32), dtype=rt.u8)
+    packed, scales = x.new_empty(T * K, H // 2, dtype=rt.u8), x.new_empty(T * K, H // 32, dtype=rt.u8)
     _launch(rt, "k3c_moe_permute_mxfp4", dev, packed.data_ptr(), scales.data_ptr(), x.data_ptr(), rt.code[x.dtype], ld,
             pos.data_ptr(), T, K, H)
     return packed, scales
@@ -1144,7 +1150,7 @@ def moe_unpermute(y, pos, wt, out=None, out_dtype=None):
     H = _mat_arg(y, "y", dev, rt.floats, T * K)[1]
     _mat_arg(wt, "wt", dev, (rt.f32,), T, K)
     if out is None:
-        out = y.new_empty((T, H), dtype=out_dtype or y.dtype)
+        out = y.new_empty(T, H, dtype=out_dtype or y.dtype)
     _mat_arg(out, "out", dev, rt.floats if out_dtype is None else (out_dtype,), T, H)
     if out.dtype not in rt.code:
         raise K3CError(f"out_dtype {out_dtype}: fp32 or bf16")
@@ -1183,7 +1189,7 @@ def mxfp4_quant(x):
     rt = _runtime(x)
     dev = x.get_device()
     M, K, ld = _rows_arg(x, "x", dev, rt.floats)
-    packed, scales = x.new_empty((M, K // 2), dtype=rt.u8), x.new_empty((M, (K + 31) // 32), dtype=rt.u8)
+    packed, scales = x.new_empty(M, K // 2, dtype=rt.u8), x.new_empty(M, (K + 31) // 32, dtype=rt.u8)
     _launch(rt, "k3c_mxfp4_quant", dev, packed.data_ptr(), scales.data_ptr(), x.data_ptr(), rt.code[x.dtype], ld, M, K)
     return packed, scales
 
@@ -1267,7 +1273,7 @@ def _mm_groups(rt, W, off, dev):
 
 def _mm_out(rt, like, M, n, dev, out, out_dtype):
     if out is None:
-        out = like.new_empty((M, n), dtype=out_dtype or rt.torch.bfloat16)
+        out = like.new_empty(M, n, dtype=out_dtype or rt.torch.bfloat16)
     rows, cols, ld = _rows_arg(out, "out", dev, rt.floats if out_dtype is None else (out_dtype,))
     if rows != M or cols != n or out.dtype not in rt.code:
         _bad(out, "out", f"fp32 or bf16 {(M, n)}")
