@@ -59,21 +59,27 @@ __device__ __forceinline__ uint32_t f32x8_to_e2m1(const float *f) {
     return d;
 }
 
+// The scale byte of a group whose largest magnitude has these bits (magnitudes order as their bits,
+// NaN above infinity), and 2^(127-byte); byte 255, a NaN, has no multiplier and zero codes.
+__device__ __forceinline__ uint32_t mx4_scale_byte(uint32_t top) {
+    if (top > 0x7F800000u) return 255;
+    const uint32_t e = top >> 23;
+    return e > 2 ? e - 2 : 0;
+}
+__device__ __forceinline__ float mx4_multiplier(uint32_t byte) { return __uint_as_float((254u - min(byte, 253u)) << 23); }
+
 // Quantises v, returns the scale byte.
 __device__ __forceinline__ uint8_t mx4_quant32(const float (&v)[32], uint4 &codes) {
-    uint32_t top = 0;   // magnitudes order as their bits, NaN above infinity
+    uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < 32; i++) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    if (top > 0x7F800000u) {
-        codes = make_uint4(0, 0, 0, 0);
-        return 255;
-    }
-    const int e = (int)(top >> 23), byte = e > 2 ? e - 2 : 0;
-    const float m = __uint_as_float((uint32_t)(254 - byte) << 23);   // 2^(127-byte), byte <= 253
+    const uint32_t byte = mx4_scale_byte(top);
+    const float m = mx4_multiplier(byte);
     float f[32];
 #pragma unroll
     for (int i = 0; i < 32; i++) f[i] = v[i] * m;
     codes = make_uint4(f32x8_to_e2m1(f), f32x8_to_e2m1(f + 8), f32x8_to_e2m1(f + 16), f32x8_to_e2m1(f + 24));
+    if (byte == 255) codes = make_uint4(0, 0, 0, 0);
     return (uint8_t)byte;
 }
 

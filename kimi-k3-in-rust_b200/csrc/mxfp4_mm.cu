@@ -49,10 +49,69 @@ __device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.w
 __device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // ------------------------------------------------------------------ quantisation
-// One thread per 32-element group.
-template <typename T>
+// Rows of whole groups on 16-byte boundaries: four lanes share a group, so that a warp's loads and
+// stores are contiguous (with a lane per group, 64 bytes apart, L1 was 72% busy and DRAM 56%).
+// QUANT_U pieces of 8 elements per thread, all loaded first. DENSE: rows lie side by side.
+constexpr int QUANT_U = 4;
+template <typename T, bool DENSE>
 __global__ void __launch_bounds__(256) k_mx4_quant(uint8_t *__restrict__ packed, uint8_t *__restrict__ scales,
-                                                   const T *__restrict__ x, int64_t ldx, int rows, int in, int vec) {
+                                                   const T *__restrict__ x, int64_t ldx, int rows, int in) {
+    grid_dep_launch();
+    constexpr int L = sizeof(T) / 2;             // 16-byte loads per piece
+    const size_t per = in / 8, n = (size_t)rows * per;
+    for (size_t b0 = (size_t)blockIdx.x * (256 * QUANT_U); b0 < n; b0 += (size_t)gridDim.x * (256 * QUANT_U)) {   // whole blocks
+        const size_t i0 = b0 + threadIdx.x;
+        uint4 u[QUANT_U][L];
+#pragma unroll
+        for (int k = 0; k < QUANT_U; k++) {
+            const size_t i = i0 + 256 * k;
+            if (i < n) {
+                const T *src = DENSE ? x + i * 8 : x + (i / per) * ldx + (i % per) * 8;
+#pragma unroll
+                for (int l = 0; l < L; l++) u[k][l] = ldg_nc_v4(src + 8 / L * l);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < QUANT_U; k++) {
+            const size_t i = i0 + 256 * k;
+            float f[8];   // of a piece past the end: nothing is stored
+            if constexpr (L == 1) {
+                const uint32_t w[4] = {u[k][0].x, u[k][0].y, u[k][0].z, u[k][0].w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    f[2 * j] = __uint_as_float(w[j] << 16);
+                    f[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+                }
+            } else {
+#pragma unroll
+                for (int l = 0; l < L; l++) {
+                    f[4 * l] = __uint_as_float(u[k][l].x);
+                    f[4 * l + 1] = __uint_as_float(u[k][l].y);
+                    f[4 * l + 2] = __uint_as_float(u[k][l].z);
+                    f[4 * l + 3] = __uint_as_float(u[k][l].w);
+                }
+            }
+            uint32_t top = 0;
+#pragma unroll
+            for (int j = 0; j < 8; j++) top = max(top, __float_as_uint(f[j]) & 0x7FFFFFFFu);
+            // n and the strides are multiples of four pieces: a group's lanes are all here or all not
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            if (i >= n) continue;
+            const uint32_t byte = mx4_scale_byte(top);
+            const float m = mx4_multiplier(byte);
+#pragma unroll
+            for (int j = 0; j < 8; j++) f[j] *= m;
+            reinterpret_cast<uint32_t *>(packed)[i] = byte == 255 ? 0u : f32x8_to_e2m1(f);
+            if ((threadIdx.x & 3) == 0) scales[i / 4] = (uint8_t)byte;
+        }
+    }
+}
+
+// Any other rows: one thread per group.
+template <typename T>
+__global__ void __launch_bounds__(256) k_mx4_quant_any(uint8_t *__restrict__ packed, uint8_t *__restrict__ scales,
+                                                       const T *__restrict__ x, int64_t ldx, int rows, int in) {
     grid_dep_launch();
     const int G = (in + 31) / 32;
     const size_t n = (size_t)rows * G;
@@ -60,17 +119,14 @@ __global__ void __launch_bounds__(256) k_mx4_quant(uint8_t *__restrict__ packed,
         const size_t r = i / G;
         const int g = (int)(i - r * G), left = min(32, in - 32 * g);
         float v[32];
-        mx4_load32(v, x + r * ldx + (size_t)g * 32, left, vec);
+        mx4_load32(v, x + r * ldx + (size_t)g * 32, left, 0);
         uint4 c;
         scales[i] = mx4_quant32(v, c);
         uint8_t *d = packed + r * (in / 2) + (size_t)g * 16;
-        if (vec && left == 32) *reinterpret_cast<uint4 *>(d) = c;
-        else {
-            const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+        const uint32_t w[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
-            for (int b = 0; b < 16; b++)
-                if (2 * b < left) d[b] = (uint8_t)(w[b >> 2] >> (8 * (b & 3)));
-        }
+        for (int b = 0; b < 16; b++)
+            if (2 * b < left) d[b] = (uint8_t)(w[b >> 2] >> (8 * (b & 3)));
     }
 }
 
@@ -1481,12 +1537,22 @@ extern "C" int k3c_mxfp4_quant(uint8_t *packed, uint8_t *scales, const void *x, 
     if (!rows) return K3C_OK;
     if (!packed || !scales || !x) return set_error(K3C_EINVAL, "mxfp4_quant: NULL array");
     cudaStream_t s = (cudaStream_t)stream;
-    const size_t groups = (size_t)rows * ((in + 31) / 32);
-    const unsigned grid = (unsigned)((groups + 255) / 256 < 148 * 64 ? (groups + 255) / 256 : 148 * 64);
     const int esz = x_dtype == K3C_F32 ? 4 : 2;
-    const int vec = al16(x) && al16(packed) && in % 32 == 0 && (ldx * esz) % 16 == 0;
-    if (x_dtype == K3C_F32) k_mx4_quant<<<grid, 256, 0, s>>>(packed, scales, (const float *)x, ldx, rows, in, vec);
-    else k_mx4_quant<<<grid, 256, 0, s>>>(packed, scales, (const uint16_t *)x, ldx, rows, in, vec);
+    const bool wide = al16(x) && ((uintptr_t)packed & 3) == 0 && in % 32 == 0 && (ldx * esz) % 16 == 0;
+    const size_t work = wide ? (size_t)rows * (in / 8) / QUANT_U : (size_t)rows * ((in + 31) / 32);
+    const unsigned grid = (unsigned)(work / 256 + 1 < 148 * 64 ? work / 256 + 1 : 148 * 64);
+    const bool dense = ldx == in || rows == 1;
+    if (x_dtype == K3C_F32) {
+        const float *xf = (const float *)x;
+        if (wide && dense) k_mx4_quant<float, true><<<grid, 256, 0, s>>>(packed, scales, xf, ldx, rows, in);
+        else if (wide) k_mx4_quant<float, false><<<grid, 256, 0, s>>>(packed, scales, xf, ldx, rows, in);
+        else k_mx4_quant_any<<<grid, 256, 0, s>>>(packed, scales, xf, ldx, rows, in);
+    } else {
+        const uint16_t *xb = (const uint16_t *)x;
+        if (wide && dense) k_mx4_quant<uint16_t, true><<<grid, 256, 0, s>>>(packed, scales, xb, ldx, rows, in);
+        else if (wide) k_mx4_quant<uint16_t, false><<<grid, 256, 0, s>>>(packed, scales, xb, ldx, rows, in);
+        else k_mx4_quant_any<<<grid, 256, 0, s>>>(packed, scales, xb, ldx, rows, in);
+    }
     K3C_CHECK_LAUNCH();
     return K3C_OK;
 }
