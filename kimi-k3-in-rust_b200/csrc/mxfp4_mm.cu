@@ -938,17 +938,21 @@ constexpr int MB_WIDE0 = 3;                      // warps: dY, MMA, W, widening,
 // (cta_group::2); each widens NT of them and the MMA reads both CTAs' halves. Shared memory's
 // bandwidth bounds these kernels: a K block of 128 x 256 takes one CTA 121 KB through it (copies
 // in, packed tile out, widened tile in, both operands out), 950 cycles at 128 bytes a cycle, for
-// 512 cycles of MMAs; a pair's CTA 73 KB, 580 cycles.
-template <int NT, bool PAIR>
+// 512 cycles of MMAs; a pair's CTA 73 KB, 580 cycles. ACCS = 2: a pair takes 512 rows in two
+// accumulators, so a widened tile serves both; what that saves is mostly power, which bounds the
+// clock under large products. It leaves no TMEM for the next item's accumulators.
+template <int NT, bool PAIR, int ACCS>
 struct MbCfg {
     static constexpr int TN = PAIR ? 2 * NT : NT;            // columns of an item
-    static constexpr int A = 128 * 128;                      // dY: 128 rows x 64 bf16
+    static constexpr int A = ACCS * 128 * 128;               // dY: 128 rows x 64 bf16 per accumulator
     static constexpr int B = NT * MB_KB * 2;                 // widened W: NT/64 blocks of 64 columns x 64 rows
     static constexpr int WB = NT / 2;                        // bytes of a packed W row
     static constexpr int W = MB_KB * WB;
     static constexpr int R = (W + NT / 128 * 512 + 1023) / 1024 * 1024;   // and its scale atoms
     static constexpr int RING = NT == 256 ? 3 : 4;           // slots of dY and widened W
-    static constexpr int RAW = NT == 256 ? 6 : 12;           // slots of packed W
+    static constexpr int RAW = ACCS == 2 ? 4 : NT == 256 ? 6 : 12;        // slots of packed W
+    static constexpr int NBUF = ACCS == 2 ? 1 : 2;           // items whose accumulators TMEM holds
+    static constexpr int ROWS = (PAIR ? 256 : 128) * ACCS;   // rows of an item
     // Groups of widening warps. Both rings hold a multiple of TURNS, so a slot is always the same
     // group's, which then awaits each of the slot's phases in turn: a group that skipped a phase
     // could take the one before it, of the same parity, for the one it needs.
@@ -956,6 +960,7 @@ struct MbCfg {
     static constexpr int EPI0 = MB_WIDE0 + TURNS * MB_GROUP, THREADS = 32 * (EPI0 + MB_EPI);
     static constexpr int BYTES = 1024 + RING * (A + B) + RAW * R + 512;
     static_assert(B % 1024 == 0, "slots stay 1024-byte aligned");
+    static_assert(NBUF * ACCS * TN <= 512, "TMEM columns");
     static_assert(RING % TURNS == 0 && RAW % TURNS == 0, "a slot belongs to one group");
     static_assert((4 * RING + 2 * RAW + 4) * 8 + 4 <= 512, "barriers");
     static_assert(BYTES + sizeof(Plan) + 64 <= 227 * 1024, "one CTA per SM");
@@ -1041,11 +1046,11 @@ __device__ __forceinline__ void put8(const MxArgs &p, int64_t row, int col, cons
     }
 }
 
-template <int NT, bool PAIR>
-__global__ void __launch_bounds__(MbCfg<NT, PAIR>::THREADS, 1) k_mx4_bwd(const __grid_constant__ CUtensorMap tmD,
+template <int NT, bool PAIR, int ACCS>
+__global__ void __launch_bounds__(MbCfg<NT, PAIR, ACCS>::THREADS, 1) k_mx4_bwd(const __grid_constant__ CUtensorMap tmD,
                                                            const __grid_constant__ CUtensorMap tmD1,
                                                            const __grid_constant__ CUtensorMap tmW, MxArgs p) {
-    using C = MbCfg<NT, PAIR>;
+    using C = MbCfg<NT, PAIR, ACCS>;
     extern __shared__ uint8_t mb_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)mb_raw + 1023) & ~(uintptr_t)1023);
     uint8_t *s_a = smem, *s_b = s_a + C::RING * C::A, *s_r = s_b + C::RING * C::B;
@@ -1069,7 +1074,7 @@ __global__ void __launch_bounds__(MbCfg<NT, PAIR>::THREADS, 1) k_mx4_bwd(const _
             tc::mbar_init(&rfull[i], 1);
             tc::mbar_init(&rempty[i], MB_GROUP);
         }
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < C::NBUF; i++) {
             tc::mbar_init(&tfull[i], 1);
             tc::mbar_init(&tempty[i], (PAIR ? 2 : 1) * MB_EPI);
         }
@@ -1087,20 +1092,16 @@ __global__ void __launch_bounds__(MbCfg<NT, PAIR>::THREADS, 1) k_mx4_bwd(const _
     tc::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     grid_dep_wait();
-    const int tiles = plan_tiles<C::THREADS>(plan, p.off, p.G, p.M, PAIR ? 256 : 128);
+    const int tiles = plan_tiles<C::THREADS>(plan, p.off, p.G, p.M, C::ROWS);
     const int n_items = tiles * p.NTL;
     const int KB = (p.N + MB_KB - 1) / MB_KB;      // contracted: W's rows
     const int KA = (p.K + 127) / 128;
     const int it0 = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
-    Walk walk{plan, p.mat_of, p.n_mats, p.G, p.NTL, PAIR ? 256 : 128};
-    auto item = [&](int it) {   // this CTA's rows of an item; a thread takes one role
-        Item x = walk.at(it);
-        if constexpr (PAIR) {
-            x.row0 += rank * 128;
-            x.n = min(max(x.n - (int)rank * 128, 0), 128);
-        }
-        return x;
-    };
+    Walk walk{plan, p.mat_of, p.n_mats, p.G, p.NTL, C::ROWS};
+    auto item = [&](int it) { return walk.at(it); };   // a thread takes one role
+    // This CTA's rows of an item in accumulator j: 128 j and, in pairs, 256 j + 128 rank on.
+    auto first_row = [&](int j) { return (PAIR ? 256 : 128) * j + (int)rank * 128; };
+    auto row_count = [&](const Item &x, int j) { return min(max(x.n - first_row(j), 0), 128); };
 
     if (warp == 0) {
         // ------------------------------------------------------------ dY copies
@@ -1110,15 +1111,24 @@ __global__ void __launch_bounds__(MbCfg<NT, PAIR>::THREADS, 1) k_mx4_bwd(const _
             for (int it = it0; ok && it < n_items; it += step) {
                 const Item x = item(it);
                 if (x.mat < 0) continue;
-                const int boxes = (x.n + 31) / 32;
+                int boxes[ACCS], all = 0;
+#pragma unroll
+                for (int j = 0; j < ACCS; j++) {
+                    boxes[j] = (row_count(x, j) + 31) / 32;
+                    all += boxes[j];
+                }
                 for (int kb = 0; kb < KB; kb++, n++) {
                     if (!tc::mbar_wait(&empty[st], ph, p.err, 91)) { ok = false; break; }
                     uint8_t *sa = s_a + st * C::A;
-                    tc::mbar_expect_tx(&afull[st], boxes * 32 * 128);
-                    if (boxes == 4) tc::tma_load_3d(sa, &tmD, &afull[st], kb * MB_KB, x.row0, 0);
-                    else
-                        for (int b = 0; b < boxes; b++)
-                            tc::tma_load_3d(sa + b * (32 * 128), &tmD1, &afull[st], kb * MB_KB, x.row0 + b * 32, 0);
+                    tc::mbar_expect_tx(&afull[st], all * 32 * 128);
+#pragma unroll
+                    for (int j = 0; j < ACCS; j++) {
+                        const int row = x.row0 + first_row(j);
+                        if (boxes[j] == 4) tc::tma_load_3d(sa + j * (128 * 128), &tmD, &afull[st], kb * MB_KB, row, 0);
+                        else
+                            for (int b = 0; b < boxes[j]; b++)
+                                tc::tma_load_3d(sa + j * (128 * 128) + b * (32 * 128), &tmD1, &afull[st], kb * MB_KB, row + b * 32, 0);
+                    }
                     if (++st == C::RING) {
                         st = 0;
                         ph ^= 1u;
@@ -1184,7 +1194,8 @@ __global__ void __launch_bounds__(MbCfg<NT, PAIR>::THREADS, 1) k_mx4_bwd(const _
                 if (x.mat < 0) continue;
                 if (!tc::mbar_wait(&tempty[a], aph, p.err, 95)) { ok = false; break; }
                 tc::tc_fence_after();
-                const uint32_t d = tmem + a * C::TN;
+                const uint32_t d = tmem + a * ACCS * C::TN;
+                const bool two = ACCS == 2 && x.n > C::ROWS / 2;
                 for (int kb = 0; kb < KB; kb++) {
                     if (!tc::mbar_wait(&afull[st], ph, p.err, 96) || !tc::mbar_wait(&wide[st], ph, p.err, 97)) { ok = false; break; }
                     if (PAIR && !tc::mbar_wait(&pfull[st], ph, p.err, 103)) { ok = false; break; }
@@ -1192,6 +1203,11 @@ __global__ void __launch_bounds__(MbCfg<NT, PAIR>::THREADS, 1) k_mx4_bwd(const _
                     const uint64_t da = da0 + st * (C::A >> 4), db = db0 + st * (C::B >> 4);
 #pragma unroll
                     for (int k = 0; k < 4; k++) tc_mma_bf16<PAIR>(d, da + 2 * k, db + 128 * k, idesc, (kb | k) != 0);
+                    if (two) {
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            tc_mma_bf16<PAIR>(d + C::TN, da + (128 * 128 >> 4) + 2 * k, db + 128 * k, idesc, (kb | k) != 0);
+                    }
                     if constexpr (PAIR) tc_commit_pair(&empty[st]);
                     else tc::tc_commit(&empty[st]);
                     if (++st == C::RING) {
@@ -1203,7 +1219,7 @@ __global__ void __launch_bounds__(MbCfg<NT, PAIR>::THREADS, 1) k_mx4_bwd(const _
                     if constexpr (PAIR) tc_commit_pair(&tfull[a]);
                     else tc::tc_commit(&tfull[a]);
                 }
-                if (++a == 2) {
+                if (++a == C::NBUF) {
                     a = 0;
                     aph ^= 1u;
                 }
@@ -1287,31 +1303,34 @@ __global__ void __launch_bounds__(MbCfg<NT, PAIR>::THREADS, 1) k_mx4_bwd(const _
     } else if (warp >= C::EPI0) {
         // ------------------------------------------------------------ epilogue
         // A store covers 8 rows x 64 bytes (bf16); with a row per lane it was 32 rows x 16, and
-        // the accumulators stayed taken for 12000 cycles an item instead of EPI_CYCLES.
+        // the accumulators stayed taken for 12000 cycles an item instead of 8600.
         const int q = warp & 3, half = (warp - C::EPI0) >> 2;   // TMEM lane quadrant, half of the columns
         const uint32_t lanes = (uint32_t)(32 * q) << 16;
         uint32_t a = 0, aph = 0;
         bool alive = true;
         for (int it = it0; it < n_items; it += step) {
             const Item x = item(it);
-            const int r0 = 32 * q;                                             // the warp's first row
-            const int first = half * (C::TN / 2);                              // and its columns of the tile
+            const int first = half * (C::TN / 2);                              // the warp's columns of the tile
             const int c0 = x.nt * C::TN, last = min(first + C::TN / 2, p.K - c0);   // a multiple of 32
-            const uint32_t taddr = tmem + lanes + a * C::TN;
+            const uint32_t taddr = tmem + lanes + a * ACCS * C::TN;
             const bool real = x.mat >= 0;
             if (real) {
                 alive = alive && tc::mbar_wait(&tfull[a], aph, p.err, 100);
                 __syncwarp();
                 tc::tc_fence_after();
             }
-            if (r0 < x.n) {
+#pragma unroll
+            for (int j = 0; j < ACCS; j++) {
+                const int n = row_count(x, j) - 32 * q;                        // rows of the warp's 32
+                const int64_t row = x.row0 + first_row(j) + 32 * q;
+                if (n <= 0) continue;
 #pragma unroll 2
                 for (int c = first; c < last; c += 32) {
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {                      // rows r0 + 16h ..
+                    for (int h = 0; h < 2; h++) {                      // rows 16h ..
                         uint32_t v[16];
                         if (real) {
-                            tmem_ld_16x32(taddr + ((uint32_t)(16 * h) << 16) + c, v);
+                            tmem_ld_16x32(taddr + ((uint32_t)(16 * h) << 16) + j * C::TN + c, v);
                             tc::tmem_ld_wait();
                         }
                         if (!real || !alive)
@@ -1319,10 +1338,10 @@ __global__ void __launch_bounds__(MbCfg<NT, PAIR>::THREADS, 1) k_mx4_bwd(const _
                             for (int i = 0; i < 16; i++) v[i] = real ? 0x7FC00000u : 0u;
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
-                            const int r = r0 + 16 * h + 8 * e + (lane >> 2);
+                            const int r = 16 * h + 8 * e + (lane >> 2);
                             const uint32_t u[8] = {v[2 * e], v[2 * e + 1], v[4 + 2 * e], v[5 + 2 * e],
                                                    v[8 + 2 * e], v[9 + 2 * e], v[12 + 2 * e], v[13 + 2 * e]};
-                            if (r < x.n) put8(p, x.row0 + r, c0 + c + 8 * (lane & 3), u);
+                            if (r < n) put8(p, row + r, c0 + c + 8 * (lane & 3), u);
                         }
                     }
                 }
@@ -1334,7 +1353,7 @@ __global__ void __launch_bounds__(MbCfg<NT, PAIR>::THREADS, 1) k_mx4_bwd(const _
                     if constexpr (PAIR) mbar_arrive_cta(&tempty[a], 0);
                     else tc::mbar_arrive(&tempty[a]);
                 }
-                if (++a == 2) {
+                if (++a == C::NBUF) {
                     a = 0;
                     aph ^= 1u;
                 }
@@ -1497,9 +1516,9 @@ int launch_mm_pair(const CUtensorMap &ma, const CUtensorMap &ma1, const CUtensor
     return K3C_OK;
 }
 
-template <int NT, bool PAIR>
+template <int NT, bool PAIR, int ACCS>
 int launch_bwd(MxArgs p, const k3c_mxfp4_mat *W, const void *dy, int64_t lddy, cudaStream_t s) {
-    using C = MbCfg<NT, PAIR>;
+    using C = MbCfg<NT, PAIR, ACCS>;
     CUtensorMap md, md1, mw;
     K3C_TRY(make_map3(&md, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dy, p.N, p.M, 1, lddy * 2, (uint64_t)lddy * 2 * p.M, 64, 128));
     K3C_TRY(make_map3(&md1, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dy, p.N, p.M, 1, lddy * 2, (uint64_t)lddy * 2 * p.M, 64, 32));
@@ -1507,18 +1526,18 @@ int launch_bwd(MxArgs p, const k3c_mxfp4_mat *W, const void *dy, int64_t lddy, c
     static bool attr_of[64] = {};
     bool &attr = attr_of[cur_dev()];
     if (!attr) {
-        K3C_TRY_CUDA(cudaFuncSetAttribute(k_mx4_bwd<NT, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES));
+        K3C_TRY_CUDA(cudaFuncSetAttribute(k_mx4_bwd<NT, PAIR, ACCS>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES));
         attr = true;
     }
     p.NTL = (p.K + C::TN - 1) / C::TN;
-    const int64_t items = most_tiles(p.M, p.G, PAIR ? 256 : 128) * p.NTL;
+    const int64_t items = most_tiles(p.M, p.G, C::ROWS) * p.NTL;
     K3C_TRY(check_items("mxfp4_mm_bwd", items));
     if constexpr (PAIR) {
         const int grid = 2 * (int)(items < sm_count() / 2 ? items : sm_count() / 2);
-        K3C_TRY_CUDA(launch_pairs(k_mx4_bwd<NT, PAIR>, grid, C::THREADS, C::BYTES, s, md, md1, mw, p));
+        K3C_TRY_CUDA(launch_pairs(k_mx4_bwd<NT, PAIR, ACCS>, grid, C::THREADS, C::BYTES, s, md, md1, mw, p));
     } else {
         const int grid = (int)(items < sm_count() ? items : sm_count());
-        K3C_TRY_CUDA(launch_pdl(k_mx4_bwd<NT, PAIR>, dim3(grid), dim3(C::THREADS), C::BYTES, s, md, md1, mw, p));
+        K3C_TRY_CUDA(launch_pdl(k_mx4_bwd<NT, PAIR, ACCS>, dim3(grid), dim3(C::THREADS), C::BYTES, s, md, md1, mw, p));
     }
     K3C_CHECK_LAUNCH();
     return K3C_OK;
@@ -1645,13 +1664,17 @@ extern "C" int k3c_mxfp4_mm_bwd(void *da, int da_dtype, int64_t ldda, const void
     p.n_mats = W->n_mats;
     p.atoms = W->atoms;
     p.atom_stride = W->atom_stride;
-    // (112 K blocks: pair 43.8 us at 512 x 7168, 256 columns 69, 128 78; at 64 x 7168 42, 68, 41)
-    static const TileCost kinds[] = {{256, 256, 2, 335, 300, 6300},
+    // (112 K blocks: pair 43.8 us at 512 x 7168, 256 columns 69, 128 78; at 64 x 7168 42, 68, 41;
+    // the pair's two accumulators 72 us and one 83 at 2400 x 2048, 692 and 824 at 32768 x 2048, but
+    // 64 K blocks 45 and 28 at 1200 x 2048)
+    static const TileCost kinds[] = {{512, 256, 2, 560, 4500, 6300},
+                                     {256, 256, 2, 335, 300, 6300},
                                      {128, 256, 1, 555, 500, 5900},
                                      {128, 128, 1, 320, 400, 4800}};
-    const int kind = cheapest(kinds, 3, M, n_groups, off != nullptr, p.K, (p.N + MB_KB - 1) / MB_KB);
-    if (kind == 0) K3C_TRY((launch_bwd<128, true>(p, W, dy, lddy, s)));
-    else if (kind == 1) K3C_TRY((launch_bwd<256, false>(p, W, dy, lddy, s)));
-    else K3C_TRY((launch_bwd<128, false>(p, W, dy, lddy, s)));
+    const int kind = cheapest(kinds, 4, M, n_groups, off != nullptr, p.K, (p.N + MB_KB - 1) / MB_KB);
+    if (kind == 0) K3C_TRY((launch_bwd<128, true, 2>(p, W, dy, lddy, s)));
+    else if (kind == 1) K3C_TRY((launch_bwd<128, true, 1>(p, W, dy, lddy, s)));
+    else if (kind == 2) K3C_TRY((launch_bwd<256, false, 1>(p, W, dy, lddy, s)));
+    else K3C_TRY((launch_bwd<128, false, 1>(p, W, dy, lddy, s)));
     return check_waits("mxfp4_mm_bwd", p.err, s);
 }

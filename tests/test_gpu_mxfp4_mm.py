@@ -165,7 +165,7 @@ def test_mm(k3, dev, M, N, K, out):
 
 @pytest.mark.parametrize("out", ["f32", "bf16"])
 @pytest.mark.parametrize("M,N,K", [m for m in DENSE if m[1] % 8 == 0]
-                         + [(4000, 72, 2592), (128, 200, 60000), (300, 136, 19232), (2200, 4096, 64)])
+                         + [(4000, 72, 2592), (128, 200, 60000), (300, 136, 19232), (2200, 4096, 64), (2700, 4096, 1824)])
 def test_mm_bwd(k3, dev, M, N, K, out):
     import torch
     W, w = matrices(k3, dev, 7, 1, N, K)
@@ -184,7 +184,7 @@ GROUPS = [[0], [1], [0, 0, 5, 0], [1] * 9, [130, 0, 1, 257, 32], [0, 40, 33, 128
 # and sizes that reach every tile shape of both products
 SHAPES = [(g, N, K) for g in GROUPS for N, K in ((64, 32), (200, 416), (520, 1056))] + [
     ([700, 0, 900, 1300] + [300] * 30, 1304, 1312), ([1000, 0] + [1000] * 7, 2104, 1312), ([9] * 100, 200, 2080),
-    ([100] * 100, 72, 1056)]
+    ([100] * 100, 72, 1056), ([1400, 1, 0, 1290], 4104, 1824)]
 
 
 @pytest.mark.parametrize("sizes,N,K", SHAPES, ids=lambda v: "-".join(map(str, v[:8])) if isinstance(v, list) else str(v))
