@@ -565,7 +565,8 @@ int k3c_moe_combine(float *out, const float *contrib, const float *wt, const int
  * a token's experts one by one, src/core/k3_ops.c:630-645). Pair p = t * topk + j is token t's
  * j-th expert idx[t][j]. An id outside [0, n_experts) (another rank's expert, a dropped one) has
  * no row: pos = -1, and every operator below passes over it. A token may name an expert more
- * than once. ntok may be 0. Nothing here synchronises the host or allocates.
+ * than once. ntok may be 0, topk is at most 64, ntok * topk at most 2^31 - 2^19 - 1. No output
+ * may overlap an input. Nothing here synchronises the host or allocates.
  * ------------------------------------------------------------------------------------ */
 /* Stable sort of the pairs by expert: off[n_experts + 1] first rows (off[n_experts] rows in
  * all), pos[ntok][topk] each pair's row or -1, pair[ntok * topk] each row's pair, -1 behind the
@@ -582,7 +583,8 @@ int k3c_moe_permute(void *rows, const void *x, int dtype, int64_t ldx, const int
  * token without rows gets zeros. */
 int k3c_moe_permute_bwd(void *dx, const void *drows, int dtype, const int *pos, int ntok, int topk,
                         int hidden, k3c_stream_t stream);
-/* The permute and k3c_mxfp4_quant in one pass: packed [ntok * topk][hidden / 2] and scales
+/* The permute and k3c_mxfp4_quant in one pass (its gradient, the quantisation passed straight
+ * through, is k3c_moe_permute_bwd): packed [ntok * topk][hidden / 2] and scales
  * [ntok * topk][hidden / 32] rows, as k3c_mxfp4_mm reads them. hidden a multiple of 32, packed
  * 16-byte aligned. */
 int k3c_moe_permute_mxfp4(uint8_t *packed, uint8_t *scales, const void *x, int x_dtype, int64_t ldx,
@@ -593,7 +595,7 @@ int k3c_moe_unpermute(void *out, int out_dtype, const void *y, int y_dtype, cons
                       int ntok, int topk, int hidden, k3c_stream_t stream);
 /* Its gradients: dy[pos[t][j]] = wt[t][j] * dout[t] (y's type; rows no pair has are left as they
  * were) and dwt[t][j] = <dout[t], y[pos[t][j]]> (fp32; 0 for a pair without a row). Either may be
- * NULL; y is not read when dwt is. dy must not overlap y. */
+ * NULL; y is not read when dwt is. */
 int k3c_moe_unpermute_bwd(void *dy, float *dwt, const void *dout, int out_dtype, const void *y, int y_dtype,
                           const float *wt, const int *pos, int ntok, int topk, int hidden,
                           k3c_stream_t stream);

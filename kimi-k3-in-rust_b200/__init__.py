@@ -1048,6 +1048,14 @@ def _bad(t, name, want):
     raise K3CError(f"{name}: {t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}, expected {want}")
 
 
+def _apart(out, name, *inputs):
+    """A given output is none of the inputs (rows move: nothing can run in place)."""
+    p = out.data_ptr()
+    for t in inputs:
+        if t.data_ptr() == p and p:
+            raise K3CError(f"{name}: may not be an input")
+
+
 def _mat_arg(t, name, dev, dtypes, d0=None, d1=None):
     """A contiguous 2-D tensor on device dev; its extents (None: any)."""
     sh = t.shape
@@ -1110,6 +1118,7 @@ def moe_permute(x, pos, out=None):
         out = x.new_empty(T * K, H)
     else:
         _mat_arg(out, "out", dev, (x.dtype,), T * K, H)
+        _apart(out, "out", x)
     _launch(rt, "k3c_moe_permute", dev, out.data_ptr(), x.data_ptr(), rt.code[x.dtype], ld, pos.data_ptr(), T, K, H)
     return out
 
@@ -1124,6 +1133,7 @@ def moe_permute_bwd(drows, pos, out=None):
         out = drows.new_empty(T, H)
     else:
         _mat_arg(out, "out", dev, (drows.dtype,), T, H)
+        _apart(out, "out", drows)
     _launch(rt, "k3c_moe_permute_bwd", dev, out.data_ptr(), drows.data_ptr(), rt.code[drows.dtype], pos.data_ptr(), T, K, H)
     return out
 
@@ -1151,6 +1161,8 @@ def moe_unpermute(y, pos, wt, out=None, out_dtype=None):
     _mat_arg(wt, "wt", dev, (rt.f32,), T, K)
     if out is None:
         out = y.new_empty(T, H, dtype=out_dtype or y.dtype)
+    else:
+        _apart(out, "out", y, wt)
     _mat_arg(out, "out", dev, rt.floats if out_dtype is None else (out_dtype,), T, H)
     if out.dtype not in rt.code:
         raise K3CError(f"out_dtype {out_dtype}: fp32 or bf16")
@@ -1161,7 +1173,7 @@ def moe_unpermute(y, pos, wt, out=None, out_dtype=None):
 
 def moe_unpermute_bwd(dout, y, pos, wt, dy=None, dwt=None):
     """moe_unpermute's gradients (dy [T * topk][H] of y's type, dwt [T][topk] fp32). Rows of dy no
-    pair has are left as they were (in a new dy: undefined). dy may not be y."""
+    pair has are left as they were (in a new dy: undefined)."""
     rt = _runtime(y)
     dev = y.get_device()
     T, K = _mat_arg(pos, "pos", dev, (rt.i32,))
@@ -1172,12 +1184,12 @@ def moe_unpermute_bwd(dout, y, pos, wt, dy=None, dwt=None):
         dy = rt.torch.empty_like(y)
     else:
         _mat_arg(dy, "dy", dev, (y.dtype,), T * K, H)
-        if dy.data_ptr() == y.data_ptr() and dy.numel():
-            raise K3CError("dy: may not be y")
+        _apart(dy, "dy", y, dout, wt)
     if dwt is None:
         dwt = rt.torch.empty_like(wt)
     else:
         _mat_arg(dwt, "dwt", dev, (rt.f32,), T, K)
+        _apart(dwt, "dwt", y, dout, wt, dy)
     _launch(rt, "k3c_moe_unpermute_bwd", dev, dy.data_ptr(), dwt.data_ptr(), dout.data_ptr(), rt.code[dout.dtype],
             y.data_ptr(), rt.code[y.dtype], wt.data_ptr(), pos.data_ptr(), T, K, H)
     return dy, dwt

@@ -524,7 +524,7 @@ int row_blocks(int ntok, int units) {
 }
 
 int check_pairs(const char *what, int ntok, int topk, int hidden) {
-    if (ntok < 0 || topk < 1 || topk > K3_MAX_TOPK || hidden < 1)
+    if (ntok < 0 || topk < 1 || topk > K3_MAX_TOPK || hidden < 1 || hidden > 1 << 28)
         return set_error(K3C_EINVAL, "%s: ntok=%d topk=%d (1..%d) hidden=%d", what, ntok, topk, K3_MAX_TOPK, hidden);
     if ((int64_t)ntok * topk > 0x7FFFFFFF - 2 * SORT_BLOCKS * SORT_SUB)
         return set_error(K3C_EINVAL, "%s: %d x %d pairs exceed 32 bits", what, ntok, topk);

@@ -255,3 +255,30 @@ def test_captured_and_on_two_streams(k3, dev):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+def test_outputs_may_not_be_inputs(k3, dev):
+    import torch
+    pos = torch.arange(6, dtype=torch.int32, device=dev).view(6, 1)
+    x, wt = torch.randn(6, 32, device=dev), torch.ones(6, 1, device=dev)
+    for call in (lambda: k3.moe_permute(x, pos, out=x), lambda: k3.moe_permute_bwd(x, pos, out=x),
+                 lambda: k3.moe_unpermute(x, pos, wt, out=x), lambda: k3.moe_unpermute_bwd(x, x.clone(), pos, wt, dy=x),
+                 lambda: k3.moe_unpermute_bwd(x, x.clone(), pos, wt, dwt=wt)):
+        with pytest.raises(k3.K3CError, match="may not be an input"):
+            call()
+
+
+def test_offsets_past_32_bits(k3, dev):
+    """Rows more than 4 GiB from the first: 40000 x 8 rows of 14336 bytes."""
+    import torch
+    T, K, E, H = 40000, 8, 3, 7168
+    g = torch.Generator(device=dev).manual_seed(1)
+    idx = torch.randint(0, E, (T, K), generator=g, device=dev, dtype=torch.int32)
+    x = torch.randn(T, H, generator=g, device=dev).bfloat16()
+    pos, pair, off = k3.moe_sort(idx, E)
+    rows = k3.moe_permute(x, pos)
+    last = pair[-2000:].long()
+    assert torch.equal(rows[-2000:], x[last // K])
+    assert torch.equal(rows[pos[::997].long()], x[::997].unsqueeze(1).expand(-1, K, -1))
+    wt = torch.full((T, K), 0.125, device=dev)          # eight equal rows: exact
+    assert torch.equal(k3.moe_unpermute(rows, pos, wt), x)

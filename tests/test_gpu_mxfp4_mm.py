@@ -424,3 +424,44 @@ def test_products_match_the_gemv_and_dequant(k3, dev):
     ref = k3.mxfp4_gemv(k3.mxfp4_dequant(a, sa), p, s)
     mag = np.abs(values(unpack(a.cpu().numpy()), sa.cpu().numpy())) @ np.abs(values(c, b)).T
     assert (np.abs((y - ref).double().cpu().numpy()) <= (K + 16) * 2.0 ** -23 * mag).all()
+
+
+def test_results_past_32_bits(k3, dev):
+    """Product and gradient rows more than 4 GiB from the first, against the same rows alone."""
+    import torch
+    M, N, K = 600000, 4096, 64
+    W, _ = matrices(k3, dev, 81, 1, N, K)
+    g = torch.Generator(device=dev).manual_seed(1)
+    a, s = k3.mxfp4_quant(torch.randn(M, K, generator=g, device=dev))
+    y = k3.mxfp4_mm(a, s, W)
+    assert torch.equal(y[-300:], k3.mxfp4_mm(a[-300:].contiguous(), s[-300:].contiguous(), W))
+    assert torch.equal(y[:300], k3.mxfp4_mm(a[:300].contiguous(), s[:300].contiguous(), W))
+    da = k3.mxfp4_mm_bwd(y, W)
+    assert torch.equal(da[-300:], k3.mxfp4_mm_bwd(y[-300:], W)) and torch.equal(da[:300], k3.mxfp4_mm_bwd(y[:300], W))
+
+
+def test_large_products_on_two_streams(k3, dev):
+    """Kernels of CTA pairs from two streams at once, both products, eager and captured."""
+    import torch
+    W, _ = matrices(k3, dev, 91, 1, 4096, 2048)
+    g = torch.Generator().manual_seed(4)
+    x = [torch.randn((5000, 2048), generator=g).to(dev) for _ in range(2)]
+
+    def chain(t):
+        y = k3.mxfp4_mm(*k3.mxfp4_quant(t), W)
+        return y, k3.mxfp4_mm_bwd(y, W)
+    want = [chain(t) for t in x]
+    torch.cuda.synchronize()
+    st = [torch.cuda.Stream(), torch.cuda.Stream()]
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        cap = chain(x[0])
+    for _ in range(5):
+        got = []
+        for t, q in zip(x, st):
+            with torch.cuda.stream(q):
+                got.append(chain(t))
+        gr.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got + [cap], want + [want[0]]):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
