@@ -1020,6 +1020,10 @@ class _Runtime:
         torch.cuda.init()
         self.device = torch._C._cuda_getDevice
         self.stream = torch._C._cuda_getCurrentRawStream
+        try:     # torch's own short way to an uninitialised tensor on the current device
+            self.empty = torch._C._dynamo.guards._empty_strided_cuda
+        except AttributeError:
+            self.empty = lambda size, stride, dtype: torch.empty_strided(size, stride, dtype=dtype, device="cuda")
 
 
 def _runtime(t):
@@ -1030,6 +1034,14 @@ def _runtime(t):
     if _rt is None:
         _rt = _Runtime()
     return _rt
+
+
+def _new(rt, dev, dtype, rows, cols=None):
+    """An uninitialised contiguous tensor on device dev."""
+    size, stride = ((rows,), (1,)) if cols is None else ((rows, cols), (cols or 1, 1))
+    if rt.device() == dev:
+        return rt.empty(size, stride, dtype)
+    return rt.torch.empty(size, dtype=dtype, device=rt.torch.device("cuda", dev))
 
 
 def _launch(rt, name, dev, *args):
@@ -1099,8 +1111,9 @@ def moe_sort(idx, n_experts):
     dev = idx.get_device()
     T, K = _mat_arg(idx, "idx", dev, (rt.i32,))
     n = _sort_scratch(T, K, n_experts)
-    pos, pair, off = rt.torch.empty_like(idx), idx.new_empty(T * K), idx.new_empty(max(n_experts, 0) + 1)
-    ws = idx.new_empty(n // 4) if n else None
+    pos, pair = _new(rt, dev, rt.i32, T, K), _new(rt, dev, rt.i32, T * K)
+    off = _new(rt, dev, rt.i32, max(n_experts, 0) + 1)
+    ws = _new(rt, dev, rt.i32, n // 4) if n else None
     _launch(rt, "k3c_moe_sort", dev, pos.data_ptr(), pair.data_ptr(), off.data_ptr(), idx.data_ptr(), T, K, n_experts,
             ws.data_ptr() if n else None, n)
     return pos, pair, off
@@ -1115,7 +1128,7 @@ def moe_permute(x, pos, out=None):
     T, H, ld = _rows_arg(x, "x", dev, rt.floats)
     K = _mat_arg(pos, "pos", dev, (rt.i32,), T)[1]
     if out is None:
-        out = x.new_empty(T * K, H)
+        out = _new(rt, dev, x.dtype, T * K, H)
     else:
         _mat_arg(out, "out", dev, (x.dtype,), T * K, H)
         _apart(out, "out", x)
@@ -1130,7 +1143,7 @@ def moe_permute_bwd(drows, pos, out=None):
     T, K = _mat_arg(pos, "pos", dev, (rt.i32,))
     H = _mat_arg(drows, "drows", dev, rt.floats, T * K)[1]
     if out is None:
-        out = drows.new_empty(T, H)
+        out = _new(rt, dev, drows.dtype, T, H)
     else:
         _mat_arg(out, "out", dev, (drows.dtype,), T, H)
         _apart(out, "out", drows)
@@ -1145,10 +1158,18 @@ def moe_permute_mxfp4(x, pos):
     dev = x.get_device()
     T, H, ld = _rows_arg(x, "x", dev, rt.floats)
     K = _mat_arg(pos, "pos", dev, (rt.i32,), T)[1]
-    packed, scales = x.new_empty(T * K, H // 2, dtype=rt.u8), x.new_empty(T * K, H // 32, dtype=rt.u8)
+    packed, scales = _new(rt, dev, rt.u8, T * K, H // 2), _new(rt, dev, rt.u8, T * K, H // 32)
     _launch(rt, "k3c_moe_permute_mxfp4", dev, packed.data_ptr(), scales.data_ptr(), x.data_ptr(), rt.code[x.dtype], ld,
             pos.data_ptr(), T, K, H)
     return packed, scales
+
+
+def _out_type(rt, out_dtype, default):
+    if out_dtype is None:
+        return default
+    if out_dtype not in rt.code:
+        raise K3CError(f"out_dtype {out_dtype}: fp32 or bf16")
+    return out_dtype
 
 
 def moe_unpermute(y, pos, wt, out=None, out_dtype=None):
@@ -1160,12 +1181,10 @@ def moe_unpermute(y, pos, wt, out=None, out_dtype=None):
     H = _mat_arg(y, "y", dev, rt.floats, T * K)[1]
     _mat_arg(wt, "wt", dev, (rt.f32,), T, K)
     if out is None:
-        out = y.new_empty(T, H, dtype=out_dtype or y.dtype)
+        out = _new(rt, dev, _out_type(rt, out_dtype, y.dtype), T, H)
     else:
+        _mat_arg(out, "out", dev, rt.floats if out_dtype is None else (_out_type(rt, out_dtype, None),), T, H)
         _apart(out, "out", y, wt)
-    _mat_arg(out, "out", dev, rt.floats if out_dtype is None else (out_dtype,), T, H)
-    if out.dtype not in rt.code:
-        raise K3CError(f"out_dtype {out_dtype}: fp32 or bf16")
     _launch(rt, "k3c_moe_unpermute", dev, out.data_ptr(), rt.code[out.dtype], y.data_ptr(), rt.code[y.dtype], wt.data_ptr(),
             pos.data_ptr(), T, K, H)
     return out
@@ -1181,12 +1200,12 @@ def moe_unpermute_bwd(dout, y, pos, wt, dy=None, dwt=None):
     _mat_arg(dout, "dout", dev, rt.floats, T, H)
     _mat_arg(wt, "wt", dev, (rt.f32,), T, K)
     if dy is None:
-        dy = rt.torch.empty_like(y)
+        dy = _new(rt, dev, y.dtype, T * K, H)
     else:
         _mat_arg(dy, "dy", dev, (y.dtype,), T * K, H)
         _apart(dy, "dy", y, dout, wt)
     if dwt is None:
-        dwt = rt.torch.empty_like(wt)
+        dwt = _new(rt, dev, rt.f32, T, K)
     else:
         _mat_arg(dwt, "dwt", dev, (rt.f32,), T, K)
         _apart(dwt, "dwt", y, dout, wt, dy)
@@ -1201,7 +1220,7 @@ def mxfp4_quant(x):
     rt = _runtime(x)
     dev = x.get_device()
     M, K, ld = _rows_arg(x, "x", dev, rt.floats)
-    packed, scales = x.new_empty(M, K // 2, dtype=rt.u8), x.new_empty(M, (K + 31) // 32, dtype=rt.u8)
+    packed, scales = _new(rt, dev, rt.u8, M, K // 2), _new(rt, dev, rt.u8, M, (K + 31) // 32)
     _launch(rt, "k3c_mxfp4_quant", dev, packed.data_ptr(), scales.data_ptr(), x.data_ptr(), rt.code[x.dtype], ld, M, K)
     return packed, scales
 
@@ -1283,11 +1302,12 @@ def _mm_groups(rt, W, off, dev):
     return off.data_ptr(), G
 
 
-def _mm_out(rt, like, M, n, dev, out, out_dtype):
+def _mm_out(rt, M, n, dev, out, out_dtype):
+    """(out, its row stride)."""
     if out is None:
-        out = like.new_empty(M, n, dtype=out_dtype or rt.torch.bfloat16)
-    rows, cols, ld = _rows_arg(out, "out", dev, rt.floats if out_dtype is None else (out_dtype,))
-    if rows != M or cols != n or out.dtype not in rt.code:
+        return _new(rt, dev, _out_type(rt, out_dtype, rt.torch.bfloat16), M, n), n
+    rows, cols, ld = _rows_arg(out, "out", dev, rt.floats if out_dtype is None else (_out_type(rt, out_dtype, None),))
+    if rows != M or cols != n:
         _bad(out, "out", f"fp32 or bf16 {(M, n)}")
     return out, ld
 
@@ -1303,7 +1323,7 @@ def mxfp4_mm(a, a_scales, W, off=None, out=None, out_dtype=None):
     M = _mat_arg(a, "a", dev, (rt.u8,), None, W.in_ // 2)[0]
     _mat_arg(a_scales, "a_scales", dev, (rt.u8,), M, W.in_ // 32)
     po, G = _mm_groups(rt, W, off, dev)
-    out, ld = _mm_out(rt, a, M, W.rows, dev, out, out_dtype)
+    out, ld = _mm_out(rt, M, W.rows, dev, out, out_dtype)
     _launch(rt, "k3c_mxfp4_mm", dev, out.data_ptr(), rt.code[out.dtype], ld, a.data_ptr(), a_scales.data_ptr(), M, W.ref, po, G)
     return out
 
@@ -1317,7 +1337,7 @@ def mxfp4_mm_bwd(dy, W, off=None, out=None, out_dtype=None):
     if n != W.rows:
         _bad(dy, "dy", f"{W.rows} columns")
     po, G = _mm_groups(rt, W, off, dev)
-    out, ld = _mm_out(rt, dy, M, W.in_, dev, out, out_dtype)
+    out, ld = _mm_out(rt, M, W.in_, dev, out, out_dtype)
     _launch(rt, "k3c_mxfp4_mm_bwd", dev, out.data_ptr(), rt.code[out.dtype], ld, dy.data_ptr(), ldd, M, W.ref, po, G)
     return out
 
