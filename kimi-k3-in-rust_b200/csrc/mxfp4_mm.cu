@@ -51,6 +51,7 @@ __device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol
 // ------------------------------------------------------------------ quantisation
 // Rows of whole groups on 16-byte boundaries: four lanes share a group, so that a warp's loads and
 // stores are contiguous (with a lane per group, 64 bytes apart, L1 was 72% busy and DRAM 56%).
+// Bound by HBM: 8192 x 7168 bf16 in 24.3 us, 6.1 TB/s.
 // QUANT_U pieces of 8 elements per thread, all loaded first. DENSE: rows lie side by side.
 constexpr int QUANT_U = 4;
 template <typename T, bool DENSE>
@@ -425,7 +426,7 @@ __device__ __forceinline__ void copy_a(const MxArgs &p, int n_items, const ItemF
 // 32+i, 64+i and 96+i and stores the four rows' words of each atom as one 16-byte piece (sf_byte's
 // order). MM_KS K blocks are fetched at a time, while the MM_KS before them are stored, across
 // items. The stores become visible to tcgen05.cp by a proxy fence of the thread that waits on
-// `full`: one here would wait for the fetches in flight. sf: the scales' place in stage 0; item(it)
+// `full`: one here would wait for the fetches in flight. sf0: the scales' place in stage 0; item(it)
 // gives the rows of this CTA.
 template <int STAGES, typename ItemFn>
 __device__ __forceinline__ void a_scales(const MxArgs &p, int n_items, const ItemFn &item, uint8_t *sf0, int stage_bytes,
@@ -505,6 +506,10 @@ __device__ __forceinline__ void a_scales(const MxArgs &p, int n_items, const Ite
     }
 }
 
+// 128 rows x NT columns per item, one CTA per SM. A K block is 256 codes of a row, 128 bytes: four
+// MMAs of K = 64 and two TMEM copies of scale atoms per operand. Bound by HBM for few rows (16 x 8
+// rows over 64 experts of 4096 x 7168: 122 us, the weights at 7.1 TB/s), by the MMA thread's 0.24 us
+// a K block for one tile in a row (one token, 7168 x 7168: 10.4 us), by L2 and power above.
 template <int NT>
 __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant__ CUtensorMap tmA,
                                                           const __grid_constant__ CUtensorMap tmA1,
@@ -683,8 +688,9 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant_
 // ------------------------------------------------------------------ two CTAs on one tile
 // k_mx4_mm on 256 rows x 256 columns per pair of CTAs (cta_group::2): each holds its 128 rows of A
 // and its 128 rows of W, and the MMA reads both halves of W, so an SM fetches 32 KB of codes per
-// 256 x 256 x 128 products instead of 48: at 8192 x 7168 x 7168 those fetches from L2 set the
-// one-CTA kernel's pace (PAIR_FIGURES). W's scales of all 256 columns are in both CTAs.
+// K block instead of 48. 8192 x 7168 x 7168: 155 us, 5.4 PFLOP/s (one CTA 165); 16384 x 7168 x 2048:
+// 113 (141). 470 cycles a K block, the MMAs' own time, at the 1.5 GHz that power leaves; the first
+// blocks of an item and the last wave are the rest. W's scales of all 256 columns are in both CTAs.
 // The pair's first CTA issues all MMAs. Its partner's warp 1 passes each filled stage on: it waits
 // for the local copies, fences A's scales and arrives on pfull in the first CTA. MMA commits free
 // the stage in both.
@@ -1046,6 +1052,9 @@ __device__ __forceinline__ void put8(const MxArgs &p, int64_t row, int col, cons
     }
 }
 
+// Dense 32768 x 7168 x 2048 (rows, contracted, columns): 627 us, 1.53 PFLOP/s, 692 after some
+// seconds at the power limit. 32768 rows in 48 groups: 840-920 us at 1.37 GHz, 600 cycles a K block
+// against 512 of MMAs, 15% of the tiles' rows empty. 2400 rows in 48 groups of 1432 x 992: 32 us.
 template <int NT, bool PAIR, int ACCS>
 __global__ void __launch_bounds__(MbCfg<NT, PAIR, ACCS>::THREADS, 1) k_mx4_bwd(const __grid_constant__ CUtensorMap tmD,
                                                            const __grid_constant__ CUtensorMap tmD1,
