@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(PM_TH) k_unpermute_bwd(T *__restrict__ dy, flo
 // ------------------------------------------------------------------ quantising permute
 // One thread per 32-element group of a token: read and quantised once, its 16 bytes of codes
 // and its scale byte stored into each of the token's rows. Bound by HBM: 4096 x 8 rows of 7168 in
-// 32 us, 5.8 TB/s (the permute and a quantisation of its rows: 88 + 97).
+// 32 us, 5.8 TB/s (the permute and a quantisation of its rows: 88 + 93).
 template <typename T>
 __global__ void __launch_bounds__(PM_TH) k_permute_mx4(uint8_t *__restrict__ packed, uint8_t *__restrict__ scales,
                                                        const T *__restrict__ x, int64_t ldx,

@@ -282,3 +282,15 @@ def test_offsets_past_32_bits(k3, dev):
     assert torch.equal(rows[pos[::997].long()], x[::997].unsqueeze(1).expand(-1, K, -1))
     wt = torch.full((T, K), 0.125, device=dev)          # eight equal rows: exact
     assert torch.equal(k3.moe_unpermute(rows, pos, wt), x)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("first,pad", [(0, 8), (0, 3), (1, 7), (8, 0)])
+def test_permute_of_strided_rows(k3, dev, first, pad, dtype):
+    """x as a slice of wider rows: aligned and odd strides and bases."""
+    import torch
+    T, K, E, H = 50, 3, 6, 72
+    pos, pair, off = k3.moe_sort(torch.from_numpy(routing(T, K, E, "holes", 8)).to(dev), E)
+    n = int(off[-1])
+    x = rand((T, first + H + pad), dtype, 1, dev)[:, first:first + H]
+    assert torch.equal(k3.moe_permute(x, pos)[:n], x[(pair[:n] // K).long()])

@@ -465,3 +465,44 @@ def test_large_products_on_two_streams(k3, dev):
         torch.cuda.synchronize()
         for a, b in zip(got + [cap], want + [want[0]]):
             assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_one_mapped_matrix_for_all_rows_and_no_rows(k3, dev):
+    """Without offsets the rows multiply matrix mat_of[0]; no rows give empty results."""
+    import torch
+    N, K = 72, 96
+    W, w = matrices(k3, dev, 101, 3, N, K)
+    W = k3.Mxfp4Mat(W.keep[0], W.keep[1], mat_of=torch.tensor([2, 0], dtype=torch.int32, device=dev))
+    c, b = operand(102, 10, K)
+    a, s = to_dev(dev, pack_nibbles(c), b)
+    dy = torch.randn(10, N, device=dev).bfloat16()
+    av, dv = values(c, b), dy.double().cpu().numpy()
+    check(k3.mxfp4_mm(a, s, W, out_dtype=torch.float32).double().cpu().numpy(), av @ w[2].T, np.abs(av) @ np.abs(w[2]).T, 2, False)
+    check(k3.mxfp4_mm_bwd(dy, W, out_dtype=torch.float32).double().cpu().numpy(), dv @ w[2], np.abs(dv) @ np.abs(w[2]), 5, False)
+    off = torch.zeros(3, dtype=torch.int32, device=dev)
+    for o in (None, off):
+        assert k3.mxfp4_mm(a[:0], s[:0], W, off=o).shape == (0, N)
+        assert k3.mxfp4_mm_bwd(dy[:0], W, off=o).shape == (0, K)
+    assert k3.mxfp4_quant(torch.empty(0, 64, device=dev))[1].shape == (0, 2)
+
+
+def test_the_most_groups(k3, dev):
+    """512 groups, most of them empty, sharing three matrices."""
+    import torch
+    G, N, K, M = 512, 136, 160, 700
+    g = np.random.default_rng(5)
+    cuts = np.sort(np.concatenate([np.repeat(g.integers(0, M + 1, 120), 4), np.zeros(20, int), np.full(11, M)]))
+    off = np.concatenate([[0], cuts, [M]]).astype(np.int32)
+    assert off.size == G + 1
+    mat_of = g.integers(0, 3, G).astype(np.int32)
+    W, w = matrices(k3, dev, 111, 3, N, K)
+    c, b = operand(112, M, K)
+    a, s, po, pm = to_dev(dev, pack_nibbles(c), b, off, mat_of)
+    W = k3.Mxfp4Mat(W.keep[0], W.keep[1], mat_of=pm)
+    y = k3.mxfp4_mm(a, s, W, off=po, out_dtype=torch.float32).double().cpu().numpy()
+    dy = torch.randn(M, N, device=dev).bfloat16()
+    da = k3.mxfp4_mm_bwd(dy, W, off=po, out_dtype=torch.float32).double().cpu().numpy()
+    row_w = w[np.repeat(mat_of, np.diff(off))]          # [M][N][K]
+    av, dv = values(c, b), dy.double().cpu().numpy()
+    check(y, np.einsum("mk,mnk->mn", av, row_w), np.einsum("mk,mnk->mn", np.abs(av), np.abs(row_w)), 3, False)
+    check(da, np.einsum("mn,mnk->mk", dv, row_w), np.einsum("mn,mnk->mk", np.abs(dv), np.abs(row_w)), 9, False)
