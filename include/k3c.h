@@ -634,7 +634,7 @@ size_t k3c_mxfp4_atom_bytes(int rows, int in);
 int k3c_mxfp4_pack(uint8_t *codes, uint8_t *atoms, const uint8_t *packed, const uint8_t *scales, int n_mats,
                    int rows, int in, k3c_stream_t stream);
 /* y[r][o] = sum_i A[r][i] W_g[o][i], A as k3c_mxfp4_quant writes it (a [M][in/2] 16-byte aligned,
- * a_scales [M][in/32] 4-byte aligned); rows off[g] .. off[g+1] - 1 (device, n_groups + 1 ints, ascending;
+ * a_scales [M][in/32]); rows off[g] .. off[g+1] - 1 (device, n_groups + 1 ints, ascending;
  * offsets outside 0..M are clamped) belong to group g, rows outside every group are left as they
  * were; off NULL with n_groups 1: all rows. Exact products, fp32 accumulation, one rounding to
  * y_dtype; y rows ldy >= rows elements apart. n_groups <= 512. The result does not depend on

@@ -1313,8 +1313,8 @@ def _mm_out(rt, M, n, dev, out, out_dtype):
 
 
 def mxfp4_mm(a, a_scales, W, off=None, out=None, out_dtype=None):
-    """y[r] = W_g a[r]: a [M][in/2] and a_scales [M][in/32] (on a 4-byte boundary) as mxfp4_quant
-    or moe_permute_mxfp4 return them, W an Mxfp4Mat. Without off every row multiplies W's first matrix (mat_of[0]);
+    """y[r] = W_g a[r]: a [M][in/2] and a_scales [M][in/32] as mxfp4_quant or moe_permute_mxfp4
+    return them, W an Mxfp4Mat. Without off every row multiplies W's first matrix (mat_of[0]);
     with off [G + 1] int32 (moe_sort's) rows off[g]..off[g+1]-1 multiply group g's and rows
     outside every group are left as they were (in a new out: undefined). out [M][rows] of
     out_dtype (default bf16), rows may be strided."""

@@ -328,31 +328,6 @@ __device__ __forceinline__ void store_rows(uint8_t *stg, const uint32_t (&v)[32]
 }
 
 // ------------------------------------------------------------------ MXFP4 x MXFP4
-// Scale rows that do not start on 16-byte boundaries: 4 * W scale bytes at s as words. Word
-// loads only, nine for eight words, shifted together. A word that ends past the array (hi) reads
-// as `tail`, its bytes below hi, and one past it as 0; their loads go to `any` instead, without a
-// branch, so that all loads stay in flight together. n bytes from s on belong to the row, the
-// rest read as 127 (scale 1). The array starts on a word boundary.
-template <int W>
-__device__ __forceinline__ void scales_at(uint32_t (&v)[W], const uint8_t *s, int n, const uint8_t *any, const uint8_t *hi,
-                                          uint32_t tail) {
-    const uint8_t *a = reinterpret_cast<const uint8_t *>((uintptr_t)s & ~(uintptr_t)3);
-    const uint32_t sh = 8 * (uint32_t)((uintptr_t)s & 3);
-    uint32_t w[W + 1];
-#pragma unroll
-    for (int i = 0; i <= W; i++) {
-        const uint8_t *c = a + 4 * i;
-        const bool in = c + 4 <= hi;
-        const uint32_t u = __ldg(reinterpret_cast<const uint32_t *>(in ? c : any));
-        w[i] = in ? u : c < hi ? tail : 0u;
-    }
-#pragma unroll
-    for (int i = 0; i < W; i++) {
-        const int left = n - 4 * i;
-        const uint32_t keep = left >= 4 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
-        v[i] = (__funnelshift_r(w[i], w[i + 1], sh) & keep) | (0x7F7F7F7Fu & ~keep);
-    }
-}
 // kind::mxf4: E2M1 A and B, K-major, UE8M0 scales per 32 (scale_vec::2X), M = 128, K = 64.
 __host__ __device__ constexpr uint32_t idesc_mxf4(uint32_t n, uint32_t sf_id) {
     return (sf_id << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((128u >> 4) << 24) | (sf_id << 29);
@@ -422,59 +397,144 @@ __device__ __forceinline__ void copy_a(const MxArgs &p, int n_items, const ItemF
         tc::mbar_wait(&full[i % STAGES], (i / STAGES) & 1u, p.err, 88);
 }
 
+// The scale bytes of four rows and MM_KS K blocks (32 bytes a row) as one lane holds them: the aligned
+// 16-byte pieces they lie in, whatever the row's alignment, as loaded. They are shifted into words
+// only when the K blocks before them are stored: right after the loads the shift would wait for
+// them (8192 x 7168 x 7136: 315 us then, 196 now; 178 with a K of 7168).
+// EVEN: every row starts on a piece.
+template <bool EVEN>
+struct ScaleRows {
+    uint4 u[4][EVEN ? 2 : 3];
+    uint32_t off[4];    // the rows' first byte within their first piece
+};
+// The 16 bytes at c of an array [lo, hi), zeros outside it: each of 16 lanes has loaded one byte.
+__device__ __forceinline__ uint4 edge_piece(uint32_t byte, int at) {   // at: the byte's place, -1 for none
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) w[k] = __reduce_or_sync(0xFFFFFFFFu, at >> 2 == k ? byte << (8 * (at & 3)) : 0u);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // A's scales of every K block of this CTA's items, by one warp. Lane i fetches the bytes of rows i,
 // 32+i, 64+i and 96+i and stores the four rows' words of each atom as one 16-byte piece (sf_byte's
 // order). MM_KS K blocks are fetched at a time, while the MM_KS before them are stored, across
 // items. The stores become visible to tcgen05.cp by a proxy fence of the thread that waits on
 // `full`: one here would wait for the fetches in flight. sf0: the scales' place in stage 0; item(it)
 // gives the rows of this CTA.
-template <int STAGES, typename ItemFn>
-__device__ __forceinline__ void a_scales(const MxArgs &p, int n_items, const ItemFn &item, uint8_t *sf0, int stage_bytes,
-                                         uint64_t *full, uint64_t *empty, int KB, int it0, int step) {
+template <int STAGES, bool EVEN, typename ItemFn>
+__device__ __forceinline__ void a_scales_of(const MxArgs &p, int n_items, const ItemFn &item, uint8_t *sf0, int stage_bytes,
+                                            uint64_t *full, uint64_t *empty, int KB, int it0, int step) {
     const int lane = threadIdx.x & 31;
     const int SR = p.K / 32;
-    const int wide = SR % 16 == 0 && ((uintptr_t)p.as & 15) == 0;
     const uint8_t *as_end = p.as + (size_t)p.M * SR;
-    uint32_t tail = 0;   // the bytes of the array's last word, if it is no whole one
-    for (const uint8_t *c = reinterpret_cast<const uint8_t *>((uintptr_t)as_end & ~(uintptr_t)3); c < as_end; c++)
-        tail |= (uint32_t)__ldg(c) << (8 * ((uintptr_t)c & 3));
-    uint32_t st = 0, ph = 1, w[4][2 * MM_KS];
+    uint32_t st = 0, ph = 1;
     bool ok = true;
+    // the array's first and last piece, which a 16-byte load would leave: a byte per lane
+    const uint8_t *first = nullptr, *last = nullptr;
+    uint32_t edge_byte = 0;
+    if constexpr (!EVEN) {
+        first = reinterpret_cast<const uint8_t *>((uintptr_t)p.as & ~(uintptr_t)15);
+        last = reinterpret_cast<const uint8_t *>((uintptr_t)(as_end - 1) & ~(uintptr_t)15);
+        const uint8_t *c = (lane < 16 ? first : last) + (lane & 15);
+        if (c >= p.as && c < as_end) edge_byte = __ldg(c);
+    }
     auto next_item = [&](int &it, Item &x) {   // the first item from `it` on that has a matrix
         for (; it < n_items; it += step) {
             x = item(it);
             if (x.mat >= 0) return;
         }
     };
-    auto fetch = [&](uint32_t (&v)[4][2 * MM_KS], const Item &x, int k0) {
+    const uint4 ones = make_uint4(0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+    auto fetch = [&](ScaleRows<EVEN> &v, const Item &x, int k0) {
+        if constexpr (EVEN) {
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+#pragma unroll
+                for (int h = 0; h < 2; h++) v.u[q][h] = ones;   // rows past the tile: scale 1
+                if (32 * q + lane < x.n) {
+                    const uint8_t *s = p.as + (size_t)(x.row0 + 32 * q + lane) * SR + 8 * k0;
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+                        if (k0 + 2 * h < KB) v.u[q][h] = __ldg(reinterpret_cast<const uint4 *>(s + 16 * h));
+                }
+            }
+        } else {
+            bool edge = false;
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const bool live = 32 * q + lane < x.n;
+                const uint8_t *row = p.as + (size_t)(x.row0 + (live ? 32 * q + lane : 0)) * SR, *s = row + 8 * k0;
+                v.off[q] = (uint32_t)((uintptr_t)s & 15);
+#pragma unroll
+                for (int h = 0; h < 3; h++) {
+                    const uint8_t *c = s - v.off[q] + 16 * h;
+                    v.u[q][h] = ones;
+                    const bool want = live && c < row + SR && (h < 2 || v.off[q] != 0);
+                    if (want && c >= p.as && c + 16 <= as_end) v.u[q][h] = __ldg(reinterpret_cast<const uint4 *>(c));
+                    edge |= want && (c < p.as || c + 16 > as_end);
+                }
+            }
+            if (__any_sync(0xFFFFFFFFu, edge)) {
+                const uint4 head = edge_piece(edge_byte, lane < 16 ? lane : -1), tail = edge_piece(edge_byte, lane < 16 ? -1 : lane - 16);
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+                    if (32 * q + lane < x.n) {
+                        const uint8_t *row = p.as + (size_t)(x.row0 + 32 * q + lane) * SR, *s = row + 8 * k0;
+#pragma unroll
+                        for (int h = 0; h < 3; h++) {
+                            const uint8_t *c = s - v.off[q] + 16 * h;
+                            if (c < row + SR && (c < p.as || c + 16 > as_end)) v.u[q][h] = c == last ? tail : head;
+                        }
+                    }
+            }
+        }
+    };
+    // The rows' 32 bytes as words, once the pieces are there; `left` bytes of a row remain, what lies
+    // past them reads as scale 1.
+    auto words = [&](uint32_t (&w)[4][8], const ScaleRows<EVEN> &v, int left) {
 #pragma unroll
         for (int q = 0; q < 4; q++) {
+            if constexpr (EVEN) {
 #pragma unroll
-            for (int i = 0; i < 2 * MM_KS; i++) v[q][i] = 0x7F7F7F7Fu;   // rows past the tile, groups past K: scale 1
-            if (32 * q + lane < x.n) {
-                const uint8_t *s = p.as + (size_t)(x.row0 + 32 * q + lane) * SR + 8 * k0;
-                if (wide) {   // SR is a multiple of 16: two K blocks at a time, all of them inside the row
+                for (int h = 0; h < 2; h++) {
+                    w[q][4 * h] = v.u[q][h].x;
+                    w[q][4 * h + 1] = v.u[q][h].y;
+                    w[q][4 * h + 2] = v.u[q][h].z;
+                    w[q][4 * h + 3] = v.u[q][h].w;
+                }
+            } else {
+                const uint32_t r[12] = {v.u[q][0].x, v.u[q][0].y, v.u[q][0].z, v.u[q][0].w, v.u[q][1].x, v.u[q][1].y,
+                                        v.u[q][1].z, v.u[q][1].w, v.u[q][2].x, v.u[q][2].y, v.u[q][2].z, v.u[q][2].w};
+                const bool one = v.off[q] & 4, two = v.off[q] & 8;
+                const uint32_t sh = 8 * (v.off[q] & 3);
+                uint32_t a[11], b[9];
 #pragma unroll
-                    for (int h = 0; h < MM_KS / 2; h++)
-                        if (k0 + 2 * h < KB) {
-                            const uint4 u = __ldg(reinterpret_cast<const uint4 *>(s + 16 * h));
-                            v[q][4 * h] = u.x;
-                            v[q][4 * h + 1] = u.y;
-                            v[q][4 * h + 2] = u.z;
-                            v[q][4 * h + 3] = u.w;
-                        }
-                } else {
-                    scales_at<2 * MM_KS>(v[q], s, SR - 8 * k0, p.atoms, as_end, tail);
+                for (int i = 0; i < 11; i++) a[i] = one ? r[i + 1] : r[i];
+#pragma unroll
+                for (int i = 0; i < 9; i++) b[i] = two ? a[i + 2] : a[i];
+#pragma unroll
+                for (int i = 0; i < 8; i++) w[q][i] = __funnelshift_r(b[i], b[i + 1], sh);
+                if (left < 32) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int n = left - 4 * i;
+                        const uint32_t keep = n >= 4 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
+                        w[q][i] = (w[q][i] & keep) | (0x7F7F7F7Fu & ~keep);
+                    }
                 }
             }
         }
     };
+    ScaleRows<EVEN> nx;
+    uint32_t w[4][8];
     int it = it0, k0 = 0;
     Item x = {};
     next_item(it, x);
-    if (it < n_items) fetch(w, x, 0);
+    if (it < n_items) {
+        fetch(nx, x, 0);
+        words(w, nx, SR);
+    }
     while (ok && it < n_items) {
-        uint32_t nx[4][2 * MM_KS] = {};
         const int kn = min(MM_KS, KB - k0);
         k0 += MM_KS;
         if (k0 >= KB) {
@@ -499,11 +559,17 @@ __device__ __forceinline__ void a_scales(const MxArgs &p, int n_items, const Ite
                 ph ^= 1u;
             }
         }
-#pragma unroll
-        for (int q = 0; q < 4; q++)
-#pragma unroll
-            for (int i = 0; i < 2 * MM_KS; i++) w[q][i] = nx[q][i];
+        words(w, nx, SR - 8 * k0);
     }
+}
+
+template <int STAGES, typename ItemFn>
+__device__ __forceinline__ void a_scales(const MxArgs &p, int n_items, const ItemFn &item, uint8_t *sf0, int stage_bytes,
+                                         uint64_t *full, uint64_t *empty, int KB, int it0, int step) {
+    if ((p.K / 32) % 16 == 0 && ((uintptr_t)p.as & 15) == 0)
+        a_scales_of<STAGES, true>(p, n_items, item, sf0, stage_bytes, full, empty, KB, it0, step);
+    else
+        a_scales_of<STAGES, false>(p, n_items, item, sf0, stage_bytes, full, empty, KB, it0, step);
 }
 
 // 128 rows x NT columns per item, one CTA per SM. A K block is 256 codes of a row, 128 bytes: four
@@ -1612,8 +1678,7 @@ extern "C" int k3c_mxfp4_mm(void *y, int y_dtype, int64_t ldy, const uint8_t *a,
         return set_error(K3C_EINVAL, "mxfp4_mm: y_dtype=%d ldy=%lld rows=%d", y_dtype, (long long)ldy, W->rows);
     if (!M) return K3C_OK;
     if (!y || !a || !a_scales) return set_error(K3C_EINVAL, "mxfp4_mm: NULL array");
-    if (!al16(a) || ((uintptr_t)a_scales & 3))
-        return set_error(K3C_EINVAL, "mxfp4_mm: a must be 16-byte aligned, a_scales 4-byte aligned");
+    if (!al16(a)) return set_error(K3C_EINVAL, "mxfp4_mm: a must be 16-byte aligned");
     cudaStream_t s = (cudaStream_t)stream;
     MxArgs p = {};
     K3C_TRY(err_slot(&p.err));

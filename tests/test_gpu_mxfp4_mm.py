@@ -506,3 +506,22 @@ def test_the_most_groups(k3, dev):
     av, dv = values(c, b), dy.double().cpu().numpy()
     check(y, np.einsum("mk,mnk->mn", av, row_w), np.einsum("mk,mnk->mn", np.abs(av), np.abs(row_w)), 3, False)
     check(da, np.einsum("mn,mnk->mk", dv, row_w), np.einsum("mn,mnk->mk", np.abs(dv), np.abs(row_w)), 9, False)
+
+
+@pytest.mark.parametrize("K", [32, 96, 160, 512, 1056, 2016])
+@pytest.mark.parametrize("first", [0, 1, 3, 5, 8])
+def test_scale_rows_on_any_boundary(k3, dev, first, K):
+    """a_scales at every kind of address, for row lengths of odd and even bytes; nothing beside the
+    array is read as a scale (its neighbours hold the NaN byte)."""
+    import torch
+    N = 64
+    W, w = matrices(k3, dev, 121, 1, N, K)
+    for M in (1, 2, 33, 129):
+        c, b = operand(122, M, K)
+        a = to_dev(dev, pack_nibbles(c))[0]
+        buf = torch.full((first + b.size + 40,), 255, dtype=torch.uint8, device=dev)
+        s = buf[first:first + b.size].view(M, K // 32)
+        s.copy_(torch.from_numpy(b))
+        av = values(c, b)
+        y = k3.mxfp4_mm(a, s, W, out_dtype=torch.float32).double().cpu().numpy()
+        check(y, av @ w[0].T, np.abs(av) @ np.abs(w[0]).T, -(-K // 64), False)
