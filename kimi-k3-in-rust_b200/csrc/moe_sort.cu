@@ -260,6 +260,9 @@ __device__ __forceinline__ void st16(void *p, const uint4 &v) {
 }
 
 constexpr int PM_TH = 512;   // threads of a block at most
+// Rows on no 16-byte boundary move element by element, so many per thread and round (32768 rows of
+// 7167 bf16 summed to 4096: 175 us, 202 with one at a time).
+constexpr int PM_U = 4, UB_U = 2;
 
 // A token's pairs that have a row, in the order of j: rows, j and weights in shared memory, so that
 // the loops below run over those pairs alone with several loads in flight (an expert-parallel
@@ -302,19 +305,29 @@ __global__ void __launch_bounds__(PM_TH) k_permute(T *__restrict__ rows, const T
     __shared__ TokenRows s;
     const int t = blockIdx.x;
     const T *xr = x + (size_t)t * ldx;
-    constexpr int V = VEC ? Vec<T>::V : 1;
-    const int n = H / V, stride = gridDim.y * blockDim.x;
     const int m = token_rows(s, pos, nullptr, (size_t)t * topk, P, topk);
     if (!m) return;
-    for (int c = blockIdx.y * blockDim.x + threadIdx.x; c < n; c += stride) {
-        if constexpr (VEC) {
+    if constexpr (VEC) {
+        constexpr int V = Vec<T>::V;
+        const int n = H / V, stride = gridDim.y * blockDim.x;
+        for (int c = blockIdx.y * blockDim.x + threadIdx.x; c < n; c += stride) {
             const uint4 v = ld16(xr + (size_t)c * V);
 #pragma unroll 4
             for (int j = 0; j < m; j++) st16(rows + (size_t)s.row[j] * H + (size_t)c * V, v);
-        } else {
-            const T v = xr[c];
-#pragma unroll 4
-            for (int j = 0; j < m; j++) rows[(size_t)s.row[j] * H + c] = v;
+        }
+    } else {
+        const int th = blockDim.x;
+        for (int c0 = blockIdx.y * th * PM_U + threadIdx.x; c0 < H; c0 += gridDim.y * th * PM_U) {
+            T v[PM_U];
+#pragma unroll
+            for (int i = 0; i < PM_U; i++)
+                if (c0 + i * th < H) v[i] = xr[c0 + i * th];
+            for (int j = 0; j < m; j++) {
+                T *r = rows + (size_t)s.row[j] * H;
+#pragma unroll
+                for (int i = 0; i < PM_U; i++)
+                    if (c0 + i * th < H) r[c0 + i * th] = v[i];
+            }
         }
     }
 }
@@ -331,14 +344,14 @@ __global__ void __launch_bounds__(PM_TH) k_gather_sum(O *__restrict__ out, const
     __shared__ TokenRows s;
     const int t = blockIdx.x;
     const int m = token_rows(s, pos, wt, (size_t)t * topk, P, topk);
-    constexpr int V = VEC ? Vec<T>::V : 1;
-    const int n = H / V, stride = gridDim.y * blockDim.x;
-    for (int c = blockIdx.y * blockDim.x + threadIdx.x; c < n; c += stride) {
-        float acc[V];
+    if constexpr (VEC) {
+        constexpr int V = Vec<T>::V, VO = Vec<O>::V;
+        const int n = H / V, stride = gridDim.y * blockDim.x;
+        for (int c = blockIdx.y * blockDim.x + threadIdx.x; c < n; c += stride) {
+            float acc[V];
 #pragma unroll
-        for (int i = 0; i < V; i++) acc[i] = 0.0f;
-        for (int j0 = 0; j0 < m; j0 += GS_JB) {
-            if constexpr (VEC) {
+            for (int i = 0; i < V; i++) acc[i] = 0.0f;
+            for (int j0 = 0; j0 < m; j0 += GS_JB) {
                 uint4 u[GS_JB];
 #pragma unroll
                 for (int q = 0; q < GS_JB; q++)
@@ -352,21 +365,8 @@ __global__ void __launch_bounds__(PM_TH) k_gather_sum(O *__restrict__ out, const
 #pragma unroll
                         for (int i = 0; i < V; i++) acc[i] = __fadd_rn(acc[i], __fmul_rn(w, f[i]));
                     }
-            } else {
-                float f[GS_JB];
-#pragma unroll
-                for (int q = 0; q < GS_JB; q++)
-                    if (j0 + q < m) f[q] = Vec<T>::one(y[(size_t)s.row[j0 + q] * H + c]);
-#pragma unroll
-                for (int q = 0; q < GS_JB; q++)
-                    if (j0 + q < m) acc[0] = __fadd_rn(acc[0], __fmul_rn(s.w[j0 + q], f[q]));
             }
-        }
-        O *o = out + (size_t)t * H + (size_t)c * V;
-        if constexpr (!VEC) {
-            *o = Vec<O>::back(acc[0]);
-        } else {
-            constexpr int VO = Vec<O>::V;
+            O *o = out + (size_t)t * H + (size_t)c * V;
             if constexpr (VO == V) {
                 st16(o, Vec<O>::put(acc));
             } else if constexpr (VO < V) {   // bf16 rows, fp32 sums: two stores
@@ -380,6 +380,33 @@ __global__ void __launch_bounds__(PM_TH) k_gather_sum(O *__restrict__ out, const
             } else {                         // fp32 rows, bf16 sums: half a store
                 *reinterpret_cast<uint2 *>(o) = make_uint2(f32x2_to_bf16x2(acc[0], acc[1]), f32x2_to_bf16x2(acc[2], acc[3]));
             }
+        }
+    } else {
+        const int th = blockDim.x;
+        for (int c0 = blockIdx.y * th * PM_U + threadIdx.x; c0 < H; c0 += gridDim.y * th * PM_U) {
+            float acc[PM_U];
+#pragma unroll
+            for (int i = 0; i < PM_U; i++) acc[i] = 0.0f;
+            for (int j0 = 0; j0 < m; j0 += GS_JB) {
+                T u[GS_JB][PM_U];
+#pragma unroll
+                for (int q = 0; q < GS_JB; q++) {
+                    const T *r = y + (size_t)s.row[j0 + q < m ? j0 + q : 0] * H;
+#pragma unroll
+                    for (int i = 0; i < PM_U; i++)
+                        if (j0 + q < m && c0 + i * th < H) u[q][i] = r[c0 + i * th];
+                }
+#pragma unroll
+                for (int q = 0; q < GS_JB; q++)
+                    if (j0 + q < m) {
+                        const float w = s.w[j0 + q];
+#pragma unroll
+                        for (int i = 0; i < PM_U; i++) acc[i] = __fadd_rn(acc[i], __fmul_rn(w, Vec<T>::one(u[q][i])));
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < PM_U; i++)
+                if (c0 + i * th < H) out[(size_t)t * H + c0 + i * th] = Vec<O>::back(acc[i]);
         }
     }
 }
@@ -460,17 +487,33 @@ __global__ void __launch_bounds__(PM_TH) k_unpermute_bwd(T *__restrict__ dy, flo
                 }
             }
         } else {
-            for (int i = threadIdx.x; i < H; i += blockDim.x) {
-                const float d = Vec<D>::one(dr[i]);
-                float f[UB_JB];
+            constexpr int U = UB_U;
+            const int th = blockDim.x;
+            for (int c0 = threadIdx.x; c0 < H; c0 += th * U) {
+                float d[U];
+                T f[UB_JB][U];
 #pragma unroll
-                for (int q = 0; q < UB_JB; q++)
-                    if (dwt && q < jn) f[q] = Vec<T>::one(y[(size_t)s.row[j0 + q] * H + i]);
+                for (int i = 0; i < U; i++) d[i] = c0 + i * th < H ? Vec<D>::one(dr[c0 + i * th]) : 0.0f;
+                if (dwt) {
+#pragma unroll
+                    for (int q = 0; q < UB_JB; q++) {
+                        const T *r = y + (size_t)s.row[j0 + (q < jn ? q : 0)] * H;
+#pragma unroll
+                        for (int i = 0; i < U; i++)
+                            if (q < jn && c0 + i * th < H) f[q][i] = r[c0 + i * th];
+                    }
+                }
 #pragma unroll
                 for (int q = 0; q < UB_JB; q++) {
                     if (q >= jn) continue;
-                    if (dwt) dot[q] = fmaf(d, f[q], dot[q]);
-                    if (dy) dy[(size_t)s.row[j0 + q] * H + i] = Vec<T>::back(s.w[j0 + q] * d);
+                    T *r = dy + (size_t)s.row[j0 + q] * H;
+                    const float w = s.w[j0 + q];
+#pragma unroll
+                    for (int i = 0; i < U; i++)
+                        if (c0 + i * th < H) {
+                            if (dwt) dot[q] = fmaf(d[i], Vec<T>::one(f[q][i]), dot[q]);
+                            if (dy) r[c0 + i * th] = Vec<T>::back(w * d[i]);
+                        }
                 }
             }
         }
@@ -556,7 +599,7 @@ int sort_blocks(int64_t P) {
 template <typename T, typename O>
 int run_gather(O *out, const T *y, const float *wt, const int *pos, int ntok, int topk, int H, cudaStream_t s) {
     const bool vec = al16(y) && al16(out) && H % Vec<T>::V == 0 && H % Vec<O>::V == 0;
-    const Shape g = row_shape(ntok, vec ? H / Vec<T>::V : H, true);
+    const Shape g = row_shape(ntok, vec ? H / Vec<T>::V : (H + PM_U - 1) / PM_U, true);
     if (vec) k_gather_sum<T, O, true><<<g.grid, g.block, 0, s>>>(out, y, wt, pos, ntok * topk, topk, H);
     else k_gather_sum<T, O, false><<<g.grid, g.block, 0, s>>>(out, y, wt, pos, ntok * topk, topk, H);
     K3C_CHECK_LAUNCH();
@@ -567,7 +610,7 @@ template <typename T, typename D>
 int run_unpermute_bwd(T *dy, float *dwt, const D *dout, const T *y, const float *wt, const int *pos, int ntok, int topk,
                       int H, cudaStream_t s) {
     const bool vec = al16(y) && al16(dy) && al16(dout) && H % Vec<T>::V == 0 && H % Vec<D>::V == 0;
-    const Shape g = row_shape(ntok, vec ? H / Vec<T>::V : H, false);   // one block per token: it sums dwt
+    const Shape g = row_shape(ntok, vec ? H / Vec<T>::V : (H + UB_U - 1) / UB_U, false);   // one block per token: it sums dwt
     if (vec) k_unpermute_bwd<T, D, true><<<g.grid, g.block, 0, s>>>(dy, dwt, dout, y, wt, pos, ntok * topk, topk, H);
     else k_unpermute_bwd<T, D, false><<<g.grid, g.block, 0, s>>>(dy, dwt, dout, y, wt, pos, ntok * topk, topk, H);
     K3C_CHECK_LAUNCH();
@@ -632,7 +675,7 @@ extern "C" int k3c_moe_permute(void *rows, const void *x, int dtype, int64_t ldx
     cudaStream_t s = (cudaStream_t)stream;
     const int V = dtype == K3C_F32 ? 4 : 8, P = ntok * topk;
     const bool vec = al16(rows) && al16(x) && hidden % V == 0 && ldx % V == 0;
-    const Shape g = row_shape(ntok, vec ? hidden / V : hidden, true);
+    const Shape g = row_shape(ntok, vec ? hidden / V : (hidden + PM_U - 1) / PM_U, true);
     if (dtype == K3C_F32) {
         if (vec) k_permute<float, true><<<g.grid, g.block, 0, s>>>((float *)rows, (const float *)x, ldx, pos, P, topk, hidden);
         else k_permute<float, false><<<g.grid, g.block, 0, s>>>((float *)rows, (const float *)x, ldx, pos, P, topk, hidden);
