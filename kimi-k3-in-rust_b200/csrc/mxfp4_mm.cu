@@ -1525,12 +1525,13 @@ int check_items(const char *what, int64_t items) {
 // Row tiles of at most `tile` rows that n_groups groups of M rows can have together.
 int64_t most_tiles(int M, int n_groups, int tile) { return (int64_t)M / tile + (n_groups < M ? n_groups : M); }
 
-// A kernel's tile and what it costs: a launch takes about fixed + waves * (K blocks * block + item)
-// ns, a wave being one item on every SM (or pair of SMs). Fitted to measured launches of M = 1 to
-// 4096 rows, dense and in 48 groups (e.g. 8 K blocks of k3c_mxfp4_mm, 4096 x 7168: pair 33.5 us,
-// 256 columns 33.7, 128 38.8, 64 62; 1 x 7168: 9.5, 7.8, 6.4, 6.7).
+// A kernel's tile and what it costs: a launch takes about fixed + waves * max(K blocks * block + item,
+// store) ns, a wave being one item on every SM (or pair of SMs) and `store` its epilogue. Fitted to
+// measured launches of M = 1 to 16000 rows, dense and in 4 to 48 groups (e.g. 8 K blocks of
+// k3c_mxfp4_mm, 4096 x 7168: pair 33.5 us, 256 columns 33.7, 128 38.8, 64 62; 1 x 7168: 9.5, 7.8, 6.4,
+// 6.7; one K block, 8000 x 4096: 29.5, 26.1, 37.6, 65).
 struct TileCost {
-    int rows, cols, ctas, block, item, fixed;
+    int rows, cols, ctas, block, item, store, fixed;
 };
 // The cheapest of n kernels for M rows in n_groups groups (grouped: their sizes are on the device;
 // each is taken to waste half a tile) and `cols` columns, kb K blocks. Ties go to the first.
@@ -1545,7 +1546,8 @@ int cheapest(const TileCost *t, int n, int M, int n_groups, bool grouped, int co
         }
         const double items = tiles * ((cols + t[i].cols - 1) / t[i].cols), at_once = sm_count() / t[i].ctas;
         const double waves = items <= at_once ? 1 : (double)(int64_t)((items + at_once - 1) / at_once);
-        const double ns = t[i].fixed + waves * ((double)kb * t[i].block + t[i].item);
+        const double loop = (double)kb * t[i].block + t[i].item;
+        const double ns = t[i].fixed + waves * (loop > t[i].store ? loop : t[i].store);
         if (!i || ns < least) {
             best = i;
             least = ns;
@@ -1711,10 +1713,10 @@ extern "C" int k3c_mxfp4_mm(void *y, int y_dtype, int64_t ldy, const uint8_t *a,
     p.as = a_scales;
     p.atoms = W->atoms;
     p.atom_stride = W->atom_stride;
-    static const TileCost kinds[] = {{256, 256, 2, 380, 700, 5400},
-                                     {128, 256, 1, 410, 1000, 3950},
-                                     {128, 128, 1, 270, 500, 3650},
-                                     {128, 64, 1, 240, 400, 3400}};
+    static const TileCost kinds[] = {{256, 256, 2, 380, 700, 3400, 5400},
+                                     {128, 256, 1, 410, 1000, 3150, 3950},
+                                     {128, 128, 1, 270, 500, 2400, 3650},
+                                     {128, 64, 1, 240, 400, 2200, 3400}};
     const int kind = cheapest(kinds, 4, M, n_groups, off != nullptr, p.N, (p.K + 255) / 256);
     CUtensorMap ma, ma1, mw;
     K3C_TRY(make_map3(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, a, p.K / 2, M, 1, p.K / 2, (uint64_t)(p.K / 2) * M, 128, MM_M));
@@ -1756,10 +1758,10 @@ extern "C" int k3c_mxfp4_mm_bwd(void *da, int da_dtype, int64_t ldda, const void
     // (112 K blocks: pair 43.8 us at 512 x 7168, 256 columns 69, 128 78; at 64 x 7168 42, 68, 41;
     // the pair's two accumulators 72 us and one 83 at 2400 x 2048, 692 and 824 at 32768 x 2048, but
     // 64 K blocks 45 and 28 at 1200 x 2048)
-    static const TileCost kinds[] = {{512, 256, 2, 560, 4500, 6300},
-                                     {256, 256, 2, 335, 300, 6300},
-                                     {128, 256, 1, 555, 500, 5900},
-                                     {128, 128, 1, 320, 400, 4800}};
+    static const TileCost kinds[] = {{512, 256, 2, 560, 4500, 0, 6300},
+                                     {256, 256, 2, 335, 300, 0, 6300},
+                                     {128, 256, 1, 555, 500, 0, 5900},
+                                     {128, 128, 1, 320, 400, 0, 4800}};
     const int kind = cheapest(kinds, 4, M, n_groups, off != nullptr, p.K, (p.N + MB_KB - 1) / MB_KB);
     if (kind == 0) K3C_TRY((launch_bwd<128, true, 2>(p, W, dy, lddy, s)));
     else if (kind == 1) K3C_TRY((launch_bwd<128, true, 1>(p, W, dy, lddy, s)));

@@ -145,7 +145,8 @@ def matrices(k3, dev, seed, n, rows, in_):
 
 DENSE = [(1, 1, 32), (1, 64, 64), (2, 65, 96), (1, 7168, 2048), (31, 130, 160), (33, 200, 256), (127, 384, 288),
          (128, 128, 512), (129, 257, 1056), (300, 1000, 3616), (64, 7168, 7168), (1000, 640, 352), (2200, 4100, 64),
-         (2100, 2304, 1056), (256, 19000, 256), (900, 4100, 4128), (4300, 4100, 1312)]
+         (2100, 2304, 1056), (256, 19000, 256), (900, 4100, 4128), (4300, 4100, 1312),
+         (300, 4100, 1056), (5000, 4100, 2080)]
 
 
 @pytest.mark.parametrize("out", ["f32", "bf16"])
