@@ -1255,16 +1255,16 @@ class Mxfp4Mat:
     def __init__(self, codes, atoms, mat_of=None):
         """mat_of: device int32, the matrix of each group of rows (default: group g's is g)."""
         rt = _runtime(codes)
-        dev = codes.get_device()
-        if codes.dim() != 3 or codes.dtype != rt.u8 or not codes.is_contiguous():
+        dev, sh = codes.get_device(), codes.shape
+        if len(sh) != 3 or codes.dtype != rt.u8 or not codes.is_contiguous():
             _bad(codes, "codes", "contiguous uint8 [n][rows][in/2]")
-        n, rows, half = codes.shape
-        want = (n, (rows + 127) // 128, (2 * half + 127) // 128, 512)
-        if atoms.shape != want or atoms.dtype != rt.u8 or atoms.get_device() != dev or not atoms.is_contiguous():
-            _bad(atoms, "atoms", f"contiguous uint8 {want} on device {dev}")
-        groups = n if mat_of is None else _vec_arg(mat_of, "mat_of", dev, rt.i32)
-        self._set(Mxfp4MatC(codes.data_ptr(), atoms.data_ptr(), rows * half, want[1] * want[2] * 512, n, rows, 2 * half,
-                            None if mat_of is None else mat_of.data_ptr()), groups, dev, (codes, atoms, mat_of))
+        n, rows, half = sh
+        ra, ka = (rows + 127) >> 7, (2 * half + 127) >> 7
+        if atoms.shape != (n, ra, ka, 512) or atoms.dtype != rt.u8 or atoms.get_device() != dev or not atoms.is_contiguous():
+            _bad(atoms, "atoms", f"contiguous uint8 {(n, ra, ka, 512)} on device {dev}")
+        groups, mp = (n, None) if mat_of is None else (_vec_arg(mat_of, "mat_of", dev, rt.i32), mat_of.data_ptr())
+        self._set(Mxfp4MatC(codes.data_ptr(), atoms.data_ptr(), rows * half, ra * ka * 512, n, rows, 2 * half, mp), groups,
+                  dev, (codes, atoms, mat_of))
 
     def _set(self, c, groups, dev, keep):
         self.c, self.ref, self.rows, self.in_ = c, C.byref(c), c.rows, c.in_
