@@ -637,7 +637,7 @@ int k3c_mxfp4_pack(uint8_t *codes, uint8_t *atoms, const uint8_t *packed, const 
  * a_scales [M][in/32]); rows off[g] .. off[g+1] - 1 (device, n_groups + 1 ints, ascending;
  * offsets outside 0..M are clamped) belong to group g, rows outside every group are left as they
  * were; off NULL with n_groups 1: all rows. Exact products, fp32 accumulation, one rounding to
- * y_dtype; y rows ldy >= rows elements apart. n_groups <= 512. The result does not depend on
+ * y_dtype; y rows ldy >= rows elements apart. n_groups <= 1024. The result does not depend on
  * how the work is spread. */
 int k3c_mxfp4_mm(void *y, int y_dtype, int64_t ldy, const uint8_t *a, const uint8_t *a_scales, int M,
                  const k3c_mxfp4_mat *W, const int *off, int n_groups, k3c_stream_t stream);

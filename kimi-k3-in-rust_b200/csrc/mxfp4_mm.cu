@@ -31,7 +31,7 @@ namespace k3c {
 
 namespace {
 
-constexpr int MX_GMAX = 512;    // groups of a product
+constexpr int MX_GMAX = 1024;   // groups of a product: with more, the largest tiles' shared memory would not hold the Plan
 
 static __device__ int g_mx_err;
 
@@ -168,11 +168,15 @@ struct Item {
     int nt;          // column tile
 };
 
-// The groups' rows and tiles, in shared memory: group g has rows first[g] .. max(first[g],
-// first[g+1]) - 1 and row tiles tile[g] .. tile[g+1] - 1.
+// The groups' tiles, in shared memory: group g has row tiles tile[g] .. tile[g+1] - 1.
 struct Plan {
-    int first[MX_GMAX + 1], tile[MX_GMAX + 1], warp_tot[32];
+    int tile[MX_GMAX + 1], warp_tot[32];
 };
+
+// Group g's first row; its rows end before group g + 1's. Offsets cannot leave the rows.
+__device__ __forceinline__ int first_of(const int *off, int g, int M) {
+    return off ? min(max(__ldg(off + g), 0), M) : g ? M : 0;
+}
 
 // Filled by all THREADS of the block; returns the number of row tiles.
 template <int THREADS>
@@ -181,19 +185,16 @@ __device__ int plan_tiles(Plan &pl, const int *off, int G, int M, int rows) {
     if (!off) {
         const int n = (M + rows - 1) / rows;
         if (tid == 0) {
-            pl.first[0] = pl.tile[0] = 0;
-            pl.first[1] = M;
+            pl.tile[0] = 0;
             pl.tile[1] = n;
         }
         __syncthreads();
         return n;
     }
-    for (int g = tid; g <= G; g += THREADS) pl.first[g] = min(max(__ldg(off + g), 0), M);   // offsets cannot leave the rows
-    __syncthreads();
     int run = 0;
     for (int g0 = 0; g0 < G; g0 += THREADS) {
         const int g = g0 + tid;
-        const int n = g < G ? (max(pl.first[g + 1] - pl.first[g], 0) + rows - 1) / rows : 0;
+        const int n = g < G ? (max(first_of(off, g + 1, M) - first_of(off, g, M), 0) + rows - 1) / rows : 0;
         int inc = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -224,8 +225,8 @@ __device__ int plan_tiles(Plan &pl, const int *off, int G, int M, int rows) {
 constexpr int MX_RB = 16;
 struct Walk {
     const Plan &pl;
-    const int *mat_of;
-    int n_mats, G, NTL, rows;
+    const int *off, *mat_of;
+    int M, n_mats, G, NTL, rows;
     int g = -1, lo = 0, hi = 0;    // items lo .. hi - 1 belong to group g
     int mt = 0, f0 = 0, f1 = 0, mat = -1;
     __device__ __forceinline__ Item at(int it) {
@@ -240,8 +241,8 @@ struct Walk {
             mt = pl.tile[g + 1] - pl.tile[g];
             lo = pl.tile[g] * NTL;
             hi = pl.tile[g + 1] * NTL;
-            f0 = pl.first[g];
-            f1 = pl.first[g + 1];
+            f0 = first_of(off, g, M);
+            f1 = first_of(off, g + 1, M);
             mat = mat_of ? __ldg(mat_of + g) : g;
             if (mat < 0 || mat >= n_mats) mat = -1;
         }
@@ -636,7 +637,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant_
     const int n_items = tiles * p.NTL;
     const int KB = (p.K + 255) / 256;
     const int KA = (p.K + 127) / 128;              // scale atoms along K
-    Walk walk{plan, p.mat_of, p.n_mats, p.G, p.NTL, MM_M};
+    Walk walk{plan, p.off, p.mat_of, p.M, p.n_mats, p.G, p.NTL, MM_M};
     auto item = [&](int it) { return walk.at(it); };   // a thread takes one role
 
     if (warp == 0) {
@@ -865,7 +866,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm_pair(const __grid_cons
     const int n_items = tiles * p.NTL;
     const int KB = (p.K + 255) / 256, KA = (p.K + 127) / 128;
     const int it0 = blockIdx.x >> 1, step = gridDim.x >> 1;
-    Walk walk{plan, p.mat_of, p.n_mats, p.G, p.NTL, 2 * MM_M};
+    Walk walk{plan, p.off, p.mat_of, p.M, p.n_mats, p.G, p.NTL, 2 * MM_M};
     auto pair_item = [&](int it) { return walk.at(it); };   // a thread takes one role
     auto item = [&](int it) {   // this CTA's rows of the pair's item
         Item x = pair_item(it);
@@ -1187,7 +1188,7 @@ __global__ void __launch_bounds__(MbCfg<NT, PAIR, ACCS>::THREADS, 1) k_mx4_bwd(c
     const int KB = (p.N + MB_KB - 1) / MB_KB;      // contracted: W's rows
     const int KA = (p.K + 127) / 128;
     const int it0 = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
-    Walk walk{plan, p.mat_of, p.n_mats, p.G, p.NTL, C::ROWS};
+    Walk walk{plan, p.off, p.mat_of, p.M, p.n_mats, p.G, p.NTL, C::ROWS};
     auto item = [&](int it) { return walk.at(it); };   // a thread takes one role
     // This CTA's rows of an item in accumulator j: 128 j and, in pairs, 256 j + 128 rank on.
     auto first_row = [&](int j) { return (PAIR ? 256 : 128) * j + (int)rank * 128; };

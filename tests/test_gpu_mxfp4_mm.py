@@ -487,12 +487,13 @@ def test_one_mapped_matrix_for_all_rows_and_no_rows(k3, dev):
     assert k3.mxfp4_quant(torch.empty(0, 64, device=dev))[1].shape == (0, 2)
 
 
-def test_the_most_groups(k3, dev):
-    """512 groups, most of them empty, sharing three matrices."""
+@pytest.mark.parametrize("G", [512, 896, 1024])
+def test_the_most_groups(k3, dev, G):
+    """Up to 1024 groups, most of them empty, sharing three matrices."""
     import torch
-    G, N, K, M = 512, 136, 160, 700
+    N, K, M = 136, 160, 700
     g = np.random.default_rng(5)
-    cuts = np.sort(np.concatenate([np.repeat(g.integers(0, M + 1, 120), 4), np.zeros(20, int), np.full(11, M)]))
+    cuts = np.sort(np.concatenate([np.repeat(g.integers(0, M + 1, G // 4 - 8), 4), np.zeros(20, int), np.full(11, M)]))
     off = np.concatenate([[0], cuts, [M]]).astype(np.int32)
     assert off.size == G + 1
     mat_of = g.integers(0, 3, G).astype(np.int32)

@@ -83,7 +83,7 @@ def test_mm_refusals(k3):
         assert f(mat(k3), M=-1) == -1 and "M=" in err(k3)
         assert f(mat(k3), G=2) == -1 and "n_groups" in err(k3)
         assert f(mat(k3), off=BUF, G=0) == -1 and "n_groups" in err(k3)
-        assert f(mat(k3, n_mats=2000, mat_of=BUF), off=BUF, G=513) == -1 and "n_groups" in err(k3)
+        assert f(mat(k3, n_mats=2000, mat_of=BUF), off=BUF, G=1025) == -1 and "n_groups" in err(k3)
         assert f(mat(k3), off=BUF, G=2) == -1 and "matrices" in err(k3)
         assert f(mat(k3), dt=4) == -1 and "dtype" in err(k3)
         assert f(mat(k3), M=0) == 0
