@@ -602,7 +602,8 @@ int k3c_moe_unpermute_bwd(void *dy, float *dwt, const void *dout, int out_dtype,
 
 /* ------------------------------------------------------------------------------------
  * MXFP4 quantisation and products (E2M1 x E2M1 on tcgen05 kind::mxf4; no reference counterpart,
- * the packed format is the reference's). No output may overlap an input, except as said.
+ * the packed format is the reference's). No output may overlap an input, except as said. Rows and
+ * columns: at most 2^31 - 2^10.
  * ------------------------------------------------------------------------------------ */
 /* x [rows] rows of ldx elements (x_dtype K3C_F32 or K3C_BF16) to packed [rows][in/2] and scales
  * [rows][ceil(in/32)]: per 32 elements scale byte clamp(floor(log2 max|x|) - 2 + 127, 0, 254),

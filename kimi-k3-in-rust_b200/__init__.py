@@ -1056,6 +1056,9 @@ def _launch(rt, name, dev, *args):
         _check(rc, name)
 
 
+_INT_MAX = 0x7FFFFFFF      # what the entry points' int arguments hold
+
+
 def _bad(t, name, want):
     raise K3CError(f"{name}: {t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}, expected {want}")
 
@@ -1074,6 +1077,8 @@ def _mat_arg(t, name, dev, dtypes, d0=None, d1=None):
     if (t.dtype not in dtypes or len(sh) != 2 or (d0 is not None and sh[0] != d0) or (d1 is not None and sh[1] != d1)
             or t.get_device() != dev or not t.is_contiguous()):
         _bad(t, name, f"contiguous {dtypes} {(d0, d1)} on device {dev}")
+    if sh[0] > _INT_MAX or sh[1] > _INT_MAX:
+        _bad(t, name, "extents within 32 bits")
     return sh
 
 
@@ -1088,6 +1093,8 @@ def _rows_arg(t, name, dev, dtypes):
     if t.dtype not in dtypes or t.dim() != 2 or t.get_device() != dev:
         _bad(t, name, f"2-D {dtypes} on device {dev}")
     rows, n = t.shape
+    if rows > _INT_MAX or n > _INT_MAX:
+        _bad(t, name, "extents within 32 bits")
     if t.is_contiguous():
         return rows, n, n
     ld, inner = t.stride()
@@ -1110,6 +1117,8 @@ def moe_sort(idx, n_experts):
     rt = _runtime(idx)
     dev = idx.get_device()
     T, K = _mat_arg(idx, "idx", dev, (rt.i32,))
+    if n_experts > _INT_MAX:
+        raise K3CError(f"n_experts {n_experts}: 32 bits")
     n = _sort_scratch(T, K, n_experts)
     pos, pair = _new(rt, dev, rt.i32, T, K), _new(rt, dev, rt.i32, T * K)
     off = _new(rt, dev, rt.i32, max(n_experts, 0) + 1)
@@ -1235,6 +1244,8 @@ def mxfp4_pack(packed, scales):
     if packed.dim() != 3 or packed.dtype != rt.u8 or not packed.is_contiguous():
         _bad(packed, "packed", "contiguous uint8 [n][rows][in/2]")
     n, rows, half = packed.shape
+    if max(n, rows, 2 * half) > _INT_MAX:
+        _bad(packed, "packed", "extents within 32 bits")
     if (scales.shape != (n, rows, half // 16) or scales.dtype != rt.u8 or scales.get_device() != dev
             or not scales.is_contiguous()):
         _bad(scales, "scales", f"contiguous uint8 {(n, rows, half // 16)} on device {dev}")
@@ -1259,6 +1270,8 @@ class Mxfp4Mat:
         if len(sh) != 3 or codes.dtype != rt.u8 or not codes.is_contiguous():
             _bad(codes, "codes", "contiguous uint8 [n][rows][in/2]")
         n, rows, half = sh
+        if max(n, rows, 2 * half) > _INT_MAX:
+            _bad(codes, "codes", "extents within 32 bits")
         ra, ka = (rows + 127) >> 7, (2 * half + 127) >> 7
         if atoms.shape != (n, ra, ka, 512) or atoms.dtype != rt.u8 or atoms.get_device() != dev or not atoms.is_contiguous():
             _bad(atoms, "atoms", f"contiguous uint8 {(n, ra, ka, 512)} on device {dev}")
@@ -1302,13 +1315,14 @@ def _mm_groups(rt, W, off, dev):
     return off.data_ptr(), G
 
 
-def _mm_out(rt, M, n, dev, out, out_dtype):
-    """(out, its row stride)."""
+def _mm_out(rt, M, n, dev, out, out_dtype, a):
+    """(out, its row stride); a: the rows multiplied."""
     if out is None:
         return _new(rt, dev, _out_type(rt, out_dtype, rt.torch.bfloat16), M, n), n
     rows, cols, ld = _rows_arg(out, "out", dev, rt.floats if out_dtype is None else (_out_type(rt, out_dtype, None),))
     if rows != M or cols != n:
         _bad(out, "out", f"fp32 or bf16 {(M, n)}")
+    _apart(out, "out", a)
     return out, ld
 
 
@@ -1323,7 +1337,7 @@ def mxfp4_mm(a, a_scales, W, off=None, out=None, out_dtype=None):
     M = _mat_arg(a, "a", dev, (rt.u8,), None, W.in_ // 2)[0]
     _mat_arg(a_scales, "a_scales", dev, (rt.u8,), M, W.in_ // 32)
     po, G = _mm_groups(rt, W, off, dev)
-    out, ld = _mm_out(rt, M, W.rows, dev, out, out_dtype)
+    out, ld = _mm_out(rt, M, W.rows, dev, out, out_dtype, a)
     _launch(rt, "k3c_mxfp4_mm", dev, out.data_ptr(), rt.code[out.dtype], ld, a.data_ptr(), a_scales.data_ptr(), M, W.ref, po, G)
     return out
 
@@ -1337,7 +1351,7 @@ def mxfp4_mm_bwd(dy, W, off=None, out=None, out_dtype=None):
     if n != W.rows:
         _bad(dy, "dy", f"{W.rows} columns")
     po, G = _mm_groups(rt, W, off, dev)
-    out, ld = _mm_out(rt, M, W.in_, dev, out, out_dtype)
+    out, ld = _mm_out(rt, M, W.in_, dev, out, out_dtype, dy)
     _launch(rt, "k3c_mxfp4_mm_bwd", dev, out.data_ptr(), rt.code[out.dtype], ld, dy.data_ptr(), ldd, M, W.ref, po, G)
     return out
 

@@ -31,6 +31,7 @@ namespace k3c {
 
 namespace {
 
+constexpr int MX_DIM = 0x7FFFFFFF - 1023;   // rows and columns at most: sums with a tile's stay within 32 bits
 constexpr int MX_GMAX = 1024;   // groups of a product: with more, the largest tiles' shared memory would not hold the Plan
 
 static __device__ int g_mx_err;
@@ -1466,7 +1467,8 @@ bool al16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 int known(int dt) { return dt == K3C_F32 || dt == K3C_BF16; }
 
 int check_mat(const char *what, const k3c_mxfp4_mat *W, int M, const int *off, int n_groups) {
-    if (!W || !W->codes || !W->atoms || W->rows < 1 || W->in < 32 || W->in % 32 || W->n_mats < 1)
+    if (!W || !W->codes || !W->atoms || W->rows < 1 || W->rows > MX_DIM || W->in < 32 || W->in > MX_DIM || W->in % 32 ||
+        W->n_mats < 1)
         return set_error(K3C_EINVAL, "%s: matrix rows=%d in=%d (a multiple of 32) n_mats=%d", what, W ? W->rows : 0,
                          W ? W->in : 0, W ? W->n_mats : 0);
     if (!al16(W->codes) || !al16(W->atoms) || W->code_stride % 16 || W->atom_stride % 16)
@@ -1475,7 +1477,7 @@ int check_mat(const char *what, const k3c_mxfp4_mat *W, int M, const int *off, i
     if (W->n_mats > 1 && (W->code_stride < cb || W->atom_stride < ab))
         return set_error(K3C_EINVAL, "%s: strides %zu, %zu below a matrix's %zu, %zu bytes", what, W->code_stride,
                          W->atom_stride, cb, ab);
-    if (M < 0 || n_groups < 1 || n_groups > MX_GMAX || (!off && n_groups != 1))
+    if (M < 0 || M > MX_DIM || n_groups < 1 || n_groups > MX_GMAX || (!off && n_groups != 1))
         return set_error(K3C_EINVAL, "%s: M=%d n_groups=%d (1..%d; 1 without offsets)", what, M, n_groups, MX_GMAX);
     if (off && !W->mat_of && n_groups > W->n_mats)
         return set_error(K3C_EINVAL, "%s: %d groups, %d matrices", what, n_groups, W->n_mats);
@@ -1519,12 +1521,14 @@ int check_waits(const char *what, int *err, cudaStream_t s) {
     return K3C_OK;
 }
 
-int check_items(const char *what, int64_t items) {
-    return items < 0x7FFFFFFF ? K3C_OK : set_error(K3C_EINVAL, "%s: %lld tiles exceed 32 bits", what, (long long)items);
-}
-
 // Row tiles of at most `tile` rows that n_groups groups of M rows can have together.
 int64_t most_tiles(int M, int n_groups, int tile) { return (int64_t)M / tile + (n_groups < M ? n_groups : M); }
+
+// Items are numbered in 32 bits; 128 x 64 is the smallest tile.
+int check_items(const char *what, int M, int n_groups, int cols) {
+    const int64_t items = most_tiles(M, n_groups, 128) * ((cols + 63) / 64);
+    return items <= MX_DIM ? K3C_OK : set_error(K3C_EINVAL, "%s: %lld tiles exceed 32 bits", what, (long long)items);
+}
 
 // A kernel's tile and what it costs: a launch takes about fixed + waves * max(K blocks * block + item,
 // store) ns, a wave being one item on every SM (or pair of SMs) and `store` its epilogue. Fitted to
@@ -1567,7 +1571,6 @@ int launch_mm(const CUtensorMap &ma, const CUtensorMap &ma1, const CUtensorMap &
     }
     p.NTL = (p.N + NT - 1) / NT;
     const int64_t items = most_tiles(p.M, p.G, MM_M) * p.NTL;
-    K3C_TRY(check_items("mxfp4_mm", items));
     const int grid = (int)(items < sm_count() ? items : sm_count());
     K3C_TRY_CUDA(launch_pdl(k_mx4_mm<NT>, dim3(grid), dim3(MM_THREADS), MmCfg<NT>::BYTES, s, ma, ma1, mw, p));
     K3C_CHECK_LAUNCH();
@@ -1602,7 +1605,6 @@ int launch_mm_pair(const CUtensorMap &ma, const CUtensorMap &ma1, const CUtensor
     }
     p.NTL = (p.N + 255) / 256;
     const int64_t items = most_tiles(p.M, p.G, 2 * MM_M) * p.NTL;
-    K3C_TRY(check_items("mxfp4_mm", items));
     const int grid = 2 * (int)(items < sm_count() / 2 ? items : sm_count() / 2);
     K3C_TRY_CUDA(launch_pairs(k_mx4_mm_pair, grid, MM_THREADS, PrCfg::BYTES, s, ma, ma1, mw, p));
     K3C_CHECK_LAUNCH();
@@ -1624,7 +1626,6 @@ int launch_bwd(MxArgs p, const k3c_mxfp4_mat *W, const void *dy, int64_t lddy, c
     }
     p.NTL = (p.K + C::TN - 1) / C::TN;
     const int64_t items = most_tiles(p.M, p.G, C::ROWS) * p.NTL;
-    K3C_TRY(check_items("mxfp4_mm_bwd", items));
     if constexpr (PAIR) {
         const int grid = 2 * (int)(items < sm_count() / 2 ? items : sm_count() / 2);
         K3C_TRY_CUDA(launch_pairs(k_mx4_bwd<NT, PAIR, ACCS>, grid, C::THREADS, C::BYTES, s, md, md1, mw, p));
@@ -1644,7 +1645,7 @@ using namespace k3c;
 extern "C" int k3c_mxfp4_quant(uint8_t *packed, uint8_t *scales, const void *x, int x_dtype, int64_t ldx, int rows, int in,
                                k3c_stream_t stream) {
     clear_error();
-    if (rows < 0 || in < 2 || in % 2 || ldx < in || !known(x_dtype))
+    if (rows < 0 || in < 2 || in > MX_DIM || in % 2 || ldx < in || !known(x_dtype))
         return set_error(K3C_EINVAL, "mxfp4_quant: rows=%d in=%d (even) ldx=%lld dtype=%d", rows, in, (long long)ldx, x_dtype);
     if (!rows) return K3C_OK;
     if (!packed || !scales || !x) return set_error(K3C_EINVAL, "mxfp4_quant: NULL array");
@@ -1677,7 +1678,7 @@ extern "C" size_t k3c_mxfp4_atom_bytes(int rows, int in) {
 extern "C" int k3c_mxfp4_pack(uint8_t *codes, uint8_t *atoms, const uint8_t *packed, const uint8_t *scales, int n_mats,
                               int rows, int in, k3c_stream_t stream) {
     clear_error();
-    if (n_mats < 1 || rows < 1 || in < 32 || in % 32)
+    if (n_mats < 1 || rows < 1 || rows > MX_DIM || in < 32 || in > MX_DIM || in % 32)
         return set_error(K3C_EINVAL, "mxfp4_pack: n_mats=%d rows=%d in=%d (a multiple of 32)", n_mats, rows, in);
     if (!codes || !atoms || !packed || !scales) return set_error(K3C_EINVAL, "mxfp4_pack: NULL array");
     if (!al16(codes) || !al16(packed)) return set_error(K3C_EINVAL, "mxfp4_pack: codes and packed must be 16-byte aligned");
@@ -1697,6 +1698,7 @@ extern "C" int k3c_mxfp4_mm(void *y, int y_dtype, int64_t ldy, const uint8_t *a,
     if (!M) return K3C_OK;
     if (!y || !a || !a_scales) return set_error(K3C_EINVAL, "mxfp4_mm: NULL array");
     if (!al16(a)) return set_error(K3C_EINVAL, "mxfp4_mm: a must be 16-byte aligned");
+    K3C_TRY(check_items("mxfp4_mm", M, n_groups, W->rows));
     cudaStream_t s = (cudaStream_t)stream;
     MxArgs p = {};
     K3C_TRY(err_slot(&p.err));
@@ -1740,6 +1742,7 @@ extern "C" int k3c_mxfp4_mm_bwd(void *da, int da_dtype, int64_t ldda, const void
     if (!M) return K3C_OK;
     if (!da || !dy) return set_error(K3C_EINVAL, "mxfp4_mm_bwd: NULL array");
     if (!al16(dy)) return set_error(K3C_EINVAL, "mxfp4_mm_bwd: dy must be 16-byte aligned");
+    K3C_TRY(check_items("mxfp4_mm_bwd", M, n_groups, W->in));
     cudaStream_t s = (cudaStream_t)stream;
     MxArgs p = {};
     K3C_TRY(err_slot(&p.err));

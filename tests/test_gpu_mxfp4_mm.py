@@ -527,3 +527,16 @@ def test_scale_rows_on_any_boundary(k3, dev, first, K):
         av = values(c, b)
         y = k3.mxfp4_mm(a, s, W, out_dtype=torch.float32).double().cpu().numpy()
         check(y, av @ w[0].T, np.abs(av) @ np.abs(w[0]).T, -(-K // 64), False)
+
+
+def test_result_may_not_be_the_rows(k3, dev):
+    import torch
+    W, _ = matrices(k3, dev, 131, 1, 64, 64)
+    dy = torch.randn(9, 64, device=dev).bfloat16()
+    a, s = k3.mxfp4_quant(dy)
+    with pytest.raises(k3.K3CError, match="may not be an input"):
+        k3.mxfp4_mm_bwd(dy, W, out=dy)
+    with pytest.raises(k3.K3CError, match="may not be an input"):
+        k3.mxfp4_mm(a[:8], s[:8], k3.Mxfp4Mat(*k3.mxfp4_pack(*k3.mxfp4_quant(dy[:8]))), out=a.view(-1)[:256].view(torch.float32).view(8, 8))
+    with pytest.raises(k3.K3CError, match="n_experts"):
+        k3.moe_sort(torch.zeros(2, 2, dtype=torch.int32, device=dev), (1 << 32) + 4)

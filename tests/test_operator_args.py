@@ -110,6 +110,31 @@ def test_wrappers_refuse(k3):
             call()
 
 
+def test_extents_past_32_bits_are_refused(k3):
+    """Extents that the C arguments could not hold are refused, not cut; and those whose sums with a
+    tile's would not fit."""
+    import torch
+    L = k3.lib()
+    big = (1 << 31) + 32
+    for rows, n in ((big, 32), (1, big), (big, 2)):
+        t = torch.empty((rows, n), dtype=torch.bfloat16, device="meta")
+        for f in (lambda: k3._rows_arg(t, "x", -1, (torch.bfloat16,)), lambda: k3._mat_arg(t, "x", -1, (torch.bfloat16,))):
+            with pytest.raises(k3.K3CError, match="32 bits"):
+                f()
+        assert k3._rows_arg(t[:5, :2], "x", -1, (torch.bfloat16,))[:2] == (min(rows, 5), 2)
+    top = (1 << 31) - 1024
+    assert L.k3c_mxfp4_mm(BUF, 0, 64, BUF, BUF, top + 1, C.byref(mat(k3)), None, 1, None) == -1 and "M=" in err(k3)
+    assert L.k3c_mxfp4_mm_bwd(BUF, 0, 64, BUF, 64, top + 1, C.byref(mat(k3)), None, 1, None) == -1 and "M=" in err(k3)
+    for kw in (dict(rows=top + 1), dict(in_=top + 32)):
+        assert L.k3c_mxfp4_mm(BUF, 0, top + 64, BUF, BUF, 4, C.byref(mat(k3, **kw)), None, 1, None) == -1 and "matrix" in err(k3)
+    assert L.k3c_mxfp4_quant(BUF, BUF, BUF, 0, top + 32, 1, top + 2, None) == -1 and "in=" in err(k3)
+    assert L.k3c_mxfp4_pack(BUF, BUF, BUF, BUF, 1, top + 1, 32, None) == -1 and "rows=" in err(k3)
+    # more tiles than 32 bits count: 2^31 - 2^12 rows times as many columns
+    n = (1 << 31) - 4096
+    assert L.k3c_mxfp4_mm(BUF, 0, n, BUF, BUF, n, C.byref(mat(k3, rows=n)), None, 1, None) == -1 and "tiles" in err(k3)
+    assert L.k3c_mxfp4_mm_bwd(BUF, 0, n, BUF, 64, n, C.byref(mat(k3, in_=n)), None, 1, None) == -1 and "tiles" in err(k3)
+
+
 def test_mat_struct_layout_matches_header(k3, tmp_path):
     import os
     import subprocess
