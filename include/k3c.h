@@ -608,9 +608,10 @@ int k3c_moe_unpermute_bwd(void *dy, float *dwt, const void *dout, int out_dtype,
 /* x [rows] rows of ldx elements (x_dtype K3C_F32 or K3C_BF16) to packed [rows][in/2] and scales
  * [rows][ceil(in/32)]: per 32 elements scale byte clamp(floor(log2 max|x|) - 2 + 127, 0, 254),
  * codes round(x * 2^(127-byte)) to the nearest E2M1 value, ties to even, saturating at +-6. An
- * infinity makes its group's byte 253 and reads back as an infinity; a NaN makes it 255 with
- * zero codes, which k3c_mxfp4_mm reads as NaN and k3c_mxfp4_dequant, like the reference, as 0.
- * in even. */
+ * infinity makes its group's byte 253: k3c_mxfp4_dequant reads it back as an infinity, for
+ * k3c_mxfp4_mm it is 6 * 2^126 (the format has no infinity) and its group's finite elements are 0;
+ * a NaN makes the byte 255 with zero codes, which k3c_mxfp4_mm reads as NaN and k3c_mxfp4_dequant,
+ * like the reference, as 0. in even. */
 int k3c_mxfp4_quant(uint8_t *packed, uint8_t *scales, const void *x, int x_dtype, int64_t ldx, int rows, int in,
                     k3c_stream_t stream);
 /* A product's right operand: n_mats matrices [rows][in] as codes [rows][in/2], code_stride

@@ -272,6 +272,26 @@ def test_nan_scale_makes_its_row_nan(k3, dev):
     assert torch.isnan(y[2]).all() and torch.isfinite(y[[0, 1, 3, 4]]).all()
 
 
+def test_infinity_is_the_largest_value(k3, dev):
+    """An infinite activation enters a product as 6 * 2^126, exactly: infinite only where the result
+    leaves fp32's range, and no other row sees it."""
+    import torch
+    N, K = 40, 96
+    c, b = operand(141, N, K)
+    for wb in (90, 140):
+        wbyte = np.full_like(b, wb)
+        W = k3.Mxfp4Mat(*k3.mxfp4_pack(*to_dev(dev, pack_nibbles(c)[None], wbyte[None])))
+        x = torch.zeros(3, K)
+        x[0], x[2] = 1.0, 2.0
+        x[1, 40], x[1, 41] = -float("inf"), 5.0
+        y = k3.mxfp4_mm(*k3.mxfp4_quant(x.to(dev)), W, out_dtype=torch.float32).double().cpu().numpy()
+        v = x.double().numpy().copy()
+        v[1, 40], v[1, 41] = -6 * 2.0 ** 126, 0
+        want = v @ values(c, wbyte).T
+        with np.errstate(over="ignore"):
+            assert np.array_equal(y, want.astype(np.float32))
+
+
 def test_scales_over_the_whole_range(k3, dev):
     """Scale bytes 0..254 on either side; results inside fp32's range are right, and the widened
     weights of mm_bwd keep subnormal scales."""
