@@ -1259,7 +1259,7 @@ def mxfp4_pack(packed, scales):
 class Mxfp4Mat:
     """Packed matrices as the right operand of mxfp4_mm: codes [n][rows][in/2] and atoms
     [n][ceil(rows/128)][ceil(in/128)][512] as mxfp4_pack returns them, or one matrix of every run
-    of a PoolMoeLayer (from_pool). The tensors are kept, not copied."""
+    of a PoolMoeLayer or LatentMoeLayer (from_pool). The tensors are kept, not copied."""
 
     __slots__ = ("c", "ref", "rows", "in_", "groups", "dev", "keep")
 
@@ -1286,20 +1286,25 @@ class Mxfp4Mat:
 
     @classmethod
     def from_pool(cls, layer, which):
-        """The experts' matrices of a PoolMoeLayer in its arena, by expert id: "gate_up" [2 * inter]
-        [hidden] (64 gate rows, the matching 64 up rows, and so on) or "down" [hidden][inter].
-        Experts without a run give zeros."""
-        H, I = layer.c.hidden, layer.c.inter
+        """The experts' matrices of a PoolMoeLayer, or of a LatentMoeLayer (hidden: its latent width),
+        in its arena, by expert id: "gate_up" [2 * inter][hidden] (64 gate rows, the matching 64 up
+        rows, and so on) or "down" [hidden][inter]. Experts without a run give zeros."""
+        if isinstance(layer, LatentMoeLayer):
+            c, (arena, run_of) = layer.c.experts, layer._keep[:2]
+        elif isinstance(layer, PoolMoeLayer):
+            c, arena, run_of = layer.c, layer.arena, layer.run_of
+        else:
+            raise K3CError(f"from_pool: {type(layer).__name__} holds no pool-format runs")
         if which not in ("gate_up", "down"):
             raise K3CError(f"from_pool: {which!r}")
+        H, I = c.hidden, c.inter
         lay, _ = pool_layout(H, I)
         p, s = ("gu_p", "gu_s") if which == "gate_up" else ("d_p", "d_s")
         rows, in_ = (2 * I, H) if which == "gate_up" else (H, I)
-        base = layer.arena.data_ptr()
+        base = arena.data_ptr()
         m = cls.__new__(cls)
-        m._set(Mxfp4MatC(base + lay[p][0], base + lay[s][0], layer.stride, layer.stride, layer.c.n_runs, rows, in_,
-                         layer.run_of.data_ptr()), layer.run_of.numel(), layer.arena.get_device(),
-               (layer.arena, layer.run_of))
+        m._set(Mxfp4MatC(base + lay[p][0], base + lay[s][0], c.run_stride, c.run_stride, c.n_runs, rows, in_,
+                         run_of.data_ptr()), run_of.numel(), arena.get_device(), (arena, run_of))
         return m
 
 

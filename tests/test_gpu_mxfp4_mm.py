@@ -433,6 +433,45 @@ def test_experts_of_a_pool_layer_together(k3, dev):
     assert (np.abs(dx.double().cpu().numpy() - want.sum(1)) <= (K + 2) * 2.0 ** -24 * np.abs(want).sum(1)).all()
 
 
+def test_experts_of_a_latent_layer(k3, dev):
+    """A latent layer's own 896 experts at the latent width, 16 a token: both of its matrices from its
+    arena and run table, each against 64 bits, and the gradient through the first."""
+    import torch
+    g = k3.synth.rng(79)
+    H, Lw, I, E, K, T = 512, 256, 128, 896, 16, 40
+    lat = k3.synth.latent_layer(g, H, Lw, I, 5, 4, n_shared=1, wdt=1)
+    few = lat["experts"]
+    lat.update(experts=[few[e % 5] for e in range(E)], topk=K, router_w=np.zeros((E, H), np.float32),
+               router_bias=np.zeros(E, np.float32))
+    layer = k3.LatentMoeLayer.from_host(lat, dev)
+    gn = torch.Generator().manual_seed(3)
+    idx = torch.stack([torch.randperm(E, generator=gn)[:K] for _ in range(T)]).int().to(dev)
+    pos, _, off = k3.moe_sort(idx, E)
+    row_e = np.zeros(T * K, int)
+    row_e[pos.cpu().numpy()] = idx.cpu().numpy() % 5
+
+    def mat(e, name):
+        return values(unpack(e[name + "_p"]), e[name + "_s"])
+    gate_up = np.stack([np.stack([mat(e, "gate").reshape(I // 64, 64, Lw), mat(e, "up").reshape(I // 64, 64, Lw)], 1)
+                        .reshape(2 * I, Lw) for e in few])
+    down = np.stack([mat(e, "down") for e in few])
+    for which, w in (("gate_up", gate_up), ("down", down)):
+        x = torch.randn((T, w.shape[2]), generator=gn).to(dev)
+        a, s = k3.moe_permute_mxfp4(x, pos)
+        W = k3.Mxfp4Mat.from_pool(layer, which)
+        y = k3.mxfp4_mm(a, s, W, off=off, out_dtype=torch.float32).double().cpu().numpy()
+        av = values(unpack(a.cpu().numpy()), s.cpu().numpy())
+        check(y, np.einsum("mk,mnk->mn", av, w[row_e]), np.einsum("mk,mnk->mn", np.abs(av), np.abs(w[row_e])),
+              w.shape[2] // 64, False)
+        dy = torch.randn((T * K, w.shape[1]), generator=gn).bfloat16().to(dev)
+        da = k3.mxfp4_mm_bwd(dy, W, off=off, out_dtype=torch.float32).double().cpu().numpy()
+        dv = dy.double().cpu().numpy()
+        check(da, np.einsum("mn,mnk->mk", dv, w[row_e]), np.einsum("mn,mnk->mk", np.abs(dv), np.abs(w[row_e])),
+              w.shape[1] // 16, False)
+    with pytest.raises(k3.K3CError, match="no pool-format runs"):
+        k3.Mxfp4Mat.from_pool(lat, "down")
+
+
 def test_products_match_the_gemv_and_dequant(k3, dev):
     """The same codes through the framework's own fp32-activation GEMV and dequantiser."""
     import torch
