@@ -599,8 +599,11 @@ __device__ __forceinline__ void a_scales(const MxArgs &p, int n_items, const Ite
 
 // 128 rows x NT columns per item, one CTA per SM. A K block is 256 codes of a row, 128 bytes: four
 // MMAs of K = 64 and two TMEM copies of scale atoms per operand. Bound by HBM for few rows (16 x 8
-// rows over 64 experts of 4096 x 7168: 122 us, the weights at 7.1 TB/s), by the MMA thread's 0.24 us
-// a K block for one tile in a row (one token, 7168 x 7168: 10.4 us), by L2 and power above.
+// rows over 64 experts of 4096 x 7168: 122 us, the weights at 7.1 TB/s), by the chain of K
+// blocks for one tile in a row (one token, 7168 x 7168: 9.8 us, 0.20 us a K block: about half of it
+// waits, copies and commits, 25 ns an MMA however few its columns; fewer stages, a second accumulator
+// or no proxy fence left it as it was, and a K split would make a row's result depend on how many
+// rows are beside it), by L2 and power above.
 template <int NT>
 __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant__ CUtensorMap tmA,
                                                           const __grid_constant__ CUtensorMap tmA1,
