@@ -782,7 +782,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant_
 // 113 (141). 470 cycles a K block, the MMAs' own time, at the 1.5 GHz that power leaves; the first
 // blocks of an item and the last wave are the rest. W's scales of all 256 columns are in both CTAs.
 // The pair's first CTA issues all MMAs. Its partner's warp 1 passes each filled stage on: it waits
-// for the local copies, fences A's scales and arrives on pfull in the first CTA. MMA commits free
+// for the local copies, fences A's scales and arrives on `full` in the first CTA. MMA commits free
 // the stage in both.
 struct PrCfg {
     static constexpr int B = 128 * 128;
@@ -840,7 +840,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm_pair(const __grid_cons
     extern __shared__ uint8_t pr_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)pr_raw + 1023) & ~(uintptr_t)1023);
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::STAGES * C::STAGE);
-    uint64_t *pfull = full + C::STAGES, *empty = pfull + C::STAGES, *tfull = empty + C::STAGES, *tempty = tfull + 1;
+    uint64_t *empty = full + C::STAGES, *tfull = empty + C::STAGES, *tempty = tfull + 1;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tempty + 1);
     uint8_t *stg_all = smem + C::STAGES * C::STAGE + 256;
     __shared__ Plan plan;
@@ -849,8 +849,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm_pair(const __grid_cons
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::STAGES; i++) {
-            tc::mbar_init(&full[i], 3);
-            tc::mbar_init(&pfull[i], 1);
+            tc::mbar_init(&full[i], rank == 0 ? 4 : 3);   // the first CTA's: the partner's stage too
             tc::mbar_init(&empty[i], 1);
         }
         tc::mbar_init(tfull, 1);
@@ -919,7 +918,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm_pair(const __grid_cons
                 for (int kb = 0; kb < KB; kb++) {
                     if (!tc::mbar_wait(&full[st], ph, p.err, 113)) { ok = false; break; }
                     tc::fence_proxy_async_smem();
-                    mbar_arrive_cta(&pfull[st], 0);
+                    mbar_arrive_cta(&full[st], 0);
                     if (++st == C::STAGES) {
                         st = 0;
                         ph ^= 1u;
@@ -940,7 +939,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm_pair(const __grid_cons
                 tph ^= 1u;
                 tc::tc_fence_after();
                 for (int kb = 0; kb < KB; kb++) {
-                    if (!tc::mbar_wait(&full[st], ph, p.err, 115) || !tc::mbar_wait(&pfull[st], ph, p.err, 116)) { ok = false; break; }
+                    if (!tc::mbar_wait(&full[st], ph, p.err, 115)) { ok = false; break; }
                     tc::fence_proxy_async_smem();
                     tc::tc_fence_after();
                     const uint64_t so = (uint64_t)(st * (C::STAGE >> 4));
@@ -1053,8 +1052,8 @@ struct MbCfg {
     static constexpr int BYTES = 1024 + RING * (A + B) + RAW * R + 512;
     static_assert(B % 1024 == 0, "slots stay 1024-byte aligned");
     static_assert(NBUF * ACCS * TN <= 512, "TMEM columns");
-    static_assert(RING % TURNS == 0 && RAW % TURNS == 0, "a slot belongs to one group");
-    static_assert((4 * RING + 2 * RAW + 4) * 8 + 4 <= 512, "barriers");
+    static_assert(RING == TURNS && RAW % TURNS == 0, "a slot belongs to one group");
+    static_assert((2 * RING + 2 * RAW + 4) * 8 + 4 <= 512, "barriers");
     static_assert(BYTES + sizeof(Plan) + 64 <= 227 * 1024, "one CTA per SM");
 };
 
@@ -1149,9 +1148,8 @@ __global__ void __launch_bounds__(MbCfg<NT, PAIR, ACCS>::THREADS, 1) k_mx4_bwd(c
     extern __shared__ uint8_t mb_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)mb_raw + 1023) & ~(uintptr_t)1023);
     uint8_t *s_a = smem, *s_b = s_a + C::RING * C::A, *s_r = s_b + C::RING * C::B;
-    uint64_t *afull = reinterpret_cast<uint64_t *>(s_r + C::RAW * C::R);
-    uint64_t *wide = afull + C::RING, *empty = wide + C::RING, *pfull = empty + C::RING;
-    uint64_t *rfull = pfull + C::RING, *rempty = rfull + C::RAW;
+    uint64_t *full = reinterpret_cast<uint64_t *>(s_r + C::RAW * C::R), *empty = full + C::RING;
+    uint64_t *rfull = empty + C::RING, *rempty = rfull + C::RAW;
     uint64_t *tfull = rempty + C::RAW, *tempty = tfull + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tempty + 2);
     __shared__ Plan plan;
@@ -1160,10 +1158,9 @@ __global__ void __launch_bounds__(MbCfg<NT, PAIR, ACCS>::THREADS, 1) k_mx4_bwd(c
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::RING; i++) {
-            tc::mbar_init(&afull[i], 1);
-            tc::mbar_init(&wide[i], MB_GROUP);
+            // dY's copy, the widening warps and, in a pair's first CTA, the partner's slot
+            tc::mbar_init(&full[i], 1 + MB_GROUP + (PAIR && rank == 0 ? 1 : 0));
             tc::mbar_init(&empty[i], 1);
-            tc::mbar_init(&pfull[i], 1);
         }
         for (int i = 0; i < C::RAW; i++) {
             tc::mbar_init(&rfull[i], 1);
@@ -1215,14 +1212,14 @@ __global__ void __launch_bounds__(MbCfg<NT, PAIR, ACCS>::THREADS, 1) k_mx4_bwd(c
                 for (int kb = 0; kb < KB; kb++, n++) {
                     if (!tc::mbar_wait(&empty[st], ph, p.err, 91)) { ok = false; break; }
                     uint8_t *sa = s_a + st * C::A;
-                    tc::mbar_expect_tx(&afull[st], all * 32 * 128);
+                    tc::mbar_expect_tx(&full[st], all * 32 * 128);
 #pragma unroll
                     for (int j = 0; j < ACCS; j++) {
                         const int row = x.row0 + first_row(j);
-                        if (boxes[j] == 4) tc::tma_load_3d(sa + j * (128 * 128), &tmD, &afull[st], kb * MB_KB, row, 0);
+                        if (boxes[j] == 4) tc::tma_load_3d(sa + j * (128 * 128), &tmD, &full[st], kb * MB_KB, row, 0);
                         else
                             for (int b = 0; b < boxes[j]; b++)
-                                tc::tma_load_3d(sa + j * (128 * 128) + b * (32 * 128), &tmD1, &afull[st], kb * MB_KB, row + b * 32, 0);
+                                tc::tma_load_3d(sa + j * (128 * 128) + b * (32 * 128), &tmD1, &full[st], kb * MB_KB, row + b * 32, 0);
                     }
                     if (++st == C::RING) {
                         st = 0;
@@ -1232,7 +1229,7 @@ __global__ void __launch_bounds__(MbCfg<NT, PAIR, ACCS>::THREADS, 1) k_mx4_bwd(c
             }
             // no copy may still be landing when the CTA exits
             for (uint32_t i = n > C::RING ? n - C::RING : 0; i < n; i++)
-                tc::mbar_wait(&afull[i % C::RING], (i / C::RING) & 1u, p.err, 92);
+                tc::mbar_wait(&full[i % C::RING], (i / C::RING) & 1u, p.err, 92);
         }
     } else if (warp == 2) {
         // ------------------------------------------------------------ W copies
@@ -1268,8 +1265,8 @@ __global__ void __launch_bounds__(MbCfg<NT, PAIR, ACCS>::THREADS, 1) k_mx4_bwd(c
             for (int it = it0; ok && it < n_items; it += step) {
                 if (item(it).mat < 0) continue;
                 for (int kb = 0; kb < KB; kb++) {
-                    if (!tc::mbar_wait(&afull[st], ph, p.err, 101) || !tc::mbar_wait(&wide[st], ph, p.err, 102)) { ok = false; break; }
-                    mbar_arrive_cta(&pfull[st], 0);
+                    if (!tc::mbar_wait(&full[st], ph, p.err, 101)) { ok = false; break; }
+                    mbar_arrive_cta(&full[st], 0);
                     if (++st == C::RING) {
                         st = 0;
                         ph ^= 1u;
@@ -1292,8 +1289,7 @@ __global__ void __launch_bounds__(MbCfg<NT, PAIR, ACCS>::THREADS, 1) k_mx4_bwd(c
                 const uint32_t d = tmem + a * ACCS * C::TN;
                 const bool two = ACCS == 2 && x.n > C::ROWS / 2;
                 for (int kb = 0; kb < KB; kb++) {
-                    if (!tc::mbar_wait(&afull[st], ph, p.err, 96) || !tc::mbar_wait(&wide[st], ph, p.err, 97)) { ok = false; break; }
-                    if (PAIR && !tc::mbar_wait(&pfull[st], ph, p.err, 103)) { ok = false; break; }
+                    if (!tc::mbar_wait(&full[st], ph, p.err, 96)) { ok = false; break; }
                     tc::tc_fence_after();
                     const uint64_t da = da0 + st * (C::A >> 4), db = db0 + st * (C::B >> 4);
 #pragma unroll
@@ -1324,76 +1320,75 @@ __global__ void __launch_bounds__(MbCfg<NT, PAIR, ACCS>::THREADS, 1) k_mx4_bwd(c
         // ------------------------------------------------------------ widening
         const int w4 = (warp - MB_WIDE0) % MB_GROUP;
         const uint32_t turn = (warp - MB_WIDE0) / MB_GROUP;
-        uint32_t n = 0, st = 0, ph = 1, rt = 0, rph = 0;   // slot and awaited parity of the two rings
+        // A group steps straight from one of its K blocks to the next (counting through the others' cost
+        // 250 cycles a block, a third of a group's time): its slot of the widened ring is number
+        // `turn`, and its packed slots come round by TURNS.
+        uint32_t n = 0, ph = 1, rt = turn, rph = 0;   // K blocks before the item; awaited parities, packed slot
+        uint8_t *const sb = s_b + turn * C::B;
         bool ok = true;
         for (int it = it0; ok && it < n_items; it += step) {
-            const Item x = item(it);
-            if (x.mat < 0) continue;
-            for (int kb = 0; ok && kb < KB; kb++, n++) {
-                if (n % C::TURNS == turn) {
-                    ok = __all_sync(0xFFFFFFFFu, tc::mbar_wait(&rfull[rt], rph, p.err, 98));
-                    if (!ok) break;
-                    // a lane widens 32 codes of MB_RJ W rows in each 128 columns: groups g and g + 4
-                    // (eight lanes touch eight rows: the swizzle spreads them over the banks)
-                    constexpr int GH = NT / 128, RJ = 8 / MB_GROUP;
-                    const uint8_t *sw = s_r + rt * C::R;
-                    const int r0 = 8 * RJ * w4 + (lane & 7), g = lane >> 3;
-                    uint4 c[RJ][GH];
-                    uint32_t s[RJ][GH];
+            if (item(it).mat < 0) continue;
+            for (int kb = (int)((turn + C::TURNS - n % C::TURNS) % C::TURNS); kb < KB; kb += C::TURNS) {
+                ok = __all_sync(0xFFFFFFFFu, tc::mbar_wait(&rfull[rt], rph, p.err, 98));
+                if (!ok) break;
+                // a lane widens 32 codes of MB_RJ W rows in each 128 columns: groups g and g + 4
+                // (eight lanes touch eight rows: the swizzle spreads them over the banks)
+                constexpr int GH = NT / 128, RJ = 8 / MB_GROUP;
+                const uint8_t *sw = s_r + rt * C::R;
+                const int r0 = 8 * RJ * w4 + (lane & 7), g = lane >> 3;
+                uint4 c[RJ][GH];
+                uint32_t s[RJ][GH];
 #pragma unroll
-                    for (int j = 0; j < RJ; j++)
+                for (int j = 0; j < RJ; j++)
 #pragma unroll
-                        for (int i = 0; i < GH; i++) {
-                            const int r = r0 + 8 * j;
-                            const int at = NT == 256 ? (g + 4 * i) ^ (r & 7) : g ^ ((r >> 1) & 3);   // 128- and 64-byte swizzle
-                            c[j][i] = *reinterpret_cast<const uint4 *>(sw + r * C::WB + 16 * at);
-                            s[j][i] = sw[C::W + i * 512 + sf_byte((kb & 1) * 64 + r, g)];
+                    for (int i = 0; i < GH; i++) {
+                        const int r = r0 + 8 * j;
+                        const int at = NT == 256 ? (g + 4 * i) ^ (r & 7) : g ^ ((r >> 1) & 3);   // 128- and 64-byte swizzle
+                        c[j][i] = *reinterpret_cast<const uint4 *>(sw + r * C::WB + 16 * at);
+                        s[j][i] = sw[C::W + i * 512 + sf_byte((kb & 1) * 64 + r, g)];
+                    }
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&rempty[rt]);
+                ok = __all_sync(0xFFFFFFFFu, tc::mbar_wait(&empty[turn], ph, p.err, 99));
+                if (!ok) break;
+#pragma unroll
+                for (int j = 0; j < RJ; j++)
+#pragma unroll
+                    for (int i = 0; i < GH; i++) {
+                        const int r = r0 + 8 * j;
+                        const uint32_t e = min(s[j][i], 128u) + 126u;    // 2^(min(byte, 128) - 1)
+                        const uint32_t f1 = e << 7 | e << 23;
+                        const uint32_t cw[4] = {c[j][i].x, c[j][i].y, c[j][i].z, c[j][i].w};
+                        uint32_t o[4][4];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) e2m1x8_widen(cw[k], f1, o[k]);
+                        if (s[j][i] > 128) {                             // the rest of a scale above 2^1
+                            const uint32_t h = s[j][i] - 1u, f2 = h << 7 | h << 23;   // 2^(byte - 128)
+#pragma unroll
+                            for (int k = 0; k < 4; k++)
+#pragma unroll
+                                for (int q = 0; q < 4; q++) o[k][q] = mul_bf16x2(o[k][q], f2);
                         }
-                    __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(&rempty[rt]);
-                    ok = __all_sync(0xFFFFFFFFu, tc::mbar_wait(&empty[st], ph, p.err, 99));
-                    if (!ok) break;
-                    uint8_t *sb = s_b + st * C::B;
+                        // Column order within the 32: piece q holds codes q and q + 4 of each of
+                        // the four words, so that a lane of the epilogue's 16x256b loads, which
+                        // gets columns 2l and 2l + 1 of every piece, gets word l: eight neighbours.
+                        uint8_t *row = sb + ((g + 4 * i) >> 1) * (MB_KB * 128) + r * 128;
 #pragma unroll
-                    for (int j = 0; j < RJ; j++)
-#pragma unroll
-                        for (int i = 0; i < GH; i++) {
-                            const int r = r0 + 8 * j;
-                            const uint32_t e = min(s[j][i], 128u) + 126u;    // 2^(min(byte, 128) - 1)
-                            const uint32_t f1 = e << 7 | e << 23;
-                            const uint32_t cw[4] = {c[j][i].x, c[j][i].y, c[j][i].z, c[j][i].w};
-                            uint32_t o[4][4];
-#pragma unroll
-                            for (int k = 0; k < 4; k++) e2m1x8_widen(cw[k], f1, o[k]);
-                            if (s[j][i] > 128) {                             // the rest of a scale above 2^1
-                                const uint32_t h = s[j][i] - 1u, f2 = h << 7 | h << 23;   // 2^(byte - 128)
-#pragma unroll
-                                for (int k = 0; k < 4; k++)
-#pragma unroll
-                                    for (int q = 0; q < 4; q++) o[k][q] = mul_bf16x2(o[k][q], f2);
-                            }
-                            // Column order within the 32: piece q holds codes q and q + 4 of each of
-                            // the four words, so that a lane of the epilogue's 16x256b loads, which
-                            // gets columns 2l and 2l + 1 of every piece, gets word l: eight neighbours.
-                            uint8_t *row = sb + ((g + 4 * i) >> 1) * (MB_KB * 128) + r * 128;
-#pragma unroll
-                            for (int q = 0; q < 4; q++)
-                                *reinterpret_cast<uint4 *>(row + 16 * (((g & 1) * 4 + q) ^ (r & 7))) =
-                                    make_uint4(o[0][q], o[1][q], o[2][q], o[3][q]);
-                        }
-                    tc::fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(&wide[st]);
-                }
-                if (++st == C::RING) {
-                    st = 0;
-                    ph ^= 1u;
-                }
-                if (++rt == C::RAW) {
-                    rt = 0;
+                        for (int q = 0; q < 4; q++)
+                            *reinterpret_cast<uint4 *>(row + 16 * (((g & 1) * 4 + q) ^ (r & 7))) =
+                                make_uint4(o[0][q], o[1][q], o[2][q], o[3][q]);
+                    }
+                tc::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&full[turn]);
+                ph ^= 1u;
+                rt += C::TURNS;
+                if (rt >= C::RAW) {
+                    rt -= C::RAW;
                     rph ^= 1u;
                 }
             }
+            n += KB;
         }
     } else if (warp >= C::EPI0) {
         // ------------------------------------------------------------ epilogue
