@@ -1089,11 +1089,14 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
 }
 // Eight E2M1 codes to bf16: a code's exponent and mantissa bits at bits 8..6 of a bf16 are its
 // value times 2^-126, subnormals included, so f1 = 2^(byte-1) under both halves gives the scaled
-// value in one exact product. Codes j and j + 4 share word j, as they lie 16 bits apart.
+// value in one exact product. Codes j and j + 4 share word j, as they lie 16 bits apart. A multiply
+// puts a code's magnitude and sign in place at once (the bits between are masked), shifts and masks
+// do the same on the other pipe: two words each (64 x 7168 x 2048: 35.2 us; all by shifts 35.7, all by
+// multiplies 36.3).
 __device__ __forceinline__ void e2m1x8_widen(uint32_t w, uint32_t f1, uint32_t (&o)[4]) {
     constexpr uint32_t mag = 0x01C001C0u, sign = 0x80008000u;
-    o[0] = mul_bf16x2(((w << 6) & mag) | ((w << 12) & sign), f1);
-    o[1] = mul_bf16x2(((w << 2) & mag) | ((w << 8) & sign), f1);
+    o[0] = mul_bf16x2(((w & 0x000F000Fu) * 0x1040u) & (mag | sign), f1);
+    o[1] = mul_bf16x2(((w & 0x00F000F0u) * 0x0104u) & (mag | sign), f1);
     o[2] = mul_bf16x2(((w >> 2) & mag) | ((w << 4) & sign), f1);
     o[3] = mul_bf16x2(((w >> 6) & mag) | (w & sign), f1);
 }
