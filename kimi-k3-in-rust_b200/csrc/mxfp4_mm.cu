@@ -1021,7 +1021,6 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm_pair(const __grid_cons
 // one ring for all three a slot was held through copy, widening and MMA, 3900 cycles for 1024
 // of MMAs: three slots' worth of them set the pace.
 constexpr int MB_KB = 64;                        // W rows per K block
-constexpr int MB_GROUP = 4;                      // warps that widen one K block; groups take turns
 constexpr int MB_EPI = 8;
 constexpr int MB_WIDE0 = 3;                      // warps: dY, MMA, W, widening, epilogue
 // 128 rows x NT columns (W's in) per CTA and item; columns narrower than 256 make more items where
@@ -1048,7 +1047,12 @@ struct MbCfg {
     // group's, which then awaits each of the slot's phases in turn: a group that skipped a phase
     // could take the one before it, of the same parity, for the one it needs.
     static constexpr int TURNS = RING;
-    static constexpr int EPI0 = MB_WIDE0 + TURNS * MB_GROUP, THREADS = 32 * (EPI0 + MB_EPI);
+    // Warps that widen one K block. Where a single CTA widens 128 columns of it two do, with more in
+    // flight each: four warps' issue slots are what few rows wait for (64 x 7168 x 2048 34.0 us,
+    // 35.0 with four; 39.5 with one). Pairs and 256 columns need four (1200 x 7168 x 2048 39.1, 41.9
+    // with two; 128 x 7168 x 37888 70 and 92).
+    static constexpr int GROUP = !PAIR && NT == 128 ? 2 : 4;
+    static constexpr int EPI0 = MB_WIDE0 + TURNS * GROUP, THREADS = 32 * (EPI0 + MB_EPI);
     static constexpr int BYTES = 1024 + RING * (A + B) + RAW * R + 512;
     static_assert(B % 1024 == 0, "slots stay 1024-byte aligned");
     static_assert(NBUF * ACCS * TN <= 512, "TMEM columns");
@@ -1162,12 +1166,12 @@ __global__ void __launch_bounds__(MbCfg<NT, PAIR, ACCS>::THREADS, 1) k_mx4_bwd(c
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::RING; i++) {
             // dY's copy, the widening warps and, in a pair's first CTA, the partner's slot
-            tc::mbar_init(&full[i], 1 + MB_GROUP + (PAIR && rank == 0 ? 1 : 0));
+            tc::mbar_init(&full[i], 1 + C::GROUP + (PAIR && rank == 0 ? 1 : 0));
             tc::mbar_init(&empty[i], 1);
         }
         for (int i = 0; i < C::RAW; i++) {
             tc::mbar_init(&rfull[i], 1);
-            tc::mbar_init(&rempty[i], MB_GROUP);
+            tc::mbar_init(&rempty[i], C::GROUP);
         }
         for (int i = 0; i < C::NBUF; i++) {
             tc::mbar_init(&tfull[i], 1);
@@ -1321,8 +1325,8 @@ __global__ void __launch_bounds__(MbCfg<NT, PAIR, ACCS>::THREADS, 1) k_mx4_bwd(c
         }
     } else if (warp >= MB_WIDE0 && warp < C::EPI0) {
         // ------------------------------------------------------------ widening
-        const int w4 = (warp - MB_WIDE0) % MB_GROUP;
-        const uint32_t turn = (warp - MB_WIDE0) / MB_GROUP;
+        const int w4 = (warp - MB_WIDE0) % C::GROUP;
+        const uint32_t turn = (warp - MB_WIDE0) / C::GROUP;
         // A group steps straight from one of its K blocks to the next (counting through the others' cost
         // 250 cycles a block, a third of a group's time): its slot of the widened ring is number
         // `turn`, and its packed slots come round by TURNS.
@@ -1334,9 +1338,9 @@ __global__ void __launch_bounds__(MbCfg<NT, PAIR, ACCS>::THREADS, 1) k_mx4_bwd(c
             for (int kb = (int)((turn + C::TURNS - n % C::TURNS) % C::TURNS); kb < KB; kb += C::TURNS) {
                 ok = __all_sync(0xFFFFFFFFu, tc::mbar_wait(&rfull[rt], rph, p.err, 98));
                 if (!ok) break;
-                // a lane widens 32 codes of MB_RJ W rows in each 128 columns: groups g and g + 4
+                // a lane widens 32 codes of RJ W rows in each 128 columns: groups g and g + 4
                 // (eight lanes touch eight rows: the swizzle spreads them over the banks)
-                constexpr int GH = NT / 128, RJ = 8 / MB_GROUP;
+                constexpr int GH = NT / 128, RJ = 8 / C::GROUP;
                 const uint8_t *sw = s_r + rt * C::R;
                 const int r0 = 8 * RJ * w4 + (lane & 7), g = lane >> 3;
                 uint4 c[RJ][GH];
@@ -1760,13 +1764,13 @@ extern "C" int k3c_mxfp4_mm_bwd(void *da, int da_dtype, int64_t ldda, const void
     p.n_mats = W->n_mats;
     p.atoms = W->atoms;
     p.atom_stride = W->atom_stride;
-    // (112 K blocks: pair 43.8 us at 512 x 7168, 256 columns 69, 128 78; at 64 x 7168 42, 68, 41;
-    // the pair's two accumulators 72 us and one 83 at 2400 x 2048, 692 and 824 at 32768 x 2048, but
-    // 64 K blocks 45 and 28 at 1200 x 2048)
-    static const TileCost kinds[] = {{512, 256, 2, 560, 4500, 0, 6300},
-                                     {256, 256, 2, 335, 300, 0, 6300},
-                                     {128, 256, 1, 555, 500, 0, 5900},
-                                     {128, 128, 1, 320, 400, 0, 4800}};
+    // (112 K blocks, 2048 columns: 64 rows take the pair 41 us, 256 columns 58, 128 columns 35; 2000 rows
+    // 43, 61, 70; two accumulators 72 there, but 257 and one 305 at 12000 rows. 4 K blocks, 2000 x 2048:
+    // the pair 9.2, 128 columns 7.4)
+    static const TileCost kinds[] = {{512, 256, 2, 555, 4050, 0, 5150},
+                                     {256, 256, 2, 325, 1100, 0, 6200},
+                                     {128, 256, 1, 505, 550, 0, 5100},
+                                     {128, 128, 1, 295, 300, 1700, 3850}};
     const int kind = cheapest(kinds, 4, M, n_groups, off != nullptr, p.K, (p.N + MB_KB - 1) / MB_KB);
     if (kind == 0) K3C_TRY((launch_bwd<128, true, 2>(p, W, dy, lddy, s)));
     else if (kind == 1) K3C_TRY((launch_bwd<128, true, 1>(p, W, dy, lddy, s)));
