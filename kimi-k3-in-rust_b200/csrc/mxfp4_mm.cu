@@ -1028,7 +1028,9 @@ constexpr int MB_WIDE0 = 3;                      // warps: dY, MMA, W, widening,
 // (cta_group::2); each widens NT of them and the MMA reads both CTAs' halves. Shared memory's
 // bandwidth bounds these kernels: a K block of 128 x 256 takes one CTA 121 KB through it (copies
 // in, packed tile out, widened tile in, both operands out), 950 cycles at 128 bytes a cycle, for
-// 512 cycles of MMAs; a pair's CTA 73 KB, 580 cycles. ACCS = 2: a pair takes 512 rows in two
+// 512 cycles of MMAs; a pair's CTA 73 KB, 580 cycles; 128 x 128 72 KB, 560 cycles, to which the
+// widening's instructions add (without its arithmetic 64 x 7168 x 2048 takes 30 us of 34, with half its
+// stores 30, without dY's copies 31, with a deeper ring for them 34). ACCS = 2: a pair takes 512 rows in two
 // accumulators, so a widened tile serves both; what that saves is mostly power, which bounds the
 // clock under large products. It leaves no TMEM for the next item's accumulators.
 template <int NT, bool PAIR, int ACCS>
@@ -1145,8 +1147,9 @@ __device__ __forceinline__ void put8(const MxArgs &p, int64_t row, int col, cons
 }
 
 // Dense 32768 x 7168 x 2048 (rows, contracted, columns): 627 us, 1.53 PFLOP/s, 692 after some
-// seconds at the power limit. 32768 rows in 48 groups: 840-920 us at 1.37 GHz, 600 cycles a K block
-// against 512 of MMAs, 15% of the tiles' rows empty. 2400 rows in 48 groups of 1432 x 992: 32 us.
+// seconds at the power limit. 32768 rows in 48 groups: 780-880 us at 1.37 GHz, 600 cycles a K block
+// against 512 of MMAs, 15% of the tiles' rows empty. 2400 rows in 48 groups of 1432 x 992: 26 us, 28 with
+// a cold L2.
 template <int NT, bool PAIR, int ACCS>
 __global__ void __launch_bounds__(MbCfg<NT, PAIR, ACCS>::THREADS, 1) k_mx4_bwd(const __grid_constant__ CUtensorMap tmD,
                                                            const __grid_constant__ CUtensorMap tmD1,
