@@ -294,3 +294,32 @@ def test_permute_of_strided_rows(k3, dev, first, pad, dtype):
     n = int(off[-1])
     x = rand((T, first + H + pad), dtype, 1, dev)[:, first:first + H]
     assert torch.equal(k3.moe_permute(x, pos)[:n], x[(pair[:n] // K).long()])
+
+
+@pytest.mark.parametrize("first", [0, 1])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_one_gradient_of_the_sum_alone(k3, dev, dtype, first):
+    """k3c_moe_unpermute_bwd with dy or dwt left out gives the other as with both (y is not read
+    without dwt); rows on odd addresses (first = 1) and a width no vector divides among them."""
+    import torch
+    L, st = k3.lib(), torch.cuda.current_stream(dev).cuda_stream
+    code = {"bf16": k3.K3C_BF16, "f32": k3.K3C_F32}[dtype]
+    T, K, E = 21, 5, 9
+    pos, _, _ = k3.moe_sort(torch.from_numpy(routing(T, K, E, "holes", 4)).to(dev), E)
+    wt = rand((T, K), "f32", 6, dev)
+    for H in (64, 4097):
+        def odd(rows, seed):
+            return rand((rows * H + first,), dtype, seed, dev)[first:].view(rows, H)
+        y, dout = odd(T * K, 7), odd(T, 8)
+        both = [torch.full_like(y, 3.0), torch.full((T, K), 3.0, device=dev)]
+        k3.moe_unpermute_bwd(dout, y, pos, wt, dy=both[0], dwt=both[1])
+        dy, dwt = odd(T * K, 9).fill_(3.0), torch.full((T, K), 3.0, device=dev)
+        for a, b, yy in ((dy, None, None), (None, dwt, y)):
+            rc = L.k3c_moe_unpermute_bwd(*(None if t is None else t.data_ptr() for t in (a, b)), dout.data_ptr(), code,
+                                         None if yy is None else yy.data_ptr(), code, wt.data_ptr(), pos.data_ptr(), T, K, H, st)
+            assert rc == 0
+        assert torch.equal(dy, both[0])
+        # the sums' split over threads goes with the width alone, but not over vectors and elements
+        want = (dout[:, None].double() * y[pos.clamp(min=0).long()].double())
+        lim = (H // 256 * 8 + 32) * 2.0 ** -24 * want.abs().sum(-1) * (pos >= 0)
+        assert ((dwt.double() - want.sum(-1) * (pos >= 0)).abs() <= lim).all()

@@ -599,3 +599,16 @@ def test_result_may_not_be_the_rows(k3, dev):
         k3.mxfp4_mm(a[:8], s[:8], k3.Mxfp4Mat(*k3.mxfp4_pack(*k3.mxfp4_quant(dy[:8]))), out=a.view(-1)[:256].view(torch.float32).view(8, 8))
     with pytest.raises(k3.K3CError, match="n_experts"):
         k3.moe_sort(torch.zeros(2, 2, dtype=torch.int32, device=dev), (1 << 32) + 4)
+
+
+def test_pack_in_place(k3, dev):
+    """The codes written over the packed nibbles they come from."""
+    import torch
+    g = np.random.default_rng(8)
+    n, rows, in_ = 3, 70, 160
+    p, s = to_dev(dev, g.integers(0, 256, (n, rows, in_ // 2), dtype=np.uint8), g.integers(250, 256, (n, rows, in_ // 32), dtype=np.uint8))
+    codes, atoms = k3.mxfp4_pack(p, s)
+    mine = torch.empty_like(atoms)
+    assert k3.lib().k3c_mxfp4_pack(p.data_ptr(), mine.data_ptr(), p.data_ptr(), s.data_ptr(), n, rows, in_,
+                                   torch.cuda.current_stream(dev).cuda_stream) == 0
+    assert torch.equal(p, codes) and torch.equal(mine, atoms)
