@@ -1057,6 +1057,7 @@ def _launch(rt, name, dev, *args):
 
 
 _INT_MAX = 0x7FFFFFFF      # what the entry points' int arguments hold
+_SORT_EMAX = 2048          # experts that k3c_moe_sort takes
 
 
 def _bad(t, name, want):
@@ -1113,15 +1114,17 @@ def _sort_scratch(T, K, n_experts):
 def moe_sort(idx, n_experts):
     """Stable sort of a routing's pairs by expert: idx [T][topk] int32 -> (pos [T][topk], pair
     [T * topk], off [n_experts + 1]) int32. pos is a pair's row, -1 for ids outside
-    0..n_experts-1; pair a row's pair t * topk + j, -1 behind the last row (off[n_experts])."""
+    0..n_experts-1 (n_experts at most 2048); pair a row's pair t * topk + j, -1 behind the last row
+    (off[n_experts])."""
+    # off's length hangs on it, and an int argument would be cut to 32 bits without a word
+    if not 1 <= n_experts <= _SORT_EMAX:
+        raise K3CError(f"n_experts {n_experts}: 1..{_SORT_EMAX}")
     rt = _runtime(idx)
     dev = idx.get_device()
     T, K = _mat_arg(idx, "idx", dev, (rt.i32,))
-    if n_experts > _INT_MAX:
-        raise K3CError(f"n_experts {n_experts}: 32 bits")
     n = _sort_scratch(T, K, n_experts)
     pos, pair = _new(rt, dev, rt.i32, T, K), _new(rt, dev, rt.i32, T * K)
-    off = _new(rt, dev, rt.i32, max(n_experts, 0) + 1)
+    off = _new(rt, dev, rt.i32, n_experts + 1)
     ws = _new(rt, dev, rt.i32, n // 4) if n else None
     _launch(rt, "k3c_moe_sort", dev, pos.data_ptr(), pair.data_ptr(), off.data_ptr(), idx.data_ptr(), T, K, n_experts,
             ws.data_ptr() if n else None, n)

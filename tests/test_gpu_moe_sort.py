@@ -323,3 +323,11 @@ def test_one_gradient_of_the_sum_alone(k3, dev, dtype, first):
         want = (dout[:, None].double() * y[pos.clamp(min=0).long()].double())
         lim = (H // 256 * 8 + 32) * 2.0 ** -24 * want.abs().sum(-1) * (pos >= 0)
         assert ((dwt.double() - want.sum(-1) * (pos >= 0)).abs() <= lim).all()
+
+
+@pytest.mark.parametrize("n", [0, 2049, -(1 << 32) + 2048, (1 << 32) + 1])
+def test_expert_counts_the_sort_refuses(k3, dev, n):
+    import torch
+    with pytest.raises(k3.K3CError, match="n_experts"):
+        k3.moe_sort(torch.zeros((4, 2), dtype=torch.int32, device=dev), n)
+    assert k3.moe_sort(torch.zeros((4, 2), dtype=torch.int32, device=dev), 2048)[2].shape == (2049,)

@@ -147,3 +147,12 @@ def test_mat_struct_layout_matches_header(k3, tmp_path):
     got = [int(v) for v in subprocess.run([str(tmp_path / "t")], capture_output=True, text=True).stdout.split()]
     m = k3.Mxfp4MatC
     assert got == [C.sizeof(m), m.code_stride.offset, m.rows.offset, m.mat_of.offset]
+
+
+@pytest.mark.parametrize("n", [0, -1, 2049, 1 << 31, (1 << 32) + 4, -(1 << 32) + 2048, -(1 << 33) + 1, 1 << 64])
+def test_sort_refuses_expert_counts_before_it_allocates(k3, n):
+    """Counts outside 1..2048, those among them that 32 bits would cut to one inside: off is as
+    long as the count given, the entry point would write as many as the count it sees."""
+    import torch
+    with pytest.raises(k3.K3CError, match="n_experts"):
+        k3.moe_sort(torch.zeros((4, 2), dtype=torch.int32), n)
