@@ -637,8 +637,8 @@ int k3c_mxfp4_pack(uint8_t *codes, uint8_t *atoms, const uint8_t *packed, const 
                    int rows, int in, k3c_stream_t stream);
 /* y[r][o] = sum_i A[r][i] W_g[o][i], A as k3c_mxfp4_quant writes it (a [M][in/2] 16-byte aligned,
  * a_scales [M][in/32]); rows off[g] .. off[g+1] - 1 (device, n_groups + 1 ints, ascending;
- * offsets outside 0..M are clamped) belong to group g, rows outside every group are left as they
- * were; off NULL with n_groups 1: all rows. Exact products, fp32 accumulation, one rounding to
+ * offsets outside 0..M are clamped, and where offsets descend some groups' rows may be left out) belong
+ * to group g, rows outside every group are left as they were; off NULL with n_groups 1: all rows. Exact products, fp32 accumulation, one rounding to
  * y_dtype; y rows ldy >= rows elements apart. n_groups <= 1024. The result does not depend on
  * how the work is spread. */
 int k3c_mxfp4_mm(void *y, int y_dtype, int64_t ldy, const uint8_t *a, const uint8_t *a_scales, int M,

@@ -179,7 +179,15 @@ __device__ __forceinline__ int first_of(const int *off, int g, int M) {
     return off ? min(max(__ldg(off + g), 0), M) : g ? M : 0;
 }
 
-// Filled by all THREADS of the block; returns the number of row tiles.
+// Row tiles of at most `tile` rows that n_groups groups of M rows can have together.
+__host__ __device__ __forceinline__ int64_t most_tiles(int M, int n_groups, int tile) {
+    return (int64_t)M / tile + (n_groups < M ? n_groups : M);
+}
+
+// Filled by all THREADS of the block; returns the number of row tiles. Ascending offsets have no more than
+// most_tiles of them. Offsets that descend in places can name the same rows again and again (0, M, 0, M, ...: 512
+// times M), more tiles than 32 bits count and items than the launch was checked for: tiles past
+// most_tiles are left out, so that every sum here and in a Walk stays within what the host has checked.
 template <int THREADS>
 __device__ int plan_tiles(Plan &pl, const int *off, int G, int M, int rows) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -192,11 +200,12 @@ __device__ int plan_tiles(Plan &pl, const int *off, int G, int M, int rows) {
         __syncthreads();
         return n;
     }
+    const int most = (int)most_tiles(M, G, rows);
     int run = 0;
     for (int g0 = 0; g0 < G; g0 += THREADS) {
         const int g = g0 + tid;
         const int n = g < G ? (max(first_of(off, g + 1, M) - first_of(off, g, M), 0) + rows - 1) / rows : 0;
-        int inc = n;
+        int inc = n;   // n < 2^25: a warp's sum stays below 2^30
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, inc, o);
@@ -204,14 +213,14 @@ __device__ int plan_tiles(Plan &pl, const int *off, int G, int M, int rows) {
         }
         if (lane == 31) pl.warp_tot[warp] = inc;
         __syncthreads();
-        int pre = 0, all = 0;
+        int pre = run, all = run;
 #pragma unroll
         for (int w = 0; w < THREADS / 32; w++) {
-            pre += w < warp ? pl.warp_tot[w] : 0;
-            all += pl.warp_tot[w];
+            if (w < warp) pre = min(pre + pl.warp_tot[w], most);
+            all = min(all + pl.warp_tot[w], most);
         }
-        if (g < G) pl.tile[g] = run + pre + inc - n;
-        run += all;
+        if (g < G) pl.tile[g] = min(pre + inc - n, most);
+        run = all;
         __syncthreads();
     }
     if (tid == 0) pl.tile[G] = run;
@@ -1528,9 +1537,6 @@ int check_waits(const char *what, int *err, cudaStream_t s) {
     }
     return K3C_OK;
 }
-
-// Row tiles of at most `tile` rows that n_groups groups of M rows can have together.
-int64_t most_tiles(int M, int n_groups, int tile) { return (int64_t)M / tile + (n_groups < M ? n_groups : M); }
 
 // Items are numbered in 32 bits; 128 x 64 is the smallest tile.
 int check_items(const char *what, int M, int n_groups, int cols) {

@@ -612,3 +612,22 @@ def test_pack_in_place(k3, dev):
     assert k3.lib().k3c_mxfp4_pack(p.data_ptr(), mine.data_ptr(), p.data_ptr(), s.data_ptr(), n, rows, in_,
                                    torch.cuda.current_stream(dev).cuda_stream) == 0
     assert torch.equal(p, codes) and torch.equal(mine, atoms)
+
+
+def test_offsets_that_name_rows_again_and_again(k3, dev):
+    """Descending offsets that let 512 groups name all rows each: more tiles than 32 bits count. The
+    first of them is done, and nothing outside the result is touched."""
+    import torch
+    torch.cuda.empty_cache()
+    G, M, N, K = 1024, (1 << 29) + 384, 1, 32
+    W, _ = matrices(k3, dev, 151, 1, N, K)
+    W = k3.Mxfp4Mat(W.keep[0], W.keep[1], mat_of=torch.zeros(G, dtype=torch.int32, device=dev))
+    g = torch.Generator(device=dev).manual_seed(2)
+    a = torch.randint(0, 256, (M, K // 2), dtype=torch.uint8, device=dev, generator=g)
+    s = torch.full((M, 1), 127, dtype=torch.uint8, device=dev)
+    off = torch.zeros(G + 1, dtype=torch.int32, device=dev)
+    off[1::2] = M
+    buf = torch.full((M + 256, N), 7.0, dtype=torch.bfloat16, device=dev)
+    k3.mxfp4_mm(a, s, W, off=off, out=buf[128:M + 128])
+    assert (buf[:128] == 7).all() and (buf[M + 128:] == 7).all()
+    assert torch.equal(buf[128:M + 128], k3.mxfp4_mm(a, s, W))
