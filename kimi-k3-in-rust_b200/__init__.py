@@ -1016,6 +1016,7 @@ class _Runtime:
         self.lib = lib()
         self.floats = (torch.float32, torch.bfloat16)
         self.code = {torch.float32: K3C_F32, torch.bfloat16: K3C_BF16}
+        self.size = {torch.float32: 4, torch.bfloat16: 2}
         self.i32, self.u8, self.f32 = torch.int32, torch.uint8, torch.float32
         torch.cuda.init()
         self.device = torch._C._cuda_getDevice
@@ -1064,12 +1065,33 @@ def _bad(t, name, want):
     raise K3CError(f"{name}: {t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}, expected {want}")
 
 
-def _apart(out, name, *inputs):
-    """A given output is none of the inputs (rows move: nothing can run in place)."""
-    p = out.data_ptr()
+# Memory as (address, rows, bytes of a row, bytes from a row to the next).
+def _flat(p, n):
+    return p, 1, n, n
+
+
+def _share(a, b):
+    """Whether two pieces of memory have a byte in common."""
+    (p, ra, wa, sa), (q, rb, wb, sb) = a, b
+    if min(ra, wa, rb, wb) < 1:
+        return False
+    if ra > 1 and rb > 1 and sa != sb:   # row by row; two slices of one buffer have one stride
+        if ra > rb:
+            (p, ra, wa, sa), b = b, a
+        return any(_share(_flat(p + i * sa, wa), b) for i in range(ra))
+    # row j of b begins d + (j - i) * s bytes behind row i of a
+    d, s = q - p, sa if ra > 1 else sb
+    return max(1 - ra, -((d + wb - 1) // s)) <= min(rb - 1, (wa - 1 - d) // s)
+
+
+def _apart(name, out, *inputs):
+    """A given result shares no memory with an input (rows move: nothing can run in place)."""
+    p, r, w, s = out
+    end = p + (r - 1) * s + w
     for t in inputs:
-        if t.data_ptr() == p and p:
-            raise K3CError(f"{name}: may not be an input")
+        q, r, w, s = t
+        if q < end and p < q + (r - 1) * s + w and _share(out, t):
+            raise K3CError(f"{name}: may not be an input, nor share memory with one")
 
 
 def _mat_arg(t, name, dev, dtypes, d0=None, d1=None):
@@ -1139,12 +1161,15 @@ def moe_permute(x, pos, out=None):
     dev = x.get_device()
     T, H, ld = _rows_arg(x, "x", dev, rt.floats)
     K = _mat_arg(pos, "pos", dev, (rt.i32,), T)[1]
+    px, pp = x.data_ptr(), pos.data_ptr()
     if out is None:
         out = _new(rt, dev, x.dtype, T * K, H)
+        po = out.data_ptr()
     else:
         _mat_arg(out, "out", dev, (x.dtype,), T * K, H)
-        _apart(out, "out", x)
-    _launch(rt, "k3c_moe_permute", dev, out.data_ptr(), x.data_ptr(), rt.code[x.dtype], ld, pos.data_ptr(), T, K, H)
+        po, b = out.data_ptr(), rt.size[x.dtype]
+        _apart("out", _flat(po, T * K * H * b), (px, T, H * b, ld * b), _flat(pp, 4 * T * K))
+    _launch(rt, "k3c_moe_permute", dev, po, px, rt.code[x.dtype], ld, pp, T, K, H)
     return out
 
 
@@ -1158,7 +1183,8 @@ def moe_permute_bwd(drows, pos, out=None):
         out = _new(rt, dev, drows.dtype, T, H)
     else:
         _mat_arg(out, "out", dev, (drows.dtype,), T, H)
-        _apart(out, "out", drows)
+        b = rt.size[drows.dtype]
+        _apart("out", _flat(out.data_ptr(), T * H * b), _flat(drows.data_ptr(), T * K * H * b), _flat(pos.data_ptr(), 4 * T * K))
     _launch(rt, "k3c_moe_permute_bwd", dev, out.data_ptr(), drows.data_ptr(), rt.code[drows.dtype], pos.data_ptr(), T, K, H)
     return out
 
@@ -1184,6 +1210,11 @@ def _out_type(rt, out_dtype, default):
     return out_dtype
 
 
+def _pair_inputs(rt, y, pos, wt, T, K, H):
+    return (_flat(y.data_ptr(), T * K * H * rt.size[y.dtype]), _flat(pos.data_ptr(), 4 * T * K),
+            _flat(wt.data_ptr(), 4 * T * K))
+
+
 def moe_unpermute(y, pos, wt, out=None, out_dtype=None):
     """out[t] = sum_j wt[t][j] * y[pos[t][j]]: y [T * topk][H] in expert order, wt [T][topk] fp32;
     out [T][H] of out_dtype (default: y's)."""
@@ -1196,7 +1227,7 @@ def moe_unpermute(y, pos, wt, out=None, out_dtype=None):
         out = _new(rt, dev, _out_type(rt, out_dtype, y.dtype), T, H)
     else:
         _mat_arg(out, "out", dev, rt.floats if out_dtype is None else (_out_type(rt, out_dtype, None),), T, H)
-        _apart(out, "out", y, wt)
+        _apart("out", _flat(out.data_ptr(), T * H * rt.size[out.dtype]), *_pair_inputs(rt, y, pos, wt, T, K, H))
     _launch(rt, "k3c_moe_unpermute", dev, out.data_ptr(), rt.code[out.dtype], y.data_ptr(), rt.code[y.dtype], wt.data_ptr(),
             pos.data_ptr(), T, K, H)
     return out
@@ -1211,16 +1242,18 @@ def moe_unpermute_bwd(dout, y, pos, wt, dy=None, dwt=None):
     H = _mat_arg(y, "y", dev, rt.floats, T * K)[1]
     _mat_arg(dout, "dout", dev, rt.floats, T, H)
     _mat_arg(wt, "wt", dev, (rt.f32,), T, K)
+    if dy is not None or dwt is not None:
+        ins = (_flat(dout.data_ptr(), T * H * rt.size[dout.dtype]), *_pair_inputs(rt, y, pos, wt, T, K, H))
     if dy is None:
         dy = _new(rt, dev, y.dtype, T * K, H)
     else:
         _mat_arg(dy, "dy", dev, (y.dtype,), T * K, H)
-        _apart(dy, "dy", y, dout, wt)
+        _apart("dy", _flat(dy.data_ptr(), T * K * H * rt.size[y.dtype]), *ins)
     if dwt is None:
         dwt = _new(rt, dev, rt.f32, T, K)
     else:
         _mat_arg(dwt, "dwt", dev, (rt.f32,), T, K)
-        _apart(dwt, "dwt", y, dout, wt, dy)
+        _apart("dwt", _flat(dwt.data_ptr(), 4 * T * K), *ins, _flat(dy.data_ptr(), T * K * H * rt.size[y.dtype]))
     _launch(rt, "k3c_moe_unpermute_bwd", dev, dy.data_ptr(), dwt.data_ptr(), dout.data_ptr(), rt.code[dout.dtype],
             y.data_ptr(), rt.code[y.dtype], wt.data_ptr(), pos.data_ptr(), T, K, H)
     return dy, dwt
@@ -1287,6 +1320,12 @@ class Mxfp4Mat:
         self.groups = groups      # groups of rows that `off` may name
         self.dev, self.keep = dev, keep
 
+    def _memory(self):
+        c = self.c
+        return ((c.codes or 0, c.n_mats, c.rows * (c.in_ // 2), c.code_stride),
+                (c.atoms or 0, c.n_mats, ((c.rows + 127) >> 7) * ((c.in_ + 127) >> 7) * 512, c.atom_stride),
+                _flat(c.mat_of or 0, 4 * self.groups if c.mat_of else 0))
+
     @classmethod
     def from_pool(cls, layer, which):
         """The experts' matrices of a PoolMoeLayer, or of a LatentMoeLayer (hidden: its latent width),
@@ -1323,14 +1362,15 @@ def _mm_groups(rt, W, off, dev):
     return off.data_ptr(), G
 
 
-def _mm_out(rt, M, n, dev, out, out_dtype, a):
-    """(out, its row stride); a: the rows multiplied."""
+def _mm_out(rt, M, n, dev, out, out_dtype, W, *memory):
+    """(out, its row stride); memory: what the product reads besides W."""
     if out is None:
         return _new(rt, dev, _out_type(rt, out_dtype, rt.torch.bfloat16), M, n), n
     rows, cols, ld = _rows_arg(out, "out", dev, rt.floats if out_dtype is None else (_out_type(rt, out_dtype, None),))
     if rows != M or cols != n:
         _bad(out, "out", f"fp32 or bf16 {(M, n)}")
-    _apart(out, "out", a)
+    b = rt.size[out.dtype]
+    _apart("out", (out.data_ptr(), M, n * b, ld * b), *memory, *W._memory())
     return out, ld
 
 
@@ -1345,8 +1385,10 @@ def mxfp4_mm(a, a_scales, W, off=None, out=None, out_dtype=None):
     M = _mat_arg(a, "a", dev, (rt.u8,), None, W.in_ // 2)[0]
     _mat_arg(a_scales, "a_scales", dev, (rt.u8,), M, W.in_ // 32)
     po, G = _mm_groups(rt, W, off, dev)
-    out, ld = _mm_out(rt, M, W.rows, dev, out, out_dtype, a)
-    _launch(rt, "k3c_mxfp4_mm", dev, out.data_ptr(), rt.code[out.dtype], ld, a.data_ptr(), a_scales.data_ptr(), M, W.ref, po, G)
+    pa, ps = a.data_ptr(), a_scales.data_ptr()
+    out, ld = _mm_out(rt, M, W.rows, dev, out, out_dtype, W, _flat(pa, M * (W.in_ // 2)), _flat(ps, M * (W.in_ // 32)),
+                      _flat(po or 0, 4 * (G + 1) if po else 0))
+    _launch(rt, "k3c_mxfp4_mm", dev, out.data_ptr(), rt.code[out.dtype], ld, pa, ps, M, W.ref, po, G)
     return out
 
 
@@ -1359,8 +1401,9 @@ def mxfp4_mm_bwd(dy, W, off=None, out=None, out_dtype=None):
     if n != W.rows:
         _bad(dy, "dy", f"{W.rows} columns")
     po, G = _mm_groups(rt, W, off, dev)
-    out, ld = _mm_out(rt, M, W.in_, dev, out, out_dtype, dy)
-    _launch(rt, "k3c_mxfp4_mm_bwd", dev, out.data_ptr(), rt.code[out.dtype], ld, dy.data_ptr(), ldd, M, W.ref, po, G)
+    pd = dy.data_ptr()
+    out, ld = _mm_out(rt, M, W.in_, dev, out, out_dtype, W, (pd, M, 2 * n, 2 * ldd), _flat(po or 0, 4 * (G + 1) if po else 0))
+    _launch(rt, "k3c_mxfp4_mm_bwd", dev, out.data_ptr(), rt.code[out.dtype], ld, pd, ldd, M, W.ref, po, G)
     return out
 
 

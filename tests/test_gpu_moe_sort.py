@@ -331,3 +331,41 @@ def test_expert_counts_the_sort_refuses(k3, dev, n):
     with pytest.raises(k3.K3CError, match="n_experts"):
         k3.moe_sort(torch.zeros((4, 2), dtype=torch.int32, device=dev), n)
     assert k3.moe_sort(torch.zeros((4, 2), dtype=torch.int32, device=dev), 2048)[2].shape == (2049,)
+
+
+def test_outputs_may_not_overlap_inputs(k3, dev):
+    """A result that shares part of its memory with any input is refused, one that lies beside them in
+    the same buffer is not."""
+    import torch
+    T, K, H = 6, 2, 32
+    buf = torch.zeros(4 * T * K * H, device=dev)
+    pos = torch.arange(T * K, dtype=torch.int32, device=dev).view(T, K)
+    wt = torch.ones(T, K, device=dev)
+
+    def at(first, rows, cols=H):
+        return buf[first:first + rows * cols].view(rows, cols)
+
+    n, one = T * K * H, T * H
+    ip = pos.view(torch.float32)
+    for call in (lambda: k3.moe_permute(at(n - 1, T), pos, out=at(0, T * K)),
+                 lambda: k3.moe_permute(at(0, T), pos, out=at(one - 1, T * K)),
+                 lambda: k3.moe_permute(buf[:T * 2 * H].view(T, 2 * H)[:, H:], pos, out=at(H, T * K)),
+                 lambda: k3.moe_permute_bwd(at(one - 1, T * K), pos, out=at(0, T)),
+                 lambda: k3.moe_unpermute(at(H, T * K), pos, wt, out=at(0, T)),
+                 lambda: k3.moe_unpermute(at(0, T * K), pos, at(n + 3, T, K), out=at(n, T)),
+                 lambda: k3.moe_unpermute(torch.zeros(T * K, K, device=dev), pos, wt, out=ip),
+                 lambda: k3.moe_unpermute_bwd(at(0, T), at(one, T * K), pos, wt, dy=at(one + n - 1, T * K)),
+                 lambda: k3.moe_unpermute_bwd(at(0, T), at(one, T * K), pos, wt, dwt=at(one - 1, T, K)),
+                 lambda: k3.moe_unpermute_bwd(at(0, T), at(one, T * K), pos, wt, dy=at(one + n, T * K), dwt=at(one + 2 * n - 2, T, K))):
+        with pytest.raises(k3.K3CError, match="may not be an input"):
+            call()
+    x = torch.randn(T, H, device=dev)
+    wide = torch.zeros(T * K, 4 * H, device=dev)     # side by side
+    at(0, T).copy_(x)
+    assert torch.equal(k3.moe_permute(at(0, T), pos, out=at(one, T * K)), x.repeat_interleave(K, 0))
+    src = wide[:T, H:2 * H]
+    src.copy_(x)
+    assert torch.equal(k3.moe_permute(src, pos, out=at(one, T * K)), x.repeat_interleave(K, 0))
+    gap = buf[:2 * T * 2 * K * H].view(T, 4 * K * H)       # x's rows in the first columns, one token's rows behind them
+    gap[:1, :H].copy_(x[:1])
+    assert torch.equal(k3.moe_permute(gap[:2, :H][:1], pos[:1], out=gap.view(-1)[H:H + K * H].view(K, H)), x[:1].repeat_interleave(K, 0))

@@ -631,3 +631,44 @@ def test_offsets_that_name_rows_again_and_again(k3, dev):
     k3.mxfp4_mm(a, s, W, off=off, out=buf[128:M + 128])
     assert (buf[:128] == 7).all() and (buf[M + 128:] == 7).all()
     assert torch.equal(buf[128:M + 128], k3.mxfp4_mm(a, s, W))
+
+
+def test_result_may_not_overlap_what_is_read(k3, dev):
+    """A product's result in part of its rows, scales, offsets, matrices or map is refused; columns
+    of one buffer side by side are not."""
+    import torch
+    N, K, M = 64, 64, 40
+    W, w = matrices(k3, dev, 161, 2, N, K)
+    big = torch.zeros(1 << 16, dtype=torch.uint8, device=dev)
+    raw = k3.Mxfp4Mat(W.keep[0], W.keep[1], mat_of=big[4096:4104].view(torch.int32))
+    c, b = operand(162, M, K)
+    a, s = to_dev(dev, pack_nibbles(c), b)
+
+    def put(t, at):
+        v = big[at:at + t.nbytes].view(t.dtype).view(t.shape)
+        v.copy_(t)
+        return v
+
+    off = torch.tensor([0, 20, M], dtype=torch.int32, device=dev)
+    nb = M * N * 2
+    out = big[8192:8192 + nb].view(torch.bfloat16).view(M, N)
+    dy = torch.randn(M, N, device=dev).bfloat16()
+    codes, atoms = W.keep[0], W.keep[1]
+    for call in (lambda: k3.mxfp4_mm(put(a, 8192 + nb - 16), s, W, out=out),
+                 lambda: k3.mxfp4_mm(a, put(s, 8192 - s.nbytes + 1), W, out=out),
+                 lambda: k3.mxfp4_mm(a, s, W, off=put(off, 8192 + 400), out=out),
+                 lambda: k3.mxfp4_mm(a, s, k3.Mxfp4Mat(put(codes, 8192 + nb - 16), atoms), out=out),
+                 lambda: k3.mxfp4_mm(a, s, k3.Mxfp4Mat(codes, put(atoms, 8192 - 512)), out=out),
+                 lambda: k3.mxfp4_mm(a, s, raw, off=off, out=big[4100:4100 + nb].view(torch.bfloat16).view(M, N)),
+                 lambda: k3.mxfp4_mm_bwd(put(dy, 8192 + nb - 32), W, out=out),
+                 lambda: k3.mxfp4_mm_bwd(dy, W, off=put(off, 8192 - 4), out=out)):
+        with pytest.raises(k3.K3CError, match="may not be an input"):
+            call()
+    want = k3.mxfp4_mm(a, s, W), k3.mxfp4_mm_bwd(dy, W)
+    wide = torch.full((M, 3 * N), 7.0, dtype=torch.bfloat16, device=dev)
+    wide[:, N:2 * N].copy_(dy)
+    k3.mxfp4_mm_bwd(wide[:, N:2 * N], W, out=wide[:, 2 * N:])
+    assert torch.equal(wide[:, 2 * N:], want[1]) and torch.equal(wide[:, N:2 * N], dy) and (wide[:, :N] == 7).all()
+    with pytest.raises(k3.K3CError, match="may not be an input"):
+        k3.mxfp4_mm_bwd(wide[:, N:2 * N], W, out=wide[:, 2 * N - 8:3 * N - 8])
+    assert torch.equal(k3.mxfp4_mm(put(a, 8192 + nb), put(s, 8192 - s.nbytes), W, out=out), want[0])

@@ -156,3 +156,33 @@ def test_sort_refuses_expert_counts_before_it_allocates(k3, n):
     import torch
     with pytest.raises(k3.K3CError, match="n_experts"):
         k3.moe_sort(torch.zeros((4, 2), dtype=torch.int32), n)
+
+
+def test_memory_in_common_is_found():
+    """_share against the sets of bytes themselves: contiguous pieces, rows of one stride (slices of
+    one buffer, side by side or one inside the other) and of two."""
+    import random
+    import __graft_entry__ as ge
+    k3 = ge.load_package()
+    rng = random.Random(1)
+
+    def bytes_of(t):
+        p, r, w, s = t
+        return {p + i * s + j for i in range(r) for j in range(w)}
+    met = [0, 0]
+    for _ in range(4000):
+        s = rng.randint(1, 12)
+        two = []
+        for _ in range(2):
+            if rng.random() < 0.4:
+                s = rng.randint(1, 12)
+            two.append((rng.randint(0, 40), rng.randint(0, 5), rng.randint(0, s), s))
+        want = bool(bytes_of(two[0]) & bytes_of(two[1]))
+        assert k3._share(*two) == want and k3._share(*two[::-1]) == want, two
+        met[want] += 1
+        if want:
+            with pytest.raises(k3.K3CError, match="may not be an input"):
+                k3._apart("out", two[0], (10 ** 6, 1, 4, 4), two[1])
+        else:
+            k3._apart("out", *two)
+    assert min(met) > 500
