@@ -134,6 +134,13 @@ __global__ void __launch_bounds__(256) k_mx4_quant_any(uint8_t *__restrict__ pac
     }
 }
 
+// An epilogue's wait for its item's sums. They take as long as the item's K blocks do, 0.2 to 0.6 us each: 10 s for a
+// gradient over 2^31 weight rows, so the limit grows with them (with the other waits' 2 s that
+// gradient was NaN from 430 million rows on).
+__device__ __forceinline__ bool wait_for_sums(uint64_t *bar, uint32_t parity, int *err, int code, int k_blocks) {
+    return tc::mbar_wait_ns(bar, parity, err, code, tc::kWaitLimitNs + 2000ull * (uint32_t)k_blocks);
+}
+
 // Byte of row m (0..127), group g (0..3) in a scale atom.
 __device__ __forceinline__ int sf_byte(int m, int g) { return 16 * (m & 31) + 4 * (m >> 5) + g; }
 
@@ -764,7 +771,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant_
             } else {
                 const uint32_t a = li % C::NACC, use = li / C::NACC;
                 li++;
-                ok = alive = alive && tc::mbar_wait(&tfull[a], use & 1u, p.err, 86);
+                ok = alive = alive && wait_for_sums(&tfull[a], use & 1u, p.err, 86, KB);
                 __syncwarp();
                 tc::tc_fence_after();
                 // the whole share goes to registers first, so the accumulator is free again
@@ -1003,7 +1010,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm_pair(const __grid_cons
 #pragma unroll
                     for (int i = 0; i < 32; i++) v[c][i] = 0;
             } else {
-                ok = alive = alive && tc::mbar_wait(tfull, tph, p.err, 117);
+                ok = alive = alive && wait_for_sums(tfull, tph, p.err, 117, KB);
                 tph ^= 1u;
                 __syncwarp();
                 tc::tc_fence_after();
@@ -1424,7 +1431,7 @@ __global__ void __launch_bounds__(MbCfg<NT, PAIR, ACCS>::THREADS, 1) k_mx4_bwd(c
             const uint32_t taddr = tmem + lanes + a * ACCS * C::TN;
             const bool real = x.mat >= 0;
             if (real) {
-                alive = alive && tc::mbar_wait(&tfull[a], aph, p.err, 100);
+                alive = alive && wait_for_sums(&tfull[a], aph, p.err, 100, KB);
                 __syncwarp();
                 tc::tc_fence_after();
             }

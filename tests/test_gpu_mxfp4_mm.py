@@ -672,3 +672,36 @@ def test_result_may_not_overlap_what_is_read(k3, dev):
     with pytest.raises(k3.K3CError, match="may not be an input"):
         k3.mxfp4_mm_bwd(wide[:, N:2 * N], W, out=wide[:, 2 * N - 8:3 * N - 8])
     assert torch.equal(k3.mxfp4_mm(put(a, 8192 + nb), put(s, 8192 - s.nbytes), W, out=out), want[0])
+
+
+def test_the_longest_sums(k3, dev):
+    """A gradient over 2^29 weight rows, 8.4 million K blocks of one tile (2.5 s, longer than a wait
+    inside the kernel may take otherwise), and a product over the longest rows there may be. All but
+    some elements are 0 and the others small integers: every sum is exact."""
+    import torch
+    torch.cuda.empty_cache()
+    g = torch.Generator(device=dev).manual_seed(6)
+
+    def ones(n):       # n places and +-1 there
+        at = torch.cat([torch.randint(0, n, (200,), generator=g, device=dev), torch.tensor([0, n - 1], device=dev)]).unique()
+        return at, torch.randint(0, 2, at.shape, generator=g, device=dev).double() * 2 - 1
+    N, K = (1 << 29) + 40, 32
+    codes = torch.randint(0, 256, (1, N, K // 2), dtype=torch.uint8, device=dev, generator=g) & 0x66    # 0, 1, 2, 4
+    atoms = torch.full((1, -(-N // 128), 1, 512), 127, dtype=torch.uint8, device=dev)
+    at, v = ones(N)
+    dy = torch.zeros(1, N, dtype=torch.bfloat16, device=dev)
+    dy[0, at] = v.bfloat16()
+    da = k3.mxfp4_mm_bwd(dy, k3.Mxfp4Mat(codes, atoms), out_dtype=torch.float32)
+    grid = torch.tensor(GRID, device=dev)
+    rows = grid[torch.stack([codes[0, at] & 7, codes[0, at] >> 4 & 7], -1).reshape(len(at), K).long()]
+    assert torch.equal(da[0].double(), v @ rows)
+    del codes, atoms, dy
+    K = (1 << 31) - 1024
+    a = torch.zeros(1, K // 2, dtype=torch.uint8, device=dev)
+    at, v = ones(K // 2)
+    a[0, at] = torch.where(v > 0, 0x22, 0x2A).to(torch.uint8)          # 1, 1 and -1, 1
+    codes = torch.randint(0, 256, (1, 1, K // 2), dtype=torch.uint8, device=dev, generator=g) & 0x66
+    W = k3.Mxfp4Mat(codes, torch.full((1, 1, K // 128, 512), 127, dtype=torch.uint8, device=dev))
+    y = k3.mxfp4_mm(a, torch.full((1, K // 32), 127, dtype=torch.uint8, device=dev), W, out_dtype=torch.float32)
+    w = grid[torch.stack([codes[0, 0, at] & 7, codes[0, 0, at] >> 4 & 7], -1).long()]
+    assert y.item() == (v * w[:, 0] + w[:, 1]).sum().item()
