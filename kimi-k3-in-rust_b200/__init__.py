@@ -1402,6 +1402,8 @@ def mxfp4_mm_bwd(dy, W, off=None, out=None, out_dtype=None):
         _bad(dy, "dy", f"{W.rows} columns")
     po, G = _mm_groups(rt, W, off, dev)
     pd = dy.data_ptr()
+    if M == 1:       # whatever its stride, which torch does not keep for a row that counts as contiguous
+        ldd = (n + 7) & ~7
     out, ld = _mm_out(rt, M, W.in_, dev, out, out_dtype, W, (pd, M, 2 * n, 2 * ldd), _flat(po or 0, 4 * (G + 1) if po else 0))
     _launch(rt, "k3c_mxfp4_mm_bwd", dev, out.data_ptr(), rt.code[out.dtype], ld, pd, ldd, M, W.ref, po, G)
     return out

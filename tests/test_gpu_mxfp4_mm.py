@@ -705,3 +705,20 @@ def test_the_longest_sums(k3, dev):
     y = k3.mxfp4_mm(a, torch.full((1, K // 32), 127, dtype=torch.uint8, device=dev), W, out_dtype=torch.float32)
     w = grid[torch.stack([codes[0, 0, at] & 7, codes[0, 0, at] >> 4 & 7], -1).long()]
     assert y.item() == (v * w[:, 0] + w[:, 1]).sum().item()
+
+
+@pytest.mark.parametrize("N", [1, 7, 65, 257, 4095])
+def test_gradient_of_padded_rows(k3, dev, N):
+    """dy of any number of columns in rows whose stride is a multiple of 8, one row (contiguous to
+    torch) and several, beside values that are NaN."""
+    import torch
+    K = 96
+    W, w = matrices(k3, dev, 171, 1, N, K)
+    ld = -(-N // 8) * 8 + 16
+    for M in (1, 2, 33):
+        buf = torch.full((M + 1, ld), float("nan"), dtype=torch.bfloat16, device=dev)
+        dy = buf[:M, :N]
+        dy.copy_(torch.randn((M, N), generator=torch.Generator().manual_seed(M)))
+        da = k3.mxfp4_mm_bwd(dy, W, out_dtype=torch.float32).double().cpu().numpy()
+        dv = dy.double().cpu().numpy()
+        check(da, dv @ w[0], np.abs(dv) @ np.abs(w[0]), -(-N // 16), False)
