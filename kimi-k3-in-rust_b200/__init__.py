@@ -1394,7 +1394,8 @@ def mxfp4_mm(a, a_scales, W, off=None, out=None, out_dtype=None):
 
 def mxfp4_mm_bwd(dy, W, off=None, out=None, out_dtype=None):
     """mxfp4_mm's gradient with respect to a's values: da[r] = W_g^T dy[r], dy [M][rows] bf16 (rows
-    may be strided, the stride a multiple of 8). out [M][in] of out_dtype (default bf16)."""
+    may be strided; those that do not start on 16-byte boundaries are copied to such first). out [M][in]
+    of out_dtype (default bf16)."""
     rt = _runtime(dy)
     dev = dy.get_device()
     M, n, ldd = _rows_arg(dy, "dy", dev, (rt.torch.bfloat16,))
@@ -1402,9 +1403,15 @@ def mxfp4_mm_bwd(dy, W, off=None, out=None, out_dtype=None):
         _bad(dy, "dy", f"{W.rows} columns")
     po, G = _mm_groups(rt, W, off, dev)
     pd = dy.data_ptr()
-    if M == 1:       # whatever its stride, which torch does not keep for a row that counts as contiguous
-        ldd = (n + 7) & ~7
     out, ld = _mm_out(rt, M, W.in_, dev, out, out_dtype, W, (pd, M, 2 * n, 2 * ldd), _flat(po or 0, 4 * (G + 1) if po else 0))
+    if M <= 1:       # whatever its stride, which torch does not keep for a row that counts as contiguous
+        ldd = (n + 7) & ~7
+    if pd & 15 or ldd & 7:
+        # the kernels copy dy by tiles, which start on 16 bytes: any other rows go to padded ones
+        ldd = (n + 7) & ~7
+        rows = _new(rt, dev, dy.dtype, M, ldd)
+        rows[:, :n].copy_(dy)
+        pd = rows.data_ptr()
     _launch(rt, "k3c_mxfp4_mm_bwd", dev, out.data_ptr(), rt.code[out.dtype], ld, pd, ldd, M, W.ref, po, G)
     return out
 

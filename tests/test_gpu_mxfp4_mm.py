@@ -722,3 +722,36 @@ def test_gradient_of_padded_rows(k3, dev, N):
         da = k3.mxfp4_mm_bwd(dy, W, out_dtype=torch.float32).double().cpu().numpy()
         dv = dy.double().cpu().numpy()
         check(da, dv @ w[0], np.abs(dv) @ np.abs(w[0]), -(-N // 16), False)
+
+
+@pytest.mark.parametrize("N", [1, 7, 65, 257, 4095, 4104])
+def test_gradient_of_rows_on_any_boundary(k3, dev, N):
+    """dy as the product's own result has it, contiguous whatever its width, and rows at odd addresses
+    and strides; grouped, with rows behind the last group left as they were, eager and captured."""
+    import torch
+    K, G = 160, 3
+    W, w = matrices(k3, dev, 181, G, N, K)
+    for M, sizes in ((0, [0, 0, 0]), (1, [0, 1, 0]), (2, [1, 0, 1]), (40, [3, 0, 30])):
+        off = np.concatenate([[0], np.cumsum(sizes)]).astype(np.int32)
+        po = to_dev(dev, off)[0]
+        for first, pad in ((0, 0), (1, 0), (3, 2), (8, 3)):
+            buf = torch.full(((N + pad) * M + first + 9,), float("nan"), dtype=torch.bfloat16, device=dev)
+            dy = buf[first:first + (N + pad) * M].view(M, N + pad)[:, :N]
+            dy.copy_(torch.randn((M, N), generator=torch.Generator().manual_seed(M)))
+            da = torch.full((M, K), 7.0, device=dev)
+            k3.mxfp4_mm_bwd(dy, W, off=po, out=da)
+            assert (da[off[-1]:] == 7).all()
+            got, dv = da.double().cpu().numpy(), dy.double().cpu().numpy()
+            for e in range(G):
+                r = slice(off[e], off[e + 1])
+                check(got[r], dv[r] @ w[e], np.abs(dv[r]) @ np.abs(w[e]), -(-N // 16), False)
+    held = torch.zeros_like(dy)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        cap = k3.mxfp4_mm_bwd(held, W, off=po, out=torch.zeros_like(da))
+    held.copy_(dy)
+    g.replay()
+    assert torch.equal(cap[:off[-1]], da[:off[-1]])
+    flat = torch.randn(33 * max(N, K) + 8, device=dev).bfloat16()       # a copied dy is no less an input
+    with pytest.raises(k3.K3CError, match="may not be an input"):
+        k3.mxfp4_mm_bwd(flat[1:1 + 33 * N].view(33, N), W, out=flat[:33 * K].view(33, K))
