@@ -1003,7 +1003,9 @@ class LatentMoeLayer:
 # These wrappers check what the C entry points cannot see (element types, shapes, devices), run on
 # the tensors' own device and on that device's current stream, and allocate only their results.
 # A decode step makes several of these calls on a few tokens, where the host's time is the call's:
-# hence the plain comparisons, and addresses passed as integers.
+# hence the plain comparisons, and addresses passed as integers. None of them is recorded by autograd:
+# their gradients are the _bwd calls, to be made from a torch.autograd.Function (where gradient mode is
+# off), so an input that requires grad in gradient mode is refused.
 _rt = None
 
 
@@ -1094,6 +1096,14 @@ def _apart(name, out, *inputs):
             raise K3CError(f"{name}: may not be an input, nor share memory with one")
 
 
+def _tracked(t, name):
+    """For a t that requires grad: its gradient would be lost without a word."""
+    import torch
+    if torch.is_grad_enabled():
+        raise K3CError(f"{name}: requires grad, which these calls do not record; detach it, or call them and their "
+                       "_bwd forms from a torch.autograd.Function")
+
+
 def _mat_arg(t, name, dev, dtypes, d0=None, d1=None):
     """A contiguous 2-D tensor on device dev; its extents (None: any)."""
     sh = t.shape
@@ -1102,6 +1112,8 @@ def _mat_arg(t, name, dev, dtypes, d0=None, d1=None):
         _bad(t, name, f"contiguous {dtypes} {(d0, d1)} on device {dev}")
     if sh[0] > _INT_MAX or sh[1] > _INT_MAX:
         _bad(t, name, "extents within 32 bits")
+    if t.requires_grad:
+        _tracked(t, name)
     return sh
 
 
@@ -1118,6 +1130,8 @@ def _rows_arg(t, name, dev, dtypes):
     rows, n = t.shape
     if rows > _INT_MAX or n > _INT_MAX:
         _bad(t, name, "extents within 32 bits")
+    if t.requires_grad:
+        _tracked(t, name)
     if t.is_contiguous():
         return rows, n, n
     ld, inner = t.stride()

@@ -755,3 +755,46 @@ def test_gradient_of_rows_on_any_boundary(k3, dev, N):
     flat = torch.randn(33 * max(N, K) + 8, device=dev).bfloat16()       # a copied dy is no less an input
     with pytest.raises(k3.K3CError, match="may not be an input"):
         k3.mxfp4_mm_bwd(flat[1:1 + 33 * N].view(33, N), W, out=flat[:33 * K].view(33, K))
+
+
+def test_under_autograd(k3, dev):
+    """Inputs that require grad are refused by name; inside autograd functions the calls and their
+    gradients make a differentiable layer of frozen experts, whose gradients are the calls' own."""
+    import torch
+    T, K, E, H, I = 40, 3, 7, 96, 64
+    g = torch.Generator().manual_seed(9)
+    W, _ = matrices(k3, dev, 191, E, I, H)
+    idx = torch.randint(0, E, (T, K), generator=g).int().to(dev)
+    pos, _, off = k3.moe_sort(idx, E)
+    x0, wt0 = torch.randn((T, H), generator=g).to(dev), torch.rand((T, K), generator=g).to(dev)
+    x, wt = x0.clone().requires_grad_(), wt0.clone().requires_grad_()
+    y0, d0 = torch.randn((T * K, I), generator=g).to(dev), torch.randn((T, I), generator=g).to(dev)
+    y, d = y0.clone().requires_grad_(), d0.clone().requires_grad_()
+    bf = torch.zeros((T * K, I), dtype=torch.bfloat16, device=dev, requires_grad=True)
+    rows = torch.zeros((T * K, H), device=dev, requires_grad=True)
+    for name, call in (("x", lambda: k3.moe_permute(x, pos)), ("x", lambda: k3.moe_permute_mxfp4(x, pos)),
+                       ("x", lambda: k3.mxfp4_quant(x)), ("out", lambda: k3.moe_permute(x0, pos, out=rows)),
+                       ("drows", lambda: k3.moe_permute_bwd(y, pos)), ("y", lambda: k3.moe_unpermute(y, pos, wt0)),
+                       ("wt", lambda: k3.moe_unpermute(y0, pos, wt)), ("dout", lambda: k3.moe_unpermute_bwd(d, y0, pos, wt0)),
+                       ("dy", lambda: k3.mxfp4_mm_bwd(bf, W, off=off))):
+        with pytest.raises(k3.K3CError, match=f"^{name}: requires grad"):
+            call()
+
+    class Layer(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, wt):
+            y = k3.mxfp4_mm(*k3.moe_permute_mxfp4(x, pos), W, off=off, out_dtype=torch.float32)
+            ctx.save_for_backward(y, wt)
+            return k3.moe_unpermute(y, pos, wt)
+
+        @staticmethod
+        def backward(ctx, dout):
+            y, wt = ctx.saved_tensors
+            dy, dwt = k3.moe_unpermute_bwd(dout.contiguous(), y, pos, wt)
+            return k3.moe_permute_bwd(k3.mxfp4_mm_bwd(dy.bfloat16(), W, off=off, out_dtype=torch.float32), pos), dwt
+
+    Layer.apply(x, wt).backward(d0)
+    y = k3.mxfp4_mm(*k3.moe_permute_mxfp4(x0, pos), W, off=off, out_dtype=torch.float32)
+    dy, dwt = k3.moe_unpermute_bwd(d0, y, pos, wt0)
+    assert torch.equal(wt.grad, dwt)
+    assert torch.equal(x.grad, k3.moe_permute_bwd(k3.mxfp4_mm_bwd(dy.bfloat16(), W, off=off, out_dtype=torch.float32), pos))

@@ -186,3 +186,15 @@ def test_memory_in_common_is_found():
         else:
             k3._apart("out", *two)
     assert min(met) > 500
+
+
+def test_tensors_that_require_grad_are_refused(k3):
+    """In gradient mode, whose record would lack them; not where it is off, as in autograd functions."""
+    import torch
+    t = torch.zeros((4, 6), requires_grad=True)
+    for f in (lambda: k3._mat_arg(t, "x", -1, (torch.float32,)), lambda: k3._rows_arg(t, "x", -1, (torch.float32,)),
+              lambda: k3._rows_arg(t[:, :3], "x", -1, (torch.float32,))):
+        with pytest.raises(k3.K3CError, match="x: requires grad"):
+            f()
+        with torch.no_grad():
+            assert f()[0] == 4
