@@ -1120,6 +1120,8 @@ def _mat_arg(t, name, dev, dtypes, d0=None, d1=None):
 def _vec_arg(t, name, dev, dtype):
     if t.dtype != dtype or t.dim() != 1 or t.get_device() != dev or not t.is_contiguous():
         _bad(t, name, f"contiguous 1-D {dtype} on device {dev}")
+    if not 1 <= t.shape[0] <= _INT_MAX:     # of no elements the address would be NULL, which means no array
+        _bad(t, name, "1 element to 32 bits of them")
     return t.shape[0]
 
 

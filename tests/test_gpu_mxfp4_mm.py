@@ -798,3 +798,14 @@ def test_under_autograd(k3, dev):
     dy, dwt = k3.moe_unpermute_bwd(d0, y, pos, wt0)
     assert torch.equal(wt.grad, dwt)
     assert torch.equal(x.grad, k3.moe_permute_bwd(k3.mxfp4_mm_bwd(dy.bfloat16(), W, off=off, out_dtype=torch.float32), pos))
+
+
+def test_an_empty_map_is_refused(k3, dev):
+    import torch
+    W, _ = matrices(k3, dev, 201, 2, 64, 64)
+    none = torch.zeros(0, dtype=torch.int32, device=dev)
+    with pytest.raises(k3.K3CError, match="mat_of"):
+        k3.Mxfp4Mat(W.keep[0], W.keep[1], mat_of=none)
+    a, s = k3.mxfp4_quant(torch.randn(4, 64, device=dev))
+    with pytest.raises(k3.K3CError, match="off"):
+        k3.mxfp4_mm(a, s, W, off=none)

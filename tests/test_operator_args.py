@@ -198,3 +198,13 @@ def test_tensors_that_require_grad_are_refused(k3):
             f()
         with torch.no_grad():
             assert f()[0] == 4
+
+
+def test_lengths_of_vectors(k3):
+    """off and mat_of hold 1 element to 2^31 - 1: the entry points take an empty one, whose address is
+    NULL, for none (every group its own matrix), and cut a longer one's length."""
+    import torch
+    for n in (0, 1 << 31, (1 << 32) + 3):
+        with pytest.raises(k3.K3CError, match="mat_of.*32 bits"):
+            k3._vec_arg(torch.empty(n, dtype=torch.int32, device="meta"), "mat_of", -1, torch.int32)
+    assert k3._vec_arg(torch.empty(5, dtype=torch.int32, device="meta"), "mat_of", -1, torch.int32) == 5
