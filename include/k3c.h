@@ -608,9 +608,10 @@ int k3c_moe_unpermute_bwd(void *dy, float *dwt, const void *dout, int out_dtype,
 /* x [rows] rows of ldx elements (x_dtype K3C_F32 or K3C_BF16) to packed [rows][in/2] and scales
  * [rows][ceil(in/32)]: per 32 elements scale byte clamp(floor(log2 max|x|) - 2 + 127, 0, 254),
  * codes round(x * 2^(127-byte)) to the nearest E2M1 value, ties to even, saturating at +-6. An
- * infinity makes its group's byte 253: k3c_mxfp4_dequant reads it back as an infinity, for
- * k3c_mxfp4_mm it is 6 * 2^126 (the format has no infinity) and its group's finite elements are 0;
- * a NaN makes the byte 255 with zero codes, which k3c_mxfp4_mm reads as NaN and k3c_mxfp4_dequant,
+ * infinity makes its group's byte 253 and its own code 6: k3c_mxfp4_dequant reads it back as an
+ * infinity, for k3c_mxfp4_mm it is 6 * 2^126 (the format has no infinity); its group's finite elements
+ * round as x * 2^-126, to 0 up to 2^124 and, from 3.5 * 2^126 on, to 2^128, an infinity to
+ * k3c_mxfp4_dequant; a NaN makes the byte 255 with zero codes, which k3c_mxfp4_mm reads as NaN and k3c_mxfp4_dequant,
  * like the reference, as 0. in even. */
 int k3c_mxfp4_quant(uint8_t *packed, uint8_t *scales, const void *x, int x_dtype, int64_t ldx, int rows, int in,
                     k3c_stream_t stream);
@@ -645,8 +646,8 @@ int k3c_mxfp4_mm(void *y, int y_dtype, int64_t ldy, const uint8_t *a, const uint
                  const k3c_mxfp4_mat *W, const int *off, int n_groups, k3c_stream_t stream);
 /* The gradient with respect to A's values: da[r][i] = sum_o dy[r][o] W_g[o][i], dy bf16 rows of
  * lddy elements (a multiple of 8, dy 16-byte aligned), fp32 accumulation, one rounding to
- * da_dtype. Weights past fp32's range (scale bytes above 251) enter as infinities, as in
- * k3_matmul_mxfp4. Quantisation passes gradients straight through; packed weights are constants. */
+ * da_dtype. Weights past fp32's range (magnitudes of 2^128 and more, under scale bytes 253 and 254)
+ * enter as infinities, as in k3_matmul_mxfp4. Quantisation passes gradients straight through; packed weights are constants. */
 int k3c_mxfp4_mm_bwd(void *da, int da_dtype, int64_t ldda, const void *dy, int64_t lddy, int M,
                      const k3c_mxfp4_mat *W, const int *off, int n_groups, k3c_stream_t stream);
 

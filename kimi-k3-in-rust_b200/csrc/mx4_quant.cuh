@@ -3,8 +3,8 @@
 // rounded to nearest, ties to even, saturating at +-6. floor(log2) is the fp32 exponent field of
 // the largest magnitude; the product with a power of two is exact wherever the code is not 0
 // (a result below the normal range is far below the smallest code's border). An infinity gives
-// byte 253 and the code 6, which reads back as infinity; a NaN gives byte 255 (the format's
-// NaN) and zero codes.
+// byte 253 and the code 6, which reads back as infinity, beside finite elements rounded under that byte; a
+// NaN gives byte 255 (the format's NaN) and zero codes.
 #pragma once
 
 #include "common.cuh"

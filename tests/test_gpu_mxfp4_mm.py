@@ -809,3 +809,51 @@ def test_an_empty_map_is_refused(k3, dev):
     a, s = k3.mxfp4_quant(torch.randn(4, 64, device=dev))
     with pytest.raises(k3.K3CError, match="off"):
         k3.mxfp4_mm(a, s, W, off=none)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_finite_elements_beside_an_infinity(k3, dev, dtype):
+    """Byte 253 for the group, finite elements rounded under it: 0 up to 2^124, a code above, and from
+    3.5 * 2^126 on the code 4, which is 2^128 to the dequantiser."""
+    import torch
+    near = [2.0 ** 124, 2.0 ** 124 * 1.01, 1.5 * 2.0 ** 125, 3e38, -2.0 ** 127, 2.0 ** 123, -2.0 ** 124, 1.0]
+    x = torch.zeros(3, 40)
+    x[:, 3] = torch.tensor([float("inf"), -float("inf"), float("inf")])
+    x[:, 4:12] = torch.tensor(near)
+    x[2] = x[2].roll(30)                                   # in a short group
+    x = x.bfloat16() if dtype == "bf16" else x
+    packed, scales = k3.mxfp4_quant(x.to(dev))
+    codes, byte = quant_plain(x.double().numpy())
+    assert np.array_equal(scales.cpu().numpy(), byte) and (byte == 253).sum() == 3
+    assert np.array_equal(unpack(packed.cpu().numpy())[:, :40], codes)
+    assert codes[0, 4] == 0 and codes[0, 5] == 1 and codes[0, 7] == 6
+    wide = torch.zeros(1, 64)
+    wide[0, 32:35] = torch.tensor([float("inf"), 3e38, -2.0 ** 127])
+    back = k3.mxfp4_dequant(*k3.mxfp4_quant(wide.to(dev))).cpu()
+    assert back[0, 32:35].tolist() == [float("inf"), float("inf"), -2.0 ** 127]
+
+
+@pytest.mark.parametrize("byte", [252, 253, 254])
+def test_gradient_of_the_largest_weights(k3, dev, byte):
+    """Every code under the last scale bytes, finite as long as its magnitude is below 2^128 (all of
+    them under 252), by one weight row whose gradient is the row itself."""
+    import torch
+    c = (np.arange(32, dtype=np.uint8) % 16)[None]
+    b = np.full((1, 1), byte, np.uint8)
+    W = k3.Mxfp4Mat(*k3.mxfp4_pack(*to_dev(dev, pack_nibbles(c), b)))
+    v = values(c, b)
+    v[np.abs(v) >= 2.0 ** 128] = np.inf * np.sign(v[np.abs(v) >= 2.0 ** 128])
+    assert np.isfinite(v).all() == (byte == 252)
+    dy = torch.tensor([[2.0 ** -20], [-3.0], [0.25]], device=dev).bfloat16()
+    da = k3.mxfp4_mm_bwd(dy, W, out_dtype=torch.float32).double().cpu().numpy()
+    want = dy.double().cpu().numpy() * v
+    want[np.abs(want) >= 2.0 ** 128] = np.inf * np.sign(want[np.abs(want) >= 2.0 ** 128])
+    assert np.array_equal(da, want)
+    N, K = 64, 64                                          # and sums of them
+    c, b = operand(211, N, K)
+    b[:] = byte
+    if byte == 252:
+        W = k3.Mxfp4Mat(*k3.mxfp4_pack(*to_dev(dev, pack_nibbles(c), b)))
+        dy = (torch.randint(-3, 4, (9, N), device=dev).double() * 2.0 ** -20).bfloat16()
+        da = k3.mxfp4_mm_bwd(dy, W, out_dtype=torch.float32).double().cpu().numpy()
+        assert np.array_equal(da, dy.double().cpu().numpy() @ values(c, b))
