@@ -1023,9 +1023,13 @@ class _Runtime:
         torch.cuda.init()
         self.device = torch._C._cuda_getDevice
         self.stream = torch._C._cuda_getCurrentRawStream
-        try:     # torch's own short way to an uninitialised tensor on the current device
+        try:     # torch's own short way to an uninitialised tensor on the current device: a private name
             self.empty = torch._C._dynamo.guards._empty_strided_cuda
-        except AttributeError:
+            t = self.empty((2, 3), (3, 1), self.i32)
+            short = t.is_cuda and t.dtype == self.i32 and t.shape == (2, 3) and t.is_contiguous()
+        except Exception:
+            short = False
+        if not short:
             self.empty = lambda size, stride, dtype: torch.empty_strided(size, stride, dtype=dtype, device="cuda")
 
 

@@ -369,3 +369,22 @@ def test_outputs_may_not_overlap_inputs(k3, dev):
     gap = buf[:2 * T * 2 * K * H].view(T, 4 * K * H)       # x's rows in the first columns, one token's rows behind them
     gap[:1, :H].copy_(x[:1])
     assert torch.equal(k3.moe_permute(gap[:2, :H][:1], pos[:1], out=gap.view(-1)[H:H + K * H].view(K, H)), x[:1].repeat_interleave(K, 0))
+
+
+@pytest.mark.parametrize("kind", ["missing", "other arguments", "another result"])
+def test_results_without_the_short_allocation(k3, dev, kind, monkeypatch):
+    """torch's private short way to a new tensor missing or changed: results come from its public one."""
+    import torch
+    guards = torch._C._dynamo.guards
+    if kind == "missing":
+        monkeypatch.delattr(guards, "_empty_strided_cuda", raising=False)
+    else:
+        def other(size, stride, dtype, *more):
+            if kind == "other arguments":
+                raise TypeError("four arguments")
+            return torch.empty(size)
+        monkeypatch.setattr(guards, "_empty_strided_cuda", other, raising=False)
+    monkeypatch.setattr(k3, "_rt", k3._Runtime())
+    idx = torch.tensor([[1, 0], [1, 5]], dtype=torch.int32, device=dev)
+    pos, pair, off = k3.moe_sort(idx, 2)
+    assert pos.tolist() == [[1, 0], [2, -1]] and pair.tolist() == [1, 0, 2, -1] and off.tolist() == [0, 1, 3]
