@@ -208,3 +208,118 @@ def test_lengths_of_vectors(k3):
         with pytest.raises(k3.K3CError, match="mat_of.*32 bits"):
             k3._vec_arg(torch.empty(n, dtype=torch.int32, device="meta"), "mat_of", -1, torch.int32)
     assert k3._vec_arg(torch.empty(5, dtype=torch.int32, device="meta"), "mat_of", -1, torch.int32) == 5
+
+
+# Each wrapper's valid call, and per tensor the defects that its own check has to find: another type,
+# another rank, one more row or column, elements or rows that are not as they have to lie.
+T, K, E, H, ROWS, IN, M = 4, 2, 3, 64, 6, 64, 5
+PAIRS = {"x": ("f32", T, H), "pos": ("i32", T, K), "wt": ("f32", T, K), "y": ("f32", T * K, H), "drows": ("f32", T * K, H),
+         "dout": ("bf16", T, H), "dy": ("f32", T * K, H), "dwt": ("f32", T, K)}
+ANY = "type rank stride"                 # extents that this argument itself sets
+OWN = ANY + " rows cols"
+CALLS = {
+    "moe_sort": (dict(idx=("i32", T, K)), (E,), dict(idx=ANY)),
+    "moe_permute": (dict(x=PAIRS["x"], pos=PAIRS["pos"], out=("f32", T * K, H)), (),
+                    dict(x=ANY + " overlap", pos=ANY + " rows", out=OWN)),
+    "moe_permute_bwd": (dict(drows=PAIRS["drows"], pos=PAIRS["pos"], out=("f32", T, H)), (),
+                        dict(drows=ANY + " rows", pos=ANY, out=OWN)),
+    "moe_permute_mxfp4": (dict(x=PAIRS["x"], pos=PAIRS["pos"]), (), dict(x=ANY + " overlap", pos=ANY + " rows")),
+    "moe_unpermute": (dict(y=PAIRS["y"], pos=PAIRS["pos"], wt=PAIRS["wt"], out=("bf16", T, H)), (),
+                      dict(y=ANY + " rows", pos=ANY, wt=OWN, out=OWN)),
+    "moe_unpermute_bwd": (dict(dout=PAIRS["dout"], y=PAIRS["y"], pos=PAIRS["pos"], wt=PAIRS["wt"], dy=PAIRS["dy"],
+                               dwt=PAIRS["dwt"]), (),
+                          dict(dout=OWN, y=ANY + " rows", pos=ANY, wt=OWN, dy=OWN, dwt=OWN)),
+    "mxfp4_quant": (dict(x=("bf16", M, IN)), (), dict(x=ANY + " overlap")),
+    "mxfp4_pack": (dict(packed=("u8", 2, ROWS, IN // 2), scales=("u8", 2, ROWS, IN // 32)), (),
+                   dict(packed="type rank stride", scales="type rank stride rows cols mats")),
+    "Mxfp4Mat": (dict(codes=("u8", 2, ROWS, IN // 2), atoms=("u8", 2, 1, 1, 512), mat_of=("i32", 4)), (),
+                 dict(codes="type rank stride", atoms="type rank stride rows cols mats", mat_of="type rank stride")),
+    "mxfp4_mm": (dict(a=("u8", M, IN // 2), a_scales=("u8", M, IN // 32), W=None, off=("i32", 3), out=("bf16", M, ROWS)), (),
+                 dict(a=ANY + " cols", a_scales=OWN, off="type rank stride cols", out=OWN + " overlap")),
+    "mxfp4_mm_bwd": (dict(dy=("bf16", M, ROWS), W=None, off=("i32", 3), out=("f32", M, IN)), (),
+                     dict(dy=ANY + " cols overlap", off="type rank stride cols", out=OWN + " overlap")),
+}
+CASES = [(f, a, d) for f, (_, _, own) in CALLS.items() for a, ds in own.items() for d in ds.split()]
+
+
+def one_defect(torch, dev, spec, defect):
+    """A tensor of the spec with one defect, or None of them."""
+    types = {"f32": torch.float32, "bf16": torch.bfloat16, "i32": torch.int32, "u8": torch.uint8}
+    other = {"f32": torch.float16, "bf16": torch.float64, "i32": torch.int64, "u8": torch.int8}
+    name, *shape = spec
+    dt = types[name]
+    if defect == "type":
+        dt = other[name]
+    elif defect == "rank":
+        shape.append(1)
+    elif defect in ("rows", "cols", "mats"):
+        shape[{"rows": max(len(shape) - 2, 0), "cols": len(shape) - 1, "mats": 0}[defect]] += 1
+    if defect == "stride":
+        return torch.zeros(*shape[:-1], 2 * shape[-1], dtype=dt, device=dev)[..., ::2]
+    if defect == "overlap":
+        return torch.zeros(1, shape[-1], dtype=dt, device=dev).expand(*shape)
+    return torch.zeros(*shape, dtype=dt, device=dev)
+
+
+def refused(k3, torch, dev, case, monkeypatch):
+    """The call with that one defect raises by the argument's name, and reaches no entry point; the
+    same call without it does."""
+    fn, arg, defect = case
+    specs, rest, _ = CALLS[fn]
+    launched = []
+
+    def kept(n, *a):
+        launched.append(n)
+    monkeypatch.setattr(k3, "_launch", lambda rt, name, *a: kept(name))
+    W = k3.Mxfp4Mat(*(one_defect(torch, dev, s, None) for s in (("u8", 2, ROWS, IN // 2), ("u8", 2, 1, 1, 512))))
+
+    def call(bad):
+        args = {n: W if s is None else one_defect(torch, dev, s, defect if n == bad else None) for n, s in specs.items()}
+        if fn == "mxfp4_mm" and bad == "off" and defect == "cols":
+            assert args["off"].shape == (4,)               # three groups, two matrices
+        return getattr(k3, fn)(*list(args.values())[:1], *rest, **dict(list(args.items())[1:]))
+    with pytest.raises(k3.K3CError, match=f"^{arg}: "):
+        call(arg)
+    assert not launched
+    call(None)
+    assert launched or fn == "Mxfp4Mat"
+
+
+@pytest.mark.parametrize("case", CASES, ids="-".join)
+def test_one_defect_is_refused_by_name(k3, case, monkeypatch):
+    """On the CPU: the wrappers with tensors and a runtime of no device."""
+    import types
+    import torch
+    rt = types.SimpleNamespace(
+        torch=torch, lib=None, floats=(torch.float32, torch.bfloat16), code={torch.float32: 0, torch.bfloat16: 1},
+        size={torch.float32: 4, torch.bfloat16: 2}, i32=torch.int32, u8=torch.uint8, f32=torch.float32, device=lambda: -1,
+        empty=lambda size, stride, dtype: torch.empty_strided(size, stride, dtype=dtype))
+    monkeypatch.setattr(k3, "_runtime", lambda t: rt)
+    refused(k3, torch, "cpu", case, monkeypatch)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", CASES, ids="-".join)
+def test_one_defect_is_refused_by_name_on_a_gpu(k3, case, monkeypatch):
+    import torch
+    refused(k3, torch, "cuda", case, monkeypatch)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fn,arg", [(f, a) for f, (s, _, _) in CALLS.items() for a in list(s)[1:] if s[a]])
+def test_a_tensor_elsewhere_is_refused(k3, fn, arg, monkeypatch):
+    """The first argument on the GPU, one of the others on the CPU."""
+    import torch
+    monkeypatch.setattr(k3, "_launch", lambda *a: pytest.fail("launched"))
+    W = k3.Mxfp4Mat(*(one_defect(torch, "cuda", s, None) for s in (("u8", 2, ROWS, IN // 2), ("u8", 2, 1, 1, 512))))
+    specs, rest, _ = CALLS[fn]
+    args = {n: W if s is None else one_defect(torch, "cpu" if n == arg else "cuda", s, None) for n, s in specs.items()}
+    with pytest.raises(k3.K3CError, match=f"^{arg}: |a CUDA tensor expected"):    # y leads moe_unpermute_bwd
+        getattr(k3, fn)(*list(args.values())[:1], *rest, **dict(list(args.items())[1:]))
+
+
+def test_a_gpu_is_asked_for(k3):
+    import torch
+    for t in (torch.zeros(4, 2, dtype=torch.int32), torch.zeros(4, 2)):
+        with pytest.raises(k3.K3CError, match="a CUDA tensor expected"):
+            k3._runtime(t)
