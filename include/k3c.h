@@ -651,6 +651,11 @@ int k3c_mxfp4_mm(void *y, int y_dtype, int64_t ldy, const uint8_t *a, const uint
 int k3c_mxfp4_mm_bwd(void *da, int da_dtype, int64_t ldda, const void *dy, int64_t lddy, int M,
                      const k3c_mxfp4_mat *W, const int *off, int n_groups, k3c_stream_t stream);
 
+/* The tiles in which k3c_mxfp4_mm (gradient 0) or k3c_mxfp4_mm_bwd (1) computes M rows in n_groups
+ * groups (grouped 0: no offsets) with matrices [rows][in]: rows << 16 | columns, or -1. For tests
+ * and measurements; no result depends on it. */
+int k3c_mxfp4_mm_tile(int M, int n_groups, int grouped, int rows, int in, int gradient);
+
 /* ---- Expert-parallel prefill over peer memory (no reference counterpart: the reference is
  * a single-process CPU engine). The ranks of one node each own a set of routed experts (the
  * layer's run table marks the others -1) and their own tokens. Per layer, with a cross-rank

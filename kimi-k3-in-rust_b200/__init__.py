@@ -283,6 +283,7 @@ def lib():
         "k3c_mxfp4_pack": ([vp, vp, vp, vp, i, i, i, vp], i),
         "k3c_mxfp4_mm": ([vp, i, C.c_int64, vp, vp, i, C.POINTER(Mxfp4MatC), vp, i, vp], i),
         "k3c_mxfp4_mm_bwd": ([vp, i, C.c_int64, vp, C.c_int64, i, C.POINTER(Mxfp4MatC), vp, i, vp], i),
+        "k3c_mxfp4_mm_tile": ([i, i, i, i, i, i], i),
         "k3c_moe_latent_decode": ([vp, vp, i, C.POINTER(MoeLatentLayerC), vp, vp, vp, vp, sz, vp], i),
     }
     for name, (args, res) in sig.items():

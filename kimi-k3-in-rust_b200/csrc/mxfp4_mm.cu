@@ -1582,6 +1582,24 @@ int cheapest(const TileCost *t, int n, int M, int n_groups, bool grouped, int co
     return best;
 }
 
+const TileCost MM_KINDS[] = {{256, 256, 2, 380, 700, 3400, 5400},
+                             {128, 256, 1, 410, 1000, 3150, 3950},
+                             {128, 128, 1, 270, 500, 2400, 3650},
+                             {128, 64, 1, 240, 400, 2200, 3400}};
+int mm_kind(int M, int n_groups, bool grouped, int rows, int in) {
+    return cheapest(MM_KINDS, 4, M, n_groups, grouped, rows, (in + 255) / 256);
+}
+// (112 K blocks, 2048 columns: 64 rows take the pair 41 us, 256 columns 58, 128 columns 35; 2000 rows
+// 43, 61, 70; two accumulators 72 there, but 257 and one 305 at 12000 rows. 4 K blocks, 2000 x 2048:
+// the pair 9.2, 128 columns 7.4)
+const TileCost BWD_KINDS[] = {{512, 256, 2, 555, 4050, 0, 5150},
+                              {256, 256, 2, 325, 1100, 0, 6200},
+                              {128, 256, 1, 505, 550, 0, 5100},
+                              {128, 128, 1, 295, 300, 1700, 3850}};
+int bwd_kind(int M, int n_groups, bool grouped, int rows, int in) {
+    return cheapest(BWD_KINDS, 4, M, n_groups, grouped, in, (rows + MB_KB - 1) / MB_KB);
+}
+
 template <int NT>
 int launch_mm(const CUtensorMap &ma, const CUtensorMap &ma1, const CUtensorMap &mw, MxArgs p, cudaStream_t s) {
     static bool attr_of[64] = {};
@@ -1710,6 +1728,15 @@ extern "C" int k3c_mxfp4_pack(uint8_t *codes, uint8_t *atoms, const uint8_t *pac
     return K3C_OK;
 }
 
+extern "C" int k3c_mxfp4_mm_tile(int M, int n_groups, int grouped, int rows, int in, int gradient) {
+    clear_error();
+    if (M < 1 || M > MX_DIM || n_groups < 1 || n_groups > MX_GMAX || rows < 1 || rows > MX_DIM || in < 32 || in > MX_DIM)
+        return set_error(K3C_EINVAL, "mxfp4_mm_tile: M=%d n_groups=%d rows=%d in=%d", M, n_groups, rows, in);
+    const TileCost &t = gradient ? BWD_KINDS[bwd_kind(M, n_groups, grouped != 0, rows, in)]
+                                 : MM_KINDS[mm_kind(M, n_groups, grouped != 0, rows, in)];
+    return t.rows << 16 | t.cols;
+}
+
 extern "C" int k3c_mxfp4_mm(void *y, int y_dtype, int64_t ldy, const uint8_t *a, const uint8_t *a_scales, int M,
                             const k3c_mxfp4_mat *W, const int *off, int n_groups, k3c_stream_t stream) {
     clear_error();
@@ -1737,15 +1764,11 @@ extern "C" int k3c_mxfp4_mm(void *y, int y_dtype, int64_t ldy, const uint8_t *a,
     p.as = a_scales;
     p.atoms = W->atoms;
     p.atom_stride = W->atom_stride;
-    static const TileCost kinds[] = {{256, 256, 2, 380, 700, 3400, 5400},
-                                     {128, 256, 1, 410, 1000, 3150, 3950},
-                                     {128, 128, 1, 270, 500, 2400, 3650},
-                                     {128, 64, 1, 240, 400, 2200, 3400}};
-    const int kind = cheapest(kinds, 4, M, n_groups, off != nullptr, p.N, (p.K + 255) / 256);
+    const int kind = mm_kind(M, n_groups, off != nullptr, p.N, p.K);
     CUtensorMap ma, ma1, mw;
     K3C_TRY(make_map3(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, a, p.K / 2, M, 1, p.K / 2, (uint64_t)(p.K / 2) * M, 128, MM_M));
     K3C_TRY(make_map3(&ma1, CU_TENSOR_MAP_DATA_TYPE_UINT8, a, p.K / 2, M, 1, p.K / 2, (uint64_t)(p.K / 2) * M, 128, MM_ABOX));
-    K3C_TRY(map_weights(&mw, W, 128, kind == 0 ? 128 : kinds[kind].cols));   // a pair's CTAs copy half the columns each
+    K3C_TRY(map_weights(&mw, W, 128, kind == 0 ? 128 : MM_KINDS[kind].cols));   // a pair's CTAs copy half the columns each
     if (kind == 0) K3C_TRY(launch_mm_pair(ma, ma1, mw, p, s));
     else if (kind == 1) K3C_TRY(launch_mm<256>(ma, ma1, mw, p, s));
     else if (kind == 2) K3C_TRY(launch_mm<128>(ma, ma1, mw, p, s));
@@ -1780,14 +1803,7 @@ extern "C" int k3c_mxfp4_mm_bwd(void *da, int da_dtype, int64_t ldda, const void
     p.n_mats = W->n_mats;
     p.atoms = W->atoms;
     p.atom_stride = W->atom_stride;
-    // (112 K blocks, 2048 columns: 64 rows take the pair 41 us, 256 columns 58, 128 columns 35; 2000 rows
-    // 43, 61, 70; two accumulators 72 there, but 257 and one 305 at 12000 rows. 4 K blocks, 2000 x 2048:
-    // the pair 9.2, 128 columns 7.4)
-    static const TileCost kinds[] = {{512, 256, 2, 555, 4050, 0, 5150},
-                                     {256, 256, 2, 325, 1100, 0, 6200},
-                                     {128, 256, 1, 505, 550, 0, 5100},
-                                     {128, 128, 1, 295, 300, 1700, 3850}};
-    const int kind = cheapest(kinds, 4, M, n_groups, off != nullptr, p.K, (p.N + MB_KB - 1) / MB_KB);
+    const int kind = bwd_kind(M, n_groups, off != nullptr, p.N, p.K);
     if (kind == 0) K3C_TRY((launch_bwd<128, true, 2>(p, W, dy, lddy, s)));
     else if (kind == 1) K3C_TRY((launch_bwd<128, true, 1>(p, W, dy, lddy, s)));
     else if (kind == 2) K3C_TRY((launch_bwd<256, false, 1>(p, W, dy, lddy, s)));

@@ -857,3 +857,51 @@ def test_gradient_of_the_largest_weights(k3, dev, byte):
         dy = (torch.randint(-3, 4, (9, N), device=dev).double() * 2.0 ** -20).bfloat16()
         da = k3.mxfp4_mm_bwd(dy, W, out_dtype=torch.float32).double().cpu().numpy()
         assert np.array_equal(da, dy.double().cpu().numpy() @ values(c, b))
+
+
+# ragged groups, and the tiles (rows, columns) that the product and its gradient take for them
+TILED = [([1400, 1, 0, 1290], 4104, 1824, (256, 256), (512, 256)),
+         ([700, 0, 900, 1300] + [300] * 30, 1304, 1312, (128, 256), (256, 256)),
+         ([100, 9, 0, 130] * 12, 200, 2080, (128, 128), (128, 256)),
+         ([40, 30, 1, 0, 33, 9, 20, 60], 520, 1056, (128, 64), (128, 128))]
+
+
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("roll", [0, 4, 7])
+@pytest.mark.parametrize("sizes,N,K,tile,tile_bwd", TILED, ids=["%dx%d" % t[3] for t in TILED])
+def test_groups_without_a_matrix_in_every_tile(k3, dev, sizes, N, K, tile, tile_bwd, roll, out):
+    """Both products in every tile shape, where groups at the start, at the end and side by side have
+    no matrix: zeros for those, the others' results beside them, rows behind the last group as they
+    were; with roll 7 the offsets leave the rows at both ends."""
+    import torch
+    G, n = len(sizes), sum(sizes)
+    M = n if roll == 7 else n + 3
+    L = k3.lib()
+    assert divmod(L.k3c_mxfp4_mm_tile(M, G, 1, N, K, 0), 65536) == tile
+    assert divmod(L.k3c_mxfp4_mm_tile(M, G, 1, N, K, 1), 65536) == tile_bwd
+    off = np.concatenate([[0], np.cumsum(sizes)]).astype(np.int32)
+    mat_of = np.roll(np.array([-1, 0, 7, 1, -1, -3, 2, 0], np.int32), -roll)[np.arange(G) % 8]
+    given = off.copy()
+    if roll == 7:
+        given[0], given[-1] = -9, n + 10 ** 6
+    W, w = matrices(k3, dev, 221, 3, N, K)
+    c, b = operand(222, M, K)
+    a, s, po, pm = to_dev(dev, pack_nibbles(c), b, given, mat_of)
+    W = k3.Mxfp4Mat(W.keep[0], W.keep[1], mat_of=pm)
+    dt = torch.float32 if out == "f32" else torch.bfloat16
+    y = torch.full((M, N), 7.0, dtype=dt, device=dev)
+    da = torch.full((M, K), 7.0, dtype=dt, device=dev)
+    dy = torch.randn((M, N), generator=torch.Generator().manual_seed(N)).bfloat16().to(dev)
+    k3.mxfp4_mm(a, s, W, off=po, out=y)
+    k3.mxfp4_mm_bwd(dy, W, off=po, out=da)
+    assert (y[n:] == 7).all() and (da[n:] == 7).all()
+    av, wv = to_dev(dev, values(c, b), w)
+    dv = dy.double()
+    for e in range(G):
+        r = slice(off[e], off[e + 1])
+        if not 0 <= mat_of[e] < 3:
+            assert (y[r] == 0).all() and (da[r] == 0).all()
+            continue
+        m = wv[mat_of[e]]
+        check(*(t.double().cpu().numpy() for t in (y[r], av[r] @ m.T, av[r].abs() @ m.abs().T)), -(-K // 64), out == "bf16")
+        check(*(t.double().cpu().numpy() for t in (da[r], dv[r] @ m, dv[r].abs() @ m.abs())), -(-N // 16), out == "bf16")

@@ -323,3 +323,21 @@ def test_a_gpu_is_asked_for(k3):
     for t in (torch.zeros(4, 2, dtype=torch.int32), torch.zeros(4, 2)):
         with pytest.raises(k3.K3CError, match="a CUDA tensor expected"):
             k3._runtime(t)
+
+
+def test_products_tests_reach_every_tile(k3):
+    """The sizes of the products' GPU tests take all four tile shapes of each product, dense and
+    grouped: a changed rule that leaves one of them untested shows here."""
+    import test_gpu_mxfp4_mm as mm
+    L = k3.lib()
+
+    def tile(*a):
+        return divmod(L.k3c_mxfp4_mm_tile(*a), 65536)
+    dense, grouped = mm.DENSE, [(s, n, k) for s, n, k, *_ in mm.TILED]
+    both = {0: {(256, 256), (128, 256), (128, 128), (128, 64)}, 1: {(512, 256), (256, 256), (128, 256), (128, 128)}}
+    more = [(128, 200, 60000), (300, 136, 19232)]      # the gradient's own
+    for gradient in (0, 1):
+        assert {tile(m, 1, 0, n, k, gradient) for m, n, k in dense + more * gradient} == both[gradient]
+        assert {tile(sum(s), len(s), 1, n, k, gradient) for s, n, k in grouped} == both[gradient]
+    for bad in ((0, 1, 0, 64, 64, 0), (4, 0, 0, 64, 64, 0), (4, 1025, 1, 64, 64, 0), (4, 1, 0, 0, 64, 0), (4, 1, 0, 64, 16, 1)):
+        assert L.k3c_mxfp4_mm_tile(*bad) == -1 and "mxfp4_mm_tile" in err(k3)
