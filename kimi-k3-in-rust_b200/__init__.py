@@ -1350,8 +1350,9 @@ class Mxfp4Mat:
     @classmethod
     def from_pool(cls, layer, which):
         """The experts' matrices of a PoolMoeLayer, or of a LatentMoeLayer (hidden: its latent width),
-        in its arena, by expert id: "gate_up" [2 * inter][hidden] (64 gate rows, the matching 64 up
-        rows, and so on) or "down" [hidden][inter]. Experts without a run give zeros."""
+        in its arena or its ExpertPool's slots, by expert id: "gate_up" [2 * inter][hidden] (64 gate rows,
+        the matching 64 up rows, and so on) or "down" [hidden][inter]. A product takes the runs that
+        the layer's table names when it runs; experts without one give zeros."""
         if isinstance(layer, LatentMoeLayer):
             c, (arena, run_of) = layer.c.experts, layer._keep[:2]
         elif isinstance(layer, PoolMoeLayer):
@@ -1367,7 +1368,7 @@ class Mxfp4Mat:
         base = arena.data_ptr()
         m = cls.__new__(cls)
         m._set(Mxfp4MatC(base + lay[p][0], base + lay[s][0], c.run_stride, c.run_stride, c.n_runs, rows, in_,
-                         run_of.data_ptr()), run_of.numel(), arena.get_device(), (arena, run_of))
+                         run_of.data_ptr()), run_of.numel(), run_of.get_device(), (arena, run_of))
         return m
 
 

@@ -905,3 +905,56 @@ def test_groups_without_a_matrix_in_every_tile(k3, dev, sizes, N, K, tile, tile_
         m = wv[mat_of[e]]
         check(*(t.double().cpu().numpy() for t in (y[r], av[r] @ m.T, av[r].abs() @ m.abs().T)), -(-K // 64), out == "bf16")
         check(*(t.double().cpu().numpy() for t in (da[r], dv[r] @ m, dv[r].abs() @ m.abs())), -(-N // 16), out == "bf16")
+
+
+def test_experts_of_a_pool_that_are_loaded_and_evicted(k3, dev):
+    """The matrices of a layer over an ExpertPool's slots: each product takes what the run table names
+    when it runs, zeros for experts that are not resident."""
+    import torch
+    H, I, NE, NS = 256, 128, 8, 4
+    g = k3.synth.rng(83)
+    experts = [k3.synth.expert(g, H, I) for _ in range(NE)]
+    run = torch.empty(k3.pool_run_bytes(H, I), dtype=torch.uint8, device=dev)
+    host = []
+    for e in experts:
+        k3.pool_pack(run, k3.DeviceExpert.from_host(e, dev).q(), H, I)
+        host.append(run.cpu().pin_memory())
+    pool = k3.ExpertPool(H, I, 1, NE, NS, lambda layer, e: host[e])
+    run_of = pool.run_table()
+    Wr = torch.zeros((NE, H), dtype=torch.bfloat16, device=dev)
+    layer = pool.layer(Wr, H, I, 2, NE, run_of)
+    D, GU = k3.Mxfp4Mat.from_pool(layer, "down"), k3.Mxfp4Mat.from_pool(layer, "gate_up")
+    assert (D.rows, D.in_, GU.rows, GU.in_, D.groups) == (H, I, 2 * I, H, NE)
+    idx = torch.arange(24, dtype=torch.int32, device=dev).view(12, 2) % NE
+    pos, _, off = k3.moe_sort(idx, NE)
+    gn = torch.Generator().manual_seed(1)
+    x = torch.randn((12, H), generator=gn).to(dev)
+    h, dy = torch.randn((24, I), generator=gn).to(dev), torch.randn((24, H), generator=gn).bfloat16().to(dev)
+    a, sa = k3.moe_permute_mxfp4(x, pos)
+    b, sb = k3.mxfp4_quant(h)
+    av, bv = values(unpack(a.cpu().numpy()), sa.cpu().numpy()), values(unpack(b.cpu().numpy()), sb.cpu().numpy())
+    dv, offn = dy.double().cpu().numpy(), off.cpu().numpy()
+
+    def mat(e, name):
+        return values(unpack(e[name + "_p"]), e[name + "_s"])
+    for ids in ([0, 3, 5, 6], [7, 1, 3]):
+        pool.acquire(0, ids, run_of)
+        table = run_of.cpu().numpy()
+        gu = k3.mxfp4_mm(a, sa, GU, off=off, out_dtype=torch.float32).double().cpu().numpy()
+        y = k3.mxfp4_mm(b, sb, D, off=off, out_dtype=torch.float32).double().cpu().numpy()
+        dh = k3.mxfp4_mm_bwd(dy, D, off=off, out_dtype=torch.float32).double().cpu().numpy()
+        assert all(table[e] >= 0 for e in ids) and (table < 0).sum() >= NE - NS
+        for e in range(NE):
+            r = slice(offn[e], offn[e + 1])
+            if table[e] < 0:
+                assert (gu[r] == 0).all() and (y[r] == 0).all() and (dh[r] == 0).all()
+                continue
+            wg, wu, wd = mat(experts[e], "gate"), mat(experts[e], "up"), mat(experts[e], "down")
+            blocks = gu[r].reshape(-1, I // 64, 2, 64)
+            check(blocks[:, :, 0].reshape(-1, I), av[r] @ wg.T, np.abs(av[r]) @ np.abs(wg).T, H // 64, False)
+            check(blocks[:, :, 1].reshape(-1, I), av[r] @ wu.T, np.abs(av[r]) @ np.abs(wu).T, H // 64, False)
+            check(y[r], bv[r] @ wd.T, np.abs(bv[r]) @ np.abs(wd).T, I // 64, False)
+            check(dh[r], dv[r] @ wd, np.abs(dv[r]) @ np.abs(wd), H // 16, False)
+        pool.release(0, ids)
+    torch.cuda.synchronize()
+    pool.close()
