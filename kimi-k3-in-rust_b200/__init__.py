@@ -1112,10 +1112,11 @@ def _tracked(t, name):
 def _mat_arg(t, name, dev, dtypes, d0=None, d1=None):
     """A contiguous 2-D tensor on device dev; its extents (None: any)."""
     sh = t.shape
-    if (t.dtype not in dtypes or len(sh) != 2 or (d0 is not None and sh[0] != d0) or (d1 is not None and sh[1] != d1)
+    a, b = sh if len(sh) == 2 else (None, None)
+    if (a is None or t.dtype not in dtypes or (d0 is not None and a != d0) or (d1 is not None and b != d1)
             or t.get_device() != dev or not t.is_contiguous()):
         _bad(t, name, f"contiguous {dtypes} {(d0, d1)} on device {dev}")
-    if sh[0] > _INT_MAX or sh[1] > _INT_MAX:
+    if a > _INT_MAX or b > _INT_MAX:
         _bad(t, name, "extents within 32 bits")
     if t.requires_grad:
         _tracked(t, name)
@@ -1132,9 +1133,10 @@ def _vec_arg(t, name, dev, dtype):
 
 def _rows_arg(t, name, dev, dtypes):
     """A 2-D tensor on device dev whose rows are contiguous: (rows, columns, row stride)."""
-    if t.dtype not in dtypes or t.dim() != 2 or t.get_device() != dev:
+    sh = t.shape
+    if len(sh) != 2 or t.dtype not in dtypes or t.get_device() != dev:
         _bad(t, name, f"2-D {dtypes} on device {dev}")
-    rows, n = t.shape
+    rows, n = sh
     if rows > _INT_MAX or n > _INT_MAX:
         _bad(t, name, "extents within 32 bits")
     if t.requires_grad:
@@ -1189,7 +1191,9 @@ def moe_permute(x, pos, out=None):
     else:
         _mat_arg(out, "out", dev, (x.dtype,), T * K, H)
         po, b = out.data_ptr(), rt.size[x.dtype]
-        _apart("out", _flat(po, T * K * H * b), (px, T, H * b, ld * b), _flat(pp, 4 * T * K))
+        end = po + T * K * H * b
+        if px < end and po < px + T * ld * b or pp < end and po < pp + 4 * T * K:   # they may: look closer
+            _apart("out", _flat(po, end - po), (px, T, H * b, ld * b), _flat(pp, 4 * T * K))
     _launch(rt, "k3c_moe_permute", dev, po, px, rt.code[x.dtype], ld, pp, T, K, H)
     return out
 
@@ -1385,15 +1389,13 @@ def _mm_groups(rt, W, off, dev):
 
 
 def _mm_out(rt, M, n, dev, out, out_dtype, W, *memory):
-    """(out, its row stride); memory: what the product reads besides W."""
-    if out is None:
-        return _new(rt, dev, _out_type(rt, out_dtype, rt.torch.bfloat16), M, n), n
+    """A given result's row stride; memory: what the product reads besides W."""
     rows, cols, ld = _rows_arg(out, "out", dev, rt.floats if out_dtype is None else (_out_type(rt, out_dtype, None),))
     if rows != M or cols != n:
         _bad(out, "out", f"fp32 or bf16 {(M, n)}")
     b = rt.size[out.dtype]
     _apart("out", (out.data_ptr(), M, n * b, ld * b), *memory, *W._memory())
-    return out, ld
+    return ld
 
 
 def mxfp4_mm(a, a_scales, W, off=None, out=None, out_dtype=None):
@@ -1408,8 +1410,12 @@ def mxfp4_mm(a, a_scales, W, off=None, out=None, out_dtype=None):
     _mat_arg(a_scales, "a_scales", dev, (rt.u8,), M, W.in_ // 32)
     po, G = _mm_groups(rt, W, off, dev)
     pa, ps = a.data_ptr(), a_scales.data_ptr()
-    out, ld = _mm_out(rt, M, W.rows, dev, out, out_dtype, W, _flat(pa, M * (W.in_ // 2)), _flat(ps, M * (W.in_ // 32)),
-                      _flat(po or 0, 4 * (G + 1) if po else 0))
+    if out is None:
+        ld = W.rows
+        out = _new(rt, dev, _out_type(rt, out_dtype, rt.torch.bfloat16), M, ld)
+    else:
+        ld = _mm_out(rt, M, W.rows, dev, out, out_dtype, W, _flat(pa, M * (W.in_ // 2)), _flat(ps, M * (W.in_ // 32)),
+                     _flat(po or 0, 4 * (G + 1) if po else 0))
     _launch(rt, "k3c_mxfp4_mm", dev, out.data_ptr(), rt.code[out.dtype], ld, pa, ps, M, W.ref, po, G)
     return out
 
@@ -1425,7 +1431,11 @@ def mxfp4_mm_bwd(dy, W, off=None, out=None, out_dtype=None):
         _bad(dy, "dy", f"{W.rows} columns")
     po, G = _mm_groups(rt, W, off, dev)
     pd = dy.data_ptr()
-    out, ld = _mm_out(rt, M, W.in_, dev, out, out_dtype, W, (pd, M, 2 * n, 2 * ldd), _flat(po or 0, 4 * (G + 1) if po else 0))
+    if out is None:
+        ld = W.in_
+        out = _new(rt, dev, _out_type(rt, out_dtype, rt.torch.bfloat16), M, ld)
+    else:
+        ld = _mm_out(rt, M, W.in_, dev, out, out_dtype, W, (pd, M, 2 * n, 2 * ldd), _flat(po or 0, 4 * (G + 1) if po else 0))
     if M <= 1:       # whatever its stride, which torch does not keep for a row that counts as contiguous
         ldd = (n + 7) & ~7
     if pd & 15 or ldd & 7:
