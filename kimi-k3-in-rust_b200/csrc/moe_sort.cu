@@ -261,7 +261,8 @@ __device__ __forceinline__ void st16(void *p, const uint4 &v) {
 
 constexpr int PM_TH = 512;   // threads of a block at most
 // Rows on no 16-byte boundary move element by element, so many per thread and round (32768 rows of
-// 7167 bf16 summed to 4096: 175 us, 202 with one at a time).
+// 7167 bf16 summed to 4096: 175 us, 202 with one at a time). Bound by the number of loads and stores: 2 bytes
+// each where aligned rows of 7168 move 16 in 78 us; in fp32 (3583 and 3584 wide) 99 and 80.
 constexpr int PM_U = 4, UB_U = 2;
 
 // A token's pairs that have a row, in the order of j: rows, j and weights in shared memory, so that
@@ -537,7 +538,7 @@ __global__ void __launch_bounds__(PM_TH) k_unpermute_bwd(T *__restrict__ dy, flo
 // ------------------------------------------------------------------ quantising permute
 // One thread per 32-element group of a token: read and quantised once, its 16 bytes of codes
 // and its scale byte stored into each of the token's rows. Bound by HBM: 4096 x 8 rows of 7168 in
-// 32 us, 5.8 TB/s (the permute and a quantisation of its rows: 88 + 93).
+// 32 us, 5.8 TB/s (the permute and a quantisation of its rows: 88 + 93), 66 us with x on odd addresses.
 template <typename T>
 __global__ void __launch_bounds__(PM_TH) k_permute_mx4(uint8_t *__restrict__ packed, uint8_t *__restrict__ scales,
                                                        const T *__restrict__ x, int64_t ldx,

@@ -112,7 +112,8 @@ __global__ void __launch_bounds__(256) k_mx4_quant(uint8_t *__restrict__ packed,
     }
 }
 
-// Any other rows: one thread per group.
+// Any other rows: one thread per group. Bound by its loads of single elements and stores of single bytes:
+// 8192 x 7168 bf16 on odd addresses 128 us (1.2 TB/s), 8192 x 7166 134.
 template <typename T>
 __global__ void __launch_bounds__(256) k_mx4_quant_any(uint8_t *__restrict__ packed, uint8_t *__restrict__ scales,
                                                        const T *__restrict__ x, int64_t ldx, int rows, int in) {
@@ -145,7 +146,7 @@ __device__ __forceinline__ bool wait_for_sums(uint64_t *bar, uint32_t parity, in
 __device__ __forceinline__ int sf_byte(int m, int g) { return 16 * (m & 31) + 4 * (m >> 5) + g; }
 
 // One thread per group of the padded matrix: scale byte into its atom, codes copied (packed and
-// codes may be the same array).
+// codes may be the same array). Done once per weight: 48 matrices of 4096 x 7168 in 260 us, 5.8 TB/s.
 __global__ void __launch_bounds__(256) k_mx4_pack(uint8_t *codes, uint8_t *__restrict__ atoms, const uint8_t *packed,
                                                   const uint8_t *__restrict__ scales, int n_mats, int rows, int in) {
     const int G = in / 32, RA = (rows + 127) / 128, KA = (in + 127) / 128;
@@ -616,10 +617,10 @@ __device__ __forceinline__ void a_scales(const MxArgs &p, int n_items, const Ite
 // 128 rows x NT columns per item, one CTA per SM. A K block is 256 codes of a row, 128 bytes: four
 // MMAs of K = 64 and two TMEM copies of scale atoms per operand. Bound by HBM for few rows (16 x 8
 // rows over 64 experts of 4096 x 7168: 122 us, the weights at 7.1 TB/s), by the chain of K
-// blocks for one tile in a row (one token, 7168 x 7168: 9.8 us, 0.20 us a K block: about half of it
+// blocks for one tile in a row (one token, 7168 x 7168: 9.8 to 10.4 us, 0.20 us a K block: about half of it
 // waits, copies and commits, 25 ns an MMA however few its columns; fewer stages, a second accumulator
-// or no proxy fence left it as it was, and a K split would make a row's result depend on how many
-// rows are beside it), by L2 and power above.
+// or no proxy fence left it as it was. A K split would make a row's result depend on how many rows
+// are beside it; more codes per wait and commit would not, and have not been tried), by L2 and power above.
 template <int NT>
 __global__ void __launch_bounds__(MM_THREADS, 1) k_mx4_mm(const __grid_constant__ CUtensorMap tmA,
                                                           const __grid_constant__ CUtensorMap tmA1,
@@ -1045,8 +1046,8 @@ constexpr int MB_WIDE0 = 3;                      // warps: dY, MMA, W, widening,
 // bandwidth bounds these kernels: a K block of 128 x 256 takes one CTA 121 KB through it (copies
 // in, packed tile out, widened tile in, both operands out), 950 cycles at 128 bytes a cycle, for
 // 512 cycles of MMAs; a pair's CTA 73 KB, 580 cycles; 128 x 128 72 KB, 560 cycles, to which the
-// widening's instructions add (without its arithmetic 64 x 7168 x 2048 takes 30 us of 34, with half its
-// stores 30, without dY's copies 31, with a deeper ring for them 34). ACCS = 2: a pair takes 512 rows in two
+// widening's instructions add (without its arithmetic 64 x 7168 x 2048 takes 29.1 us of 33.6, with
+// half its stores 30.2, without dY's copies 31.2). ACCS = 2: a pair takes 512 rows in two
 // accumulators, so a widened tile serves both; what that saves is mostly power, which bounds the
 // clock under large products. It leaves no TMEM for the next item's accumulators.
 template <int NT, bool PAIR, int ACCS>
@@ -1066,9 +1067,9 @@ struct MbCfg {
     // could take the one before it, of the same parity, for the one it needs.
     static constexpr int TURNS = RING;
     // Warps that widen one K block. Where a single CTA widens 128 columns of it two do, with more in
-    // flight each: four warps' issue slots are what few rows wait for (64 x 7168 x 2048 34.0 us,
+    // flight each: four warps' issue slots are what few rows wait for (64 x 7168 x 2048 33.6 us,
     // 35.0 with four; 39.5 with one). Pairs and 256 columns need four (1200 x 7168 x 2048 39.1, 41.9
-    // with two; 128 x 7168 x 37888 70 and 92).
+    // with two; 128 x 7168 x 37888 71 and 93).
     static constexpr int GROUP = !PAIR && NT == 128 ? 2 : 4;
     static constexpr int EPI0 = MB_WIDE0 + TURNS * GROUP, THREADS = 32 * (EPI0 + MB_EPI);
     static constexpr int BYTES = 1024 + RING * (A + B) + RAW * R + 512;
@@ -1113,8 +1114,8 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
 // value times 2^-126, subnormals included, so f1 = 2^(byte-1) under both halves gives the scaled
 // value in one exact product. Codes j and j + 4 share word j, as they lie 16 bits apart. A multiply
 // puts a code's magnitude and sign in place at once (the bits between are masked), shifts and masks
-// do the same on the other pipe: two words each (64 x 7168 x 2048: 35.2 us; all by shifts 35.7, all by
-// multiplies 36.3).
+// do the same on the other pipe: two words each (64 x 7168 x 2048: 33.6 us; all by shifts 35.4, all by
+// multiplies 34.6).
 __device__ __forceinline__ void e2m1x8_widen(uint32_t w, uint32_t f1, uint32_t (&o)[4]) {
     constexpr uint32_t mag = 0x01C001C0u, sign = 0x80008000u;
     o[0] = mul_bf16x2(((w & 0x000F000Fu) * 0x1040u) & (mag | sign), f1);
@@ -1560,7 +1561,10 @@ struct TileCost {
     int rows, cols, ctas, block, item, store, fixed;
 };
 // The cheapest of n kernels for M rows in n_groups groups (grouped: their sizes are on the device;
-// each is taken to waste half a tile) and `cols` columns, kb K blocks. Ties go to the first.
+// each is taken to waste half a tile) and `cols` columns, kb K blocks. Ties go to the first. All M rows are
+// taken to belong to groups: where an expert-parallel rank holds 4608 of 32768, in 48 groups, a
+// product with 4096 x 7168 matrices takes 160 us on pairs and 144 on 128 x 256 tiles, which the rows alone
+// would take (the gradient of 7168 x 2048 takes pairs either way).
 int cheapest(const TileCost *t, int n, int M, int n_groups, bool grouped, int cols, int kb) {
     int best = 0;
     double least = 0;
@@ -1589,9 +1593,9 @@ const TileCost MM_KINDS[] = {{256, 256, 2, 380, 700, 3400, 5400},
 int mm_kind(int M, int n_groups, bool grouped, int rows, int in) {
     return cheapest(MM_KINDS, 4, M, n_groups, grouped, rows, (in + 255) / 256);
 }
-// (112 K blocks, 2048 columns: 64 rows take the pair 41 us, 256 columns 58, 128 columns 35; 2000 rows
-// 43, 61, 70; two accumulators 72 there, but 257 and one 305 at 12000 rows. 4 K blocks, 2000 x 2048:
-// the pair 9.2, 128 columns 7.4)
+// (112 K blocks, 2048 columns: 64 rows take the pair 39 us, 256 columns 56, 128 columns 34; 2000 rows
+// 44, 63, 72; two accumulators 75 there, but 261 to 282 and one 304 at 12000 rows. 4 K blocks, 2000 x 2048:
+// the pair 8.8, 256 and 128 columns 8.3)
 const TileCost BWD_KINDS[] = {{512, 256, 2, 555, 4050, 0, 5150},
                               {256, 256, 2, 325, 1100, 0, 6200},
                               {128, 256, 1, 505, 550, 0, 5100},
