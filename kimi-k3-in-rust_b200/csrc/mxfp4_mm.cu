@@ -1046,8 +1046,8 @@ constexpr int MB_WIDE0 = 3;                      // warps: dY, MMA, W, widening,
 // bandwidth bounds these kernels: a K block of 128 x 256 takes one CTA 121 KB through it (copies
 // in, packed tile out, widened tile in, both operands out), 950 cycles at 128 bytes a cycle, for
 // 512 cycles of MMAs; a pair's CTA 73 KB, 580 cycles; 128 x 128 72 KB, 560 cycles, to which the
-// widening's instructions add (without its arithmetic 64 x 7168 x 2048 takes 29.1 us of 33.6, with
-// half its stores 30.2, without dY's copies 31.2). ACCS = 2: a pair takes 512 rows in two
+// widening's instructions add (without its arithmetic 64 x 7168 x 2048 takes 29 us of 34, with
+// half its stores 30, without dY's copies 31). ACCS = 2: a pair takes 512 rows in two
 // accumulators, so a widened tile serves both; what that saves is mostly power, which bounds the
 // clock under large products. It leaves no TMEM for the next item's accumulators.
 template <int NT, bool PAIR, int ACCS>
@@ -1067,7 +1067,7 @@ struct MbCfg {
     // could take the one before it, of the same parity, for the one it needs.
     static constexpr int TURNS = RING;
     // Warps that widen one K block. Where a single CTA widens 128 columns of it two do, with more in
-    // flight each: four warps' issue slots are what few rows wait for (64 x 7168 x 2048 33.6 us,
+    // flight each: four warps' issue slots are what few rows wait for (64 x 7168 x 2048 34.1 us,
     // 35.0 with four; 39.5 with one). Pairs and 256 columns need four (1200 x 7168 x 2048 39.1, 41.9
     // with two; 128 x 7168 x 37888 71 and 93).
     static constexpr int GROUP = !PAIR && NT == 128 ? 2 : 4;
@@ -1114,8 +1114,8 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
 // value times 2^-126, subnormals included, so f1 = 2^(byte-1) under both halves gives the scaled
 // value in one exact product. Codes j and j + 4 share word j, as they lie 16 bits apart. A multiply
 // puts a code's magnitude and sign in place at once (the bits between are masked), shifts and masks
-// do the same on the other pipe: two words each (64 x 7168 x 2048: 33.6 us; all by shifts 35.4, all by
-// multiplies 34.6).
+// do the same on the other pipe: two words each (64 x 7168 x 2048: 34.1 us; all by shifts 35.4, all by
+// multiplies 34.7).
 __device__ __forceinline__ void e2m1x8_widen(uint32_t w, uint32_t f1, uint32_t (&o)[4]) {
     constexpr uint32_t mag = 0x01C001C0u, sign = 0x80008000u;
     o[0] = mul_bf16x2(((w & 0x000F000Fu) * 0x1040u) & (mag | sign), f1);
@@ -1374,8 +1374,6 @@ __global__ void __launch_bounds__(MbCfg<NT, PAIR, ACCS>::THREADS, 1) k_mx4_bwd(c
                         c[j][i] = *reinterpret_cast<const uint4 *>(sw + r * C::WB + 16 * at);
                         s[j][i] = sw[C::W + i * 512 + sf_byte((kb & 1) * 64 + r, g)];
                     }
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&rempty[rt]);
                 ok = __all_sync(0xFFFFFFFFu, tc::mbar_wait(&empty[turn], ph, p.err, 99));
                 if (!ok) break;
 #pragma unroll
@@ -1405,9 +1403,15 @@ __global__ void __launch_bounds__(MbCfg<NT, PAIR, ACCS>::THREADS, 1) k_mx4_bwd(c
                             *reinterpret_cast<uint4 *>(row + 16 * (((g & 1) * 4 + q) ^ (r & 7))) =
                                 make_uint4(o[0][q], o[1][q], o[2][q], o[3][q]);
                     }
+                // The packed slot is given back only here, where the stores above have used every load from
+                // it and the proxy fence stands behind them. Given back right after the loads were issued, a
+                // load that waited behind the epilogue's element stores came after the next copy into the slot.
                 tc::fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&full[turn]);
+                if (lane == 0) {
+                    tc::mbar_arrive(&full[turn]);
+                    tc::mbar_arrive(&rempty[rt]);
+                }
                 ph ^= 1u;
                 rt += C::TURNS;
                 if (rt >= C::RAW) {

@@ -958,3 +958,37 @@ def test_experts_of_a_pool_that_are_loaded_and_evicted(k3, dev):
         pool.release(0, ids)
     torch.cuda.synchronize()
     pool.close()
+
+
+# 60 groups of 0 to 181 rows with a matrix in most of them
+RAGGED = [39, 17, 2, 44, 72, 48, 7, 20, 2, 29, 18, 76, 63, 56, 1, 56, 72, 8, 80, 8, 35, 31, 181, 8, 4, 101, 7, 23, 42, 13, 2,
+          29, 20, 14, 31, 6, 23, 5, 35, 39, 9, 41, 17, 6, 75, 13, 4, 0, 14, 14, 55, 2, 37, 71, 28, 13, 3, 6, 3, 61]
+
+
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("sizes,N,K", [t[:3] for t in TILED] + [(RAGGED, 819, 1440), ([1100], 832, 2048)],
+                         ids=["%dx%d" % t[3] for t in TILED] + ["ragged", "dense"])
+def test_slow_stores_change_no_result(k3, dev, sizes, N, K, out):
+    """Results in rows on odd addresses, which are stored element by element, are those in rows that are
+    not, bit for bit and every time: the epilogue's slow stores hold up whatever shares their way to
+    memory, so that waits which fast ones never test are."""
+    import torch
+    G, M = len(sizes), sum(sizes)
+    off = np.concatenate([[0], np.cumsum(sizes)]).astype(np.int32)
+    mat_of = np.array([0, 1, 2, 0, -1], np.int32)[np.arange(G) % 5]
+    W, _ = matrices(k3, dev, 231, 3, N, K)
+    c, b = operand(232, M, K)
+    a, s, po, pm = to_dev(dev, pack_nibbles(c), b, off, mat_of)
+    W = k3.Mxfp4Mat(W.keep[0], W.keep[1], mat_of=pm)
+    dt = torch.float32 if out == "f32" else torch.bfloat16
+    dy = torch.randn((M, N), generator=torch.Generator().manual_seed(N)).bfloat16().to(dev)
+    want = k3.mxfp4_mm(a, s, W, off=po, out_dtype=dt), k3.mxfp4_mm_bwd(dy, W, off=po, out_dtype=dt)
+    got = [torch.zeros(M * (n + 1) + 1, dtype=dt, device=dev)[1:].view(M, n + 1)[:, :n] for n in (N, K)]
+    bad = torch.zeros((), dtype=torch.int64, device=dev)
+    for _ in range(25):
+        k3.mxfp4_mm(a, s, W, off=po, out=got[0])
+        k3.mxfp4_mm_bwd(dy, W, off=po, out=got[1])
+        for g, w in zip(got, want):
+            bad += (g != w).sum()
+            g.zero_()
+    assert bad.item() == 0
