@@ -388,3 +388,74 @@ def test_results_without_the_short_allocation(k3, dev, kind, monkeypatch):
     idx = torch.tensor([[1, 0], [1, 5]], dtype=torch.int32, device=dev)
     pos, pair, off = k3.moe_sort(idx, 2)
     assert pos.tolist() == [[1, 0], [2, -1]] and pair.tolist() == [1, 0, 2, -1] and off.tolist() == [0, 1, 3]
+
+
+def test_the_most_pairs(k3, dev):
+    """As many pairs as 32 bits allow, with rows of one element: pair p goes to expert p % 3 - 1, the
+    first third of them nowhere."""
+    import torch
+    torch.cuda.empty_cache()
+    K, E = 8, 2
+    T = ((1 << 31) - (1 << 19) - 1) // K
+    P = T * K
+    idx = torch.arange(P, dtype=torch.int32, device=dev).remainder_(3).sub_(1).view(T, K)
+    pos, pair, off = k3.moe_sort(idx, E)
+    n = [(P - e - 1 + 2) // 3 for e in range(E)]
+    assert off.tolist() == [0, n[0], n[0] + n[1]]
+    pos = pos.view(-1)
+    x = (torch.arange(T, dtype=torch.int32, device=dev) % 251).bfloat16().view(T, 1)
+    rows = k3.moe_permute(x, pos.view(T, K))
+    out = k3.moe_permute_bwd(rows, pos.view(T, K))
+    for lo in range(0, P, 1 << 27):
+        p = torch.arange(lo, min(lo + (1 << 27), P), dtype=torch.int32, device=dev)
+        e = p % 3 - 1
+        want = torch.where(e < 0, -1, p // 3 + torch.where(e == 1, n[0], 0))
+        assert torch.equal(pos[p[0]:p[-1] + 1], want)
+        live = want >= 0
+        assert torch.equal(pair[want[live].long()], p[live])
+        assert torch.equal(rows.view(-1)[want[live].long()], x.view(-1)[(p[live] // K).long()])
+        t = p[::K] // K
+        held = (idx.view(-1)[lo:lo + p.numel()].view(-1, K) >= 0).sum(1)
+        assert torch.equal(out.view(-1)[t[0]:t[-1] + 1], (x.view(-1)[t[0]:t[-1] + 1].float() * held).bfloat16())
+    assert (pair[n[0] + n[1]:] == -1).all()
+    with pytest.raises(k3.K3CError, match="32 bits"):
+        k3.moe_sort(torch.empty((T + 1, K), dtype=torch.int32, device=dev), E)
+    del idx, pos, pair, rows, out, x
+    torch.cuda.empty_cache()
+
+
+def test_two_threads(k3, dev):
+    """Threads with streams of their own, each through all the calls, get what one alone does."""
+    import threading
+    import torch
+    T, K, E, H, N = 700, 4, 19, 96, 72
+    g = torch.Generator(device=dev).manual_seed(5)
+    codes = torch.randint(0, 256, (E, N, H // 2), dtype=torch.uint8, device=dev, generator=g)
+    W = k3.Mxfp4Mat(*k3.mxfp4_pack(codes, torch.randint(118, 125, (E, N, H // 32), dtype=torch.uint8, device=dev, generator=g)))
+
+    def layer(idx, x, wt):
+        pos, _, off = k3.moe_sort(idx, E)
+        y = k3.mxfp4_mm(*k3.moe_permute_mxfp4(x, pos), W, off=off)
+        out = k3.moe_unpermute(y, pos, wt)
+        dy, dwt = k3.moe_unpermute_bwd(out, y, pos, wt)
+        return out, dwt, k3.moe_permute_bwd(k3.mxfp4_mm_bwd(dy, W, off=off), pos)
+
+    ins = [(torch.randint(0, E, (T, K), device=dev, generator=g, dtype=torch.int32), torch.randn(T, H, device=dev, generator=g),
+            torch.rand(T, K, device=dev, generator=g)) for _ in range(4)]
+    want = [layer(*i) for i in ins]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                got = layer(*ins[i])
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    wrong.append(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong

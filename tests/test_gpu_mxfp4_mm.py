@@ -992,3 +992,44 @@ def test_slow_stores_change_no_result(k3, dev, sizes, N, K, out):
             bad += (g != w).sum()
             g.zero_()
     assert bad.item() == 0
+
+
+def test_quantising_and_packing_past_32_bits(k3, dev):
+    """More than 2^32 elements in and bytes out: the last rows and matrices as they come out alone."""
+    import torch
+    torch.cuda.empty_cache()
+    g = torch.Generator(device=dev).manual_seed(7)
+    H = 7168
+    x = torch.randn((600008, H + 8), device=dev, generator=g, dtype=torch.bfloat16)
+    for v in (x.view(-1)[:600000 * H].view(600000, H), x[:, :H], x[:, 1:H + 1], x[:, :H - 2]):
+        p, s = k3.mxfp4_quant(v)
+        for i in (slice(0, 300), slice(-300, None)):
+            wp, ws = k3.mxfp4_quant(v[i].contiguous())
+            assert torch.equal(p[i], wp) and torch.equal(s[i], ws)
+        del p, s
+    T, K = 80000, 16
+    idx = torch.randint(0, 5, (T, K), device=dev, generator=g, dtype=torch.int32)
+    pos, pair, _ = k3.moe_sort(idx, 5)
+    p, s = k3.moe_permute_mxfp4(x[:T, :H], pos)
+    wp, ws = k3.mxfp4_quant(x[:T, :H])
+    for i in (slice(0, 300), slice(-300, None)):
+        tok = (pair[i] // K).long()
+        assert torch.equal(p[i], wp[tok]) and torch.equal(s[i], ws[tok])
+    del p, s, wp, ws, x
+    n, rows = 320, 4096
+    p = torch.randint(0, 256, (n, rows, H // 2), dtype=torch.uint8, device=dev, generator=g)
+    s = torch.randint(118, 256, (n, rows, H // 32), dtype=torch.uint8, device=dev, generator=g)
+    codes, atoms = k3.mxfp4_pack(p, s)
+    for i in (0, n - 1):
+        wc, wa = k3.mxfp4_pack(p[i], s[i])
+        assert torch.equal(codes[i], wc[0]) and torch.equal(atoms[i], wa[0])
+    a, sa = k3.mxfp4_quant(torch.randn((40, H), device=dev, generator=g))
+    off = torch.zeros(n + 1, dtype=torch.int32, device=dev)
+    off[n:] = 40                                    # all rows at the last matrix
+    W = k3.Mxfp4Mat(codes, atoms)
+    y = k3.mxfp4_mm(a, sa, W, off=off)
+    last = k3.Mxfp4Mat(wc, wa)
+    assert torch.equal(y.view(torch.int16), k3.mxfp4_mm(a, sa, last).view(torch.int16))      # the bits: infinities and NaN
+    assert torch.equal(k3.mxfp4_mm_bwd(y, W, off=off).view(torch.int16), k3.mxfp4_mm_bwd(y, last).view(torch.int16))
+    del p, s, codes, atoms, W
+    torch.cuda.empty_cache()
