@@ -1566,9 +1566,9 @@ struct TileCost {
 };
 // The cheapest of n kernels for M rows in n_groups groups (grouped: their sizes are on the device;
 // each is taken to waste half a tile) and `cols` columns, kb K blocks. Ties go to the first. All M rows are
-// taken to belong to groups: where an expert-parallel rank holds 4608 of 32768, in 48 groups, a
-// product with 4096 x 7168 matrices takes 160 us on pairs and 144 on 128 x 256 tiles, which the rows alone
-// would take (the gradient of 7168 x 2048 takes pairs either way).
+// taken to belong to groups: where an expert-parallel rank holds 3637 of 32768, in 48 groups, a
+// product with 4096 x 7168 matrices takes 159 us on pairs and 135 on 128 x 256 tiles, which the rows alone
+// would take; the gradient of 7168 x 2048 takes 247 us on pairs and 275 on those tiles.
 int cheapest(const TileCost *t, int n, int M, int n_groups, bool grouped, int cols, int kb) {
     int best = 0;
     double least = 0;
